@@ -856,6 +856,100 @@ int tris_route_predecode_all_reduce(const float* router_logits, int32_t num_toke
                                     const tris_gr_predecode_job* jobs, int32_t num_jobs,
                                     const tris_backbone_pair_job* bb, void* stream);
 
+/*
+ * The attention side of a decoder layer, around the compact3 Q/K/V and output linears (no native counterpart in the
+ * reference: its models run the norms, the rotation, the cache and the attention as torch ops,
+ * modeling_mixtral.py:610-757).  Serving only, no gradients.
+ *
+ * Element types of activations, weights and caches:
+ */
+#define TRIS_DTYPE_F16 0
+#define TRIS_DTYPE_BF16 1
+#define TRIS_DTYPE_F32 2
+#define TRIS_DTYPE_E4M3 3 /* OCP 8-bit float, 4 exponent bits, largest value 448 */
+
+/*
+ * Root-mean-square norm of each row with the residual's addition, in one launch:
+ *   h = x + residual (fp32; h = x without one),  residual_out = h rounded to residual_type,
+ *   out = h * rsqrt(mean(h^2) + eps) * (weight + weight_offset), fp32, rounded once to out_type.
+ * The norm reads the unrounded sum.  x [rows, width] of x_type (F16 or BF16), rows x_stride elements apart; residual
+ * and residual_out likewise of residual_type (both NULL without one; residual_out may be residual itself); weight
+ * [width] of weight_type (F16, BF16 or F32); out of out_type (may be x itself if types and strides agree).  Buffers
+ * may not overlap otherwise.  1 <= width <= 32768; any alignment (16-byte loads where everything is 16-byte aligned).
+ */
+int tris_rms_norm(const void* x, int32_t x_type, int64_t x_stride, const void* residual, int32_t residual_type,
+                  int64_t residual_stride, const void* weight, int32_t weight_type, float weight_offset, float eps,
+                  int64_t rows, int32_t width, void* out, int32_t out_type, int64_t out_stride, void* residual_out,
+                  int64_t residual_out_stride, void* stream);
+
+/*
+ * A paged key / value cache and the sequences that live in it.  Position p of sequence b is slot p % page_size of page
+ * block_table[b][p / page_size].  k and v hold [num_pages][kv_heads][page_size][head_dim] elements of `dtype` (F16,
+ * BF16 or E4M3) with any strides over the first three dimensions that keep each row of head_dim contiguous values
+ * 16-byte aligned (strides in elements; page_size * slot stride below 2^31 bytes).  With E4M3, k_scale and v_scale
+ * hold an fp32 factor per (page, head, slot): value = element * scale; NULL otherwise.  seq_lens[b] counts the
+ * sequence's positions, new tokens included; a length <= 0 is an idle sequence, and lengths past
+ * max_pages * page_size are cut there.  Page numbers outside [0, num_pages) are never dereferenced: tokens that would
+ * go there are not stored, and keys there are left out of the attention.  head_dim 64, 128 or 256; page_size >= 1.
+ */
+typedef struct tris_paged_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* block_table; /* [batch][max_pages], rows table_stride apart */
+  const int32_t* seq_lens;    /* [batch] */
+  int64_t k_page_stride, k_head_stride, k_slot_stride;
+  int64_t v_page_stride, v_head_stride, v_slot_stride;
+  int64_t k_scale_page_stride, k_scale_head_stride, k_scale_slot_stride;
+  int64_t v_scale_page_stride, v_scale_head_stride, v_scale_slot_stride;
+  int64_t table_stride;
+  int32_t num_pages, page_size, kv_heads, head_dim;
+  int32_t batch, max_pages, dtype;
+} tris_paged_cache;
+
+/*
+ * Rotates the queries and keys of `tokens` new tokens by their positions and appends keys and values to the cache, in
+ * one launch.  Token t of sequence b (query_start[b] <= t < query_start[b + 1], query_start [batch + 1] non-decreasing;
+ * NULL: token t is sequence t's one new token, tokens == batch) has position
+ * p = seq_lens[b] - (query_start[b + 1] - t).  With cos, sin fp32 [positions][rotary_dim / 2], r = rotary_dim / 2:
+ *   y[i] = x[i] cos[p][i] - x[i + r] sin[p][i],  y[i + r] = x[i + r] cos[p][i] + x[i] sin[p][i],  i < r,
+ * fp32 with each product rounded, and y[i] = x[i] from rotary_dim on; values are not rotated.  q_out takes the rotated
+ * queries (may be q itself with the same strides), the cache the keys and values, each rounded once.  E4M3:
+ * scale = max(max_i |y[i]| * (1 / 448), 2^-126) and the element y[i] / scale rounded to nearest even; a row with an
+ * infinity or NaN is stored as NaN.  Tokens past query_start[batch], and those of a negative position, are not
+ * stored; their rows of q_out are left as they were, or set to zero with zero_unplaced.  Two sequences whose tables
+ * name the same page for a position being written race there.
+ * q [tokens][q_heads][head_dim] (NULL with q_heads 0: keys and values only), k, v [tokens][kv_heads][head_dim] of
+ * act_type (F16 or BF16; a 16-bit cache has the same type), strides in elements over tokens and heads, rows 16-byte
+ * aligned.  rotary_dim a multiple of 16 up to head_dim; positions >= max_pages * page_size.
+ */
+int tris_rotary_append_paged(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                             int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                             int64_t v_head_stride, int32_t act_type, int32_t tokens, int32_t q_heads,
+                             const float* cos, const float* sin, int32_t rotary_dim, int32_t positions,
+                             const int32_t* query_start, const tris_paged_cache* cache, void* q_out,
+                             int64_t q_out_token_stride, int64_t q_out_head_stride, int32_t zero_unplaced,
+                             void* stream);
+
+/*
+ * Attention of one new token a sequence over the paged cache: with n = seq_lens[b] (cut as above), query head h of
+ * sequence b reads kv head h / (q_heads / kv_heads) and keys j in [first, n), first = 0 or, with window > 0,
+ * max(0, n - window):
+ *   out[b][h] = sum_j softmax_j(scale * q[b][h] . k_j) v_j,
+ * scores, softmax statistics and sums in fp32, rounded once to q's type.  A sequence without keys (idle, or none of
+ * its pages valid) gives zeros.  Slots past the sequence's end, before its window, or on invalid pages may hold
+ * anything.  q, out [batch][q_heads][head_dim] of q_type (F16 or BF16; a 16-bit cache has the same type), strides in
+ * elements, rows 16-byte aligned; q_heads a multiple of kv_heads.  workspace: tris_paged_attention_workspace_bytes of
+ * the same sizes, 16-byte aligned, no initial contents; calls that may overlap need one each.
+ */
+int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, int64_t q_head_stride, int32_t q_type,
+                                int32_t q_heads, const tris_paged_cache* cache, float scale, int32_t window, void* out,
+                                int64_t out_seq_stride, int64_t out_head_stride, void* workspace,
+                                int64_t workspace_bytes, void* stream);
+int64_t tris_paged_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                             int32_t max_pages, int32_t page_size);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,184 @@
+// Rotation of queries and keys by their positions, and the append of keys and values to the paged cache.
+//
+// One launch does the three tensors: a workgroup has one token, whose position, page and table row are the same for
+// all its threads, and a thread has 16 of a head's values: in a rotated part eight of the lower half and the eight
+// that pair with them, elsewhere sixteen in a row.  An 8-bit row's largest magnitude is a maximum over the head's
+// head_dim / 16 neighbouring lanes.
+#include "tris_paged.h"
+
+// The rotation's two products and their sum are rounded one by one, as the same torch expression rounds them, so that
+// the values (and the 8-bit elements made of them) do not depend on which of the two wrote a cache.
+#pragma clang fp contract(off)
+
+namespace tris {
+
+struct AppendArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* q_out;
+  const float* cos;
+  const float* sin;
+  const int32_t* query_start;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, qo_token, qo_head;
+  int32_t act_bf16, tokens, q_heads, rotary_dim, zero_unplaced;
+  tris_paged_cache c;
+};
+
+// The sequence whose new tokens hold token t, or -1; *end: one past its last new token.
+__device__ __forceinline__ int token_sequence(const AppendArgs& a, int t, int* end) {
+  if (a.query_start == nullptr) {
+    *end = t + 1;
+    return t < a.c.batch ? t : -1;
+  }
+  int lo = 0, hi = a.c.batch;  // the first b with query_start[b + 1] > t
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (a.query_start[mid + 1] > t) hi = mid;
+    else lo = mid + 1;
+  }
+  if (lo == a.c.batch || a.query_start[lo] > t) return -1;
+  *end = a.query_start[lo + 1];
+  return lo;
+}
+
+// 16 values of one row as e4m3 pairs: v / scale, round to nearest even
+__device__ __forceinline__ uint2 e4m3x8(const float v[8], float scale) {
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int p = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i] / scale, v[4 * i + 1] / scale, 0, false);
+    p = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2] / scale, v[4 * i + 3] / scale, p, true);
+    w[i] = static_cast<uint32_t>(p);
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+template <bool kE4m3>
+__global__ __launch_bounds__(512) void rotary_append_kernel(const AppendArgs a) {
+  const int t = blockIdx.x;
+  const int dim = a.c.head_dim, lanes = dim / 16, half = a.rotary_dim / 2;
+  const bool bf16 = a.act_bf16 != 0;
+  int end = 0;
+  const int seq = token_sequence(a, t, &end);
+  int pos = -1;
+  if (seq >= 0) {
+    const int64_t p = static_cast<int64_t>(a.c.seq_lens[seq]) - (end - t);
+    pos = p >= 0 && p < cache_positions(a.c) ? static_cast<int>(p) : -1;
+  }
+  int page = -1, slot = 0;
+  if (pos >= 0) {
+    page = a.c.block_table[seq * a.c.table_stride + pos / a.c.page_size];
+    slot = pos % a.c.page_size;
+    if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.c.num_pages)) page = -1;
+  }
+  const int units = (a.q_heads + 2 * a.c.kv_heads) * lanes;
+  for (int u = threadIdx.x; u < units; u += blockDim.x) {
+    const int h = u / lanes, part = u % lanes;
+    const bool is_q = h < a.q_heads, is_k = !is_q && h < a.q_heads + a.c.kv_heads;
+    const int hh = is_q ? h : is_k ? h - a.q_heads : h - a.q_heads - a.c.kv_heads;
+    const bool rotated = (is_q || is_k) && part * 8 < half;
+    const int lo = rotated ? part * 8 : (is_q || is_k) ? a.rotary_dim + (part - half / 8) * 16 : part * 16;
+    const int hi = rotated ? lo + half : lo + 8;
+    if (is_q && pos < 0) {
+      if (a.zero_unplaced) {
+        uint16_t* o = a.q_out + t * a.qo_token + hh * a.qo_head;
+        *reinterpret_cast<uint4*>(o + lo) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(o + hi) = make_uint4(0, 0, 0, 0);
+      }
+      continue;
+    }
+    if (!is_q && page < 0) continue;
+    const uint16_t* src = is_q   ? a.q + t * a.q_token + hh * a.q_head
+                          : is_k ? a.k + t * a.k_token + hh * a.k_head
+                                 : a.v + t * a.v_token + hh * a.v_head;
+    float x[8], y[8];
+    widen8(*reinterpret_cast<const uint4*>(src + lo), bf16, x);
+    widen8(*reinterpret_cast<const uint4*>(src + hi), bf16, y);
+    if (rotated) {
+      const float* cs = a.cos + static_cast<int64_t>(pos) * half + lo;
+      const float* sn = a.sin + static_cast<int64_t>(pos) * half + lo;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float c = cs[i], s = sn[i], xi = x[i], yi = y[i];
+        x[i] = xi * c - yi * s;
+        y[i] = yi * c + xi * s;
+      }
+    }
+    if (is_q) {
+      uint16_t* o = a.q_out + t * a.qo_token + hh * a.qo_head;
+      *reinterpret_cast<uint4*>(o + lo) = narrow8(x, bf16);
+      *reinterpret_cast<uint4*>(o + hi) = narrow8(y, bf16);
+      continue;
+    }
+    const int64_t at = is_k ? page * a.c.k_page_stride + hh * a.c.k_head_stride + slot * a.c.k_slot_stride
+                            : page * a.c.v_page_stride + hh * a.c.v_head_stride + slot * a.c.v_slot_stride;
+    if constexpr (!kE4m3) {
+      uint16_t* o = static_cast<uint16_t*>(is_k ? a.c.k : a.c.v) + at;
+      *reinterpret_cast<uint4*>(o + lo) = narrow8(x, bf16);
+      *reinterpret_cast<uint4*>(o + hi) = narrow8(y, bf16);
+    } else {
+      // magnitudes compare as their bits, and a NaN's are above infinity's, so that one in the row becomes the scale
+      uint32_t most = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        most = max(most, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+        most = max(most, __float_as_uint(y[i]) & 0x7FFFFFFFu);
+      }
+      for (int d = 1; d < lanes; d *= 2) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), d)));
+      float scale = __uint_as_float(most) * (1.0f / kE4m3Max);
+      if (scale < kSmallestScale) scale = kSmallestScale;
+      uint8_t* o = static_cast<uint8_t*>(is_k ? a.c.k : a.c.v) + at;
+      *reinterpret_cast<uint2*>(o + lo) = e4m3x8(x, scale);
+      *reinterpret_cast<uint2*>(o + hi) = e4m3x8(y, scale);
+      if (part == 0) {
+        if (is_k) a.c.k_scale[page * a.c.k_scale_page_stride + hh * a.c.k_scale_head_stride + slot * a.c.k_scale_slot_stride] = scale;
+        else a.c.v_scale[page * a.c.v_scale_page_stride + hh * a.c.v_scale_head_stride + slot * a.c.v_scale_slot_stride] = scale;
+      }
+    }
+  }
+}
+
+}  // namespace tris
+
+using namespace tris;
+
+extern "C" int tris_rotary_append_paged(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                                        int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                                        int64_t v_token_stride, int64_t v_head_stride, int32_t act_type,
+                                        int32_t tokens, int32_t q_heads, const float* cos, const float* sin,
+                                        int32_t rotary_dim, int32_t positions, const int32_t* query_start,
+                                        const tris_paged_cache* cache, void* q_out, int64_t q_out_token_stride,
+                                        int64_t q_out_head_stride, int32_t zero_unplaced, void* stream) {
+  const char* who = "tris_rotary_append_paged";
+  if (const int rc = check_paged_cache(who, cache, act_type)) return rc;
+  TRIS_REQUIRE(tokens >= 0 && q_heads >= 0, "%s: negative shape", who);
+  TRIS_REQUIRE(query_start || tokens == cache->batch, "%s: without query_start there is one token a sequence", who);
+  TRIS_REQUIRE(rotary_dim >= 16 && rotary_dim % 16 == 0 && rotary_dim <= cache->head_dim,
+               "%s: rotary_dim must be a multiple of 16 up to head_dim", who);
+  TRIS_REQUIRE(positions >= cache_positions(*cache), "%s: cos and sin must cover max_pages * page_size positions", who);
+  if (tokens == 0) return TRIS_OK;
+  TRIS_REQUIRE(cache->batch > 0, "%s: tokens without sequences", who);
+  TRIS_REQUIRE(k && v && cos && sin && (q_heads == 0 || (q && q_out)), "%s: null pointer", who);
+  for (const int64_t s : {q_heads ? q_token_stride : 0, q_heads ? q_head_stride : 0, k_token_stride, k_head_stride,
+                          v_token_stride, v_head_stride, q_heads ? q_out_token_stride : 0,
+                          q_heads ? q_out_head_stride : 0})
+    TRIS_REQUIRE(s >= 0 && s % 8 == 0, "%s: rows must be 16-byte aligned", who);
+  TRIS_REQUIRE(aligned16(k) && aligned16(v) && aligned16(cos) && aligned16(sin) &&
+                   (q_heads == 0 || (aligned16(q) && aligned16(q_out))),
+               "%s: rows must be 16-byte aligned", who);
+  const int64_t units = (static_cast<int64_t>(q_heads) + 2LL * cache->kv_heads) * (cache->head_dim / 16);
+  TRIS_REQUIRE(units < (1 << 24), "%s: too many heads", who);
+  AppendArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
+               static_cast<uint16_t*>(q_out), cos, sin, query_start, q_token_stride, q_head_stride, k_token_stride,
+               k_head_stride, v_token_stride, v_head_stride, q_out_token_stride, q_out_head_stride,
+               act_type == TRIS_DTYPE_BF16, tokens, q_heads, rotary_dim, zero_unplaced, *cache};
+  const dim3 block(static_cast<unsigned>(units >= 512 ? 512 : (units + kWave - 1) / kWave * kWave));
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (cache->dtype == TRIS_DTYPE_E4M3) {
+    hipLaunchKernelGGL(rotary_append_kernel<true>, dim3(tokens), block, 0, st, a);
+  } else {
+    hipLaunchKernelGGL(rotary_append_kernel<false>, dim3(tokens), block, 0, st, a);
+  }
+  return check_launch(who);
+}

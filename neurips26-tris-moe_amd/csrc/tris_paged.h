@@ -1,0 +1,44 @@
+// The paged key / value cache: host checks and addressing shared by the append and the attention.
+#pragma once
+
+#include "tris_dtype.h"
+
+namespace tris {
+
+constexpr float kE4m3Max = 448.0f;
+constexpr float kSmallestScale = 1.17549435e-38f;  // 2^-126
+
+// Positions that a sequence's row of the block table can address (the entry checks keep it below 2^31).
+__host__ __device__ inline int32_t cache_positions(const tris_paged_cache& c) { return c.max_pages * c.page_size; }
+
+// The cache's own contract; `who` names the entry point in the message.
+inline int check_paged_cache(const char* who, const tris_paged_cache* c, int32_t act_type) {
+  TRIS_REQUIRE(c != nullptr, "%s: null cache", who);
+  TRIS_REQUIRE(c->batch >= 0 && c->num_pages >= 1 && c->kv_heads >= 1 && c->max_pages >= 0,
+               "%s: a cache has at least one page and one head", who);
+  TRIS_REQUIRE(c->page_size >= 1, "%s: page_size must be positive", who);
+  TRIS_REQUIRE(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, "%s: head_dim must be 64, 128 or 256",
+               who);
+  TRIS_REQUIRE(is_16bit(act_type), "%s: activations must be fp16 or bf16", who);
+  const bool e4m3 = c->dtype == TRIS_DTYPE_E4M3;
+  TRIS_REQUIRE(e4m3 || c->dtype == act_type, "%s: the cache must be e4m3 or of the activations' type", who);
+  TRIS_REQUIRE(e4m3 == (c->k_scale != nullptr) && e4m3 == (c->v_scale != nullptr),
+               "%s: an e4m3 cache, and no other, has k_scale and v_scale", who);
+  TRIS_REQUIRE(c->batch == 0 || (c->k && c->v && c->seq_lens && (c->block_table || c->max_pages == 0)),
+               "%s: null pointer", who);
+  TRIS_REQUIRE(static_cast<int64_t>(c->max_pages) * c->page_size < 2147483647LL, "%s: block table too wide", who);
+  TRIS_REQUIRE(c->table_stride >= 0, "%s: negative table stride", who);
+  const int size = e4m3 ? 1 : 2;
+  for (const int64_t s : {c->k_page_stride, c->k_head_stride, c->k_slot_stride, c->v_page_stride, c->v_head_stride,
+                          c->v_slot_stride})
+    TRIS_REQUIRE(s >= 0 && s * size % 16 == 0, "%s: cache rows must be 16-byte aligned", who);
+  TRIS_REQUIRE(aligned16(c->k) && aligned16(c->v), "%s: cache rows must be 16-byte aligned", who);
+  for (const int64_t s : {c->k_slot_stride, c->v_slot_stride, c->k_scale_slot_stride, c->v_scale_slot_stride})
+    TRIS_REQUIRE(s >= 0 && s < 2147483648LL && s * 4 * c->page_size < 2147483648LL, "%s: slot stride too large", who);
+  for (const int64_t s : {c->k_scale_page_stride, c->k_scale_head_stride, c->v_scale_page_stride,
+                          c->v_scale_head_stride})
+    TRIS_REQUIRE(!e4m3 || s >= 0, "%s: negative scale stride", who);
+  return TRIS_OK;
+}
+
+}  // namespace tris

@@ -126,6 +126,21 @@ class TrisNsPayload(ctypes.Structure):
     ]
 
 
+class TrisPagedCache(ctypes.Structure):
+    """Mirror of struct tris_paged_cache."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "block_table", "seq_lens")]
+                + [(n, ctypes.c_int64) for n in (
+                    "k_page_stride", "k_head_stride", "k_slot_stride",
+                    "v_page_stride", "v_head_stride", "v_slot_stride",
+                    "k_scale_page_stride", "k_scale_head_stride", "k_scale_slot_stride",
+                    "v_scale_page_stride", "v_scale_head_stride", "v_scale_slot_stride", "table_stride")]
+                + [(n, ctypes.c_int32) for n in ("num_pages", "page_size", "kv_heads", "head_dim", "batch", "max_pages",
+                                                 "dtype")])
+
+
+DTYPE_F16, DTYPE_BF16, DTYPE_F32, DTYPE_E4M3 = range(4)  # TRIS_DTYPE_*
+
 MAX_PREDECODE_JOBS = 4
 
 _P = ctypes.c_void_p
@@ -134,6 +149,7 @@ _I64 = ctypes.c_int64
 _PAY = ctypes.POINTER(TrisPayload)
 _P4 = ctypes.POINTER(TrisPacked4)
 _PNS = ctypes.POINTER(TrisNsPayload)
+_PPC = ctypes.POINTER(TrisPagedCache)
 SIGNATURES = {
     "tris_abi_version": (ctypes.c_int, []),
     "tris_last_error": (ctypes.c_char_p, []),
@@ -215,6 +231,13 @@ SIGNATURES = {
                                                      _I64, _P]),
     "tris_compact3_linears_workspace_bytes": (_I64, [_I32, _I32, ctypes.POINTER(_I32), _I32]),
     "tris_dense_linear_f32": (ctypes.c_int, [_P, _P, _I32, _I32, _P, _I32, _P, _P]),
+    "tris_rms_norm": (ctypes.c_int, [_P, _I32, _I64, _P, _I32, _I64, _P, _I32, ctypes.c_float, ctypes.c_float, _I64,
+                                     _I32, _P, _I32, _I64, _P, _I64, _P]),
+    "tris_rotary_append_paged": (ctypes.c_int, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _I32, _I32, _P,
+                                                _P, _I32, _I32, _P, _PPC, _P, _I64, _I64, _I32, _P]),
+    "tris_paged_attention_decode": (ctypes.c_int, [_P, _I64, _I64, _I32, _I32, _PPC, ctypes.c_float, _I32, _P, _I64,
+                                                   _I64, _P, _I64, _P]),
+    "tris_paged_attention_workspace_bytes": (_I64, [_I32] * 6),
 }
 
 _lib = None

@@ -1981,6 +1981,258 @@ def swiglu_mul(gate: torch.Tensor, up: torch.Tensor, out: torch.Tensor | None = 
     return out
 
 
+# ------------------------------------------------------------------ attention side of a decoder layer
+_DTYPE_IDS = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32,
+              torch.float8_e4m3fn: _lib.DTYPE_E4M3}
+_ACT_DTYPES = (torch.float16, torch.bfloat16)
+RMS_NORM_MAX_WIDTH = 32768
+PAGED_HEAD_DIMS = (64, 128, 256)
+
+
+def _launch(device, fn, *args):
+    """Calls a C entry with its device current: a stream takes launches from its own device only."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return fn(*args)
+    return fn(*args)
+
+
+def _serving_inputs(who, *tensors):
+    """These entries have no backward: an input that would need one is refused, not cut from its graph."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{who}: no gradient is defined; call it under torch.no_grad()")
+
+
+def _check_on(who, name, t, dims, dtypes, device=None):
+    """A CUDA tensor of `dims` dimensions and one of `dtypes` (on `device`), any strides."""
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{who}: {name} must be a tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{who}: {name} must be a CUDA tensor")
+    if device is not None and t.device != device:
+        raise RuntimeError(f"{who}: {name} must be on {device}")
+    if t.dtype not in dtypes:
+        raise RuntimeError(f"{who}: {name} must be {' or '.join(str(d) for d in dtypes)}")
+    if dims is not None and t.ndim != dims:
+        raise RuntimeError(f"{who}: {name} must be {dims}D")
+
+
+def _norm_rows(who, name, t, width):
+    """(rows, row stride) of t [..., width] whose leading dimensions collapse to one stride."""
+    if t.shape[-1] != width:
+        raise RuntimeError(f"{who}: {name} must have {width} columns")
+    if t.is_contiguous():
+        return t.numel() // width, width
+    try:
+        flat = t.view(-1, width)
+    except RuntimeError:
+        flat = None
+    if flat is None or (flat.stride(1) != 1 and width > 1):
+        raise RuntimeError(f"{who}: the rows of {name} must be contiguous, one stride apart")
+    return flat.size(0), flat.stride(0)
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.Tensor | None = None,
+             weight_offset: float = 0.0, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
+             residual_out: torch.Tensor | None = None):
+    """Root-mean-square norm over the last dimension with the residual's addition, in one launch (tris_rms_norm):
+    h = x + residual in fp32, residual_out = h in residual's dtype, out = h * rsqrt(mean(h^2) + eps) * (weight +
+    weight_offset), rounded once to out_dtype (x's by default).  Returns out, or (out, residual_out) with a residual.
+
+    x [..., width] fp16 or bf16 (the norm of each head: [tokens, heads, head_dim]), rows contiguous and one stride
+    apart; residual of x's shape, fp16 or bf16 (x may be the fp16 output of a compact3 linear and the residual stream
+    bf16); weight [width] fp16, bf16 or fp32.  residual_out may be residual, and out may be x; buffers may not
+    overlap otherwise.  width up to RMS_NORM_MAX_WIDTH.  No gradient."""
+    who = "rms_norm"
+    _check_on(who, "x", x, None, _ACT_DTYPES)
+    dev = x.device
+    _check_on(who, "weight", weight, 1, (torch.float16, torch.bfloat16, torch.float32), dev)
+    _serving_inputs(who, x, weight, residual)
+    width = weight.numel()
+    if x.ndim < 1 or not 1 <= width <= RMS_NORM_MAX_WIDTH:
+        raise RuntimeError(f"{who}: width must be 1 to {RMS_NORM_MAX_WIDTH}")
+    if not weight.is_contiguous():
+        raise RuntimeError(f"{who}: weight must be contiguous")
+    rows, x_stride = _norm_rows(who, "x", x, width)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype if out_dtype is None else out_dtype, device=dev)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise RuntimeError(f"{who}: out must be {out_dtype}")
+    _check_on(who, "out", out, None, _ACT_DTYPES, dev)
+    if out.shape != x.shape:
+        raise RuntimeError(f"{who}: out must have the shape of x")
+    out_stride = _norm_rows(who, "out", out, width)[1]
+    r_type = r_stride = ro_stride = 0
+    if residual is not None:
+        _check_on(who, "residual", residual, None, _ACT_DTYPES, dev)
+        if residual.shape != x.shape:
+            raise RuntimeError(f"{who}: residual must have the shape of x")
+        if residual_out is None:
+            residual_out = torch.empty(x.shape, dtype=residual.dtype, device=dev)
+        _check_on(who, "residual_out", residual_out, None, (residual.dtype,), dev)
+        if residual_out.shape != x.shape:
+            raise RuntimeError(f"{who}: residual_out must have the shape of x")
+        r_type = _DTYPE_IDS[residual.dtype]
+        r_stride = _norm_rows(who, "residual", residual, width)[1]
+        ro_stride = _norm_rows(who, "residual_out", residual_out, width)[1]
+    elif residual_out is not None:
+        raise RuntimeError(f"{who}: residual_out needs a residual")
+    _lib.check(_launch(dev, _lib.load().tris_rms_norm, _ptr(x), _DTYPE_IDS[x.dtype], x_stride, _ptr(residual), r_type,
+                       r_stride, _ptr(weight), _DTYPE_IDS[weight.dtype], weight_offset, eps, rows, width, _ptr(out),
+                       _DTYPE_IDS[out.dtype], out_stride, _ptr(residual_out), ro_stride, _stream(x)), "tris_rms_norm")
+    return out if residual is None else (out, residual_out)
+
+
+def _heads(who, name, t, dtypes, device, dim):
+    """t [tokens, heads, dim] with 16-byte-aligned contiguous rows, or a copy of it that has them."""
+    _check_on(who, name, t, 3, dtypes, device)
+    if t.size(2) != dim:
+        raise RuntimeError(f"{who}: {name} must have the cache's head_dim {dim}")
+    if t.stride(2) == 1 and not (t.data_ptr() % 16 or t.stride(0) % 8 or t.stride(1) % 8):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _paged_cache(who, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, device):
+    """The C descriptor of a paged cache (struct tris_paged_cache)."""
+    _check_on(who, "k_cache", k_cache, 4, _CACHE_DTYPES, device)
+    _check_on(who, "v_cache", v_cache, 4, (k_cache.dtype,), device)
+    _check_on(who, "block_table", block_table, 2, (torch.int32,), device)
+    _check_on(who, "seq_lens", seq_lens, 1, (torch.int32,), device)
+    pages, heads, page, dim = k_cache.shape
+    if v_cache.shape != k_cache.shape:
+        raise RuntimeError(f"{who}: v_cache must have the shape of k_cache")
+    ks, vs = k_cache.stride(), v_cache.stride()
+    if ks[3] != 1 or vs[3] != 1:
+        raise RuntimeError(f"{who}: each cache row of head_dim values must be contiguous")
+    batch, max_pages = block_table.shape
+    if seq_lens.size(0) != batch or not seq_lens.is_contiguous():
+        raise RuntimeError(f"{who}: seq_lens must be contiguous, one length for each row of block_table")
+    if block_table.stride(1) != 1 and max_pages > 1:
+        raise RuntimeError(f"{who}: the rows of block_table must be contiguous")
+    sks = svs = (0, 0, 0)
+    if k_cache.dtype is torch.float8_e4m3fn:
+        if k_scale is None or v_scale is None:
+            raise RuntimeError(f"{who}: an e4m3 cache needs k_scale and v_scale")
+        for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+            _check_on(who, name, s, 3, (torch.float32,), device)
+            if s.shape != (pages, heads, page):
+                raise RuntimeError(f"{who}: {name} must be [pages, kv_heads, page_size]")
+        sks, svs = k_scale.stride(), v_scale.stride()
+    elif k_scale is not None or v_scale is not None:
+        raise RuntimeError(f"{who}: k_scale and v_scale belong to an e4m3 cache")
+    # by position, in the order of TrisPagedCache's fields
+    return _lib.TrisPagedCache(
+        k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), block_table.data_ptr(),
+        seq_lens.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], *sks, *svs, block_table.stride(0), pages, page,
+        heads, dim, batch, max_pages, _DTYPE_IDS[k_cache.dtype])
+
+
+_CACHE_DTYPES = (torch.float16, torch.bfloat16, torch.float8_e4m3fn)
+
+
+def rotary_append_paged(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                        k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                        seq_lens: torch.Tensor, query_start: torch.Tensor | None = None,
+                        k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                        q_out: torch.Tensor | None = None):
+    """Rotates queries and keys by their positions and appends keys and values to the paged cache, in one launch
+    (tris_rotary_append_paged).  Returns the rotated queries (None without q).
+
+    q [tokens, q_heads, head_dim], k and v [tokens, kv_heads, head_dim], fp16 or bf16 (rows that are not 16-byte
+    aligned are copied first).  cos, sin fp32 [positions, rotary_dim / 2] (``attention.rotary_tables``), covering
+    every position the block table can address; the first rotary_dim of head_dim values are rotated by halves
+    (y[i] = x[i] cos - x[i + r] sin, y[i + r] = x[i + r] cos + x[i] sin, r = rotary_dim / 2).
+
+    k_cache, v_cache [pages, kv_heads, page_size, head_dim] in q's dtype or float8_e4m3fn, any strides that keep rows
+    contiguous and 16-byte aligned (a [pages, page_size, kv_heads, head_dim] pool: pass it permuted); e4m3 with
+    k_scale, v_scale fp32 [pages, kv_heads, page_size].  block_table int32 [batch, max_pages]; seq_lens int32 [batch],
+    the lengths with the new tokens.  query_start int32 [batch + 1]: sequence b's new tokens are rows
+    query_start[b] to query_start[b + 1], its last ones; None: one new token a sequence, token b is sequence b's.
+
+    A row past query_start[-1], or of an idle sequence (length 0), is not stored and its rotated query is zero (left
+    as it was in a given q_out).  A page number outside the pool is skipped.  q_out may be q.  No gradient."""
+    who = "rotary_append_paged"
+    _check_on(who, "k", k, 3, _ACT_DTYPES)
+    dev, dt = k.device, (k.dtype,)
+    _serving_inputs(who, q, k, v)
+    cache = _paged_cache(who, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, dev)
+    dim, heads, tokens = cache.head_dim, cache.kv_heads, k.size(0)
+    k, v = _heads(who, "k", k, dt, dev, dim), _heads(who, "v", v, dt, dev, dim)
+    if k.size(1) != heads or v.shape != k.shape:
+        raise RuntimeError(f"{who}: k and v must be [tokens, kv_heads, head_dim] of the cache's kv_heads")
+    for name, t in (("cos", cos), ("sin", sin)):
+        _check_cuda(name, t, torch.float32, 2, dev)
+    if sin.shape != cos.shape:
+        raise RuntimeError(f"{who}: cos and sin must have one shape")
+    if query_start is not None:
+        _check_cuda("query_start", query_start, torch.int32, 1, dev)
+        if query_start.size(0) != cache.batch + 1:
+            raise RuntimeError(f"{who}: query_start must hold batch + 1 entries")
+    q_heads, zero, qs, qos = 0, 0, (0, 0), (0, 0)
+    if q is not None:
+        inplace = q_out is q
+        q = _heads(who, "q", q, dt, dev, dim)
+        if q.size(0) != tokens:
+            raise RuntimeError(f"{who}: q, k and v must have one number of tokens")
+        q_heads = q.size(1)
+        if q_out is None:
+            q_out, zero = torch.empty(q.shape, dtype=q.dtype, device=dev), 1
+        elif inplace and q is not q_out:
+            raise RuntimeError(f"{who}: q_out must have 16-byte-aligned contiguous rows")
+        _check_on(who, "q_out", q_out, 3, dt, dev)
+        if q_out.shape != q.shape or q_out.stride(2) != 1:
+            raise RuntimeError(f"{who}: q_out must have the shape of q and contiguous rows")
+        qs, qos = q.stride(), q_out.stride()
+    elif q_out is not None:
+        raise RuntimeError(f"{who}: q_out needs q")
+    ks, vs = k.stride(), v.stride()
+    _lib.check(_launch(dev, _lib.load().tris_rotary_append_paged, _ptr(q), qs[0], qs[1], _ptr(k), ks[0], ks[1], _ptr(v),
+                       vs[0], vs[1], _DTYPE_IDS[k.dtype], tokens, q_heads, _ptr(cos), _ptr(sin), 2 * cos.size(1),
+                       cos.size(0), _ptr(query_start), ctypes.byref(cache), _ptr(q_out), qos[0], qos[1], zero,
+                       _stream(k)), "tris_rotary_append_paged")
+    return q_out
+
+
+def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                           seq_lens: torch.Tensor, scale: float | None = None, window: int = 0,
+                           k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                           out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one new token a sequence over the paged cache (tris_paged_attention_decode): out[b, h] =
+    sum_j softmax_j(scale * q[b, h] . k_j) v_j over sequence b's seq_lens[b] positions, or its last ``window`` of
+    them; fp32 inside, rounded once.  scale: head_dim ** -0.5 by default.
+
+    q [batch, q_heads, head_dim] fp16 or bf16, q_heads a multiple of kv_heads (query head h reads kv head
+    h // (q_heads / kv_heads)); the cache, block_table, seq_lens and scales as rotary_append_paged takes them.  An
+    idle sequence (length 0) gives zeros; slots outside a sequence may hold anything.  The launch depends on no value
+    on the device, so a captured call may be replayed with other lengths and tables.  No gradient."""
+    who = "paged_attention_decode"
+    _check_on(who, "q", q, 3, _ACT_DTYPES)
+    dev = q.device
+    _serving_inputs(who, q)
+    cache = _paged_cache(who, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, dev)
+    q = _heads(who, "q", q, (q.dtype,), dev, cache.head_dim)
+    batch, q_heads, dim = q.shape
+    if batch != cache.batch:
+        raise RuntimeError(f"{who}: q must hold one token for each row of block_table")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    _check_on(who, "out", out, 3, (q.dtype,), dev)
+    if out.shape != q.shape or out.stride(2) != 1:
+        raise RuntimeError(f"{who}: out must have the shape of q and contiguous rows")
+    lib = _lib.load()
+    need = lib.tris_paged_attention_workspace_bytes(batch, q_heads, cache.kv_heads, dim, cache.max_pages,
+                                                    cache.page_size)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    qs, os_ = q.stride(), out.stride()
+    _lib.check(_launch(dev, lib.tris_paged_attention_decode, _ptr(q), qs[0], qs[1], _DTYPE_IDS[q.dtype], q_heads,
+                       ctypes.byref(cache), dim ** -0.5 if scale is None else scale, int(window), _ptr(out), os_[0],
+                       os_[1], _ptr(ws), need, _stream(q)), "tris_paged_attention_decode")
+    return out
+
+
 def gr_encode(packed, k_min: int = 0, k_max: int = 7, force_raw: bool = False):
     """Host block-GR encoder: int32 [packed_rows, N] (numpy or CPU tensor) -> (words, offsets, meta) int32 numpy."""
     import numpy as np
