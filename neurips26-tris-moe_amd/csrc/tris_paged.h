@@ -8,7 +8,8 @@ namespace tris {
 constexpr float kE4m3Max = 448.0f;
 constexpr float kSmallestScale = 1.17549435e-38f;  // 2^-126
 
-// Positions that a sequence's row of the block table can address (the entry checks keep it below 2^31).
+// Positions that a sequence's row of the block table can address (the entry checks keep it below 2^31 - 2^16, so that a
+// few tiles past the end are still int32).
 __host__ __device__ inline int32_t cache_positions(const tris_paged_cache& c) { return c.max_pages * c.page_size; }
 
 // The cache's own contract; `who` names the entry point in the message.
@@ -26,7 +27,8 @@ inline int check_paged_cache(const char* who, const tris_paged_cache* c, int32_t
                "%s: an e4m3 cache, and no other, has k_scale and v_scale", who);
   TRIS_REQUIRE(c->batch == 0 || (c->k && c->v && c->seq_lens && (c->block_table || c->max_pages == 0)),
                "%s: null pointer", who);
-  TRIS_REQUIRE(static_cast<int64_t>(c->max_pages) * c->page_size < 2147483647LL, "%s: block table too wide", who);
+  TRIS_REQUIRE(static_cast<int64_t>(c->max_pages) * c->page_size < (1LL << 31) - (1 << 16),
+               "%s: block table too wide", who);
   TRIS_REQUIRE(c->table_stride >= 0, "%s: negative table stride", who);
   const int size = e4m3 ? 1 : 2;
   for (const int64_t s : {c->k_page_stride, c->k_head_stride, c->k_slot_stride, c->v_page_stride, c->v_head_stride,
