@@ -42,16 +42,12 @@ struct AttentionArgs {
   int64_t q_seq, q_head, out_seq, out_head;
   float scale_log2;                  // scale * log2(e): the softmax runs on powers of two
   int32_t window, q_heads, group, head_tiles, tile_heads, max_slots;
-  uint32_t page_magic, page_shift;   // division by page_size (below 2^31)
+  PageDivision page_of;
   int2* plan;                        // [batch]: first slot and number of the sequence's pieces
   float2* part_ml;                   // [slots][kv_heads * head_tiles][tile_heads]: maximum and sum
   float* part_o;                     // the same rows of head_dim sums
   tris_paged_cache c;
 };
-
-__device__ __forceinline__ int page_of(const AttentionArgs& a, int key) {
-  return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(key)) * a.page_magic) >> a.page_shift);
-}
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
@@ -191,7 +187,7 @@ __global__ __launch_bounds__(kWaves * kWave, kDim == 256 ? 1 : 2) void attention
     for (int i = 0; i < kPages; ++i) {
       const int key = key_of(tile, i);
       int id = -1;
-      if (tile < p.t1 && key < n && (kWhole || key >= first)) id = table[page_of(a, key)];
+      if (tile < p.t1 && key < n && (kWhole || key >= first)) id = table[a.page_of(key)];
       pg.id[i] = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.c.num_pages) ? id : -1;
       if constexpr (kWhole) pg.id[i] = uniform(pg.id[i]);
     }
@@ -206,7 +202,7 @@ __global__ __launch_bounds__(kWaves * kWave, kDim == 256 ? 1 : 2) void attention
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int page = max(pg.id[t], 0), key = key_of(tile, t);
-      const int slot = key - page_of(a, key) * a.c.page_size;
+      const int slot = key - a.page_of(key) * a.c.page_size;
       const char* row = kbase + page * a.c.k_page_stride * kSize;
       uint32_t off;
       if constexpr (kWhole) {
@@ -226,7 +222,7 @@ __global__ __launch_bounds__(kWaves * kWave, kDim == 256 ? 1 : 2) void attention
     if constexpr (kE4m3 && !kWhole) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int key = key_of(tile, 2 + j), slot = key - page_of(a, key) * a.c.page_size;
+        const int key = key_of(tile, 2 + j), slot = key - a.page_of(key) * a.c.page_size;
         ks[j] = ksbase[max(pg.id[2 + j], 0) * a.c.k_scale_page_stride + slot * ks_slot];
       }
     }
@@ -236,7 +232,7 @@ __global__ __launch_bounds__(kWaves * kWave, kDim == 256 ? 1 : 2) void attention
     for (int j = 0; j < 8; ++j) {
       const int i = kWhole ? j / 4 : 2 + j;
       const int page = max(pg.id[i], 0), key = key_of(tile, i);
-      const int slot = key - page_of(a, key) * a.c.page_size;
+      const int slot = key - a.page_of(key) * a.c.page_size;
       const char* row = vbase + page * a.c.v_page_stride * kSize;
       uint32_t off;
       if constexpr (kWhole) {
@@ -584,19 +580,24 @@ extern "C" int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, 
   const AttentionSpace w = attention_space(s, cache->batch, cache->head_dim);
   TRIS_REQUIRE(w.bytes == 0 || (workspace && aligned16(workspace) && workspace_bytes >= w.bytes),
                "%s: workspace of %lld bytes needed", who, static_cast<long long>(w.bytes));
-  AttentionArgs a{};
-  a.q = static_cast<const uint16_t*>(q);
-  a.out = static_cast<uint16_t*>(out);
-  a.q_seq = q_seq_stride, a.q_head = q_head_stride, a.out_seq = out_seq_stride, a.out_head = out_head_stride;
-  a.scale_log2 = scale * 1.44269504088896341f;
-  a.window = window, a.q_heads = q_heads, a.group = s.group, a.head_tiles = s.head_tiles;
-  a.tile_heads = s.tile_heads;
-  a.c = *cache;
-  // x / d = x * m >> (31 + e), m = 2^(31 + e) / d + 1, 2^e >= d, for x < 2^31
-  uint32_t e = 0;
-  while ((1u << e) < static_cast<uint32_t>(cache->page_size)) ++e;
-  a.page_magic = static_cast<uint32_t>((1ull << (31 + e)) / cache->page_size + 1);
-  a.page_shift = 31 + e;
+  AttentionArgs a{static_cast<const uint16_t*>(q),
+                  static_cast<uint16_t*>(out),
+                  q_seq_stride,
+                  q_head_stride,
+                  out_seq_stride,
+                  out_head_stride,
+                  scale * 1.44269504088896341f,
+                  window,
+                  q_heads,
+                  s.group,
+                  s.head_tiles,
+                  s.tile_heads,
+                  0,
+                  PageDivision(cache->page_size),
+                  nullptr,
+                  nullptr,
+                  nullptr,
+                  *cache};
   if (s.splits) {
     char* at = static_cast<char*>(workspace);
     a.max_slots = static_cast<int32_t>(s.slots);

@@ -22,24 +22,29 @@ struct AppendArgs {
   const int32_t* query_start;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, qo_token, qo_head;
   int32_t act_bf16, tokens, q_heads, rotary_dim, zero_unplaced;
+  PageDivision page_of;
   tris_paged_cache c;
 };
 
-// The sequence whose new tokens hold token t, or -1; *end: one past its last new token.
+// The sequence whose new tokens hold token t, or -1; *end: one past its last new token.  The wavefront reads 64
+// boundaries at a time and takes the first past t.
 __device__ __forceinline__ int token_sequence(const AppendArgs& a, int t, int* end) {
   if (a.query_start == nullptr) {
     *end = t + 1;
     return t < a.c.batch ? t : -1;
   }
-  int lo = 0, hi = a.c.batch;  // the first b with query_start[b + 1] > t
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (a.query_start[mid + 1] > t) hi = mid;
-    else lo = mid + 1;
+  const int lane = threadIdx.x % kWave, begin = a.query_start[0];
+  for (int b0 = 0; b0 < a.c.batch; b0 += kWave) {
+    const int b = b0 + lane;
+    const int e = b < a.c.batch ? a.query_start[b + 1] : 0;
+    const uint64_t past = __ballot(b < a.c.batch && e > t);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      *end = __builtin_amdgcn_readlane(e, l);
+      return t >= begin ? b0 + l : -1;
+    }
   }
-  if (lo == a.c.batch || a.query_start[lo] > t) return -1;
-  *end = a.query_start[lo + 1];
-  return lo;
+  return -1;
 }
 
 // 16 values of one row as e4m3 pairs: v / scale, round to nearest even
@@ -57,8 +62,38 @@ __device__ __forceinline__ uint2 e4m3x8(const float v[8], float scale) {
 template <bool kE4m3>
 __global__ __launch_bounds__(512) void rotary_append_kernel(const AppendArgs a) {
   const int t = blockIdx.x;
-  const int dim = a.c.head_dim, lanes = dim / 16, half = a.rotary_dim / 2;
+  const int lanes = a.c.head_dim / 16, half = a.rotary_dim / 2;
   const bool bf16 = a.act_bf16 != 0;
+  const int units = (a.q_heads + 2 * a.c.kv_heads) * lanes;
+
+  // a thread's unit: 16 values of one head, as two runs of eight columns
+  struct Unit {
+    bool is_q, is_k, rotated;
+    int head, part, lo, hi;
+    uint4 x, y;
+  };
+  const auto load = [&](int u) {
+    Unit w;
+    const int h = u / lanes;
+    w.part = u % lanes;
+    w.is_q = h < a.q_heads;
+    w.is_k = !w.is_q && h < a.q_heads + a.c.kv_heads;
+    w.head = w.is_q ? h : w.is_k ? h - a.q_heads : h - a.q_heads - a.c.kv_heads;
+    w.rotated = (w.is_q || w.is_k) && w.part * 8 < half;
+    w.lo = w.rotated ? w.part * 8 : (w.is_q || w.is_k) ? a.rotary_dim + (w.part - half / 8) * 16 : w.part * 16;
+    w.hi = w.rotated ? w.lo + half : w.lo + 8;
+    if (u < units) {
+      const uint16_t* src = w.is_q   ? a.q + t * a.q_token + w.head * a.q_head
+                            : w.is_k ? a.k + t * a.k_token + w.head * a.k_head
+                                     : a.v + t * a.v_token + w.head * a.v_head;
+      w.x = *reinterpret_cast<const uint4*>(src + w.lo);
+      w.y = *reinterpret_cast<const uint4*>(src + w.hi);
+    }
+    return w;
+  };
+  // the values first: they are in flight while the token's place is looked up
+  Unit w = load(threadIdx.x);
+
   int end = 0;
   const int seq = token_sequence(a, t, &end);
   int pos = -1;
@@ -68,74 +103,67 @@ __global__ __launch_bounds__(512) void rotary_append_kernel(const AppendArgs a) 
   }
   int page = -1, slot = 0;
   if (pos >= 0) {
-    page = a.c.block_table[seq * a.c.table_stride + pos / a.c.page_size];
-    slot = pos % a.c.page_size;
+    const int i = a.page_of(pos);
+    page = a.c.block_table[seq * a.c.table_stride + i];
+    slot = pos - i * a.c.page_size;
     if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.c.num_pages)) page = -1;
   }
-  const int units = (a.q_heads + 2 * a.c.kv_heads) * lanes;
-  for (int u = threadIdx.x; u < units; u += blockDim.x) {
-    const int h = u / lanes, part = u % lanes;
-    const bool is_q = h < a.q_heads, is_k = !is_q && h < a.q_heads + a.c.kv_heads;
-    const int hh = is_q ? h : is_k ? h - a.q_heads : h - a.q_heads - a.c.kv_heads;
-    const bool rotated = (is_q || is_k) && part * 8 < half;
-    const int lo = rotated ? part * 8 : (is_q || is_k) ? a.rotary_dim + (part - half / 8) * 16 : part * 16;
-    const int hi = rotated ? lo + half : lo + 8;
-    if (is_q && pos < 0) {
+
+  for (int u = threadIdx.x;;) {
+    uint16_t* q_out = a.q_out + t * a.qo_token + w.head * a.qo_head;
+    if (u < units && w.is_q && pos < 0) {
       if (a.zero_unplaced) {
-        uint16_t* o = a.q_out + t * a.qo_token + hh * a.qo_head;
-        *reinterpret_cast<uint4*>(o + lo) = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(o + hi) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(q_out + w.lo) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(q_out + w.hi) = make_uint4(0, 0, 0, 0);
       }
-      continue;
-    }
-    if (!is_q && page < 0) continue;
-    const uint16_t* src = is_q   ? a.q + t * a.q_token + hh * a.q_head
-                          : is_k ? a.k + t * a.k_token + hh * a.k_head
-                                 : a.v + t * a.v_token + hh * a.v_head;
-    float x[8], y[8];
-    widen8(*reinterpret_cast<const uint4*>(src + lo), bf16, x);
-    widen8(*reinterpret_cast<const uint4*>(src + hi), bf16, y);
-    if (rotated) {
-      const float* cs = a.cos + static_cast<int64_t>(pos) * half + lo;
-      const float* sn = a.sin + static_cast<int64_t>(pos) * half + lo;
+    } else if (u < units && (w.is_q || page >= 0)) {
+      float x[8], y[8];
+      widen8(w.x, bf16, x);
+      widen8(w.y, bf16, y);
+      if (w.rotated) {
+        const float* cs = a.cos + static_cast<int64_t>(pos) * half + w.lo;
+        const float* sn = a.sin + static_cast<int64_t>(pos) * half + w.lo;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float c = cs[i], s = sn[i], xi = x[i], yi = y[i];
-        x[i] = xi * c - yi * s;
-        y[i] = yi * c + xi * s;
+        for (int i = 0; i < 8; ++i) {
+          const float c = cs[i], s = sn[i], xi = x[i], yi = y[i];
+          x[i] = xi * c - yi * s;
+          y[i] = yi * c + xi * s;
+        }
       }
-    }
-    if (is_q) {
-      uint16_t* o = a.q_out + t * a.qo_token + hh * a.qo_head;
-      *reinterpret_cast<uint4*>(o + lo) = narrow8(x, bf16);
-      *reinterpret_cast<uint4*>(o + hi) = narrow8(y, bf16);
-      continue;
-    }
-    const int64_t at = is_k ? page * a.c.k_page_stride + hh * a.c.k_head_stride + slot * a.c.k_slot_stride
-                            : page * a.c.v_page_stride + hh * a.c.v_head_stride + slot * a.c.v_slot_stride;
-    if constexpr (!kE4m3) {
-      uint16_t* o = static_cast<uint16_t*>(is_k ? a.c.k : a.c.v) + at;
-      *reinterpret_cast<uint4*>(o + lo) = narrow8(x, bf16);
-      *reinterpret_cast<uint4*>(o + hi) = narrow8(y, bf16);
-    } else {
-      // magnitudes compare as their bits, and a NaN's are above infinity's, so that one in the row becomes the scale
-      uint32_t most = 0;
+      const int64_t at = w.is_k ? page * a.c.k_page_stride + w.head * a.c.k_head_stride + slot * a.c.k_slot_stride
+                                : page * a.c.v_page_stride + w.head * a.c.v_head_stride + slot * a.c.v_slot_stride;
+      void* rows = w.is_k ? a.c.k : a.c.v;
+      if (w.is_q || !kE4m3) {
+        uint16_t* o = w.is_q ? q_out : static_cast<uint16_t*>(rows) + at;
+        *reinterpret_cast<uint4*>(o + w.lo) = narrow8(x, bf16);
+        *reinterpret_cast<uint4*>(o + w.hi) = narrow8(y, bf16);
+      } else {
+        // magnitudes compare as their bits, and a NaN's are above infinity's, so that one in the row becomes the scale
+        uint32_t most = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        most = max(most, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-        most = max(most, __float_as_uint(y[i]) & 0x7FFFFFFFu);
-      }
-      for (int d = 1; d < lanes; d *= 2) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), d)));
-      float scale = __uint_as_float(most) * (1.0f / kE4m3Max);
-      if (scale < kSmallestScale) scale = kSmallestScale;
-      uint8_t* o = static_cast<uint8_t*>(is_k ? a.c.k : a.c.v) + at;
-      *reinterpret_cast<uint2*>(o + lo) = e4m3x8(x, scale);
-      *reinterpret_cast<uint2*>(o + hi) = e4m3x8(y, scale);
-      if (part == 0) {
-        if (is_k) a.c.k_scale[page * a.c.k_scale_page_stride + hh * a.c.k_scale_head_stride + slot * a.c.k_scale_slot_stride] = scale;
-        else a.c.v_scale[page * a.c.v_scale_page_stride + hh * a.c.v_scale_head_stride + slot * a.c.v_scale_slot_stride] = scale;
+        for (int i = 0; i < 8; ++i) {
+          most = max(most, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+          most = max(most, __float_as_uint(y[i]) & 0x7FFFFFFFu);
+        }
+        for (int d = 1; d < lanes; d *= 2) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), d)));
+        float scale = __uint_as_float(most) * (1.0f / kE4m3Max);
+        if (scale < kSmallestScale) scale = kSmallestScale;
+        uint8_t* o = static_cast<uint8_t*>(rows) + at;
+        *reinterpret_cast<uint2*>(o + w.lo) = e4m3x8(x, scale);
+        *reinterpret_cast<uint2*>(o + w.hi) = e4m3x8(y, scale);
+        if (w.part == 0) {
+          if (w.is_k)
+            a.c.k_scale[page * a.c.k_scale_page_stride + w.head * a.c.k_scale_head_stride +
+                        slot * a.c.k_scale_slot_stride] = scale;
+          else
+            a.c.v_scale[page * a.c.v_scale_page_stride + w.head * a.c.v_scale_head_stride +
+                        slot * a.c.v_scale_slot_stride] = scale;
+        }
       }
     }
+    u += blockDim.x;
+    if (u >= units) break;
+    w = load(u);
   }
 }
 
@@ -172,7 +200,8 @@ extern "C" int tris_rotary_append_paged(const void* q, int64_t q_token_stride, i
   AppendArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
                static_cast<uint16_t*>(q_out), cos, sin, query_start, q_token_stride, q_head_stride, k_token_stride,
                k_head_stride, v_token_stride, v_head_stride, q_out_token_stride, q_out_head_stride,
-               act_type == TRIS_DTYPE_BF16, tokens, q_heads, rotary_dim, zero_unplaced, *cache};
+               act_type == TRIS_DTYPE_BF16, tokens, q_heads, rotary_dim, zero_unplaced,
+               PageDivision(cache->page_size), *cache};
   const dim3 block(static_cast<unsigned>(units >= 512 ? 512 : (units + kWave - 1) / kWave * kWave));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (cache->dtype == TRIS_DTYPE_E4M3) {

@@ -12,6 +12,21 @@ constexpr float kSmallestScale = 1.17549435e-38f;  // 2^-126
 // few tiles past the end are still int32).
 __host__ __device__ inline int32_t cache_positions(const tris_paged_cache& c) { return c.max_pages * c.page_size; }
 
+// Division of positions (below 2^31) by the page size d: x / d = x * m >> (31 + e), 2^e >= d, m = 2^(31 + e) / d + 1,
+// exact since m d - 2^(31 + e) <= 2^e.
+struct PageDivision {
+  uint32_t magic, shift;
+  explicit PageDivision(int32_t d) {
+    uint32_t e = 0;
+    while ((1u << e) < static_cast<uint32_t>(d)) ++e;
+    magic = static_cast<uint32_t>((1ull << (31 + e)) / static_cast<uint32_t>(d) + 1);
+    shift = 31 + e;
+  }
+  __device__ int operator()(int x) const {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(x)) * magic) >> shift);
+  }
+};
+
 // The cache's own contract; `who` names the entry point in the message.
 inline int check_paged_cache(const char* who, const tris_paged_cache* c, int32_t act_type) {
   TRIS_REQUIRE(c != nullptr, "%s: null cache", who);

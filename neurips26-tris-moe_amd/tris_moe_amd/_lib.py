@@ -149,7 +149,7 @@ _I64 = ctypes.c_int64
 _PAY = ctypes.POINTER(TrisPayload)
 _P4 = ctypes.POINTER(TrisPacked4)
 _PNS = ctypes.POINTER(TrisNsPayload)
-_PPC = ctypes.POINTER(TrisPagedCache)
+_PPC = _P  # a TrisPagedCache by reference, or its bytes
 SIGNATURES = {
     "tris_abi_version": (ctypes.c_int, []),
     "tris_last_error": (ctypes.c_char_p, []),
