@@ -15,10 +15,11 @@
 //                                 product m of eight takes the m-th dimension of every lane's run.
 // No operand goes through LDS, the statistics of a head stay in its lanes, and rescaling is a product in a lane.
 //
-// The work is split over the length: every wavefront of the grid derives the same plan from seq_lens (the total of
-// tiles, a chunk per workgroup, the workgroups of each sequence), so the launch needs no lengths on the host and a long
-// sequence beside short ones gets its share of the GPU.  A sequence in one piece is written at once, the pieces of a
-// longer one leave fp32 sums in the workspace, and a second launch joins them.
+// The work is split over the length: the tiles of all sequences and head groups form one line, and each workgroup takes
+// an equal stretch of it, so that a long sequence beside short ones is shared by the whole GPU and all workgroups end
+// together.  Every wavefront derives the same line from seq_lens, so the launch needs no lengths on the host.  A
+// (sequence, head group) that one workgroup has whole is written at once; the pieces of one that several share leave
+// fp32 sums in the workspace, and a second launch joins them.
 #include <algorithm>
 
 #include "tris_paged.h"
@@ -28,7 +29,11 @@ namespace tris {
 constexpr int kTileKeys = 32;
 constexpr int kWaves = 4;          // wavefronts of a workgroup, taking its tiles in turn
 constexpr int kHeadTile = 16;      // query heads of a workgroup
-constexpr int kTargetWorkgroups = 1024;
+constexpr int kCus = 256;
+// wavefronts a SIMD, and so workgroups a CU, that a head dimension's registers leave room for; a grid of as many runs in
+// one go
+__host__ __device__ constexpr int resident(int head_dim) { return head_dim == 64 ? 4 : head_dim == 128 ? 3 : 2; }
+constexpr int kLoadOnce = 2;       // cache policy of loads that are not read again: non-temporal
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -41,68 +46,62 @@ struct AttentionArgs {
   uint16_t* out;
   int64_t q_seq, q_head, out_seq, out_head;
   float scale_log2;                  // scale * log2(e): the softmax runs on powers of two
-  int32_t window, q_heads, group, head_tiles, tile_heads, max_slots;
+  int32_t window, q_heads, group, head_tiles, tile_heads, workgroups;
   PageDivision page_of;
-  int2* plan;                        // [batch]: first slot and number of the sequence's pieces
-  float2* part_ml;                   // [slots][kv_heads * head_tiles][tile_heads]: maximum and sum
+  int2* owners;                      // [batch][kv_heads * head_tiles]: the first and the last workgroup with a piece of it
+  float2* part_ml;                   // [2 * workgroups][tile_heads]: maximum and sum of a piece
   float* part_o;                     // the same rows of head_dim sums
   tris_paged_cache c;
 };
 
+// a value that every lane holds alike, moved to a scalar register
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// A load from global memory (not a generic one, which would count as an LDS access too).
+template <typename T>
+__device__ __forceinline__ T load_global(const char* base, uint32_t offset) {
+  typedef const __attribute__((address_space(1))) char* Base;
+  typedef const __attribute__((address_space(1))) T* Typed;
+  return *(Typed)((Base)base + offset);
+}
 
 // the positions [first, n) that sequence b's token attends to
 __device__ __forceinline__ void sequence_range(const AttentionArgs& a, int b, int* n, int* first) {
   *n = b < a.c.batch ? min(max(a.c.seq_lens[b], 0), cache_positions(a.c)) : 0;
   *first = a.window > 0 ? max(0, *n - a.window) : 0;
 }
+
+// A sequence's tiles, an idle one's too: one, without keys, so that some workgroup writes its zeros.
 __device__ __forceinline__ int range_tiles(int n, int first) {
-  return n > first ? (n + kTileKeys - 1) / kTileKeys - first / kTileKeys : 0;
+  return n > first ? (n + kTileKeys - 1) / kTileKeys - first / kTileKeys : 1;
 }
 
-struct Piece {
-  int b, n, first, t0, t1, splits, slot;  // slot: of this piece; only sequences in several pieces have slots
+// The line: sequence by sequence, in each its head groups one after the other, in each its tiles and then kPieceCost
+// places for what a piece costs whatever its length (its query, the first rows' way from memory, the sums' way out), so
+// that a stretch of short sequences is a short one.  Of `total` places workgroup w of `shares` has
+// [start(w), start(w + 1)), equal to within one.
+constexpr int kPieceCost = 4;
+
+typedef const __attribute__((address_space(4))) AttentionArgs* KernelArgs;
+
+struct Line {
+  int shares, each, more;
+  __device__ Line(int total, int workgroups) {
+    shares = min(workgroups, (total + kWaves - 1) / kWaves);  // no fewer than one tile for a wavefront
+    each = total / shares;
+    more = total - each * shares;
+  }
+  __device__ int start(int w) const { return w * each + min(w, more); }
+  __device__ int owner(int x) const {
+    return x < more * (each + 1) ? x / (each + 1) : more + (x - more * (each + 1)) / each;
+  }
 };
 
-// Piece `item` of the plan (the same for every caller): with T tiles in all, a workgroup gets
-// chunk = max(4, T * head groups / kTargetWorkgroups) tiles rounded up to one for each wavefront, and sequence b is cut
-// into ceil(tiles / chunk) pieces, an idle one into one of no tiles.  At most kTargetWorkgroups / head groups + batch
-// pieces come of it.
-__device__ __forceinline__ bool find_piece(const AttentionArgs& a, int item, int head_groups, Piece* p) {
-  const int lane = threadIdx.x % kWave;
+// The places of 64 sequences from b0, one a lane.
+__device__ __forceinline__ int places_of(const AttentionArgs& a, int b0, int head_groups) {
+  const int b = b0 + static_cast<int>(threadIdx.x) % kWave;
   int n, first;
-  float total = 0.0f;
-  for (int b0 = 0; b0 < a.c.batch; b0 += kWave) {
-    sequence_range(a, b0 + lane, &n, &first);
-    total += wave_sum_f32(static_cast<float>(range_tiles(n, first)));
-  }
-  const float share = fminf(total * static_cast<float>(head_groups) / static_cast<float>(kTargetWorkgroups), 1e9f);
-  const int chunk = max(1, (static_cast<int>(ceilf(share)) + kWaves - 1) / kWaves) * kWaves;
-  int pieces = 0, slots = 0;
-  for (int b0 = 0; b0 < a.c.batch; b0 += kWave) {
-    const int b = b0 + lane;
-    sequence_range(a, b, &n, &first);
-    const int tiles = range_tiles(n, first);
-    const int s = b < a.c.batch ? max(1, (tiles + chunk - 1) / chunk) : 0;
-    const int end = pieces + wave_incl_sum_i32(s);
-    const int slot_end = slots + wave_incl_sum_i32(s > 1 ? s : 0);
-    const uint64_t hit = __ballot(item >= end - s && item < end);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      const int at = item - __builtin_amdgcn_readlane(end - s, l);
-      p->b = b0 + l;
-      p->n = __builtin_amdgcn_readlane(n, l);
-      p->first = __builtin_amdgcn_readlane(first, l);
-      p->splits = __builtin_amdgcn_readlane(s, l);
-      p->slot = __builtin_amdgcn_readlane(slot_end, l) - p->splits + at;
-      p->t0 = p->first / kTileKeys + at * chunk;
-      p->t1 = min(p->first / kTileKeys + __builtin_amdgcn_readlane(tiles, l), p->t0 + chunk);
-      return true;
-    }
-    pieces = __builtin_amdgcn_readlane(end, kWave - 1);
-    slots = __builtin_amdgcn_readlane(slot_end, kWave - 1);
-  }
-  return false;
+  sequence_range(a, b, &n, &first);
+  return b < a.c.batch ? (range_tiles(n, first) + kPieceCost) * head_groups : 0;
 }
 
 template <bool kBf16>
@@ -135,7 +134,7 @@ __device__ __forceinline__ float across_groups(float v, Op op) {
 // four at a time), so that page numbers and row addresses are the same for the whole wavefront; else each lane looks
 // up the pages of its own keys.
 template <int kDim, bool kBf16, bool kE4m3, bool kWhole>
-__global__ __launch_bounds__(kWaves * kWave, kDim == 256 ? 1 : 2) void attention_decode_kernel(const AttentionArgs a) {
+__global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_decode_kernel(const AttentionArgs args) {
   constexpr bool kBf16V = kBf16 || kE4m3;           // type of the value product (see the probabilities below)
   constexpr int kRun = kDim < 128 ? kDim / 16 : 8;  // dimensions of one of a lane's runs of a value row
   constexpr int kRuns = kDim / 16 / kRun;
@@ -145,14 +144,66 @@ __global__ __launch_bounds__(kWaves * kWave, kDim == 256 ? 1 : 2) void attention
   constexpr int kPad = kDim + 4;
   extern __shared__ float lds[];                    // [kWaves][tile_heads][kPad] sums, then [kWaves][16] factors and sums
 
-  const int head_groups = a.c.kv_heads * a.head_tiles;
-  const int hg = static_cast<int>(blockIdx.x) % head_groups;
-  Piece p;
-  if (!find_piece(a, static_cast<int>(blockIdx.x) / head_groups, head_groups, &p)) return;
-  const int b = uniform(p.b), n = uniform(p.n), first = uniform(p.first);
+  const int head_groups = args.c.kv_heads * args.head_tiles, w = blockIdx.x;
+  // the line's length, the workgroup's stretch, and the sequence where it begins
+  const int places0 = places_of(args, 0, head_groups), end0 = wave_incl_sum_i32(places0);
+  int total = __builtin_amdgcn_readlane(end0, kWave - 1);
+  for (int b0 = kWave; b0 < args.c.batch; b0 += kWave)
+    total += __builtin_amdgcn_readlane(wave_incl_sum_i32(places_of(args, b0, head_groups)), kWave - 1);
+  const Line line(total, args.workgroups);
+  if (w >= line.shares) return;
+  int at = line.start(w), begin, b;
+  const int stop = line.start(w + 1);
+  for (int b0 = 0, places = places0, end = end0;;) {
+    const uint64_t past = __ballot(at < end);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      begin = __builtin_amdgcn_readlane(end - places, l);
+      b = b0 + l;
+      break;
+    }
+    const int before = __builtin_amdgcn_readlane(end, kWave - 1);
+    b0 += kWave;
+    if (b0 >= args.c.batch) return;
+    places = places_of(args, b0, head_groups);
+    end = before + wave_incl_sum_i32(places);
+  }
+  // one piece of a (sequence, head group) after the other
+  while (at < stop && b < args.c.batch) {
+  // What a piece needs of the arguments and of the lane's number is taken anew for each: kept in registers from piece to
+  // piece, it would cost the tiles' loop a third of its wavefronts.
+  int thread = threadIdx.x;
+  KernelArgs fresh = (KernelArgs)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+v"(thread), "+s"(fresh));
+  const AttentionArgs& a = *(const AttentionArgs*)fresh;
+  int n, first;
+  sequence_range(a, b, &n, &first);
+  n = uniform(n);
+  first = uniform(first);
+  const int tiles = range_tiles(n, first), span = tiles + kPieceCost;
+  const int hg = (at - begin) / span, from = at - begin - hg * span;
+  if (hg == head_groups) {
+    begin = at;
+    ++b;
+    continue;
+  }
+  if (from >= tiles) {
+    at += span - from;
+    continue;
+  }
+  const int t1 = first / kTileKeys + min(tiles, from + stop - at), t_end = n > 0 ? t1 : 0;
   const int kvh = hg / a.head_tiles, head0 = (hg % a.head_tiles) * kHeadTile;
   const int heads = min(kHeadTile, a.group - head0);
-  const int wave = uniform(threadIdx.x / kWave), lane = threadIdx.x % kWave, col = lane % 16, g = lane / 16;
+  const int wave = uniform(thread / kWave), lane = thread % kWave, col = lane % 16, g = lane / 16;
+
+  // in bytes
+  const int64_t k_page = a.c.k_page_stride * kSize, v_page = a.c.v_page_stride * kSize;
+  const int64_t ks_page = a.c.k_scale_page_stride * 4, vs_page = a.c.v_scale_page_stride * 4;
+  const int k_slot = static_cast<int>(a.c.k_slot_stride) * kSize, v_slot = static_cast<int>(a.c.v_slot_stride) * kSize;
+  const int ks_slot = static_cast<int>(a.c.k_scale_slot_stride) * 4, vs_slot = static_cast<int>(a.c.v_scale_slot_stride) * 4;
+
+  if (from == 0 && thread == 0)
+    a.owners[b * head_groups + hg] = make_int2(w, line.owner(at + tiles - 1));
 
   // the query operand: head col, the dimensions that the K operand's lane has
   u32x4 q[kDim / 32];
@@ -166,96 +217,124 @@ __global__ __launch_bounds__(kWaves * kWave, kDim == 256 ? 1 : 2) void attention
 
   const char* kbase = static_cast<const char*>(a.c.k) + kvh * a.c.k_head_stride * kSize;
   const char* vbase = static_cast<const char*>(a.c.v) + kvh * a.c.v_head_stride * kSize;
-  const float* ksbase = kE4m3 ? a.c.k_scale + kvh * a.c.k_scale_head_stride : nullptr;
-  const float* vsbase = kE4m3 ? a.c.v_scale + kvh * a.c.v_scale_head_stride : nullptr;
+  const char* ksbase = reinterpret_cast<const char*>(a.c.k_scale) + kvh * a.c.k_scale_head_stride * 4;
+  const char* vsbase = reinterpret_cast<const char*>(a.c.v_scale) + kvh * a.c.v_scale_head_stride * 4;
   const int32_t* table = a.c.block_table + b * a.c.table_stride;
-  const int k_slot = static_cast<int>(a.c.k_slot_stride) * kSize, v_slot = static_cast<int>(a.c.v_slot_stride) * kSize;
-  const int ks_slot = static_cast<int>(a.c.k_scale_slot_stride), vs_slot = static_cast<int>(a.c.v_scale_slot_stride);
+  // wavefronts take the workgroup's tiles in turn, also over the pieces
+  int tile = first / kTileKeys + from + ((wave - at) & (kWaves - 1));
 
-  // the pages of a tile's keys, -1 where there is none: of its two halves, or of the lane's two key rows and eight
-  // value rows
-  constexpr int kPages = kWhole ? 2 : 10;
-  struct Pages { int id[kPages]; };
-  const auto key_of = [&](int tile, int i) {
-    if constexpr (kWhole) return tile * kTileKeys + i * 16;
-    else if (i < 2) return tile * kTileKeys + i * 16 + col;
-    else return tile * kTileKeys + ((i - 2) / 4) * 16 + g * 4 + (i - 2) % 4;
+  // Page numbers run ahead of the rows, so that no row waits for its page: whole, lane 2 i + t holds the block table's
+  // entry of half t of the wavefront's i-th tile from `ids0`, 32 tiles a load and the next 32 behind them; else lane
+  // 32 i + k that of key k of the next tile.  Entries past the table's end read its last one; all are checked where
+  // they are used.
+  const auto entry = [&](int key) { return table[min(a.page_of(key), a.c.max_pages - 1)]; };
+  const auto fetch_ids = [&](int from) {
+    if constexpr (kWhole) return entry((from + lane / 2 * kWaves) * kTileKeys + lane % 2 * 16);
+    else return entry(from * kTileKeys + lane % kTileKeys);
   };
-  const auto find_pages = [&](int tile) {
+  // the pages of one tile: of its halves, or of the key that the lane looked up; -1 where there is none
+  struct Pages { int id[2]; };
+  const auto checked = [&](int key, int id, int of_tile) {
+    return of_tile < t1 && key < n && static_cast<uint32_t>(id) < static_cast<uint32_t>(a.c.num_pages) ? id : -1;
+  };
+  const auto pages_of = [&](int of_tile, int ids, int i) {
     Pages pg;
+    if constexpr (kWhole) {
 #pragma unroll
-    for (int i = 0; i < kPages; ++i) {
-      const int key = key_of(tile, i);
-      int id = -1;
-      if (tile < p.t1 && key < n && (kWhole || key >= first)) id = table[a.page_of(key)];
-      pg.id[i] = static_cast<uint32_t>(id) < static_cast<uint32_t>(a.c.num_pages) ? id : -1;
-      if constexpr (kWhole) pg.id[i] = uniform(pg.id[i]);
+      for (int t = 0; t < 2; ++t)
+        pg.id[t] = checked(of_tile * kTileKeys + t * 16, __builtin_amdgcn_readlane(ids, 2 * i + t), of_tile);
+    } else {
+      pg.id[0] = checked(of_tile * kTileKeys + lane % kTileKeys, ids, of_tile);
     }
     return pg;
   };
+  // Whole: one half's 16 rows as a buffer that ends with the sequence, empty without a page or past the workgroup's
+  // tiles: rows outside read as zeros, without a memory access and without a branch.
+  const auto half_rows = [&](const char* base, int64_t page_stride, int slot_bytes, int of_tile, const Pages& pg, int t) {
+    const int key = of_tile * kTileKeys + t * 16, page = pg.id[t];
+    const int slot = key - a.page_of(key) * a.c.page_size, rows = page >= 0 ? min(16, n - key) : 0;
+    return make_rsrc(base + max(page, 0) * page_stride + static_cast<int64_t>(slot) * slot_bytes,
+                     static_cast<uint32_t>(rows * slot_bytes));
+  };
+  // Else: the page and slot of the tile's k-th key, page 0 where it has none (the key is masked).
+  const auto one_row = [&](int of_tile, const Pages& pg, int k, int* page) {
+    const int key = of_tile * kTileKeys + k;
+    *page = max(__shfl(pg.id[0], k), 0);
+    return key - a.page_of(key) * a.c.page_size;
+  };
 
-  u32x4 kr[2][kKLoads];
-  uint32_t vr[8][kRuns * kVWords];
-  float ks[8], vs[8];
-  // rows without a page read page 0; their keys are masked
+  u32x4 kr[2][kKLoads] = {};
+  uint32_t vr[8][kRuns * kVWords] = {};
+  float ks[8] = {}, vs[8] = {};
   const auto load_k = [&](int tile, const Pages& pg) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int page = max(pg.id[t], 0), key = key_of(tile, t);
-      const int slot = key - a.page_of(key) * a.c.page_size;
-      const char* row = kbase + page * a.c.k_page_stride * kSize;
-      uint32_t off;
       if constexpr (kWhole) {
-        row += static_cast<int64_t>(slot) * k_slot;
-        off = static_cast<uint32_t>(col * k_slot + g * 16);
+        const __amdgpu_buffer_rsrc_t rows = half_rows(kbase, k_page, k_slot, tile, pg, t);
+#pragma unroll
+        for (int i = 0; i < kKLoads; ++i)
+          kr[t][i] = __builtin_amdgcn_raw_buffer_load_b128(rows, col * k_slot + g * 16, i * 64, kLoadOnce);
+        if constexpr (kE4m3) {
+          const __amdgpu_buffer_rsrc_t scales = half_rows(ksbase, ks_page, 4, tile, pg, t);
+          const u32x4 s = __builtin_amdgcn_raw_buffer_load_b128(scales, g * 16, 0, 0);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) ks[t * 4 + r] = __uint_as_float(s[r]);
+        }
       } else {
-        off = static_cast<uint32_t>(slot * k_slot + g * 16);
-      }
+        int page;
+        const int slot = one_row(tile, pg, t * 16 + col, &page);
+        const char* row = kbase + page * k_page;
 #pragma unroll
-      for (int i = 0; i < kKLoads; ++i) kr[t][i] = *reinterpret_cast<const u32x4*>(row + off + i * 64);
-      if constexpr (kE4m3 && kWhole) {
-        const f32x4 s = *reinterpret_cast<const f32x4*>(ksbase + page * a.c.k_scale_page_stride + slot + g * 4);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) ks[t * 4 + r] = s[r];
+        for (int i = 0; i < kKLoads; ++i)
+          kr[t][i] = load_global<u32x4>(row, static_cast<uint32_t>(slot * k_slot + g * 16 + i * 64));
       }
     }
     if constexpr (kE4m3 && !kWhole) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int key = key_of(tile, 2 + j), slot = key - a.page_of(key) * a.c.page_size;
-        ks[j] = ksbase[max(pg.id[2 + j], 0) * a.c.k_scale_page_stride + slot * ks_slot];
+        int page;
+        const int slot = one_row(tile, pg, j / 4 * 16 + g * 4 + j % 4, &page);
+        ks[j] = load_global<float>(ksbase + page * ks_page, static_cast<uint32_t>(slot * ks_slot));
       }
     }
   };
   const auto load_v = [&](int tile, const Pages& pg) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int i = kWhole ? j / 4 : 2 + j;
-      const int page = max(pg.id[i], 0), key = key_of(tile, i);
-      const int slot = key - a.page_of(key) * a.c.page_size;
-      const char* row = vbase + page * a.c.v_page_stride * kSize;
-      uint32_t off;
-      if constexpr (kWhole) {
-        row += static_cast<int64_t>(slot) * v_slot;
-        off = static_cast<uint32_t>((g * 4 + j % 4) * v_slot + col * kRun * kSize);
-      } else {
-        off = static_cast<uint32_t>(slot * v_slot + col * kRun * kSize);
-        if constexpr (kE4m3) vs[j] = vsbase[page * a.c.v_scale_page_stride + slot * vs_slot];
-      }
+    for (int t = 0; t < 2; ++t) {
+      __amdgpu_buffer_rsrc_t rows, scales;
+      if constexpr (kWhole) rows = half_rows(vbase, v_page, v_slot, tile, pg, t);
 #pragma unroll
-      for (int c = 0; c < kRuns; ++c) {
-        const char* src = row + off + c * 16 * kRun * kSize;
-        uint32_t* dst = vr[j] + c * kVWords;
-        if constexpr (kVWords == 4) *reinterpret_cast<u32x4*>(dst) = *reinterpret_cast<const u32x4*>(src);
-        else if constexpr (kVWords == 2) *reinterpret_cast<u32x2*>(dst) = *reinterpret_cast<const u32x2*>(src);
-        else *dst = *reinterpret_cast<const uint32_t*>(src);
+      for (int r = 0; r < 4; ++r) {
+        const int j = t * 4 + r;
+        int page = 0, slot = 0;
+        if constexpr (!kWhole) slot = one_row(tile, pg, t * 16 + g * 4 + r, &page);
+#pragma unroll
+        for (int c = 0; c < kRuns; ++c) {
+          uint32_t* dst = vr[j] + c * kVWords;
+          const int in_row = col * kRun * kSize + c * 16 * kRun * kSize;
+          if constexpr (kWhole) {
+            const int at_row = (g * 4 + r) * v_slot + in_row;
+            if constexpr (kVWords == 4)
+              *reinterpret_cast<u32x4*>(dst) = __builtin_amdgcn_raw_buffer_load_b128(rows, at_row, 0, kLoadOnce);
+            else if constexpr (kVWords == 2)
+              *reinterpret_cast<u32x2*>(dst) = __builtin_amdgcn_raw_buffer_load_b64(rows, at_row, 0, kLoadOnce);
+            else
+              *dst = __builtin_amdgcn_raw_buffer_load_b32(rows, at_row, 0, kLoadOnce);
+          } else {
+            const char* base = vbase + page * v_page;
+            const uint32_t at_row = static_cast<uint32_t>(slot * v_slot + in_row);
+            if constexpr (kVWords == 4) *reinterpret_cast<u32x4*>(dst) = load_global<u32x4>(base, at_row);
+            else if constexpr (kVWords == 2) *reinterpret_cast<u32x2*>(dst) = load_global<u32x2>(base, at_row);
+            else *dst = load_global<uint32_t>(base, at_row);
+          }
+        }
+        if constexpr (kE4m3 && !kWhole) vs[j] = load_global<float>(vsbase + page * vs_page, static_cast<uint32_t>(slot * vs_slot));
       }
       if constexpr (kE4m3 && kWhole) {
-        if (j % 4 == 0) {
-          const f32x4 s = *reinterpret_cast<const f32x4*>(vsbase + page * a.c.v_scale_page_stride + slot + g * 4);
+        scales = half_rows(vsbase, vs_page, 4, tile, pg, t);
+        const u32x4 s = __builtin_amdgcn_raw_buffer_load_b128(scales, g * 16, 0, 0);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) vs[j + r] = s[r];
-        }
+        for (int r = 0; r < 4; ++r) vs[t * 4 + r] = __uint_as_float(s[r]);
       }
     }
   };
@@ -265,15 +344,30 @@ __global__ __launch_bounds__(kWaves * kWave, kDim == 256 ? 1 : 2) void attention
 #pragma unroll
   for (int i = 0; i < kRuns * kRun; ++i) acc[i] = f32x4{0, 0, 0, 0};
 
-  int tile = uniform(p.t0) + wave;
-  const int t1 = uniform(p.t1);
-  Pages cur = find_pages(tile), nxt = find_pages(tile + kWaves);
-  if (tile < t1) {
+  // A tile's keys and values are loaded while the tile before it is computed: the next tile's keys are asked for when
+  // this one's have been used, the values likewise, without a branch (past the last tile from empty buffers): behind
+  // one, the compiler waits for every load in flight before it uses the values.
+  const int tile0 = tile;
+  Pages cur = {}, nxt = {};
+  int ids = 0, ahead = 0;
+  if (tile < t_end) {
+    ids = fetch_ids(tile);
+    ahead = fetch_ids(tile + (kWhole ? kWave / 2 : 1) * kWaves);
+    cur = pages_of(tile, ids, 0);
     load_k(tile, cur);
     load_v(tile, cur);
   }
-  for (; tile < t1; tile += kWaves) {
-    const bool more = tile + kWaves < t1;
+  for (int i = 1; tile < t_end; ++i, tile += kWaves) {
+    if constexpr (kWhole) {
+      if (i % (kWave / 2) == 0) {
+        ids = ahead;
+        ahead = fetch_ids(tile0 + (i + kWave / 2) * kWaves);
+      }
+      nxt = pages_of(tile + kWaves, ids, i % (kWave / 2));
+    } else {
+      nxt = pages_of(tile + kWaves, ahead, 0);
+      ahead = fetch_ids(tile + 2 * kWaves);
+    }
     f32x4 s[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -301,24 +395,18 @@ __global__ __launch_bounds__(kWaves * kWave, kDim == 256 ? 1 : 2) void attention
     // keys outside the sequence, before its window or without a page
     const int key0 = tile * kTileKeys;
     bool edge = key0 < first || key0 + kTileKeys > n;
-    if constexpr (kWhole) {
-      edge = edge || cur.id[0] < 0 || cur.id[1] < 0;
-    } else {
-      bool hole = false;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) hole = hole || cur.id[2 + j] < 0;
-      edge = __any(hole);
-    }
+    if constexpr (kWhole) edge = edge || cur.id[0] < 0 || cur.id[1] < 0;
+    else edge = edge || __any(cur.id[0] < 0);
     bool valid[8];
     if (edge) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int key = key0 + (j / 4) * 16 + g * 4 + j % 4;
-        valid[j] = key >= first && key < n && cur.id[kWhole ? j / 4 : 2 + j] >= 0;
+        const int k = j / 4 * 16 + g * 4 + j % 4;
+        valid[j] = key0 + k >= first && key0 + k < n && (kWhole ? cur.id[j / 4] : __shfl(cur.id[0], k)) >= 0;
         x[j] = valid[j] ? x[j] : -INFINITY;
       }
     }
-    if (more) load_k(tile + kWaves, nxt);
+    load_k(tile + kWaves, nxt);
 
     float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
     if (__any(top > m)) {
@@ -334,25 +422,28 @@ __global__ __launch_bounds__(kWaves * kWave, kDim == 256 ? 1 : 2) void attention
     // cancels): a long tail far below the maximum would lose its bits to the subnormals otherwise.  An 8-bit cache's
     // product runs in bf16, whose range takes any scale; its elements are exact in either type.
     const float base = (m == -INFINITY ? 0.0f : m) - (kBf16V ? 0.0f : 15.0f);
-    float w[8];
+    float pr[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      w[j] = __builtin_amdgcn_exp2f(x[j] - base);
-      l += w[j];
-      if constexpr (kE4m3) w[j] *= vs[j];
+      pr[j] = __builtin_amdgcn_exp2f(x[j] - base);
+      l += pr[j];
+      if constexpr (kE4m3) pr[j] *= vs[j];
     }
     if (edge) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        w[j] = valid[j] ? w[j] : 0.0f;
+        pr[j] = valid[j] ? pr[j] : 0.0f;
+        // (a buffer's end has done this for rows past the sequence)
+        if (!kWhole || key0 < first) {
 #pragma unroll
-        for (int i = 0; i < kRuns * kVWords; ++i) vr[j][i] = valid[j] ? vr[j][i] : 0u;
+          for (int i = 0; i < kRuns * kVWords; ++i) vr[j][i] = valid[j] ? vr[j][i] : 0u;
+        }
       }
     }
     u32x4 hi, lo;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float w0 = w[2 * i], w1 = w[2 * i + 1];
+      const float w0 = pr[2 * i], w1 = pr[2 * i + 1];
       if constexpr (kBf16V) {
         const uint32_t u0 = __float_as_uint(w0), u1 = __float_as_uint(w1);
         hi[i] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
@@ -388,11 +479,13 @@ __global__ __launch_bounds__(kWaves * kWave, kDim == 256 ? 1 : 2) void attention
         }
       }
     }
-    if (more) load_v(tile + kWaves, nxt);
+    load_v(tile + kWaves, nxt);
     cur = nxt;
-    nxt = find_pages(tile + 2 * kWaves);
   }
 
+  asm volatile("" : "+v"(thread));
+  {
+  const int col = thread % 16, g = thread % kWave / 16, wave = uniform(thread / kWave);
   // the wavefronts' sums joined under the workgroup's maximum
   l = across_groups(l, [](float u, float v) { return u + v; });
   float* sh_o = lds;
@@ -418,99 +511,102 @@ __global__ __launch_bounds__(kWaves * kWave, kDim == 256 ? 1 : 2) void attention
     }
   }
   __syncthreads();
-  const int64_t row0 = (static_cast<int64_t>(p.slot) * head_groups + hg) * a.tile_heads;
-  for (int i = threadIdx.x * 2; i < heads * kDim; i += kWaves * kWave * 2) {
+  // a piece that begins a (sequence, head group) and is not all of it ends its workgroup's stretch: the second slot
+  const bool whole_range = from == 0 && t1 - first / kTileKeys == tiles;
+  const int64_t row0 = static_cast<int64_t>(2 * w + (from == 0)) * a.tile_heads;
+  for (int i = thread * 2; i < heads * kDim; i += kWaves * kWave * 2) {
     const int h = i / kDim, d = i % kDim;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, sh_m[w * kHeadTile + h]);
+    for (int u = 0; u < kWaves; ++u) top = fmaxf(top, sh_m[u * kHeadTile + h]);
     const float base = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f, y0 = 0.0f, y1 = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float f = __builtin_amdgcn_exp2f(sh_m[w * kHeadTile + h] - base);
-      const float* o = sh_o + (w * a.tile_heads + h) * kPad + d;
-      sum += sh_l[w * kHeadTile + h] * f;
+    for (int u = 0; u < kWaves; ++u) {
+      const float f = __builtin_amdgcn_exp2f(sh_m[u * kHeadTile + h] - base);
+      const float* o = sh_o + (u * a.tile_heads + h) * kPad + d;
+      sum += sh_l[u * kHeadTile + h] * f;
       y0 += o[0] * f;
       y1 += o[1] * f;
     }
-    if (p.splits == 1) {
+    if (whole_range) {
       const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
       uint16_t* dst = a.out + b * a.out_seq + (kvh * a.group + head0 + h) * a.out_head + d;
       *reinterpret_cast<uint32_t*>(dst) = kBf16 ? pack_bf16_rne(y0 * f, y1 * f) : pack_f16_rne(y0 * f, y1 * f);
-    } else if (p.slot < a.max_slots) {
+    } else {
       *reinterpret_cast<float2*>(a.part_o + (row0 + h) * kDim + d) = make_float2(y0, y1);
       if (d == 0) a.part_ml[row0 + h] = make_float2(top, sum);
     }
   }
-  if (a.plan != nullptr && hg == 0 && threadIdx.x == 0 && p.t0 == p.first / kTileKeys)
-    a.plan[b] = make_int2(p.splits > 1 ? p.slot : 0, p.splits);
+  }
+  at += t1 - first / kTileKeys - from;
+  __syncthreads();  // the next piece's sums go where this one's are read
+  }
 }
 
-// Joins the pieces of one (sequence, query head): the maximum over them, then each wavefront adds every fourth piece.
+// Joins the pieces of one (sequence, query head): kDim / 4 lanes a piece, as many pieces at a time as the workgroup (256
+// or 1024 threads) has room for, each lane with a running maximum of its own, then the lanes' sums.
 template <int kDim, bool kBf16>
-__global__ __launch_bounds__(kWaves * kWave) void attention_join_kernel(const AttentionArgs a) {
-  constexpr int kPer = kDim / kWave;
-  __shared__ float sh_l[kWaves], sh_o[kWaves][kDim];
+__global__ __launch_bounds__(1024) void attention_join_kernel(const AttentionArgs a) {
+  constexpr int kLanes = kDim / 4;
+  __shared__ float2 sh_ml[1024 / kLanes];
+  __shared__ f32x4 sh_o[1024];
   const int b = static_cast<int>(blockIdx.x) / a.q_heads, h = static_cast<int>(blockIdx.x) % a.q_heads;
-  const int2 plan = a.plan[b];
-  if (plan.y <= 1) return;
-  const int kvh = h / a.group, in = h % a.group, head_groups = a.c.kv_heads * a.head_tiles;
-  const int hg = kvh * a.head_tiles + in / kHeadTile;
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const int pieces = min(plan.y, a.max_slots - plan.x);
-  const auto row = [&](int i) {
-    return (static_cast<int64_t>(plan.x + i) * head_groups + hg) * a.tile_heads + in % kHeadTile;
-  };
-  float top = -INFINITY;
-  for (int i = lane; i < pieces; i += kWave) top = fmaxf(top, a.part_ml[row(i)].x);
-  top = wave_max_f32(top);
-  const float base = top == -INFINITY ? 0.0f : top;
-  float l = 0.0f, o[kPer];
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) o[e] = 0.0f;
+  const int hg = h / a.group * a.head_tiles + h % a.group / kHeadTile;
+  const int2 owners = a.owners[b * (a.c.kv_heads * a.head_tiles) + hg];
+  const int w0 = owners.x, w1 = owners.y;
+  if (w0 == w1) return;
+  const int t = threadIdx.x, rows = static_cast<int>(blockDim.x) / kLanes, in = h % a.group % kHeadTile;
+  float m = -INFINITY, l = 0.0f;
+  f32x4 o = {0, 0, 0, 0};
 #pragma unroll 4
-  for (int i = wave; i < pieces; i += kWaves) {
-    const int64_t r = row(i);
+  for (int w = w0 + t / kLanes; w <= w1; w += rows) {
+    const int64_t r = static_cast<int64_t>(2 * w + (w == w0)) * a.tile_heads + in;
     const float2 ml = a.part_ml[r];
-    const float f = __builtin_amdgcn_exp2f(ml.x - base);
-    l += ml.y * f;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) o[e] += a.part_o[r * kDim + lane * kPer + e] * f;
+    const f32x4 part = *reinterpret_cast<const f32x4*>(a.part_o + r * kDim + t % kLanes * 4);
+    const float now = fmaxf(m, ml.x), base = now == -INFINITY ? 0.0f : now;
+    const float keep = __builtin_amdgcn_exp2f(m - base), f = __builtin_amdgcn_exp2f(ml.x - base);
+    l = l * keep + ml.y * f;
+    o = o * keep + part * f;
+    m = now;
   }
-  if (lane == 0) sh_l[wave] = l;
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) sh_o[wave][lane * kPer + e] = o[e];
+  if (t % kLanes == 0) sh_ml[t / kLanes] = make_float2(m, l);
+  sh_o[t] = o;
   __syncthreads();
-  const float sum = ((sh_l[0] + sh_l[1]) + sh_l[2]) + sh_l[3];
-  const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-  for (int d = threadIdx.x; d < kDim; d += kWaves * kWave) {
-    const float y = (((sh_o[0][d] + sh_o[1][d]) + sh_o[2][d]) + sh_o[3][d]) * f;
-    store1(a.out, b * a.out_seq + h * a.out_head + d, y, kBf16 ? TRIS_DTYPE_BF16 : TRIS_DTYPE_F16);
+  if (t >= kLanes) return;
+  const int pieces = min(rows, w1 - w0 + 1);
+  float top = m;
+  for (int i = 1; i < pieces; ++i) top = fmaxf(top, sh_ml[i].x);
+  const float base = top == -INFINITY ? 0.0f : top;
+  const float keep = __builtin_amdgcn_exp2f(m - base);
+  l *= keep;
+  o *= keep;
+  for (int i = 1; i < pieces; ++i) {
+    const float f = __builtin_amdgcn_exp2f(sh_ml[i].x - base);
+    l += sh_ml[i].y * f;
+    o += sh_o[i * kLanes + t] * f;
   }
+  o *= l == 0.0f ? 0.0f : 1.0f / l;
+  const uint2 packed = kBf16 ? make_uint2(pack_bf16_rne(o[0], o[1]), pack_bf16_rne(o[2], o[3]))
+                             : make_uint2(pack_f16_rne(o[0], o[1]), pack_f16_rne(o[2], o[3]));
+  *reinterpret_cast<uint2*>(a.out + b * a.out_seq + h * a.out_head + t * 4) = packed;
 }
 
 // The launch's sizes, from shapes alone.
 struct AttentionShape {
-  int group, head_tiles, tile_heads, head_groups;
-  int64_t pieces, slots;  // bounds of the plan
-  bool splits;            // whether any sequence can be cut
+  int group, head_tiles, tile_heads, workgroups;
+  int64_t places;  // of the line, at most
 };
 
-static AttentionShape attention_shape(int64_t batch, int q_heads, int kv_heads, int64_t positions) {
+static AttentionShape attention_shape(int64_t batch, int q_heads, int kv_heads, int head_dim, int64_t positions) {
   AttentionShape s;
   s.group = q_heads / kv_heads;
   s.head_tiles = (s.group + kHeadTile - 1) / kHeadTile;
-  s.tile_heads = s.group < kHeadTile ? s.group : kHeadTile;
-  s.head_groups = kv_heads * s.head_tiles;
-  // tiles of a sequence (a window may add one by its start inside a tile), pieces of at least kWaves tiles
-  const int64_t tiles = positions / kTileKeys + 2;
-  const int64_t most = (tiles + kWaves - 1) / kWaves;
-  const int64_t shared = kTargetWorkgroups / s.head_groups + 1;
-  s.pieces = std::min(batch * most, shared + batch);
-  // pieces of sequences that are cut: each such sequence has at most twice tiles / chunk
-  s.slots = std::min(batch * most, 2 * shared);
-  s.splits = most > 1;
+  s.tile_heads = std::min(s.group, kHeadTile);
+  const int64_t head_groups = static_cast<int64_t>(kv_heads) * s.head_tiles;
+  const int64_t most = positions / kTileKeys + 2;  // of one sequence: a window may begin and end inside a tile
+  s.places = batch * (most + kPieceCost) * head_groups;
+  s.workgroups = static_cast<int>(std::min<int64_t>(kCus * resident(head_dim), (s.places + kWaves - 1) / kWaves));
   return s;
 }
 
@@ -518,25 +614,26 @@ struct AttentionSpace {
   int64_t ml, o, bytes;
 };
 
-static AttentionSpace attention_space(const AttentionShape& s, int64_t batch, int head_dim) {
+static AttentionSpace attention_space(const AttentionShape& s, int64_t batch, int kv_heads, int head_dim) {
   const auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
   AttentionSpace w;
-  const int64_t rows = s.slots * s.head_groups * s.tile_heads;
-  w.ml = up(batch * static_cast<int64_t>(sizeof(int2)));
+  const int64_t rows = 2LL * s.workgroups * s.tile_heads;
+  w.ml = up(batch * kv_heads * s.head_tiles * static_cast<int64_t>(sizeof(int2)));
   w.o = w.ml + up(rows * static_cast<int64_t>(sizeof(float2)));
-  w.bytes = s.splits ? w.o + rows * head_dim * static_cast<int64_t>(sizeof(float)) : 0;
+  w.bytes = w.o + rows * head_dim * static_cast<int64_t>(sizeof(float));
   return w;
 }
 
 template <int kDim, bool kBf16, bool kE4m3>
 static void attention_launch(const AttentionArgs& a, const AttentionShape& s, bool whole, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(s.pieces * s.head_groups)), block(kWaves * kWave);
+  const dim3 grid(static_cast<unsigned>(s.workgroups)), block(kWaves * kWave);
   const size_t lds = (kWaves * a.tile_heads * (kDim + 4) + 2 * kWaves * kHeadTile) * sizeof(float);
   if (whole) hipLaunchKernelGGL((attention_decode_kernel<kDim, kBf16, kE4m3, true>), grid, block, lds, st, a);
   else hipLaunchKernelGGL((attention_decode_kernel<kDim, kBf16, kE4m3, false>), grid, block, lds, st, a);
-  if (s.splits)
-    hipLaunchKernelGGL((attention_join_kernel<kDim, kBf16>), dim3(static_cast<unsigned>(a.c.batch * a.q_heads)), block,
-                       0, st, a);
+  // few sequences are cut into many pieces each, many into a few
+  const dim3 join(a.workgroups >= 16 * static_cast<int64_t>(a.c.batch) * a.c.kv_heads * a.head_tiles ? 1024 : 256);
+  hipLaunchKernelGGL((attention_join_kernel<kDim, kBf16>), dim3(static_cast<unsigned>(a.c.batch * a.q_heads)), join, 0,
+                     st, a);
 }
 
 template <int kDim>
@@ -557,8 +654,8 @@ using namespace tris;
 extern "C" int64_t tris_paged_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads,
                                                         int32_t head_dim, int32_t max_pages, int32_t page_size) {
   if (batch < 1 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1 || max_pages < 0 || page_size < 1) return 0;
-  return attention_space(attention_shape(batch, q_heads, kv_heads, static_cast<int64_t>(max_pages) * page_size), batch,
-                         head_dim).bytes;
+  return attention_space(attention_shape(batch, q_heads, kv_heads, head_dim, static_cast<int64_t>(max_pages) * page_size), batch,
+                         kv_heads, head_dim).bytes;
 }
 
 extern "C" int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, int64_t q_head_stride, int32_t q_type,
@@ -575,10 +672,10 @@ extern "C" int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, 
     TRIS_REQUIRE(s >= 0 && s % 8 == 0, "%s: rows must be 16-byte aligned", who);
   TRIS_REQUIRE(aligned16(q) && aligned16(out), "%s: rows must be 16-byte aligned", who);
   const int64_t rows = static_cast<int64_t>(cache->batch) * q_heads;
-  const AttentionShape s = attention_shape(cache->batch, q_heads, cache->kv_heads, cache_positions(*cache));
-  TRIS_REQUIRE(rows <= 2147483647LL && s.pieces * s.head_groups <= 2147483647LL, "%s: too many rows", who);
-  const AttentionSpace w = attention_space(s, cache->batch, cache->head_dim);
-  TRIS_REQUIRE(w.bytes == 0 || (workspace && aligned16(workspace) && workspace_bytes >= w.bytes),
+  const AttentionShape s = attention_shape(cache->batch, q_heads, cache->kv_heads, cache->head_dim, cache_positions(*cache));
+  TRIS_REQUIRE(rows <= 2147483647LL && s.places < (1LL << 31) - (1 << 16), "%s: too many positions", who);
+  const AttentionSpace w = attention_space(s, cache->batch, cache->kv_heads, cache->head_dim);
+  TRIS_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= w.bytes,
                "%s: workspace of %lld bytes needed", who, static_cast<long long>(w.bytes));
   AttentionArgs a{static_cast<const uint16_t*>(q),
                   static_cast<uint16_t*>(out),
@@ -592,19 +689,16 @@ extern "C" int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, 
                   s.group,
                   s.head_tiles,
                   s.tile_heads,
-                  0,
+                  s.workgroups,
                   PageDivision(cache->page_size),
                   nullptr,
                   nullptr,
                   nullptr,
                   *cache};
-  if (s.splits) {
-    char* at = static_cast<char*>(workspace);
-    a.max_slots = static_cast<int32_t>(s.slots);
-    a.plan = reinterpret_cast<int2*>(at);
-    a.part_ml = reinterpret_cast<float2*>(at + w.ml);
-    a.part_o = reinterpret_cast<float*>(at + w.o);
-  }
+  char* at = static_cast<char*>(workspace);
+  a.owners = reinterpret_cast<int2*>(at);
+  a.part_ml = reinterpret_cast<float2*>(at + w.ml);
+  a.part_o = reinterpret_cast<float*>(at + w.o);
   bool whole = cache->page_size % 16 == 0;
   if (cache->dtype == TRIS_DTYPE_E4M3) {  // four scales a load
     whole = whole && cache->k_scale_slot_stride == 1 && cache->v_scale_slot_stride == 1 && aligned16(cache->k_scale) &&
