@@ -64,12 +64,13 @@ __device__ __forceinline__ T load_global(const char* base, uint32_t offset) {
   return *(Typed)((Base)base + offset);
 }
 
-// the positions [first, n) that sequence b's token attends to
-__device__ __forceinline__ void sequence_range(const AttentionArgs& a, int b, int* n, int* first) {
-  *n = b < a.c.batch ? min(max(a.c.seq_lens[b], 0), cache_positions(a.c)) : 0;
-  *first = a.window > 0 ? max(0, *n - a.window) : 0;
+// a sequence's token attends to the positions [range_begin, sequence_length)
+__device__ __forceinline__ int sequence_length(const AttentionArgs& a, int b) {
+  return b < a.c.batch ? min(max(a.c.seq_lens[b], 0), cache_positions(a.c)) : 0;
 }
-
+__device__ __forceinline__ int range_begin(const AttentionArgs& a, int n) {
+  return a.window > 0 ? max(0, n - a.window) : 0;
+}
 // A sequence's tiles, an idle one's too: one, without keys, so that some workgroup writes its zeros.
 __device__ __forceinline__ int range_tiles(int n, int first) {
   return n > first ? (n + kTileKeys - 1) / kTileKeys - first / kTileKeys : 1;
@@ -96,12 +97,11 @@ struct Line {
   }
 };
 
-// The places of 64 sequences from b0, one a lane.
-__device__ __forceinline__ int places_of(const AttentionArgs& a, int b0, int head_groups) {
+// The places and lengths of 64 sequences from b0, one a lane.
+__device__ __forceinline__ int places_of(const AttentionArgs& a, int b0, int head_groups, int* n) {
   const int b = b0 + static_cast<int>(threadIdx.x) % kWave;
-  int n, first;
-  sequence_range(a, b, &n, &first);
-  return b < a.c.batch ? (range_tiles(n, first) + kPieceCost) * head_groups : 0;
+  *n = sequence_length(a, b);
+  return b < a.c.batch ? (range_tiles(*n, range_begin(a, *n)) + kPieceCost) * head_groups : 0;
 }
 
 template <bool kBf16>
@@ -142,30 +142,36 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
   constexpr int kKLoads = kDim * kSize / 64;        // 16-byte loads of a lane for one key row's quarter
   constexpr int kVWords = kRun * kSize / 4;         // words of a run
   constexpr int kPad = kDim + 4;
+  constexpr bool kQueryInLds = kDim == 256;
+  __shared__ u32x4 sh_q[kQueryInLds ? kDim / 32 : 1][kQueryInLds ? kWave : 1];
   extern __shared__ float lds[];                    // [kWaves][tile_heads][kPad] sums, then [kWaves][16] factors and sums
 
   const int head_groups = args.c.kv_heads * args.head_tiles, w = blockIdx.x;
   // the line's length, the workgroup's stretch, and the sequence where it begins
-  const int places0 = places_of(args, 0, head_groups), end0 = wave_incl_sum_i32(places0);
+  int length0;
+  const int places0 = places_of(args, 0, head_groups, &length0), end0 = wave_incl_sum_i32(places0);
   int total = __builtin_amdgcn_readlane(end0, kWave - 1);
-  for (int b0 = kWave; b0 < args.c.batch; b0 += kWave)
-    total += __builtin_amdgcn_readlane(wave_incl_sum_i32(places_of(args, b0, head_groups)), kWave - 1);
+  for (int b0 = kWave; b0 < args.c.batch; b0 += kWave) {
+    int length;
+    total += __builtin_amdgcn_readlane(wave_incl_sum_i32(places_of(args, b0, head_groups, &length)), kWave - 1);
+  }
   const Line line(total, args.workgroups);
   if (w >= line.shares) return;
-  int at = line.start(w), begin, b;
+  int at = line.start(w), begin, b, n;
   const int stop = line.start(w + 1);
-  for (int b0 = 0, places = places0, end = end0;;) {
+  for (int b0 = 0, places = places0, end = end0, length = length0;;) {
     const uint64_t past = __ballot(at < end);
     if (past) {
       const int l = __builtin_ctzll(past);
       begin = __builtin_amdgcn_readlane(end - places, l);
       b = b0 + l;
+      n = __builtin_amdgcn_readlane(length, l);
       break;
     }
     const int before = __builtin_amdgcn_readlane(end, kWave - 1);
     b0 += kWave;
     if (b0 >= args.c.batch) return;
-    places = places_of(args, b0, head_groups);
+    places = places_of(args, b0, head_groups, &length);
     end = before + wave_incl_sum_i32(places);
   }
   // one piece of a (sequence, head group) after the other
@@ -176,15 +182,12 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
   KernelArgs fresh = (KernelArgs)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+v"(thread), "+s"(fresh));
   const AttentionArgs& a = *(const AttentionArgs*)fresh;
-  int n, first;
-  sequence_range(a, b, &n, &first);
-  n = uniform(n);
-  first = uniform(first);
+  const int first = range_begin(a, n);
   const int tiles = range_tiles(n, first), span = tiles + kPieceCost;
   const int hg = (at - begin) / span, from = at - begin - hg * span;
   if (hg == head_groups) {
     begin = at;
-    ++b;
+    n = uniform(sequence_length(a, ++b));
     continue;
   }
   if (from >= tiles) {
@@ -205,14 +208,20 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
   if (from == 0 && thread == 0)
     a.owners[b * head_groups + hg] = make_int2(w, line.owner(at + tiles - 1));
 
-  // the query operand: head col, the dimensions that the K operand's lane has
-  u32x4 q[kDim / 32];
-#pragma unroll
-  for (int i = 0; i < kDim / 32; ++i) {
+  // The query operand: head col, the dimensions that the K operand's lane has.  At 256 dimensions it would push the
+  // tiles' loads out of the registers (it is 32 of them), so there it stays in LDS, read when it is used.
+  u32x4 q[kQueryInLds ? 1 : kDim / 32];
+  const auto query = [&](int i) {
     const int d = kE4m3 ? (i / 2) * 64 + g * 16 + (i % 2) * 8 : i * 32 + g * 8;
-    q[i] = u32x4{0, 0, 0, 0};
-    if (col < heads)
-      q[i] = *reinterpret_cast<const u32x4*>(a.q + b * a.q_seq + (kvh * a.group + head0 + col) * a.q_head + d);
+    return col < heads ? *reinterpret_cast<const u32x4*>(a.q + b * a.q_seq + (kvh * a.group + head0 + col) * a.q_head + d)
+                       : u32x4{0, 0, 0, 0};
+  };
+  if constexpr (kQueryInLds) {
+    for (int i = wave; i < kDim / 32; i += kWaves) sh_q[i][lane] = query(i);
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int i = 0; i < kDim / 32; ++i) q[i] = query(i);
   }
 
   const char* kbase = static_cast<const char*>(a.c.k) + kvh * a.c.k_head_stride * kSize;
@@ -232,8 +241,13 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
     if constexpr (kWhole) return entry((from + lane / 2 * kWaves) * kTileKeys + lane % 2 * 16);
     else return entry(from * kTileKeys + lane % kTileKeys);
   };
-  // the pages of one tile: of its halves, or of the key that the lane looked up; -1 where there is none
-  struct Pages { int id[2]; };
+  // the pages of one tile: of its halves, or of the key that the lane looked up, -1 where there is none; and of that
+  // key, where its rows are and its scales (page 0's where it has none: it is masked)
+  struct Pages {
+    int id[2];
+    int64_t k, v;
+    float ks, vs;
+  };
   const auto checked = [&](int key, int id, int of_tile) {
     return of_tile < t1 && key < n && static_cast<uint32_t>(id) < static_cast<uint32_t>(a.c.num_pages) ? id : -1;
   };
@@ -244,7 +258,15 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
       for (int t = 0; t < 2; ++t)
         pg.id[t] = checked(of_tile * kTileKeys + t * 16, __builtin_amdgcn_readlane(ids, 2 * i + t), of_tile);
     } else {
-      pg.id[0] = checked(of_tile * kTileKeys + lane % kTileKeys, ids, of_tile);
+      const int key = of_tile * kTileKeys + lane % kTileKeys;
+      pg.id[0] = checked(key, ids, of_tile);
+      const int64_t page = max(pg.id[0], 0), slot = key - a.page_of(key) * a.c.page_size;
+      pg.k = page * k_page + slot * k_slot;
+      pg.v = page * v_page + slot * v_slot;
+      if constexpr (kE4m3) {
+        pg.ks = load_global<float>(ksbase + page * ks_page, static_cast<uint32_t>(slot * ks_slot));
+        pg.vs = load_global<float>(vsbase + page * vs_page, static_cast<uint32_t>(slot * vs_slot));
+      }
     }
     return pg;
   };
@@ -256,11 +278,10 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
     return make_rsrc(base + max(page, 0) * page_stride + static_cast<int64_t>(slot) * slot_bytes,
                      static_cast<uint32_t>(rows * slot_bytes));
   };
-  // Else: the page and slot of the tile's k-th key, page 0 where it has none (the key is masked).
-  const auto one_row = [&](int of_tile, const Pages& pg, int k, int* page) {
-    const int key = of_tile * kTileKeys + k;
-    *page = max(__shfl(pg.id[0], k), 0);
-    return key - a.page_of(key) * a.c.page_size;
+  // Else: a row of the tile's k-th key, by the lane that looked it up.
+  const auto of_key = [&](int64_t offset, int k) {
+    const int lo = __shfl(static_cast<int>(offset), k), hi = __shfl(static_cast<int>(offset >> 32), k);
+    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo));
   };
 
   u32x4 kr[2][kKLoads] = {};
@@ -281,20 +302,9 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
           for (int r = 0; r < 4; ++r) ks[t * 4 + r] = __uint_as_float(s[r]);
         }
       } else {
-        int page;
-        const int slot = one_row(tile, pg, t * 16 + col, &page);
-        const char* row = kbase + page * k_page;
+        const char* row = kbase + of_key(pg.k, t * 16 + col);
 #pragma unroll
-        for (int i = 0; i < kKLoads; ++i)
-          kr[t][i] = load_global<u32x4>(row, static_cast<uint32_t>(slot * k_slot + g * 16 + i * 64));
-      }
-    }
-    if constexpr (kE4m3 && !kWhole) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        int page;
-        const int slot = one_row(tile, pg, j / 4 * 16 + g * 4 + j % 4, &page);
-        ks[j] = load_global<float>(ksbase + page * ks_page, static_cast<uint32_t>(slot * ks_slot));
+        for (int i = 0; i < kKLoads; ++i) kr[t][i] = load_global<u32x4>(row, static_cast<uint32_t>(g * 16 + i * 64));
       }
     }
   };
@@ -306,8 +316,8 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int j = t * 4 + r;
-        int page = 0, slot = 0;
-        if constexpr (!kWhole) slot = one_row(tile, pg, t * 16 + g * 4 + r, &page);
+        const char* row = vbase;
+        if constexpr (!kWhole) row += of_key(pg.v, t * 16 + g * 4 + r);
 #pragma unroll
         for (int c = 0; c < kRuns; ++c) {
           uint32_t* dst = vr[j] + c * kVWords;
@@ -321,14 +331,12 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
             else
               *dst = __builtin_amdgcn_raw_buffer_load_b32(rows, at_row, 0, kLoadOnce);
           } else {
-            const char* base = vbase + page * v_page;
-            const uint32_t at_row = static_cast<uint32_t>(slot * v_slot + in_row);
-            if constexpr (kVWords == 4) *reinterpret_cast<u32x4*>(dst) = load_global<u32x4>(base, at_row);
-            else if constexpr (kVWords == 2) *reinterpret_cast<u32x2*>(dst) = load_global<u32x2>(base, at_row);
-            else *dst = load_global<uint32_t>(base, at_row);
+            const uint32_t at_row = static_cast<uint32_t>(in_row);
+            if constexpr (kVWords == 4) *reinterpret_cast<u32x4*>(dst) = load_global<u32x4>(row, at_row);
+            else if constexpr (kVWords == 2) *reinterpret_cast<u32x2*>(dst) = load_global<u32x2>(row, at_row);
+            else *dst = load_global<uint32_t>(row, at_row);
           }
         }
-        if constexpr (kE4m3 && !kWhole) vs[j] = load_global<float>(vsbase + page * vs_page, static_cast<uint32_t>(slot * vs_slot));
       }
       if constexpr (kE4m3 && kWhole) {
         scales = half_rows(vsbase, vs_page, 4, tile, pg, t);
@@ -368,6 +376,8 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
       nxt = pages_of(tile + kWaves, ahead, 0);
       ahead = fetch_ids(tile + 2 * kWaves);
     }
+    int q_lane = lane;
+    if constexpr (kQueryInLds) asm volatile("" : "+v"(q_lane));  // read anew for each tile, not kept
     f32x4 s[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -383,7 +393,15 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
         } else {
           k = kr[t][i];
         }
-        s[t] = mfma<kBf16>(k, q[i], s[t]);
+        s[t] = mfma<kBf16>(k, kQueryInLds ? sh_q[i][q_lane] : q[kQueryInLds ? 0 : i], s[t]);
+      }
+    }
+    if constexpr (kE4m3 && !kWhole) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int k = j / 4 * 16 + g * 4 + j % 4;
+        ks[j] = __shfl(cur.ks, k);
+        vs[j] = __shfl(cur.vs, k);
       }
     }
     float x[8];
