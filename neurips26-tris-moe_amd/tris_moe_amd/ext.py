@@ -1984,8 +1984,8 @@ def swiglu_mul(gate: torch.Tensor, up: torch.Tensor, out: torch.Tensor | None = 
 
 # ------------------------------------------------------------------ attention side of a decoder layer
 # One decode step makes a handful of these calls a layer, each a few microseconds on the GPU, so their host path is kept
-# short (measured on the host of an MI355X node, us a call: rms_norm with a residual 13.7 -> 9.1, rotary_append_paged
-# 18.7 -> 14.2, paged_attention_decode 18.7 -> 14.4): each check is one condition over attribute reads, and a call that
+# short (measured on the host of an MI355X node, us a call: rms_norm with a residual 13.7 -> 8.9, rotary_append_paged
+# 18.7 -> 13.1, paged_attention_decode 18.7 -> 14.1): each check is one condition over attribute reads, and a call that
 # fails one goes through the named checks below for its message.
 _DTYPE_IDS = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32,
               torch.float8_e4m3fn: _lib.DTYPE_E4M3}
@@ -1998,19 +1998,18 @@ RMS_NORM_MAX_WIDTH = 32768
 PAGED_HEAD_DIMS = (64, 128, 256)
 
 
-def _launch(device, fn, *args):
-    """Calls a C entry with its device current: a stream takes launches from its own device only."""
-    if device.index != torch._C._cuda_getDevice():
-        with torch.cuda.device(device):
+def _launch(index, fn, *args):
+    """Calls a C entry with CUDA device `index` current: a stream takes launches from its own device only."""
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
             return fn(*args)
     return fn(*args)
 
 
-def _serving_inputs(who, *tensors):
+def _refuse_gradient(who):
     """These entries have no backward: an input that would need one is refused, not cut from its graph."""
-    for t in tensors:
-        if t is not None and t.requires_grad:
-            raise RuntimeError(f"{who}: no gradient is defined; call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{who}: no gradient is defined; call it under torch.no_grad()")
 
 
 def _check_on(who, name, t, dims, dtypes, device=None):
@@ -2038,10 +2037,10 @@ def _norm_stride(who, name, t, width):
     return flat.stride(0)
 
 
-def _norm_operand(who, name, t, like, dtypes, width):
-    """(dtype id, row stride) of a tensor of like's shape and device."""
-    if not (isinstance(t, torch.Tensor) and t.dtype in dtypes and t.shape == like.shape and t.device == like.device):
-        _check_on(who, name, t, None, dtypes, like.device)
+def _norm_operand(who, name, t, x, index, dtypes, width):
+    """(dtype id, row stride) of a tensor of x's shape and device."""
+    if not (isinstance(t, torch.Tensor) and t.get_device() == index and t.dtype in dtypes and t.shape == x.shape):
+        _check_on(who, name, t, None, dtypes, x.device)
         raise RuntimeError(f"{who}: {name} must have the shape of x")
     return _DTYPE_IDS[t.dtype], width if t.is_contiguous() else _norm_stride(who, name, t, width)
 
@@ -2060,13 +2059,13 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.
     who = "rms_norm"
     if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in _ACT_DTYPES):
         _check_on(who, "x", x, None, _ACT_DTYPES)
-    dev = x.device
+    index = x.get_device()
     if not (isinstance(weight, torch.Tensor) and weight.dtype in _WEIGHT_DTYPES and weight.ndim == 1
-            and weight.device == dev and weight.is_contiguous()):
-        _check_on(who, "weight", weight, 1, _WEIGHT_DTYPES, dev)
+            and weight.get_device() == index and weight.is_contiguous()):
+        _check_on(who, "weight", weight, 1, _WEIGHT_DTYPES, x.device)
         raise RuntimeError(f"{who}: weight must be contiguous")
-    if torch.is_grad_enabled():
-        _serving_inputs(who, x, weight, residual)
+    if x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad):
+        _refuse_gradient(who)
     width = weight.numel()
     if not 1 <= width <= RMS_NORM_MAX_WIDTH:
         raise RuntimeError(f"{who}: width must be 1 to {RMS_NORM_MAX_WIDTH}")
@@ -2076,62 +2075,76 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.
     rows, x_stride = x.numel() // width, width if whole else _norm_stride(who, "x", x, width)
     x_type, out_stride = _DTYPE_IDS[x.dtype], width
     if out is not None:
-        out_type, out_stride = _norm_operand(who, "out", out, x, _ACT_DTYPES, width)
+        out_type, out_stride = _norm_operand(who, "out", out, x, index, _ACT_DTYPES, width)
         if out_dtype is not None and out.dtype != out_dtype:
             raise RuntimeError(f"{who}: out must be {out_dtype}")
     elif out_dtype is None or out_dtype is x.dtype:
-        out_type, out = x_type, torch.empty_like(x) if whole else torch.empty(x.shape, dtype=x.dtype, device=dev)
+        out_type, out = x_type, torch.empty_like(x) if whole else torch.empty(x.shape, dtype=x.dtype, device=x.device)
     else:
         if out_dtype not in _ACT_DTYPES:
             raise RuntimeError(f"{who}: out_dtype must be torch.float16 or torch.bfloat16")
-        out_type, out = _DTYPE_IDS[out_dtype], torch.empty(x.shape, dtype=out_dtype, device=dev)
+        out_type, out = _DTYPE_IDS[out_dtype], torch.empty(x.shape, dtype=out_dtype, device=x.device)
     r_ptr = ro_ptr = None
     r_type = r_stride = ro_stride = 0
     if residual is not None:
-        r_type, r_stride = _norm_operand(who, "residual", residual, x, _ACT_DTYPES, width)
+        r_type, r_stride = _norm_operand(who, "residual", residual, x, index, _ACT_DTYPES, width)
         if residual_out is None:
             residual_out = (torch.empty_like(residual) if residual.is_contiguous()
-                            else torch.empty(x.shape, dtype=residual.dtype, device=dev))
+                            else torch.empty(x.shape, dtype=residual.dtype, device=x.device))
             ro_stride = width
         else:
-            _, ro_stride = _norm_operand(who, "residual_out", residual_out, x, (residual.dtype,), width)
+            _, ro_stride = _norm_operand(who, "residual_out", residual_out, x, index, (residual.dtype,), width)
         r_ptr, ro_ptr = residual.data_ptr(), residual_out.data_ptr()
     elif residual_out is not None:
         raise RuntimeError(f"{who}: residual_out needs a residual")
-    rc = _launch(dev, _lib.load().tris_rms_norm, x.data_ptr(), x_type, x_stride, r_ptr, r_type, r_stride,
+    rc = _launch(index, _lib.load().tris_rms_norm, x.data_ptr(), x_type, x_stride, r_ptr, r_type, r_stride,
                  weight.data_ptr(), _DTYPE_IDS[weight.dtype], weight_offset, eps, rows, width, out.data_ptr(), out_type,
-                 out_stride, ro_ptr, ro_stride, _stream(x))
+                 out_stride, ro_ptr, ro_stride, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, "tris_rms_norm")
     return out if residual is None else (out, residual_out)
 
 
-def _heads(who, name, t, dtype, device, dim):
-    """t [tokens, heads, dim] with 16-byte-aligned contiguous rows, or a copy of it that has them."""
-    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.ndim == 3 and t.device == device
-            and t.shape[2] == dim):
-        _check_on(who, name, t, 3, (dtype,), device)
+def _heads(who, name, t, dtype, index, dim):
+    """t [tokens, heads, dim] with 16-byte-aligned contiguous rows, or a copy of it that has them; and its strides."""
+    if not (isinstance(t, torch.Tensor) and t.get_device() == index and t.dtype is dtype and t.ndim == 3):
+        _check_on(who, name, t, 3, (dtype,), torch.device("cuda", index))
+    if t.size(2) != dim:
         raise RuntimeError(f"{who}: {name} must have the cache's head_dim {dim}")
-    a, b, c = t.stride()
+    strides = t.stride()
+    a, b, c = strides
     if c == 1 and not (t.data_ptr() & 15 or a & 7 or b & 7):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+        return t, strides
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride()
 
 
-def _paged_cache(who, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, device):
+def _heads_out(who, name, t, like, dtype, index):
+    """A given output of like's shape: its strides."""
+    if not (isinstance(t, torch.Tensor) and t.get_device() == index and t.dtype is dtype and t.shape == like.shape
+            and t.stride(2) == 1):
+        _check_on(who, name, t, 3, (dtype,), torch.device("cuda", index))
+        raise RuntimeError(f"{who}: {name} must have the shape of q and contiguous rows")
+    return t.stride()
+
+
+def _paged_cache(who, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, index):
     """The C descriptor of a paged cache (struct tris_paged_cache, its bytes) and (batch, max_pages, page_size,
     kv_heads, head_dim)."""
-    if not (isinstance(k_cache, torch.Tensor) and isinstance(v_cache, torch.Tensor) and k_cache.device == device
-            and v_cache.device == device and k_cache.dtype in _CACHE_DTYPES and v_cache.dtype is k_cache.dtype
-            and k_cache.ndim == 4 and v_cache.shape == k_cache.shape):
-        _check_on(who, "k_cache", k_cache, 4, _CACHE_DTYPES, device)
-        _check_on(who, "v_cache", v_cache, 4, (k_cache.dtype,), device)
+    dtype = getattr(k_cache, "dtype", None)
+    if not (dtype in _CACHE_DTYPES and isinstance(v_cache, torch.Tensor) and k_cache.get_device() == index
+            and v_cache.get_device() == index and v_cache.dtype is dtype and k_cache.ndim == 4
+            and v_cache.shape == k_cache.shape):
+        dev = torch.device("cuda", index)
+        _check_on(who, "k_cache", k_cache, 4, _CACHE_DTYPES, dev)
+        _check_on(who, "v_cache", v_cache, 4, (dtype,), dev)
         raise RuntimeError(f"{who}: v_cache must have the shape of k_cache")
     if not (isinstance(block_table, torch.Tensor) and isinstance(seq_lens, torch.Tensor)
             and block_table.dtype is torch.int32 and seq_lens.dtype is torch.int32 and block_table.ndim == 2
-            and seq_lens.ndim == 1 and block_table.device == device and seq_lens.device == device):
-        _check_on(who, "block_table", block_table, 2, (torch.int32,), device)
-        _check_on(who, "seq_lens", seq_lens, 1, (torch.int32,), device)
+            and seq_lens.ndim == 1 and block_table.get_device() == index and seq_lens.get_device() == index):
+        dev = torch.device("cuda", index)
+        _check_on(who, "block_table", block_table, 2, (torch.int32,), dev)
+        _check_on(who, "seq_lens", seq_lens, 1, (torch.int32,), dev)
     pages, heads, page, dim = k_cache.shape
     k0, k1, k2, k3 = k_cache.stride()
     v0, v1, v2, v3 = v_cache.stride()
@@ -2139,25 +2152,27 @@ def _paged_cache(who, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale,
         raise RuntimeError(f"{who}: each cache row of head_dim values must be contiguous")
     batch, max_pages = block_table.shape
     row, col = block_table.stride()
-    if seq_lens.shape[0] != batch or not seq_lens.is_contiguous():
+    if seq_lens.size(0) != batch or not seq_lens.is_contiguous():
         raise RuntimeError(f"{who}: seq_lens must be contiguous, one length for each row of block_table")
     if col != 1 and max_pages > 1:
         raise RuntimeError(f"{who}: the rows of block_table must be contiguous")
     ks = vs = _NO_STRIDES
     ks_ptr = vs_ptr = 0
-    if k_cache.dtype is torch.float8_e4m3fn:
-        if k_scale is None or v_scale is None:
-            raise RuntimeError(f"{who}: an e4m3 cache needs k_scale and v_scale")
-        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-            _check_on(who, name, t, 3, (torch.float32,), device)
-            if t.shape != k_cache.shape[:3]:
-                raise RuntimeError(f"{who}: {name} must be [pages, kv_heads, page_size]")
+    if dtype is torch.float8_e4m3fn:
+        if not (isinstance(k_scale, torch.Tensor) and isinstance(v_scale, torch.Tensor)
+                and k_scale.get_device() == index and v_scale.get_device() == index and k_scale.dtype is torch.float32
+                and v_scale.dtype is torch.float32 and k_scale.shape == v_scale.shape == (pages, heads, page)):
+            if k_scale is None or v_scale is None:
+                raise RuntimeError(f"{who}: an e4m3 cache needs k_scale and v_scale")
+            for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+                _check_on(who, name, t, 3, (torch.float32,), torch.device("cuda", index))
+            raise RuntimeError(f"{who}: k_scale and v_scale must be [pages, kv_heads, page_size]")
         ks, vs, ks_ptr, vs_ptr = k_scale.stride(), v_scale.stride(), k_scale.data_ptr(), v_scale.data_ptr()
     elif k_scale is not None or v_scale is not None:
         raise RuntimeError(f"{who}: k_scale and v_scale belong to an e4m3 cache")
     return _CACHE_LAYOUT.pack(
         k_cache.data_ptr(), v_cache.data_ptr(), ks_ptr, vs_ptr, block_table.data_ptr(), seq_lens.data_ptr(), k0, k1, k2,
-        v0, v1, v2, *ks, *vs, row, pages, page, heads, dim, batch, max_pages, _DTYPE_IDS[k_cache.dtype]), (
+        v0, v1, v2, *ks, *vs, row, pages, page, heads, dim, batch, max_pages, _DTYPE_IDS[dtype]), (
             batch, max_pages, page, heads, dim)
 
 
@@ -2183,50 +2198,52 @@ def rotary_append_paged(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor
     A row past query_start[-1], or of an idle sequence (length 0), is not stored and its rotated query is zero (left
     as it was in a given q_out).  A page number outside the pool is skipped.  q_out may be q.  No gradient."""
     who = "rotary_append_paged"
-    if not (isinstance(k, torch.Tensor) and k.is_cuda and k.dtype in _ACT_DTYPES and k.ndim == 3):
+    if not (isinstance(k, torch.Tensor) and k.is_cuda and k.dtype in _ACT_DTYPES):
         _check_on(who, "k", k, 3, _ACT_DTYPES)
-    dev, dt = k.device, k.dtype
-    if torch.is_grad_enabled():
-        _serving_inputs(who, q, k, v)
-    cache, (batch, _, _, heads, dim) = _paged_cache(who, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, dev)
-    k, v = _heads(who, "k", k, dt, dev, dim), _heads(who, "v", v, dt, dev, dim)
-    if k.shape[1] != heads or v.shape != k.shape:
+    index, dt = k.get_device(), k.dtype
+    cache, (batch, _, _, heads, dim) = _paged_cache(who, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale,
+                                                    index)
+    (k, ks), (v, vs) = _heads(who, "k", k, dt, index, dim), _heads(who, "v", v, dt, index, dim)
+    tokens = k.size(0)
+    if k.requires_grad or v.requires_grad or (q is not None and q.requires_grad):
+        _refuse_gradient(who)
+    if k.size(1) != heads or v.size(1) != heads or v.size(0) != tokens:
         raise RuntimeError(f"{who}: k and v must be [tokens, kv_heads, head_dim] of the cache's kv_heads")
-    _check_cuda("cos", cos, torch.float32, 2, dev)
-    _check_cuda("sin", sin, torch.float32, 2, dev)
-    positions, half = cos.shape
-    if sin.shape != cos.shape:
+    if not (isinstance(cos, torch.Tensor) and isinstance(sin, torch.Tensor) and cos.get_device() == index
+            and sin.get_device() == index and cos.dtype is torch.float32 and sin.dtype is torch.float32 and cos.ndim == 2
+            and sin.shape == cos.shape and cos.is_contiguous() and sin.is_contiguous()):
+        for name, t in (("cos", cos), ("sin", sin)):
+            _check_cuda(name, t, torch.float32, 2, k.device)
         raise RuntimeError(f"{who}: cos and sin must have one shape")
+    positions, half = cos.shape
     starts = None
     if query_start is not None:
-        _check_cuda("query_start", query_start, torch.int32, 1, dev)
-        if query_start.shape[0] != batch + 1:
+        _check_cuda("query_start", query_start, torch.int32, 1, k.device)
+        if query_start.size(0) != batch + 1:
             raise RuntimeError(f"{who}: query_start must hold batch + 1 entries")
         starts = query_start.data_ptr()
-    tokens, q_heads, zero = k.shape[0], 0, 0
+    q_heads = zero = 0
     q_ptr = qo_ptr = None
     qs = qos = _NO_STRIDES
     if q is not None:
-        inplace = q_out is q
-        q = _heads(who, "q", q, dt, dev, dim)
-        if q.shape[0] != tokens:
+        given = q
+        q, qs = _heads(who, "q", q, dt, index, dim)
+        if q.size(0) != tokens:
             raise RuntimeError(f"{who}: q, k and v must have one number of tokens")
-        q_heads = q.shape[1]
+        q_heads = q.size(1)
         if q_out is None:
-            zero, q_out = 1, torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=dt, device=dev)
-        elif inplace and q is not q_out:
+            zero, q_out = 1, torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=dt, device=q.device)
+            qos = q_out.stride()
+        elif q_out is given and q is not given:
             raise RuntimeError(f"{who}: q_out must have 16-byte-aligned contiguous rows")
         else:
-            _check_on(who, "q_out", q_out, 3, (dt,), dev)
-            if q_out.shape != q.shape or q_out.stride(2) != 1:
-                raise RuntimeError(f"{who}: q_out must have the shape of q and contiguous rows")
-        qs, qos, q_ptr, qo_ptr = q.stride(), q_out.stride(), q.data_ptr(), q_out.data_ptr()
+            qos = _heads_out(who, "q_out", q_out, q, dt, index)
+        q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise RuntimeError(f"{who}: q_out needs q")
-    ks, vs = k.stride(), v.stride()
-    rc = _launch(dev, _lib.load().tris_rotary_append_paged, q_ptr, qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
+    rc = _launch(index, _lib.load().tris_rotary_append_paged, q_ptr, qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
                  v.data_ptr(), vs[0], vs[1], _DTYPE_IDS[dt], tokens, q_heads, cos.data_ptr(), sin.data_ptr(), 2 * half,
-                 positions, starts, cache, qo_ptr, qos[0], qos[1], zero, _stream(k))
+                 positions, starts, cache, qo_ptr, qos[0], qos[1], zero, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, "tris_rotary_append_paged")
     return q_out
@@ -2245,29 +2262,28 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     idle sequence (length 0) gives zeros; slots outside a sequence may hold anything.  The launch depends on no value
     on the device, so a captured call may be replayed with other lengths and tables.  No gradient."""
     who = "paged_attention_decode"
-    if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dtype in _ACT_DTYPES and q.ndim == 3):
+    if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dtype in _ACT_DTYPES):
         _check_on(who, "q", q, 3, _ACT_DTYPES)
-    dev, dt = q.device, q.dtype
-    if torch.is_grad_enabled():
-        _serving_inputs(who, q)
+    index, dt = q.get_device(), q.dtype
     cache, (batch, max_pages, page, heads, dim) = _paged_cache(who, k_cache, v_cache, block_table, seq_lens, k_scale,
-                                                               v_scale, dev)
-    q = _heads(who, "q", q, dt, dev, dim)
-    if q.shape[0] != batch:
+                                                               v_scale, index)
+    q, qs = _heads(who, "q", q, dt, index, dim)
+    if q.requires_grad:
+        _refuse_gradient(who)
+    if q.size(0) != batch:
         raise RuntimeError(f"{who}: q must hold one token for each row of block_table")
     if out is None:
-        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=dt, device=dev)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=dt, device=q.device)
+        outs = out.stride()
     else:
-        _check_on(who, "out", out, 3, (dt,), dev)
-        if out.shape != q.shape or out.stride(2) != 1:
-            raise RuntimeError(f"{who}: out must have the shape of q and contiguous rows")
-    q_heads = q.shape[1]
+        outs = _heads_out(who, "out", out, q, dt, index)
+    q_heads = q.size(1)
     lib = _lib.load()
     need = lib.tris_paged_attention_workspace_bytes(batch, q_heads, heads, dim, max_pages, page)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    qs, os_ = q.stride(), out.stride()
-    rc = _launch(dev, lib.tris_paged_attention_decode, q.data_ptr(), qs[0], qs[1], _DTYPE_IDS[dt], q_heads, cache,
-                 dim ** -0.5 if scale is None else scale, window, out.data_ptr(), os_[0], os_[1], _ptr(ws), need, _stream(q))
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)  # (of another stream's call, another allocation)
+    rc = _launch(index, lib.tris_paged_attention_decode, q.data_ptr(), qs[0], qs[1], _DTYPE_IDS[dt], q_heads, cache,
+                 dim ** -0.5 if scale is None else scale, window, out.data_ptr(), outs[0], outs[1], ws.data_ptr(), need,
+                 torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, "tris_paged_attention_decode")
     return out
