@@ -10,6 +10,7 @@ mirrors the reference's Python interface for the path:
   ``run_grouped_structured_expert_pair_forward``, payload stacking,
   ``QuantLinear`` / ``ExpertSharedMatrix`` (``qlinear_cuda.py``);
 * ``moe``      — the sparse MoE block (``modeling_mixtral.py``);
+* ``attention`` — paged key / value cache, attention over the compact3 projections, a decoder layer's decode step;
 * ``synthetic``/``configs`` — seeded payloads of the BASELINE configurations;
 * ``packing``  — payload bit/half layouts (``utils/pack_utils.py``).
 """
