@@ -1994,6 +1994,7 @@ _WEIGHT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 _CACHE_DTYPES = (torch.float16, torch.bfloat16, torch.float8_e4m3fn)
 _CACHE_LAYOUT = struct.Struct("@6P13q7i")  # struct tris_paged_cache
 _NO_STRIDES = (0, 0, 0)
+_INT32_MAX = 2 ** 31 - 1
 RMS_NORM_MAX_WIDTH = 32768
 PAGED_HEAD_DIMS = (64, 128, 256)
 
@@ -2259,7 +2260,7 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
 
     q [batch, q_heads, head_dim] fp16 or bf16, q_heads a multiple of kv_heads (query head h reads kv head
     h // (q_heads / kv_heads)); the cache, block_table, seq_lens and scales as rotary_append_paged takes them.  An
-    idle sequence (length 0) gives zeros; slots outside a sequence may hold anything.  The launch depends on no value
+    idle sequence (length 0) gives zeros; slots outside a sequence may hold anything.  out may be q.  The launch depends on no value
     on the device, so a captured call may be replayed with other lengths and tables.  No gradient."""
     who = "paged_attention_decode"
     if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dtype in _ACT_DTYPES):
@@ -2277,6 +2278,10 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         outs = out.stride()
     else:
         outs = _heads_out(who, "out", out, q, dt, index)
+    if not 0 <= window <= _INT32_MAX:
+        if window < 0:
+            raise RuntimeError(f"{who}: negative window")
+        window = _INT32_MAX  # no sequence is longer
     q_heads = q.size(1)
     lib = _lib.load()
     need = lib.tris_paged_attention_workspace_bytes(batch, q_heads, heads, dim, max_pages, page)
