@@ -562,52 +562,77 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
   }
 }
 
-// Joins the pieces of one (sequence, query head): kDim / 4 lanes a piece, as many pieces at a time as the workgroup (256
-// or 1024 threads) has room for, each lane with a running maximum of its own, then the lanes' sums.
-template <int kDim, bool kBf16>
-__global__ __launch_bounds__(1024) void attention_join_kernel(const AttentionArgs a) {
-  constexpr int kLanes = kDim / 4;
-  __shared__ float2 sh_ml[1024 / kLanes];
-  __shared__ f32x4 sh_o[1024];
-  const int b = static_cast<int>(blockIdx.x) / a.q_heads, h = static_cast<int>(blockIdx.x) % a.q_heads;
-  const int hg = h / a.group * a.head_tiles + h % a.group / kHeadTile;
+// Pieces of a (sequence, head group) on average, from which a join takes 16 or 4 wavefronts for the same dimensions.
+constexpr int kJoinMany = 64, kJoinSome = 16;
+
+// A lane's share of a join: the running maximum, sum and four dimensions' sums, and another's added to them.
+struct Part {
+  float m, l;
+  f32x4 o;
+  __device__ __forceinline__ void add(float m2, float l2, f32x4 o2) {
+    const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top;
+    const float f = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
+    m = top;
+    l = l * f + l2 * f2;
+    o = o * f + o2 * f2;
+  }
+  // over the wavefront's lanes of the same dimensions
+  __device__ __forceinline__ void across() {
+#pragma unroll
+    for (int d = 8; d < kWave; d *= 2) {
+      const f32x4 o2 = {__shfl_xor(o[0], d), __shfl_xor(o[1], d), __shfl_xor(o[2], d), __shfl_xor(o[3], d)};
+      const float m2 = __shfl_xor(m, d), l2 = __shfl_xor(l, d);
+      // (in the same order on both sides, so that both get the same bits)
+      if (threadIdx.x & d) {
+        Part other{m2, l2, o2};
+        other.add(m, l, o);
+        *this = other;
+      } else {
+        add(m2, l2, o2);
+      }
+    }
+  }
+};
+
+// Joins the pieces of one (sequence, query head), 32 dimensions a wavefront: eight lanes a piece, eight pieces at a time.
+// kTogether: 16 or 4 wavefronts on the same dimensions, or (1) four on dimensions of their own.
+template <int kDim, bool kBf16, int kTogether>
+__global__ __launch_bounds__(kTogether == 16 ? 1024 : 256) void attention_join_kernel(const AttentionArgs a) {
+  constexpr int kParts = kDim / 32;
+  constexpr bool kMany = kTogether > 1;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int unit = static_cast<int>(blockIdx.x) * (kMany ? 1 : 4) + (kMany ? 0 : wave);
+  const int row = unit / kParts, d = unit % kParts * 32 + lane % 8 * 4;
+  const int b = row / a.q_heads, h = row % a.q_heads;
+  if (b >= a.c.batch) return;
+  const int hg = h / a.group * a.head_tiles + h % a.group / kHeadTile, in = h % a.group % kHeadTile;
   const int2 owners = a.owners[b * (a.c.kv_heads * a.head_tiles) + hg];
-  const int w0 = owners.x, w1 = owners.y;
-  if (w0 == w1) return;
-  const int t = threadIdx.x, rows = static_cast<int>(blockDim.x) / kLanes, in = h % a.group % kHeadTile;
-  float m = -INFINITY, l = 0.0f;
-  f32x4 o = {0, 0, 0, 0};
-#pragma unroll 4
-  for (int w = w0 + t / kLanes; w <= w1; w += rows) {
-    const int64_t r = static_cast<int64_t>(2 * w + (w == w0)) * a.tile_heads + in;
+  if (owners.x == owners.y) return;
+  Part p{-INFINITY, 0.0f, f32x4{0, 0, 0, 0}};
+#pragma unroll 2
+  for (int w = owners.x + (kMany ? wave * 8 : 0) + lane / 8; w <= owners.y; w += 8 * kTogether) {
+    const int64_t r = static_cast<int64_t>(2 * w + (w == owners.x)) * a.tile_heads + in;
     const float2 ml = a.part_ml[r];
-    const f32x4 part = *reinterpret_cast<const f32x4*>(a.part_o + r * kDim + t % kLanes * 4);
-    const float now = fmaxf(m, ml.x), base = now == -INFINITY ? 0.0f : now;
-    const float keep = __builtin_amdgcn_exp2f(m - base), f = __builtin_amdgcn_exp2f(ml.x - base);
-    l = l * keep + ml.y * f;
-    o = o * keep + part * f;
-    m = now;
+    p.add(ml.x, ml.y, *reinterpret_cast<const f32x4*>(a.part_o + r * kDim + d));
   }
-  if (t % kLanes == 0) sh_ml[t / kLanes] = make_float2(m, l);
-  sh_o[t] = o;
-  __syncthreads();
-  if (t >= kLanes) return;
-  const int pieces = min(rows, w1 - w0 + 1);
-  float top = m;
-  for (int i = 1; i < pieces; ++i) top = fmaxf(top, sh_ml[i].x);
-  const float base = top == -INFINITY ? 0.0f : top;
-  const float keep = __builtin_amdgcn_exp2f(m - base);
-  l *= keep;
-  o *= keep;
-  for (int i = 1; i < pieces; ++i) {
-    const float f = __builtin_amdgcn_exp2f(sh_ml[i].x - base);
-    l += sh_ml[i].y * f;
-    o += sh_o[i * kLanes + t] * f;
+  p.across();
+  if constexpr (kMany) {
+    __shared__ Part sh[kTogether][8];
+    if (lane < 8) sh[wave][lane] = p;
+    __syncthreads();
+    if (wave != 0) return;
+    p = lane / 8 < kTogether ? sh[lane / 8 % kTogether][lane % 8] : Part{-INFINITY, 0.0f, f32x4{0, 0, 0, 0}};
+    if constexpr (kTogether > 8) {
+      const Part q = sh[lane / 8 + 8][lane % 8];
+      p.add(q.m, q.l, q.o);
+    }
+    p.across();
   }
-  o *= l == 0.0f ? 0.0f : 1.0f / l;
-  const uint2 packed = kBf16 ? make_uint2(pack_bf16_rne(o[0], o[1]), pack_bf16_rne(o[2], o[3]))
-                             : make_uint2(pack_f16_rne(o[0], o[1]), pack_f16_rne(o[2], o[3]));
-  *reinterpret_cast<uint2*>(a.out + b * a.out_seq + h * a.out_head + t * 4) = packed;
+  if (lane >= 8) return;
+  const f32x4 y = p.o * (p.l == 0.0f ? 0.0f : 1.0f / p.l);
+  const uint2 packed = kBf16 ? make_uint2(pack_bf16_rne(y[0], y[1]), pack_bf16_rne(y[2], y[3]))
+                             : make_uint2(pack_f16_rne(y[0], y[1]), pack_f16_rne(y[2], y[3]));
+  *reinterpret_cast<uint2*>(a.out + b * a.out_seq + h * a.out_head + d) = packed;
 }
 
 // The launch's sizes, from shapes alone.
@@ -649,9 +674,12 @@ static void attention_launch(const AttentionArgs& a, const AttentionShape& s, bo
   if (whole) hipLaunchKernelGGL((attention_decode_kernel<kDim, kBf16, kE4m3, true>), grid, block, lds, st, a);
   else hipLaunchKernelGGL((attention_decode_kernel<kDim, kBf16, kE4m3, false>), grid, block, lds, st, a);
   // few sequences are cut into many pieces each, many into a few
-  const dim3 join(a.workgroups >= 16 * static_cast<int64_t>(a.c.batch) * a.c.kv_heads * a.head_tiles ? 1024 : 256);
-  hipLaunchKernelGGL((attention_join_kernel<kDim, kBf16>), dim3(static_cast<unsigned>(a.c.batch * a.q_heads)), join, 0,
-                     st, a);
+  const int64_t units = static_cast<int64_t>(a.c.batch) * a.q_heads * (kDim / 32);
+  const int64_t pieces = a.workgroups / (static_cast<int64_t>(a.c.batch) * a.c.kv_heads * a.head_tiles);
+  const dim3 each(static_cast<unsigned>(units)), fourth(static_cast<unsigned>((units + 3) / 4));
+  if (pieces >= kJoinMany) hipLaunchKernelGGL((attention_join_kernel<kDim, kBf16, 16>), each, dim3(1024), 0, st, a);
+  else if (pieces >= kJoinSome) hipLaunchKernelGGL((attention_join_kernel<kDim, kBf16, 4>), each, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((attention_join_kernel<kDim, kBf16, 1>), fourth, dim3(256), 0, st, a);
 }
 
 template <int kDim>
@@ -691,7 +719,7 @@ extern "C" int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, 
   TRIS_REQUIRE(aligned16(q) && aligned16(out), "%s: rows must be 16-byte aligned", who);
   const int64_t rows = static_cast<int64_t>(cache->batch) * q_heads;
   const AttentionShape s = attention_shape(cache->batch, q_heads, cache->kv_heads, cache->head_dim, cache_positions(*cache));
-  TRIS_REQUIRE(rows <= 2147483647LL && s.places < (1LL << 31) - (1 << 16), "%s: too many positions", who);
+  TRIS_REQUIRE(rows * (cache->head_dim / 32) <= 2147483647LL - 3 && s.places < (1LL << 31) - (1 << 16), "%s: too many positions", who);
   const AttentionSpace w = attention_space(s, cache->batch, cache->kv_heads, cache->head_dim);
   TRIS_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= w.bytes,
                "%s: workspace of %lld bytes needed", who, static_cast<long long>(w.bytes));
