@@ -17,7 +17,13 @@
 //
 // The work is split over the length: the tiles of all sequences and head groups form one line, and each workgroup takes
 // an equal stretch of it, so that a long sequence beside short ones is shared by the whole GPU and all workgroups end
-// together.  Every wavefront derives the same line from seq_lens, so the launch needs no lengths on the host.  A
+// together.  Every wavefront derives the same line from seq_lens, so the launch needs no lengths on the host.
+//
+// Bound by memory: a (key, kv head) is 4 head_dim bytes in 16 bits and 4 flops a byte for each query head of the group.
+// One MI355X reads 6.2 TB/s; 131072 tokens with 4 kv heads of 128 (268 MB) take 46.5 + 4.5 us, 64 sequences of 4000 to
+// 8192 tokens on an e4m3 cache (792 MB) 138 + 4.9, 32 of 300 to 6000 in a window of 4096 with 16 kv heads (473 MB) 79 + 4.6.
+// Below some 50 MB the way to the first rows (length, page, row: three memory latencies) and the second launch bound it:
+// 1000 tokens, 8 kv heads (4 MB) 6.9 + 3.4 us.  A
 // (sequence, head group) that one workgroup has whole is written at once; the pieces of one that several share leave
 // fp32 sums in the workspace, and a second launch joins them.
 #include <algorithm>
@@ -30,10 +36,14 @@ constexpr int kTileKeys = 32;
 constexpr int kWaves = 4;          // wavefronts of a workgroup, taking its tiles in turn
 constexpr int kHeadTile = 16;      // query heads of a workgroup
 constexpr int kCus = 256;
-// wavefronts a SIMD, and so workgroups a CU, that a head dimension's registers leave room for; a grid of as many runs in
-// one go
+// Wavefronts a SIMD, and so workgroups a CU, that a head dimension's registers leave room for; a grid of as many runs in
+// one go (half as many / twice as many: 128k tokens 62 / 58 against 54 us, 32 windowed sequences 100 / 87 against 84).
 __host__ __device__ constexpr int resident(int head_dim) { return head_dim == 64 ? 4 : head_dim == 128 ? 3 : 2; }
-constexpr int kLoadOnce = 2;       // cache policy of loads that are not read again: non-temporal
+// Cache policy of the rows, which are read once: non-temporal.  In a graph over four states, cached against not: 128k
+// tokens 59.6 / 52.4 us, 32 windowed sequences 94.5 / 83.5, 64 on an e4m3 cache 156 / 144, 16 ragged ones 25.9 / 25.7.
+// Where each lane has its row's address, a key row's quarters come by different instructions and may lie across lines:
+// there the keys are cached, the values not (pages of 20, head_dim 256: 31.0 with both cached, 33.8 with neither, 29.1).
+constexpr int kLoadOnce = 2;
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -56,12 +66,14 @@ struct AttentionArgs {
 
 // a value that every lane holds alike, moved to a scalar register
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-// A load from global memory (not a generic one, which would count as an LDS access too).
-template <typename T>
+// A load from global memory (not a generic one, which would count as an LDS access too).  kOnce: of what is not read
+// again.
+template <typename T, bool kOnce>
 __device__ __forceinline__ T load_global(const char* base, uint32_t offset) {
   typedef const __attribute__((address_space(1))) char* Base;
   typedef const __attribute__((address_space(1))) T* Typed;
-  return *(Typed)((Base)base + offset);
+  if constexpr (kOnce) return __builtin_nontemporal_load((Typed)((Base)base + offset));
+  else return *(Typed)((Base)base + offset);
 }
 
 // a sequence's token attends to the positions [range_begin, sequence_length)
@@ -80,6 +92,8 @@ __device__ __forceinline__ int range_tiles(int n, int first) {
 // places for what a piece costs whatever its length (its query, the first rows' way from memory, the sums' way out), so
 // that a stretch of short sequences is a short one.  Of `total` places workgroup w of `shares` has
 // [start(w), start(w + 1)), equal to within one.
+// (0, 2, 4, 8, 12 places: 16 ragged sequences 41.3, 28.2, 26.1, 26.0, 27.4 us, 32 windowed ones 86.5, 84.3, 84.0, 86.0,
+// 88.5; one or 64 long ones do not care.)
 constexpr int kPieceCost = 4;
 
 typedef const __attribute__((address_space(4))) AttentionArgs* KernelArgs;
@@ -132,7 +146,8 @@ __device__ __forceinline__ float across_groups(float v, Op op) {
 
 // kWhole: every 16 keys of a tile lie in one page (page_size a multiple of 16; with e4m3, scale rows that can be read
 // four at a time), so that page numbers and row addresses are the same for the whole wavefront; else each lane looks
-// up the pages of its own keys.
+// up one key and hands its rows' addresses around (of the same calls, whole / by lanes: 52.4 / 57.1, 83.5 / 91.3,
+// 144 / 147 and 25.7 / 26.5 us).
 template <int kDim, bool kBf16, bool kE4m3, bool kWhole>
 __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_decode_kernel(const AttentionArgs args) {
   constexpr bool kBf16V = kBf16 || kE4m3;           // type of the value product (see the probabilities below)
@@ -209,7 +224,8 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
     a.owners[b * head_groups + hg] = make_int2(w, line.owner(at + tiles - 1));
 
   // The query operand: head col, the dimensions that the K operand's lane has.  At 256 dimensions it would push the
-  // tiles' loads out of the registers (it is 32 of them), so there it stays in LDS, read when it is used.
+  // tiles' loads out of the registers (it is 32 of them), so there it stays in LDS, read when it is used (8 ragged
+  // sequences of up to 16000: 31.0 us, 39.4 with it in registers; at 128 dimensions both ways take the same time).
   u32x4 q[kQueryInLds ? 1 : kDim / 32];
   const auto query = [&](int i) {
     const int d = kE4m3 ? (i / 2) * 64 + g * 16 + (i % 2) * 8 : i * 32 + g * 8;
@@ -264,8 +280,8 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
       pg.k = page * k_page + slot * k_slot;
       pg.v = page * v_page + slot * v_slot;
       if constexpr (kE4m3) {
-        pg.ks = load_global<float>(ksbase + page * ks_page, static_cast<uint32_t>(slot * ks_slot));
-        pg.vs = load_global<float>(vsbase + page * vs_page, static_cast<uint32_t>(slot * vs_slot));
+        pg.ks = load_global<float, false>(ksbase + page * ks_page, static_cast<uint32_t>(slot * ks_slot));
+        pg.vs = load_global<float, false>(vsbase + page * vs_page, static_cast<uint32_t>(slot * vs_slot));
       }
     }
     return pg;
@@ -304,7 +320,8 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
       } else {
         const char* row = kbase + of_key(pg.k, t * 16 + col);
 #pragma unroll
-        for (int i = 0; i < kKLoads; ++i) kr[t][i] = load_global<u32x4>(row, static_cast<uint32_t>(g * 16 + i * 64));
+        for (int i = 0; i < kKLoads; ++i)
+          kr[t][i] = load_global<u32x4, false>(row, static_cast<uint32_t>(g * 16 + i * 64));
       }
     }
   };
@@ -332,9 +349,9 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
               *dst = __builtin_amdgcn_raw_buffer_load_b32(rows, at_row, 0, kLoadOnce);
           } else {
             const uint32_t at_row = static_cast<uint32_t>(in_row);
-            if constexpr (kVWords == 4) *reinterpret_cast<u32x4*>(dst) = load_global<u32x4>(row, at_row);
-            else if constexpr (kVWords == 2) *reinterpret_cast<u32x2*>(dst) = load_global<u32x2>(row, at_row);
-            else *dst = load_global<uint32_t>(row, at_row);
+            if constexpr (kVWords == 4) *reinterpret_cast<u32x4*>(dst) = load_global<u32x4, true>(row, at_row);
+            else if constexpr (kVWords == 2) *reinterpret_cast<u32x2*>(dst) = load_global<u32x2, true>(row, at_row);
+            else *dst = load_global<uint32_t, true>(row, at_row);
           }
         }
       }
@@ -436,7 +453,8 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
       for (int i = 0; i < kRuns * kRun; ++i) acc[i] *= f;
     }
     // The probabilities enter the value product as two 16-bit parts, the value and what its rounding left, so that the
-    // result has one rounding to speak of, the output's.  In fp16 they are 2^15 times as large (the sum too, so that it
+    // result has one rounding to speak of, the output's (the second product costs 0 to 1 %: the matrix cores wait for
+    // memory).  In fp16 they are 2^15 times as large (the sum too, so that it
     // cancels): a long tail far below the maximum would lose its bits to the subnormals otherwise.  An 8-bit cache's
     // product runs in bf16, whose range takes any scale; its elements are exact in either type.
     const float base = (m == -INFINITY ? 0.0f : m) - (kBf16V ? 0.0f : 15.0f);
@@ -562,7 +580,9 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
   }
 }
 
-// Pieces of a (sequence, head group) on average, from which a join takes 16 or 4 wavefronts for the same dimensions.
+// Pieces of a (sequence, head group) on average, from which a join takes 16 or 4 wavefronts for the same dimensions
+// (192 pieces, 16 together: 4.5 us, an earlier form with 32 pieces at a time 5.9; 32 pieces, 4 together: the call 31.0
+// us, 16 together 34.5; 12 pieces, 1 / 4 together: 9.05 / 9.4; 1.5 pieces: the call 144 either way, 151 with 4 from 1).
 constexpr int kJoinMany = 64, kJoinSome = 16;
 
 // A lane's share of a join: the running maximum, sum and four dimensions' sums, and another's added to them.

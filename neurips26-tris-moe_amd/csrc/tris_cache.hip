@@ -5,6 +5,10 @@
 // token: all their values are in flight while the token's position, page and table row are looked up, once for all,
 // and so are the cosines and sines, since a lane has the same part of each of its heads.  An 8-bit row's largest
 // magnitude is a maximum over the head's head_dim / 16 neighbouring lanes.
+//
+// Bound by memory where there are many tokens: 8189 of 32 query and 8 kv heads of 128, bf16 (205 MB), 39.9 us in a graph,
+// 5.15 TB/s, a large copy's rate; else by two memory latencies (boundaries and lengths, then page and angles): one token
+// for each of 16 sequences 3.7 us.
 #include "tris_paged.h"
 
 // The rotation's two products and their sum are rounded one by one, as the same torch expression rounds them, so that
@@ -61,6 +65,8 @@ __device__ __forceinline__ uint2 e4m3x8(const float v[8], float scale) {
   return make_uint2(w[0], w[1]);
 }
 
+// 1, 2, 3, 4, 6 units: 8189 tokens 43.0, 40.6, 40.0, 40.6, 44.3 us; one token for each of 16 sequences 3.3, 3.7, 4.3, 4.4,
+// 6.0.
 constexpr int kUnits = 2;
 
 template <bool kE4m3>

@@ -3,7 +3,12 @@
 //   h = x + residual,  residual_out = round(h),  out = round(h * rsqrt(mean(h^2) + eps) * (weight + offset))
 //
 // Everything between the loads and the one rounding of each output is fp32; the sum of squares of a row is a fixed
-// tree, so results do not depend on the launch.
+// tree for its width, so results do not depend on the other rows.
+//
+// Bound by memory: four 16-bit values a column with a residual.  In a graph, bf16: 8192 x 4096 with the residual (268 MB)
+// 42 us, 6.3 TB/s, above a copy's 5.2 since part of it stays in the memory-side cache; 10656 x 128 3.8 us; one row of
+// 4096 2.8 us, a launch's own time.  A width that eight does not divide costs its unaligned rows: 8192 x 4095 66 us (132
+// one value at a time).
 #include "tris_dtype.h"
 
 namespace tris {
@@ -19,71 +24,70 @@ struct RmsNormArgs {
   float weight_offset, eps;
 };
 
+// Eight 16-bit values at column i of a row that is `width` long.  Rows need no alignment: the copies are 16-byte accesses
+// whatever the address, which this GPU's global memory takes.  kTail: the row's last run may be shorter.
+template <bool kTail>
+__device__ __forceinline__ uint4 load_run(const void* p, int64_t at, int i, int width) {
+  const uint16_t* src = static_cast<const uint16_t*>(p) + at + i;
+  uint4 v = {0, 0, 0, 0};
+  if (!kTail || i + 8 <= width) {
+    __builtin_memcpy(&v, src, 16);
+  } else {
+    uint32_t u[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (i + e < width) u[e / 2] |= static_cast<uint32_t>(src[e]) << (e % 2 * 16);
+    v = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  return v;
+}
+template <bool kTail>
+__device__ __forceinline__ void store_run(void* p, int64_t at, int i, int width, const uint4 v) {
+  uint16_t* dst = static_cast<uint16_t*>(p) + at + i;
+  if (!kTail || i + 8 <= width) {
+    __builtin_memcpy(dst, &v, 16);
+  } else {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (i + e < width) dst[e] = static_cast<uint16_t>(u[e / 2] >> (e % 2 * 16));
+  }
+}
+
 // kLanes threads a row, each with kChunks runs of eight columns in registers, so that a row is read once.  Up to 64
 // lanes a row a workgroup has 256 / kLanes rows and a row's sum stays in its wavefront; above, a row has the workgroup.
-// kVector: every row is 16-byte aligned and the width a multiple of eight: 16-byte loads; else one value at a time, a
-// thread's columns kLanes apart.
-template <int kLanes, int kChunks, bool kVector>
+// Measured with the residual: 10656 x 64 and x 128, as many lanes as runs 3.06 / 3.76 us, a wavefront a row 5.25 / 5.44;
+// 4096 columns, a workgroup of 256 for 8192 rows 42.2 us and for one 2.7, a wavefront a row 44.2 and 4.4, 128 threads
+// 43.0 and 3.3; 8192 columns, 512 threads 42.1 / 2.95, 1024 44.5 / 3.05, 256 42.9 / 3.4.
+template <int kLanes, int kChunks, bool kTail>
 __global__ __launch_bounds__(kLanes > 256 ? kLanes : 256) void rms_norm_kernel(const RmsNormArgs a) {
   constexpr int kRows = kLanes <= kWave ? 256 / kLanes : 1;
   const int t = threadIdx.x % kLanes;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kLanes;
-  const bool live = row < a.rows;
-  const bool x_bf16 = a.x_type == TRIS_DTYPE_BF16, r_bf16 = a.residual_type == TRIS_DTYPE_BF16;
-  const auto column = [&](int c, int e) { return kVector ? (c * kLanes + t) * 8 : (c * 8 + e) * kLanes + t; };
-  float h[kChunks][8], w[kChunks][8];
+  const bool live = row < a.rows, r_bf16 = a.residual_type == TRIS_DTYPE_BF16, w_f32 = a.weight_type == TRIS_DTYPE_F32;
   // the row and the weights in flight together
-  uint4 xs[kChunks], rs[kChunks], ws[kChunks], ws2[kChunks];
-  if constexpr (kVector) {
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      const int i = column(c, 0);
-      if (!live || i >= a.width) continue;
-      xs[c] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + row * a.x_stride + i);
-      if (a.residual)
-        rs[c] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.residual) + row * a.residual_stride + i);
-      if (a.weight_type == TRIS_DTYPE_F32) {
-        ws[c] = *reinterpret_cast<const uint4*>(static_cast<const float*>(a.weight) + i);
-        ws2[c] = *reinterpret_cast<const uint4*>(static_cast<const float*>(a.weight) + i + 4);
-      } else {
-        ws[c] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.weight) + i);
-      }
-    }
-  }
-  float sq = 0.0f;
+  uint4 xs[kChunks], rs[kChunks], ws[kChunks];
 #pragma unroll
   for (int c = 0; c < kChunks; ++c) {
-    if constexpr (kVector) {
-      const int i = column(c, 0);
-      if (!live || i >= a.width) continue;
-      widen8(xs[c], x_bf16, h[c]);
-      if (a.residual) {
-        float r[8];
-        widen8(rs[c], r_bf16, r);
+    const int i = (c * kLanes + t) * 8;
+    if (!live || i >= a.width) continue;
+    xs[c] = load_run<kTail>(a.x, row * a.x_stride, i, a.width);
+    if (a.residual) rs[c] = load_run<kTail>(a.residual, row * a.residual_stride, i, a.width);
+    if (!w_f32) ws[c] = load_run<kTail>(a.weight, 0, i, a.width);
+  }
+  float h[kChunks][8], sq = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[c][e] += r[e];
-      }
-      if (a.weight_type == TRIS_DTYPE_F32) {
-        const uint32_t u[8] = {ws[c].x, ws[c].y, ws[c].z, ws[c].w, ws2[c].x, ws2[c].y, ws2[c].z, ws2[c].w};
+  for (int c = 0; c < kChunks; ++c) {
+    if (!live || (c * kLanes + t) * 8 >= a.width) continue;
+    widen8(xs[c], a.x_type == TRIS_DTYPE_BF16, h[c]);
+    if (a.residual) {
+      float r[8];
+      widen8(rs[c], r_bf16, r);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[c][e] = __uint_as_float(u[e]);
-      } else {
-        widen8(ws[c], a.weight_type == TRIS_DTYPE_BF16, w[c]);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sq += h[c][e] * h[c][e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int i = column(c, e);
-        h[c][e] = w[c][e] = 0.0f;
-        if (!live || i >= a.width) continue;
-        h[c][e] = load1(a.x, row * a.x_stride + i, a.x_type);
-        if (a.residual) h[c][e] += load1(a.residual, row * a.residual_stride + i, a.residual_type);
-        w[c][e] = load1(a.weight, i, a.weight_type);
-        sq += h[c][e] * h[c][e];
-      }
+      for (int e = 0; e < 8; ++e) h[c][e] += r[e];
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sq += h[c][e] * h[c][e];
   }
   if constexpr (kLanes < kWave) {
 #pragma unroll
@@ -102,34 +106,28 @@ __global__ __launch_bounds__(kLanes > 256 ? kLanes : 256) void rms_norm_kernel(c
   const float f = rsqrtf(sq / static_cast<float>(a.width) + a.eps);
 #pragma unroll
   for (int c = 0; c < kChunks; ++c) {
-    if constexpr (kVector) {
-      const int i = column(c, 0);
-      if (!live || i >= a.width) continue;
-      if (a.residual)
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.residual_out) + row * a.residual_out_stride + i) =
-            narrow8(h[c], r_bf16);
+    const int i = (c * kLanes + t) * 8;
+    if (!live || i >= a.width) continue;
+    if (a.residual) store_run<kTail>(a.residual_out, row * a.residual_out_stride, i, a.width, narrow8(h[c], r_bf16));
+    float w[8];
+    if (w_f32) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) h[c][e] = h[c][e] * f * (w[c][e] + a.weight_offset);
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.out_stride + i) =
-          narrow8(h[c], a.out_type == TRIS_DTYPE_BF16);
+      for (int e = 0; e < 8; ++e) w[e] = !kTail || i + e < a.width ? static_cast<const float*>(a.weight)[i + e] : 0.0f;
     } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int i = column(c, e);
-        if (!live || i >= a.width) continue;
-        if (a.residual) store1(a.residual_out, row * a.residual_out_stride + i, h[c][e], a.residual_type);
-        store1(a.out, row * a.out_stride + i, h[c][e] * f * (w[c][e] + a.weight_offset), a.out_type);
-      }
+      widen8(ws[c], a.weight_type == TRIS_DTYPE_BF16, w);
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = h[c][e] * f * (w[e] + a.weight_offset);
+    store_run<kTail>(a.out, row * a.out_stride, i, a.width, narrow8(w, a.out_type == TRIS_DTYPE_BF16));
   }
 }
 
 template <int kLanes, int kChunks>
-static void rms_norm_launch(const RmsNormArgs& a, bool vector, hipStream_t st) {
+static void rms_norm_launch(const RmsNormArgs& a, hipStream_t st) {
   constexpr int kRows = kLanes <= kWave ? 256 / kLanes : 1;
   const dim3 grid(static_cast<unsigned>((a.rows + kRows - 1) / kRows)), block(kLanes <= kWave ? 256 : kLanes);
-  if (vector) hipLaunchKernelGGL((rms_norm_kernel<kLanes, kChunks, true>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((rms_norm_kernel<kLanes, kChunks, false>), grid, block, 0, st, a);
+  if (a.width % 8 == 0) hipLaunchKernelGGL((rms_norm_kernel<kLanes, kChunks, false>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((rms_norm_kernel<kLanes, kChunks, true>), grid, block, 0, st, a);
 }
 
 }  // namespace tris
@@ -154,20 +152,16 @@ extern "C" int tris_rms_norm(const void* x, int32_t x_type, int64_t x_stride, co
   TRIS_REQUIRE(rows == 1 || (x_stride >= 0 && residual_stride >= 0), "%s: negative stride", who);
   RmsNormArgs a{x, residual, weight, out, residual_out, x_stride, residual_stride, out_stride, residual_out_stride,
                 rows, x_type, residual_type, weight_type, out_type, width, weight_offset, eps};
-  bool vector = width % 8 == 0 && aligned16(x) && aligned16(weight) && aligned16(out) && aligned16(residual) &&
-                aligned16(residual_out);
-  if (rows > 1)
-    for (const int64_t v : {x_stride, out_stride, residual_stride, residual_out_stride}) vector = vector && v % 8 == 0;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (width <= 64) rms_norm_launch<8, 1>(a, vector, st);
-  else if (width <= 128) rms_norm_launch<16, 1>(a, vector, st);
-  else if (width <= 256) rms_norm_launch<32, 1>(a, vector, st);
-  else if (width <= 512) rms_norm_launch<64, 1>(a, vector, st);
-  else if (width <= 1024) rms_norm_launch<64, 2>(a, vector, st);
-  else if (width <= 2048) rms_norm_launch<256, 1>(a, vector, st);
-  else if (width <= 4096) rms_norm_launch<256, 2>(a, vector, st);
-  else if (width <= 8192) rms_norm_launch<512, 2>(a, vector, st);
-  else if (width <= 16384) rms_norm_launch<1024, 2>(a, vector, st);
-  else rms_norm_launch<1024, 4>(a, vector, st);
+  if (width <= 64) rms_norm_launch<8, 1>(a, st);
+  else if (width <= 128) rms_norm_launch<16, 1>(a, st);
+  else if (width <= 256) rms_norm_launch<32, 1>(a, st);
+  else if (width <= 512) rms_norm_launch<64, 1>(a, st);
+  else if (width <= 1024) rms_norm_launch<64, 2>(a, st);
+  else if (width <= 2048) rms_norm_launch<256, 1>(a, st);
+  else if (width <= 4096) rms_norm_launch<256, 2>(a, st);
+  else if (width <= 8192) rms_norm_launch<512, 2>(a, st);
+  else if (width <= 16384) rms_norm_launch<1024, 2>(a, st);
+  else rms_norm_launch<1024, 4>(a, st);
   return check_launch(who);
 }
