@@ -859,7 +859,7 @@ int tris_route_predecode_all_reduce(const float* router_logits, int32_t num_toke
 /*
  * The attention side of a decoder layer, around the compact3 Q/K/V and output linears (no native counterpart in the
  * reference: its models run the norms, the rotation, the cache and the attention as torch ops,
- * modeling_mixtral.py:610-757).  Serving only, no gradients.
+ * modeling_mixtral.py).  Serving only, no gradients.
  *
  * Element types of activations, weights and caches:
  */

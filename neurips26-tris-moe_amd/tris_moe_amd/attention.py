@@ -1,6 +1,6 @@
 """The attention side of a decoder layer on a paged cache, and the layer's decode step around the sparse MoE block.
 
-The reference leaves attention, norms and the cache to its models' torch code (``modeling_mixtral.py:610-757``); here
+The reference leaves attention, norms and the cache to its models' torch code (``modeling_mixtral.py``); here
 they run beside the compact3 projections (``qlinear.Compact3Linear``) and the block (``moe.TrisSparseMoeBlock``):
 
 * ``rotary_tables``      cosines and sines of the positions;
