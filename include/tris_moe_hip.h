@@ -875,7 +875,7 @@ int tris_route_predecode_all_reduce(const float* router_logits, int32_t num_toke
  * The norm reads the unrounded sum.  x [rows, width] of x_type (F16 or BF16), rows x_stride elements apart; residual
  * and residual_out likewise of residual_type (both NULL without one; residual_out may be residual itself); weight
  * [width] of weight_type (F16, BF16 or F32); out of out_type (may be x itself if types and strides agree).  Buffers
- * may not overlap otherwise.  1 <= width <= 32768; any alignment (16-byte loads where everything is 16-byte aligned).
+ * may not overlap otherwise.  1 <= width <= 32768; rows need no alignment.
  */
 int tris_rms_norm(const void* x, int32_t x_type, int64_t x_stride, const void* residual, int32_t residual_type,
                   int64_t residual_stride, const void* weight, int32_t weight_type, float weight_offset, float eps,

@@ -144,73 +144,93 @@ __device__ __forceinline__ float across_groups(float v, Op op) {
   return op(__uint_as_float(y[0]), __uint_as_float(y[1]));
 }
 
+// A piece: the tiles [t0, t1) of sequence b (n positions, from `first` on) and head group hg, at place `at` of the line;
+// whole: all the tiles there are; else `slot` takes its sums.
+struct Piece {
+  int b, n, first, hg, t0, t1, at, slot;
+  bool whole;
+};
+
+constexpr bool query_in_lds(int head_dim) { return head_dim == 256; }
+
+// The wavefronts' sums of a piece joined under the workgroup's maximum: to the output, or to the piece's slot.
+// lds: [kWaves][tile_heads][head_dim + 4] sums, then [kWaves][16] maxima and sums.
+template <int kDim, bool kBf16>
+__device__ __forceinline__ void write_piece(const AttentionArgs& a, const Piece& p, int thread, float m, float l,
+                                            const f32x4* acc, float* lds) {
+  constexpr int kRun = kDim < 128 ? kDim / 16 : 8;
+  constexpr int kRuns = kDim / 16 / kRun;
+  constexpr int kPad = kDim + 4;
+  const int col = thread % 16, g = thread % kWave / 16, wave = uniform(thread / kWave);
+  const int kvh = p.hg / a.head_tiles, head0 = (p.hg % a.head_tiles) * kHeadTile;
+  const int heads = min(kHeadTile, a.group - head0);
+  l = across_groups(l, [](float u, float v) { return u + v; });
+  float* sh_o = lds;
+  float* sh_m = lds + kWaves * a.tile_heads * kPad;
+  float* sh_l = sh_m + kWaves * kHeadTile;
+  if (g == 0) {
+    sh_m[wave * kHeadTile + col] = m;
+    sh_l[wave * kHeadTile + col] = l;
+  }
+  if (col < heads) {
+    float* o = sh_o + (wave * a.tile_heads + col) * kPad;
+#pragma unroll
+    for (int c = 0; c < kRuns; ++c) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+#pragma unroll
+        for (int e = 0; e < kRun; e += 4) {
+          const int i = c * kRun + e;
+          *reinterpret_cast<f32x4*>(o + c * 16 * kRun + (g * 4 + r) * kRun + e) =
+              f32x4{acc[i][r], acc[i + 1][r], acc[i + 2][r], acc[i + 3][r]};
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int64_t row0 = static_cast<int64_t>(p.slot) * a.tile_heads;
+  for (int i = thread * 2; i < heads * kDim; i += kWaves * kWave * 2) {
+    const int h = i / kDim, d = i % kDim;
+    float top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kWaves; ++u) top = fmaxf(top, sh_m[u * kHeadTile + h]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, y0 = 0.0f, y1 = 0.0f;
+#pragma unroll
+    for (int u = 0; u < kWaves; ++u) {
+      const float f = __builtin_amdgcn_exp2f(sh_m[u * kHeadTile + h] - base);
+      const float* o = sh_o + (u * a.tile_heads + h) * kPad + d;
+      sum += sh_l[u * kHeadTile + h] * f;
+      y0 += o[0] * f;
+      y1 += o[1] * f;
+    }
+    if (p.whole) {
+      const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+      uint16_t* dst = a.out + p.b * a.out_seq + (kvh * a.group + head0 + h) * a.out_head + d;
+      *reinterpret_cast<uint32_t*>(dst) = kBf16 ? pack_bf16_rne(y0 * f, y1 * f) : pack_f16_rne(y0 * f, y1 * f);
+    } else {
+      *reinterpret_cast<float2*>(a.part_o + (row0 + h) * kDim + d) = make_float2(y0, y1);
+      if (d == 0) a.part_ml[row0 + h] = make_float2(top, sum);
+    }
+  }
+}
+
 // kWhole: every 16 keys of a tile lie in one page (page_size a multiple of 16; with e4m3, scale rows that can be read
 // four at a time), so that page numbers and row addresses are the same for the whole wavefront; else each lane looks
 // up one key and hands its rows' addresses around (of the same calls, whole / by lanes: 52.4 / 57.1, 83.5 / 91.3,
 // 144 / 147 and 25.7 / 26.5 us).
 template <int kDim, bool kBf16, bool kE4m3, bool kWhole>
-__global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_decode_kernel(const AttentionArgs args) {
+__device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece& p, int thread, u32x4 (*sh_q)[kWave],
+                                             float* lds) {
   constexpr bool kBf16V = kBf16 || kE4m3;           // type of the value product (see the probabilities below)
   constexpr int kRun = kDim < 128 ? kDim / 16 : 8;  // dimensions of one of a lane's runs of a value row
   constexpr int kRuns = kDim / 16 / kRun;
   constexpr int kSize = kE4m3 ? 1 : 2;
   constexpr int kKLoads = kDim * kSize / 64;        // 16-byte loads of a lane for one key row's quarter
   constexpr int kVWords = kRun * kSize / 4;         // words of a run
-  constexpr int kPad = kDim + 4;
-  constexpr bool kQueryInLds = kDim == 256;
-  __shared__ u32x4 sh_q[kQueryInLds ? kDim / 32 : 1][kQueryInLds ? kWave : 1];
-  extern __shared__ float lds[];                    // [kWaves][tile_heads][kPad] sums, then [kWaves][16] factors and sums
-
-  const int head_groups = args.c.kv_heads * args.head_tiles, w = blockIdx.x;
-  // the line's length, the workgroup's stretch, and the sequence where it begins
-  int length0;
-  const int places0 = places_of(args, 0, head_groups, &length0), end0 = wave_incl_sum_i32(places0);
-  int total = __builtin_amdgcn_readlane(end0, kWave - 1);
-  for (int b0 = kWave; b0 < args.c.batch; b0 += kWave) {
-    int length;
-    total += __builtin_amdgcn_readlane(wave_incl_sum_i32(places_of(args, b0, head_groups, &length)), kWave - 1);
-  }
-  const Line line(total, args.workgroups);
-  if (w >= line.shares) return;
-  int at = line.start(w), begin, b, n;
-  const int stop = line.start(w + 1);
-  for (int b0 = 0, places = places0, end = end0, length = length0;;) {
-    const uint64_t past = __ballot(at < end);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      begin = __builtin_amdgcn_readlane(end - places, l);
-      b = b0 + l;
-      n = __builtin_amdgcn_readlane(length, l);
-      break;
-    }
-    const int before = __builtin_amdgcn_readlane(end, kWave - 1);
-    b0 += kWave;
-    if (b0 >= args.c.batch) return;
-    places = places_of(args, b0, head_groups, &length);
-    end = before + wave_incl_sum_i32(places);
-  }
-  // one piece of a (sequence, head group) after the other
-  while (at < stop && b < args.c.batch) {
-  // What a piece needs of the arguments and of the lane's number is taken anew for each: kept in registers from piece to
-  // piece, it would cost the tiles' loop a third of its wavefronts.
-  int thread = threadIdx.x;
-  KernelArgs fresh = (KernelArgs)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+v"(thread), "+s"(fresh));
-  const AttentionArgs& a = *(const AttentionArgs*)fresh;
-  const int first = range_begin(a, n);
-  const int tiles = range_tiles(n, first), span = tiles + kPieceCost;
-  const int hg = (at - begin) / span, from = at - begin - hg * span;
-  if (hg == head_groups) {
-    begin = at;
-    n = uniform(sequence_length(a, ++b));
-    continue;
-  }
-  if (from >= tiles) {
-    at += span - from;
-    continue;
-  }
-  const int t1 = first / kTileKeys + min(tiles, from + stop - at), t_end = n > 0 ? t1 : 0;
-  const int kvh = hg / a.head_tiles, head0 = (hg % a.head_tiles) * kHeadTile;
+  constexpr bool kQueryInLds = query_in_lds(kDim);
+  const int n = p.n, first = p.first, t1 = p.t1, t_end = n > 0 ? t1 : 0;
+  const int kvh = p.hg / a.head_tiles, head0 = (p.hg % a.head_tiles) * kHeadTile;
   const int heads = min(kHeadTile, a.group - head0);
   const int wave = uniform(thread / kWave), lane = thread % kWave, col = lane % 16, g = lane / 16;
 
@@ -220,16 +240,13 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
   const int k_slot = static_cast<int>(a.c.k_slot_stride) * kSize, v_slot = static_cast<int>(a.c.v_slot_stride) * kSize;
   const int ks_slot = static_cast<int>(a.c.k_scale_slot_stride) * 4, vs_slot = static_cast<int>(a.c.v_scale_slot_stride) * 4;
 
-  if (from == 0 && thread == 0)
-    a.owners[b * head_groups + hg] = make_int2(w, line.owner(at + tiles - 1));
-
   // The query operand: head col, the dimensions that the K operand's lane has.  At 256 dimensions it would push the
   // tiles' loads out of the registers (it is 32 of them), so there it stays in LDS, read when it is used (8 ragged
   // sequences of up to 16000: 31.0 us, 39.4 with it in registers; at 128 dimensions both ways take the same time).
   u32x4 q[kQueryInLds ? 1 : kDim / 32];
   const auto query = [&](int i) {
     const int d = kE4m3 ? (i / 2) * 64 + g * 16 + (i % 2) * 8 : i * 32 + g * 8;
-    return col < heads ? *reinterpret_cast<const u32x4*>(a.q + b * a.q_seq + (kvh * a.group + head0 + col) * a.q_head + d)
+    return col < heads ? *reinterpret_cast<const u32x4*>(a.q + p.b * a.q_seq + (kvh * a.group + head0 + col) * a.q_head + d)
                        : u32x4{0, 0, 0, 0};
   };
   if constexpr (kQueryInLds) {
@@ -244,9 +261,9 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
   const char* vbase = static_cast<const char*>(a.c.v) + kvh * a.c.v_head_stride * kSize;
   const char* ksbase = reinterpret_cast<const char*>(a.c.k_scale) + kvh * a.c.k_scale_head_stride * 4;
   const char* vsbase = reinterpret_cast<const char*>(a.c.v_scale) + kvh * a.c.v_scale_head_stride * 4;
-  const int32_t* table = a.c.block_table + b * a.c.table_stride;
+  const int32_t* table = a.c.block_table + p.b * a.c.table_stride;
   // wavefronts take the workgroup's tiles in turn, also over the pieces
-  int tile = first / kTileKeys + from + ((wave - at) & (kWaves - 1));
+  int tile = p.t0 + ((wave - p.at) & (kWaves - 1));
 
   // Page numbers run ahead of the rows, so that no row waits for its page: whole, lane 2 i + t holds the block table's
   // entry of half t of the wavefront's i-th tile from `ids0`, 32 tiles a load and the next 32 behind them; else lane
@@ -454,9 +471,9 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
     }
     // The probabilities enter the value product as two 16-bit parts, the value and what its rounding left, so that the
     // result has one rounding to speak of, the output's (the second product costs 0 to 1 %: the matrix cores wait for
-    // memory).  In fp16 they are 2^15 times as large (the sum too, so that it
-    // cancels): a long tail far below the maximum would lose its bits to the subnormals otherwise.  An 8-bit cache's
-    // product runs in bf16, whose range takes any scale; its elements are exact in either type.
+    // memory).  In fp16 they are 2^15 times as large (the sum too, so that it cancels): a long tail far below the maximum
+    // would lose its bits to the subnormals otherwise.  An 8-bit cache's product runs in bf16, whose range takes any
+    // scale; its elements are exact in either type.
     const float base = (m == -INFINITY ? 0.0f : m) - (kBf16V ? 0.0f : 15.0f);
     float pr[8];
 #pragma unroll
@@ -487,7 +504,8 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
       } else {
         const auto h = __builtin_amdgcn_cvt_pkrtz(w0, w1);
         hi[i] = __builtin_bit_cast(uint32_t, h);
-        lo[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(w0 - static_cast<float>(h[0]), w1 - static_cast<float>(h[1])));
+        const auto rest = __builtin_amdgcn_cvt_pkrtz(w0 - static_cast<float>(h[0]), w1 - static_cast<float>(h[1]));
+        lo[i] = __builtin_bit_cast(uint32_t, rest);
       }
     }
 #pragma unroll
@@ -519,64 +537,68 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
     cur = nxt;
   }
 
-  asm volatile("" : "+v"(thread));
-  {
-  const int col = thread % 16, g = thread % kWave / 16, wave = uniform(thread / kWave);
-  // the wavefronts' sums joined under the workgroup's maximum
-  l = across_groups(l, [](float u, float v) { return u + v; });
-  float* sh_o = lds;
-  float* sh_m = lds + kWaves * a.tile_heads * kPad;
-  float* sh_l = sh_m + kWaves * kHeadTile;
-  if (g == 0) {
-    sh_m[wave * kHeadTile + col] = m;
-    sh_l[wave * kHeadTile + col] = l;
+  asm volatile("" : "+v"(thread));  // (what follows takes the lane's number anew too)
+  write_piece<kDim, kBf16>(a, p, thread, m, l, acc, lds);
+}
+
+template <int kDim, bool kBf16, bool kE4m3, bool kWhole>
+__global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_decode_kernel(const AttentionArgs args) {
+  __shared__ u32x4 sh_q[query_in_lds(kDim) ? kDim / 32 : 1][kWave];
+  extern __shared__ float lds[];
+  const int head_groups = args.c.kv_heads * args.head_tiles, w = blockIdx.x;
+  // the line's length, the workgroup's stretch, and the sequence where it begins
+  int length0;
+  const int places0 = places_of(args, 0, head_groups, &length0), end0 = wave_incl_sum_i32(places0);
+  int total = __builtin_amdgcn_readlane(end0, kWave - 1);
+  for (int b0 = kWave; b0 < args.c.batch; b0 += kWave) {
+    int length;
+    total += __builtin_amdgcn_readlane(wave_incl_sum_i32(places_of(args, b0, head_groups, &length)), kWave - 1);
   }
-  if (col < heads) {
-    float* o = sh_o + (wave * a.tile_heads + col) * kPad;
-#pragma unroll
-    for (int c = 0; c < kRuns; ++c) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-#pragma unroll
-        for (int e = 0; e < kRun; e += 4) {
-          const int i = c * kRun + e;
-          *reinterpret_cast<f32x4*>(o + c * 16 * kRun + (g * 4 + r) * kRun + e) =
-              f32x4{acc[i][r], acc[i + 1][r], acc[i + 2][r], acc[i + 3][r]};
-        }
-      }
+  const Line line(total, args.workgroups);
+  if (w >= line.shares) return;
+  int at = line.start(w), begin, b, n;
+  const int stop = line.start(w + 1);
+  for (int b0 = 0, places = places0, end = end0, length = length0;;) {
+    const uint64_t past = __ballot(at < end);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      begin = __builtin_amdgcn_readlane(end - places, l);
+      b = b0 + l;
+      n = __builtin_amdgcn_readlane(length, l);
+      break;
     }
+    const int before = __builtin_amdgcn_readlane(end, kWave - 1);
+    b0 += kWave;
+    if (b0 >= args.c.batch) return;
+    places = places_of(args, b0, head_groups, &length);
+    end = before + wave_incl_sum_i32(places);
   }
-  __syncthreads();
-  // a piece that begins a (sequence, head group) and is not all of it ends its workgroup's stretch: the second slot
-  const bool whole_range = from == 0 && t1 - first / kTileKeys == tiles;
-  const int64_t row0 = static_cast<int64_t>(2 * w + (from == 0)) * a.tile_heads;
-  for (int i = thread * 2; i < heads * kDim; i += kWaves * kWave * 2) {
-    const int h = i / kDim, d = i % kDim;
-    float top = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < kWaves; ++u) top = fmaxf(top, sh_m[u * kHeadTile + h]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, y0 = 0.0f, y1 = 0.0f;
-#pragma unroll
-    for (int u = 0; u < kWaves; ++u) {
-      const float f = __builtin_amdgcn_exp2f(sh_m[u * kHeadTile + h] - base);
-      const float* o = sh_o + (u * a.tile_heads + h) * kPad + d;
-      sum += sh_l[u * kHeadTile + h] * f;
-      y0 += o[0] * f;
-      y1 += o[1] * f;
+  // one piece of a (sequence, head group) after the other
+  while (at < stop && b < args.c.batch) {
+    // What a piece needs of the arguments and of the lane's number is taken anew for each: kept in registers from piece
+    // to piece, it would cost the tiles' loop a third of its wavefronts.
+    int thread = threadIdx.x;
+    KernelArgs fresh = (KernelArgs)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+v"(thread), "+s"(fresh));
+    const AttentionArgs& a = *(const AttentionArgs*)fresh;
+    const int first = range_begin(a, n), tiles = range_tiles(n, first), span = tiles + kPieceCost;
+    const int hg = (at - begin) / span, from = at - begin - hg * span;
+    if (hg == head_groups) {  // the next sequence
+      begin = at;
+      n = uniform(sequence_length(a, ++b));
+      continue;
     }
-    if (whole_range) {
-      const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-      uint16_t* dst = a.out + b * a.out_seq + (kvh * a.group + head0 + h) * a.out_head + d;
-      *reinterpret_cast<uint32_t*>(dst) = kBf16 ? pack_bf16_rne(y0 * f, y1 * f) : pack_f16_rne(y0 * f, y1 * f);
-    } else {
-      *reinterpret_cast<float2*>(a.part_o + (row0 + h) * kDim + d) = make_float2(y0, y1);
-      if (d == 0) a.part_ml[row0 + h] = make_float2(top, sum);
+    if (from >= tiles) {  // between two head groups
+      at += span - from;
+      continue;
     }
-  }
-  }
-  at += t1 - first / kTileKeys - from;
-  __syncthreads();  // the next piece's sums go where this one's are read
+    if (from == 0 && thread == 0) a.owners[b * head_groups + hg] = make_int2(w, line.owner(at + tiles - 1));
+    const int count = min(tiles - from, stop - at), t0 = first / kTileKeys + from;
+    // a piece that begins its (sequence, head group) and is not all of it ends its workgroup's stretch: the second slot
+    const Piece p{b, n, first, hg, t0, t0 + count, at, 2 * w + (from == 0), count == tiles};
+    attend_piece<kDim, kBf16, kE4m3, kWhole>(a, p, thread, sh_q, lds);
+    at += count;
+    __syncthreads();  // the next piece's sums go where this one's are read
   }
 }
 
@@ -720,8 +742,8 @@ using namespace tris;
 extern "C" int64_t tris_paged_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads,
                                                         int32_t head_dim, int32_t max_pages, int32_t page_size) {
   if (batch < 1 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1 || max_pages < 0 || page_size < 1) return 0;
-  return attention_space(attention_shape(batch, q_heads, kv_heads, head_dim, static_cast<int64_t>(max_pages) * page_size), batch,
-                         kv_heads, head_dim).bytes;
+  const int64_t positions = static_cast<int64_t>(max_pages) * page_size;
+  return attention_space(attention_shape(batch, q_heads, kv_heads, head_dim, positions), batch, kv_heads, head_dim).bytes;
 }
 
 extern "C" int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, int64_t q_head_stride, int32_t q_type,
@@ -738,8 +760,11 @@ extern "C" int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, 
     TRIS_REQUIRE(s >= 0 && s % 8 == 0, "%s: rows must be 16-byte aligned", who);
   TRIS_REQUIRE(aligned16(q) && aligned16(out), "%s: rows must be 16-byte aligned", who);
   const int64_t rows = static_cast<int64_t>(cache->batch) * q_heads;
-  const AttentionShape s = attention_shape(cache->batch, q_heads, cache->kv_heads, cache->head_dim, cache_positions(*cache));
-  TRIS_REQUIRE(rows * (cache->head_dim / 32) <= 2147483647LL - 3 && s.places < (1LL << 31) - (1 << 16), "%s: too many positions", who);
+  const AttentionShape s =
+      attention_shape(cache->batch, q_heads, cache->kv_heads, cache->head_dim, cache_positions(*cache));
+  // a launch has less than 2^32 threads
+  TRIS_REQUIRE(rows * (cache->head_dim / 32) < (1LL << 32) / kWave - 4, "%s: too many rows", who);
+  TRIS_REQUIRE(s.places < (1LL << 31) - (1 << 16), "%s: too many positions", who);
   const AttentionSpace w = attention_space(s, cache->batch, cache->kv_heads, cache->head_dim);
   TRIS_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= w.bytes,
                "%s: workspace of %lld bytes needed", who, static_cast<long long>(w.bytes));

@@ -208,7 +208,7 @@ extern "C" int tris_rotary_append_paged(const void* q, int64_t q_token_stride, i
   TRIS_REQUIRE(units < (1 << 24), "%s: too many heads", who);
   const int64_t token_waves = (units + kUnits * kWave - 1) / (kUnits * kWave);
   const int64_t blocks = (tokens * token_waves + 3) / 4;
-  TRIS_REQUIRE(blocks * 4 <= 2147483647LL, "%s: too many tokens", who);
+  TRIS_REQUIRE(blocks < (1LL << 32) / (4 * kWave), "%s: too many tokens", who);  // a launch has less than 2^32 threads
   AppendArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
                static_cast<uint16_t*>(q_out), cos, sin, query_start, q_token_stride, q_head_stride, k_token_stride,
                k_head_stride, v_token_stride, v_head_stride, q_out_token_stride, q_out_head_stride,

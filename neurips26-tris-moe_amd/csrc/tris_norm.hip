@@ -123,11 +123,14 @@ __global__ __launch_bounds__(kLanes > 256 ? kLanes : 256) void rms_norm_kernel(c
 }
 
 template <int kLanes, int kChunks>
-static void rms_norm_launch(const RmsNormArgs& a, hipStream_t st) {
-  constexpr int kRows = kLanes <= kWave ? 256 / kLanes : 1;
-  const dim3 grid(static_cast<unsigned>((a.rows + kRows - 1) / kRows)), block(kLanes <= kWave ? 256 : kLanes);
+static int rms_norm_launch(const char* who, const RmsNormArgs& a, hipStream_t st) {
+  constexpr int kRows = kLanes <= kWave ? 256 / kLanes : 1, kThreads = kLanes <= kWave ? 256 : kLanes;
+  const int64_t blocks = (a.rows + kRows - 1) / kRows;
+  TRIS_REQUIRE(blocks * kThreads < 1LL << 32, "%s: too many rows", who);  // of one launch
+  const dim3 grid(static_cast<unsigned>(blocks)), block(kThreads);
   if (a.width % 8 == 0) hipLaunchKernelGGL((rms_norm_kernel<kLanes, kChunks, false>), grid, block, 0, st, a);
   else hipLaunchKernelGGL((rms_norm_kernel<kLanes, kChunks, true>), grid, block, 0, st, a);
+  return check_launch(who);
 }
 
 }  // namespace tris
@@ -140,7 +143,7 @@ extern "C" int tris_rms_norm(const void* x, int32_t x_type, int64_t x_stride, co
                              int64_t out_stride, void* residual_out, int64_t residual_out_stride, void* stream) {
   const char* who = "tris_rms_norm";
   TRIS_REQUIRE(rows >= 0 && width >= 1 && width <= 32768, "%s: rows must not be negative, width 1 to 32768", who);
-  TRIS_REQUIRE(rows <= 2147483647LL, "%s: too many rows", who);
+  TRIS_REQUIRE(rows < 1LL << 32, "%s: too many rows", who);
   TRIS_REQUIRE(is_16bit(x_type) && is_16bit(out_type) && (is_16bit(weight_type) || weight_type == TRIS_DTYPE_F32),
                "%s: x and out must be fp16 or bf16, weight one of these or fp32", who);
   if (rows == 0) return TRIS_OK;
@@ -153,15 +156,14 @@ extern "C" int tris_rms_norm(const void* x, int32_t x_type, int64_t x_stride, co
   RmsNormArgs a{x, residual, weight, out, residual_out, x_stride, residual_stride, out_stride, residual_out_stride,
                 rows, x_type, residual_type, weight_type, out_type, width, weight_offset, eps};
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (width <= 64) rms_norm_launch<8, 1>(a, st);
-  else if (width <= 128) rms_norm_launch<16, 1>(a, st);
-  else if (width <= 256) rms_norm_launch<32, 1>(a, st);
-  else if (width <= 512) rms_norm_launch<64, 1>(a, st);
-  else if (width <= 1024) rms_norm_launch<64, 2>(a, st);
-  else if (width <= 2048) rms_norm_launch<256, 1>(a, st);
-  else if (width <= 4096) rms_norm_launch<256, 2>(a, st);
-  else if (width <= 8192) rms_norm_launch<512, 2>(a, st);
-  else if (width <= 16384) rms_norm_launch<1024, 2>(a, st);
-  else rms_norm_launch<1024, 4>(a, st);
-  return check_launch(who);
+  if (width <= 64) return rms_norm_launch<8, 1>(who, a, st);
+  if (width <= 128) return rms_norm_launch<16, 1>(who, a, st);
+  if (width <= 256) return rms_norm_launch<32, 1>(who, a, st);
+  if (width <= 512) return rms_norm_launch<64, 1>(who, a, st);
+  if (width <= 1024) return rms_norm_launch<64, 2>(who, a, st);
+  if (width <= 2048) return rms_norm_launch<256, 1>(who, a, st);
+  if (width <= 4096) return rms_norm_launch<256, 2>(who, a, st);
+  if (width <= 8192) return rms_norm_launch<512, 2>(who, a, st);
+  if (width <= 16384) return rms_norm_launch<1024, 2>(who, a, st);
+  return rms_norm_launch<1024, 4>(who, a, st);
 }

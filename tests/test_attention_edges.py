@@ -1,6 +1,8 @@
 """The norm, the append and the paged attention at calls that the other files do not make: many query heads a kv head at
 every head dimension, pools past 4 GiB, layer and key / value slices of one pool, expanded rows, outputs over inputs,
 windows past 32 bits, tensors of another device than the current one, long page tables, calls side by side."""
+import ctypes
+
 import pytest
 import torch
 
@@ -29,6 +31,27 @@ def test_launch_makes_the_tensors_device_current(tris, monkeypatch):
     assert ext._launch(0, lambda a, b: a + b, 1, 2) == 3 and seen == []
     assert ext._launch(1, lambda a: seen.append("call") or a, 5) == 5
     assert seen == [("enter", 1), "call", ("exit", 1)]
+
+
+def test_launches_past_their_thread_count_are_refused(tris):
+    """A launch has less than 2^32 threads; what would need more is refused before it, with a message."""
+    from test_paged_cache import c_cache
+    from tris_moe_amd import _lib
+
+    lib, p = _lib.load(), ctypes.c_void_p(4096)
+    for width, rows in ((128, 1 << 28), (4096, 1 << 24), (32768, 1 << 22), (64, 1 << 32)):
+        assert lib.tris_rms_norm(p, 0, width, None, 0, 0, p, 0, 0.0, 1e-6, rows, width, p, 0, width, None, 0, None) == -1
+        assert b"too many rows" in lib.tris_last_error()
+    c = c_cache(batch=1 << 27)
+    assert lib.tris_rotary_append_paged(p, 512, 128, p, 256, 128, p, 256, 128, 0, 1 << 27, 4, p, p, 128, 48, None,
+                                        ctypes.byref(c), p, 512, 128, 0, None) == -1
+    assert b"too many tokens" in lib.tris_last_error()
+    args = (0.1, 0, p, 512, 128, p, 1 << 60, None)
+    assert lib.tris_paged_attention_decode(p, 512, 128, 0, 4, ctypes.byref(c), *args) == -1
+    assert b"too many rows" in lib.tris_last_error()
+    c = c_cache(batch=1 << 20, max_pages=1 << 20)
+    assert lib.tris_paged_attention_decode(p, 512, 128, 0, 4, ctypes.byref(c), *args) == -1
+    assert b"too many positions" in lib.tris_last_error()
 
 
 @pytest.mark.gpu
