@@ -941,7 +941,7 @@ int tris_rotary_append_paged(const void* q, int64_t q_token_stride, int64_t q_he
  * its pages valid), and one whose scores are all -infinity, gives zeros.  out may be q with the same strides.  Slots past the sequence's end, before its window, or on invalid pages may hold
  * anything.  q, out [batch][q_heads][head_dim] of q_type (F16 or BF16; a 16-bit cache has the same type), strides in
  * elements, rows 16-byte aligned; q_heads a multiple of kv_heads.  workspace: tris_paged_attention_workspace_bytes of
- * the same sizes, 16-byte aligned, no initial contents; calls that may overlap need one each.
+ * the same sizes (0: none needed), 16-byte aligned, no initial contents; calls that may overlap need one each.
  */
 int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, int64_t q_head_stride, int32_t q_type,
                                 int32_t q_heads, const tris_paged_cache* cache, float scale, int32_t window, void* out,

@@ -17,7 +17,8 @@
 //
 // The work is split over the length: the tiles of all sequences and head groups form one line, and each workgroup takes
 // an equal stretch of it, so that a long sequence beside short ones is shared by the whole GPU and all workgroups end
-// together.  Every wavefront derives the same line from seq_lens, so the launch needs no lengths on the host.
+// together.  Every wavefront derives the same line from seq_lens, so the launch needs no lengths on the host.  (Where the
+// block table is narrow there is no line: each workgroup has a (sequence, head group), in one launch.)
 //
 // Bound by memory: a (key, kv head) is 4 head_dim bytes in 16 bits and 4 flops a byte for each query head of the group.
 // One MI355X reads 6.2 TB/s; 131072 tokens with 4 kv heads of 128 (268 MB) take 46.5 + 4.5 us, 64 sequences of 4000 to
@@ -100,6 +101,7 @@ typedef const __attribute__((address_space(4))) AttentionArgs* KernelArgs;
 
 struct Line {
   int shares, each, more;
+  Line() = default;
   __device__ Line(int total, int workgroups) {
     shares = min(workgroups, (total + kWaves - 1) / kWaves);  // no fewer than one tile for a wavefront
     each = total / shares;
@@ -116,6 +118,52 @@ __device__ __forceinline__ int places_of(const AttentionArgs& a, int b0, int hea
   const int b = b0 + static_cast<int>(threadIdx.x) % kWave;
   *n = sequence_length(a, b);
   return b < a.c.batch ? (range_tiles(*n, range_begin(a, *n)) + kPieceCost) * head_groups : 0;
+}
+
+// A workgroup's part of the line, [at, stop), and the sequence where it begins: its number, length and first place.
+struct Stretch {
+  Line line;
+  int at, stop, begin, b, n;
+};
+
+__device__ __forceinline__ bool line_stretch(const AttentionArgs& a, int head_groups, int w, Stretch* s) {
+  int length0;
+  const int places0 = places_of(a, 0, head_groups, &length0), end0 = wave_incl_sum_i32(places0);
+  int total = __builtin_amdgcn_readlane(end0, kWave - 1);
+  for (int b0 = kWave; b0 < a.c.batch; b0 += kWave) {
+    int length;
+    total += __builtin_amdgcn_readlane(wave_incl_sum_i32(places_of(a, b0, head_groups, &length)), kWave - 1);
+  }
+  s->line = Line(total, a.workgroups);
+  if (w >= s->line.shares) return false;
+  s->at = s->line.start(w);
+  s->stop = s->line.start(w + 1);
+  for (int b0 = 0, places = places0, end = end0, length = length0;;) {
+    const uint64_t past = __ballot(s->at < end);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      s->begin = __builtin_amdgcn_readlane(end - places, l);
+      s->b = b0 + l;
+      s->n = __builtin_amdgcn_readlane(length, l);
+      return true;
+    }
+    const int before = __builtin_amdgcn_readlane(end, kWave - 1);
+    b0 += kWave;
+    if (b0 >= a.c.batch) return false;
+    places = places_of(a, b0, head_groups, &length);
+    end = before + wave_incl_sum_i32(places);
+  }
+}
+
+// Without a line: workgroup w has one (sequence, head group), all of it.
+__device__ __forceinline__ bool whole_stretch(const AttentionArgs& a, int head_groups, int w, Stretch* s) {
+  s->b = w / head_groups;
+  s->n = uniform(sequence_length(a, s->b));
+  const int tiles = range_tiles(s->n, range_begin(a, s->n));
+  s->begin = 0;
+  s->at = (w - s->b * head_groups) * (tiles + kPieceCost);
+  s->stop = s->at + tiles;
+  return true;
 }
 
 template <bool kBf16>
@@ -546,33 +594,11 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
   __shared__ u32x4 sh_q[query_in_lds(kDim) ? kDim / 32 : 1][kWave];
   extern __shared__ float lds[];
   const int head_groups = args.c.kv_heads * args.head_tiles, w = blockIdx.x;
-  // the line's length, the workgroup's stretch, and the sequence where it begins
-  int length0;
-  const int places0 = places_of(args, 0, head_groups, &length0), end0 = wave_incl_sum_i32(places0);
-  int total = __builtin_amdgcn_readlane(end0, kWave - 1);
-  for (int b0 = kWave; b0 < args.c.batch; b0 += kWave) {
-    int length;
-    total += __builtin_amdgcn_readlane(wave_incl_sum_i32(places_of(args, b0, head_groups, &length)), kWave - 1);
-  }
-  const Line line(total, args.workgroups);
-  if (w >= line.shares) return;
-  int at = line.start(w), begin, b, n;
-  const int stop = line.start(w + 1);
-  for (int b0 = 0, places = places0, end = end0, length = length0;;) {
-    const uint64_t past = __ballot(at < end);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      begin = __builtin_amdgcn_readlane(end - places, l);
-      b = b0 + l;
-      n = __builtin_amdgcn_readlane(length, l);
-      break;
-    }
-    const int before = __builtin_amdgcn_readlane(end, kWave - 1);
-    b0 += kWave;
-    if (b0 >= args.c.batch) return;
-    places = places_of(args, b0, head_groups, &length);
-    end = before + wave_incl_sum_i32(places);
-  }
+  Stretch st;
+  if (!(args.owners == nullptr ? whole_stretch(args, head_groups, w, &st) : line_stretch(args, head_groups, w, &st)))
+    return;
+  int at = st.at, begin = st.begin, b = st.b, n = st.n;
+  const int stop = st.stop;
   // one piece of a (sequence, head group) after the other
   while (at < stop && b < args.c.batch) {
     // What a piece needs of the arguments and of the lane's number is taken anew for each: kept in registers from piece
@@ -592,7 +618,7 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
       at += span - from;
       continue;
     }
-    if (from == 0 && thread == 0) a.owners[b * head_groups + hg] = make_int2(w, line.owner(at + tiles - 1));
+    if (a.owners != nullptr && from == 0 && thread == 0) a.owners[b * head_groups + hg] = make_int2(w, st.line.owner(at + tiles - 1));
     const int count = min(tiles - from, stop - at), t0 = first / kTileKeys + from;
     // a piece that begins its (sequence, head group) and is not all of it ends its workgroup's stretch: the second slot
     const Piece p{b, n, first, hg, t0, t0 + count, at, 2 * w + (from == 0), count == tiles};
@@ -677,10 +703,19 @@ __global__ __launch_bounds__(kTogether == 16 ? 1024 : 256) void attention_join_k
   *reinterpret_cast<uint2*>(a.out + b * a.out_seq + h * a.out_head + d) = packed;
 }
 
+// Positions times head_dim of a block table up to which a (sequence, head group) is one workgroup's: one launch, no
+// workspace, no line; twice as many where there is one for each CU.  Only the table's width is known here, not the lengths:
+// beyond, one long sequence would hold up the call.  In a graph, on the line / whole, us: one sequence of 128, 512, 1024
+// with 8 kv heads of 128: 7.0 / 4.9, 8.2 / 8.2, 8.5 / 12.4 (called eagerly 14.6 / 10.6, 14.7 / 10.5, 14.7 / 12.5); 64 of
+// 512, 1024 and 2048: 33 / 24, 51 / 45, 94 / 86; one of 128, 256 and 512 with 2 kv heads of 256: 10.5 / 8.9, 11.8 / 12.2,
+// 11.7 / 18.3.
+constexpr int64_t kWhole = 512 * 128;
+
 // The launch's sizes, from shapes alone.
 struct AttentionShape {
   int group, head_tiles, tile_heads, workgroups;
   int64_t places;  // of the line, at most
+  bool line;
 };
 
 static AttentionShape attention_shape(int64_t batch, int q_heads, int kv_heads, int head_dim, int64_t positions) {
@@ -691,7 +726,9 @@ static AttentionShape attention_shape(int64_t batch, int q_heads, int kv_heads, 
   const int64_t head_groups = static_cast<int64_t>(kv_heads) * s.head_tiles;
   const int64_t most = positions / kTileKeys + 2;  // of one sequence: a window may begin and end inside a tile
   s.places = batch * (most + kPieceCost) * head_groups;
-  s.workgroups = static_cast<int>(std::min<int64_t>(kCus * resident(head_dim), (s.places + kWaves - 1) / kWaves));
+  s.line = positions * head_dim > kWhole * (batch * head_groups >= kCus ? 2 : 1);
+  s.workgroups = static_cast<int>(s.line ? std::min<int64_t>(kCus * resident(head_dim), (s.places + kWaves - 1) / kWaves)
+                                         : std::min<int64_t>(batch * head_groups, 2147483647LL));
   return s;
 }
 
@@ -705,7 +742,7 @@ static AttentionSpace attention_space(const AttentionShape& s, int64_t batch, in
   const int64_t rows = 2LL * s.workgroups * s.tile_heads;
   w.ml = up(batch * kv_heads * s.head_tiles * static_cast<int64_t>(sizeof(int2)));
   w.o = w.ml + up(rows * static_cast<int64_t>(sizeof(float2)));
-  w.bytes = w.o + rows * head_dim * static_cast<int64_t>(sizeof(float));
+  w.bytes = s.line ? w.o + rows * head_dim * static_cast<int64_t>(sizeof(float)) : 0;
   return w;
 }
 
@@ -715,6 +752,7 @@ static void attention_launch(const AttentionArgs& a, const AttentionShape& s, bo
   const size_t lds = (kWaves * a.tile_heads * (kDim + 4) + 2 * kWaves * kHeadTile) * sizeof(float);
   if (whole) hipLaunchKernelGGL((attention_decode_kernel<kDim, kBf16, kE4m3, true>), grid, block, lds, st, a);
   else hipLaunchKernelGGL((attention_decode_kernel<kDim, kBf16, kE4m3, false>), grid, block, lds, st, a);
+  if (!s.line) return;
   // few sequences are cut into many pieces each, many into a few
   const int64_t units = static_cast<int64_t>(a.c.batch) * a.q_heads * (kDim / 32);
   const int64_t pieces = a.workgroups / (static_cast<int64_t>(a.c.batch) * a.c.kv_heads * a.head_tiles);
@@ -763,10 +801,12 @@ extern "C" int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, 
   const AttentionShape s =
       attention_shape(cache->batch, q_heads, cache->kv_heads, cache->head_dim, cache_positions(*cache));
   // a launch has less than 2^32 threads
-  TRIS_REQUIRE(rows * (cache->head_dim / 32) < (1LL << 32) / kWave - 4, "%s: too many rows", who);
+  TRIS_REQUIRE(rows * (cache->head_dim / 32) < (1LL << 32) / kWave - 4 &&
+                   s.workgroups < (1LL << 32) / (kWaves * kWave),
+               "%s: too many rows", who);
   TRIS_REQUIRE(s.places < (1LL << 31) - (1 << 16), "%s: too many positions", who);
   const AttentionSpace w = attention_space(s, cache->batch, cache->kv_heads, cache->head_dim);
-  TRIS_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= w.bytes,
+  TRIS_REQUIRE(!s.line || (workspace && aligned16(workspace) && workspace_bytes >= w.bytes),
                "%s: workspace of %lld bytes needed", who, static_cast<long long>(w.bytes));
   AttentionArgs a{static_cast<const uint16_t*>(q),
                   static_cast<uint16_t*>(out),
@@ -786,10 +826,12 @@ extern "C" int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, 
                   nullptr,
                   nullptr,
                   *cache};
-  char* at = static_cast<char*>(workspace);
-  a.owners = reinterpret_cast<int2*>(at);
-  a.part_ml = reinterpret_cast<float2*>(at + w.ml);
-  a.part_o = reinterpret_cast<float*>(at + w.o);
+  if (s.line) {
+    char* at = static_cast<char*>(workspace);
+    a.owners = reinterpret_cast<int2*>(at);
+    a.part_ml = reinterpret_cast<float2*>(at + w.ml);
+    a.part_o = reinterpret_cast<float*>(at + w.o);
+  }
   bool whole = cache->page_size % 16 == 0;
   if (cache->dtype == TRIS_DTYPE_E4M3) {  // four scales a load
     whole = whole && cache->k_scale_slot_stride == 1 && cache->v_scale_slot_stride == 1 && aligned16(cache->k_scale) &&

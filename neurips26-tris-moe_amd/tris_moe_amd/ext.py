@@ -2285,9 +2285,9 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     q_heads = q.size(1)
     lib = _lib.load()
     need = lib.tris_paged_attention_workspace_bytes(batch, q_heads, heads, dim, max_pages, page)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device)  # (of another stream's call, another allocation)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # of this call alone
     rc = _launch(index, lib.tris_paged_attention_decode, q.data_ptr(), qs[0], qs[1], _DTYPE_IDS[dt], q_heads, cache,
-                 dim ** -0.5 if scale is None else scale, window, out.data_ptr(), outs[0], outs[1], ws.data_ptr(), need,
+                 dim ** -0.5 if scale is None else scale, window, out.data_ptr(), outs[0], outs[1], _ptr(ws), need,
                  torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, "tris_paged_attention_decode")

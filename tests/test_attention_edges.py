@@ -200,3 +200,47 @@ def test_graphs_of_one_pool_and_eager_calls_between(tris, cuda):
         second.replay()
         torch.cuda.synchronize()
         assert torch.equal(got_b, want_b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", [(F16, F16), (BF16, BF16), (F16, E4M3), (BF16, E4M3)], ids=str)
+@pytest.mark.parametrize("dim,longest", [(64, 900), (128, 470), (256, 230)])
+@pytest.mark.parametrize("page", [16, 6])
+def test_narrow_tables(tris, cuda, types, dim, longest, page):
+    """Block tables narrow enough for one launch without a workspace, and the same sequences with a wider table, which
+    are split; small batches and ones with a workgroup for each CU."""
+    from tris_moe_amd import _lib
+
+    need = _lib.load().tris_paged_attention_workspace_bytes
+    for batch, heads in ((9, (8, 2)), (70, (10, 5))):
+        print(f"[gpu-case] attention {types} dim={dim} page={page} batch={batch} narrow and wide", flush=True)
+        lengths = [(37 * i * i) % longest for i in range(batch)]
+        lengths[1] = longest
+        a = _case(cuda, *heads, dim, *types, page, lengths, seed=batch)
+        assert need(batch, *heads, dim, a["block_table"].shape[1], page) == 0
+        _check(a, lengths, tris["ext"].paged_attention_decode(**a))
+        _check(a, lengths, tris["ext"].paged_attention_decode(**a, window=40), window=40)
+        wide = torch.full((batch, 3000), -1, dtype=torch.int32, device=cuda)
+        wide[:, : a["block_table"].shape[1]] = a["block_table"]
+        a["block_table"] = wide
+        assert need(batch, *heads, dim, 3000, page) > 0
+        _check(a, lengths, tris["ext"].paged_attention_decode(**a))
+
+
+@pytest.mark.gpu
+def test_workspace_too_small_is_refused(tris, cuda):
+    from tris_moe_amd import _lib
+
+    lib = _lib.load()
+    a = _case(cuda, 4, 2, 128, F16, F16, 16, [3000])
+    cache, (batch, pages, page, heads, dim) = tris["ext"]._paged_cache(
+        "t", a["k_cache"], a["v_cache"], a["block_table"], a["seq_lens"], None, None, a["q"].get_device())
+    need = lib.tris_paged_attention_workspace_bytes(batch, 4, heads, dim, pages, page)
+    ws, out = torch.empty(need, dtype=torch.uint8, device=cuda), torch.full_like(a["q"], 7.0)
+    stream = torch.cuda.current_stream(cuda).cuda_stream
+    for p, size in ((ws.data_ptr(), need - 1), (None, need), (ws.data_ptr() + 8, need)):
+        rc = lib.tris_paged_attention_decode(a["q"].data_ptr(), 512, 128, 0, 4, cache, 0.1, 0, out.data_ptr(), 512, 128, p,
+                                             size, stream)
+        assert rc == -1 and b"workspace" in lib.tris_last_error()
+    torch.cuda.synchronize()
+    assert bool((out == 7).all())
