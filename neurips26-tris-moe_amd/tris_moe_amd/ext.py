@@ -1984,8 +1984,8 @@ def swiglu_mul(gate: torch.Tensor, up: torch.Tensor, out: torch.Tensor | None = 
 
 # ------------------------------------------------------------------ attention side of a decoder layer
 # One decode step makes a handful of these calls a layer, each a few microseconds on the GPU, so their host path is kept
-# short (measured on the host of an MI355X node, us a call: rms_norm with a residual 13.7 -> 8.9, rotary_append_paged
-# 18.7 -> 13.1, paged_attention_decode 18.7 -> 14.1): each check is one condition over attribute reads, and a call that
+# short (measured on the host of an MI355X node, us a call: rms_norm with a residual 13.7 -> 8.7, rotary_append_paged
+# 18.7 -> 12.2, paged_attention_decode 18.7 -> 13.5, 10.2 in one launch): each check is one condition over attribute reads, and a call that
 # fails one goes through the named checks below for its message.
 _DTYPE_IDS = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32,
               torch.float8_e4m3fn: _lib.DTYPE_E4M3}
@@ -2038,10 +2038,10 @@ def _norm_stride(who, name, t, width):
     return flat.stride(0)
 
 
-def _norm_operand(who, name, t, x, index, dtypes, width):
+def _norm_operand(who, name, t, shape, index, dtypes, width):
     """(dtype id, row stride) of a tensor of x's shape and device."""
-    if not (isinstance(t, torch.Tensor) and t.get_device() == index and t.dtype in dtypes and t.shape == x.shape):
-        _check_on(who, name, t, None, dtypes, x.device)
+    if not (isinstance(t, torch.Tensor) and t.get_device() == index and t.dtype in dtypes and t.shape == shape):
+        _check_on(who, name, t, None, dtypes, torch.device("cuda", index))
         raise RuntimeError(f"{who}: {name} must have the shape of x")
     return _DTYPE_IDS[t.dtype], width if t.is_contiguous() else _norm_stride(who, name, t, width)
 
@@ -2070,31 +2070,32 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.
     width = weight.numel()
     if not 1 <= width <= RMS_NORM_MAX_WIDTH:
         raise RuntimeError(f"{who}: width must be 1 to {RMS_NORM_MAX_WIDTH}")
-    if x.ndim < 1 or x.shape[-1] != width:
+    shape = x.shape
+    if not shape or shape[-1] != width:
         raise RuntimeError(f"{who}: x must have {width} columns")
     whole = x.is_contiguous()
     rows, x_stride = x.numel() // width, width if whole else _norm_stride(who, "x", x, width)
     x_type, out_stride = _DTYPE_IDS[x.dtype], width
     if out is not None:
-        out_type, out_stride = _norm_operand(who, "out", out, x, index, _ACT_DTYPES, width)
+        out_type, out_stride = _norm_operand(who, "out", out, shape, index, _ACT_DTYPES, width)
         if out_dtype is not None and out.dtype != out_dtype:
             raise RuntimeError(f"{who}: out must be {out_dtype}")
     elif out_dtype is None or out_dtype is x.dtype:
-        out_type, out = x_type, torch.empty_like(x) if whole else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out_type, out = x_type, torch.empty_like(x) if whole else torch.empty(shape, dtype=x.dtype, device=x.device)
     else:
         if out_dtype not in _ACT_DTYPES:
             raise RuntimeError(f"{who}: out_dtype must be torch.float16 or torch.bfloat16")
-        out_type, out = _DTYPE_IDS[out_dtype], torch.empty(x.shape, dtype=out_dtype, device=x.device)
+        out_type, out = _DTYPE_IDS[out_dtype], torch.empty(shape, dtype=out_dtype, device=x.device)
     r_ptr = ro_ptr = None
     r_type = r_stride = ro_stride = 0
     if residual is not None:
-        r_type, r_stride = _norm_operand(who, "residual", residual, x, index, _ACT_DTYPES, width)
+        r_type, r_stride = _norm_operand(who, "residual", residual, shape, index, _ACT_DTYPES, width)
         if residual_out is None:
-            residual_out = (torch.empty_like(residual) if residual.is_contiguous()
-                            else torch.empty(x.shape, dtype=residual.dtype, device=x.device))
+            residual_out = (torch.empty_like(residual) if r_stride == width and residual.is_contiguous()
+                            else torch.empty(shape, dtype=residual.dtype, device=x.device))
             ro_stride = width
         else:
-            _, ro_stride = _norm_operand(who, "residual_out", residual_out, x, index, (residual.dtype,), width)
+            _, ro_stride = _norm_operand(who, "residual_out", residual_out, shape, index, (residual.dtype,), width)
         r_ptr, ro_ptr = residual.data_ptr(), residual_out.data_ptr()
     elif residual_out is not None:
         raise RuntimeError(f"{who}: residual_out needs a residual")
@@ -2107,35 +2108,40 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.
 
 
 def _heads(who, name, t, dtype, index, dim):
-    """t [tokens, heads, dim] with 16-byte-aligned contiguous rows, or a copy of it that has them; and its strides."""
+    """t [tokens, heads, dim] with 16-byte-aligned contiguous rows, or a copy of it that has them; its shape and
+    strides."""
     if not (isinstance(t, torch.Tensor) and t.get_device() == index and t.dtype is dtype and t.ndim == 3):
         _check_on(who, name, t, 3, (dtype,), torch.device("cuda", index))
-    if t.size(2) != dim:
+    shape, strides = t.shape, t.stride()
+    if shape[2] != dim:
         raise RuntimeError(f"{who}: {name} must have the cache's head_dim {dim}")
-    strides = t.stride()
     a, b, c = strides
     if c == 1 and not (t.data_ptr() & 15 or a & 7 or b & 7):
-        return t, strides
+        return t, shape, strides
     t = t.clone(memory_format=torch.contiguous_format)
-    return t, t.stride()
+    return t, shape, t.stride()
 
 
-def _heads_out(who, name, t, like, dtype, index):
-    """A given output of like's shape: its strides."""
-    if not (isinstance(t, torch.Tensor) and t.get_device() == index and t.dtype is dtype and t.shape == like.shape
-            and t.stride(2) == 1):
-        _check_on(who, name, t, 3, (dtype,), torch.device("cuda", index))
+def _heads_out(who, name, out, q, shape, strides, dtype, index):
+    """An output of q's shape, given or new (contiguous), and its strides."""
+    if out is None:
+        _, heads, dim = shape
+        if strides[0] == heads * dim and strides[1] == dim:
+            return torch.empty_like(q), strides
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    elif not (isinstance(out, torch.Tensor) and out.get_device() == index and out.dtype is dtype and out.shape == shape
+              and out.stride(2) == 1):
+        _check_on(who, name, out, 3, (dtype,), torch.device("cuda", index))
         raise RuntimeError(f"{who}: {name} must have the shape of q and contiguous rows")
-    return t.stride()
+    return out, out.stride()
 
 
 def _paged_cache(who, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, index):
     """The C descriptor of a paged cache (struct tris_paged_cache, its bytes) and (batch, max_pages, page_size,
     kv_heads, head_dim)."""
-    dtype = getattr(k_cache, "dtype", None)
+    dtype, shape = getattr(k_cache, "dtype", None), getattr(k_cache, "shape", ())
     if not (dtype in _CACHE_DTYPES and isinstance(v_cache, torch.Tensor) and k_cache.get_device() == index
-            and v_cache.get_device() == index and v_cache.dtype is dtype and k_cache.ndim == 4
-            and v_cache.shape == k_cache.shape):
+            and v_cache.get_device() == index and v_cache.dtype is dtype and len(shape) == 4 and v_cache.shape == shape):
         dev = torch.device("cuda", index)
         _check_on(who, "k_cache", k_cache, 4, _CACHE_DTYPES, dev)
         _check_on(who, "v_cache", v_cache, 4, (dtype,), dev)
@@ -2146,14 +2152,14 @@ def _paged_cache(who, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale,
         dev = torch.device("cuda", index)
         _check_on(who, "block_table", block_table, 2, (torch.int32,), dev)
         _check_on(who, "seq_lens", seq_lens, 1, (torch.int32,), dev)
-    pages, heads, page, dim = k_cache.shape
+    pages, heads, page, dim = shape
     k0, k1, k2, k3 = k_cache.stride()
     v0, v1, v2, v3 = v_cache.stride()
     if k3 != 1 or v3 != 1:
         raise RuntimeError(f"{who}: each cache row of head_dim values must be contiguous")
     batch, max_pages = block_table.shape
     row, col = block_table.stride()
-    if seq_lens.size(0) != batch or not seq_lens.is_contiguous():
+    if seq_lens.numel() != batch or not seq_lens.is_contiguous():
         raise RuntimeError(f"{who}: seq_lens must be contiguous, one length for each row of block_table")
     if col != 1 and max_pages > 1:
         raise RuntimeError(f"{who}: the rows of block_table must be contiguous")
@@ -2162,7 +2168,7 @@ def _paged_cache(who, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale,
     if dtype is torch.float8_e4m3fn:
         if not (isinstance(k_scale, torch.Tensor) and isinstance(v_scale, torch.Tensor)
                 and k_scale.get_device() == index and v_scale.get_device() == index and k_scale.dtype is torch.float32
-                and v_scale.dtype is torch.float32 and k_scale.shape == v_scale.shape == (pages, heads, page)):
+                and v_scale.dtype is torch.float32 and k_scale.shape == shape[:3] and v_scale.shape == shape[:3]):
             if k_scale is None or v_scale is None:
                 raise RuntimeError(f"{who}: an e4m3 cache needs k_scale and v_scale")
             for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
@@ -2204,23 +2210,24 @@ def rotary_append_paged(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor
     index, dt = k.get_device(), k.dtype
     cache, (batch, _, _, heads, dim) = _paged_cache(who, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale,
                                                     index)
-    (k, ks), (v, vs) = _heads(who, "k", k, dt, index, dim), _heads(who, "v", v, dt, index, dim)
-    tokens = k.size(0)
+    k, (tokens, k_heads, _), ks = _heads(who, "k", k, dt, index, dim)
+    v, (v_tokens, v_heads, _), vs = _heads(who, "v", v, dt, index, dim)
     if k.requires_grad or v.requires_grad or (q is not None and q.requires_grad):
         _refuse_gradient(who)
-    if k.size(1) != heads or v.size(1) != heads or v.size(0) != tokens:
+    if k_heads != heads or v_heads != heads or v_tokens != tokens:
         raise RuntimeError(f"{who}: k and v must be [tokens, kv_heads, head_dim] of the cache's kv_heads")
+    angles = getattr(cos, "shape", ())
     if not (isinstance(cos, torch.Tensor) and isinstance(sin, torch.Tensor) and cos.get_device() == index
-            and sin.get_device() == index and cos.dtype is torch.float32 and sin.dtype is torch.float32 and cos.ndim == 2
-            and sin.shape == cos.shape and cos.is_contiguous() and sin.is_contiguous()):
+            and sin.get_device() == index and cos.dtype is torch.float32 and sin.dtype is torch.float32
+            and len(angles) == 2 and sin.shape == angles and cos.is_contiguous() and sin.is_contiguous()):
         for name, t in (("cos", cos), ("sin", sin)):
             _check_cuda(name, t, torch.float32, 2, k.device)
         raise RuntimeError(f"{who}: cos and sin must have one shape")
-    positions, half = cos.shape
+    positions, half = angles
     starts = None
     if query_start is not None:
         _check_cuda("query_start", query_start, torch.int32, 1, k.device)
-        if query_start.size(0) != batch + 1:
+        if query_start.numel() != batch + 1:
             raise RuntimeError(f"{who}: query_start must hold batch + 1 entries")
         starts = query_start.data_ptr()
     q_heads = zero = 0
@@ -2228,17 +2235,14 @@ def rotary_append_paged(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor
     qs = qos = _NO_STRIDES
     if q is not None:
         given = q
-        q, qs = _heads(who, "q", q, dt, index, dim)
-        if q.size(0) != tokens:
+        q, shape, qs = _heads(who, "q", q, dt, index, dim)
+        q_tokens, q_heads, _ = shape
+        if q_tokens != tokens:
             raise RuntimeError(f"{who}: q, k and v must have one number of tokens")
-        q_heads = q.size(1)
-        if q_out is None:
-            zero, q_out = 1, torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=dt, device=q.device)
-            qos = q_out.stride()
-        elif q_out is given and q is not given:
+        if q_out is given and q is not given:
             raise RuntimeError(f"{who}: q_out must have 16-byte-aligned contiguous rows")
-        else:
-            qos = _heads_out(who, "q_out", q_out, q, dt, index)
+        zero = int(q_out is None)
+        q_out, qos = _heads_out(who, "q_out", q_out, q, shape, qs, dt, index)
         q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise RuntimeError(f"{who}: q_out needs q")
@@ -2268,21 +2272,17 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     index, dt = q.get_device(), q.dtype
     cache, (batch, max_pages, page, heads, dim) = _paged_cache(who, k_cache, v_cache, block_table, seq_lens, k_scale,
                                                                v_scale, index)
-    q, qs = _heads(who, "q", q, dt, index, dim)
+    q, shape, qs = _heads(who, "q", q, dt, index, dim)
     if q.requires_grad:
         _refuse_gradient(who)
-    if q.size(0) != batch:
+    tokens, q_heads, _ = shape
+    if tokens != batch:
         raise RuntimeError(f"{who}: q must hold one token for each row of block_table")
-    if out is None:
-        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, dtype=dt, device=q.device)
-        outs = out.stride()
-    else:
-        outs = _heads_out(who, "out", out, q, dt, index)
+    out, outs = _heads_out(who, "out", out, q, shape, qs, dt, index)
     if not 0 <= window <= _INT32_MAX:
         if window < 0:
             raise RuntimeError(f"{who}: negative window")
         window = _INT32_MAX  # no sequence is longer
-    q_heads = q.size(1)
     lib = _lib.load()
     need = lib.tris_paged_attention_workspace_bytes(batch, q_heads, heads, dim, max_pages, page)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # of this call alone
