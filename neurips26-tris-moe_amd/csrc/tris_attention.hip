@@ -24,9 +24,8 @@
 // One MI355X reads 6.2 TB/s; 131072 tokens with 4 kv heads of 128 (268 MB) take 46.5 + 4.5 us, 64 sequences of 4000 to
 // 8192 tokens on an e4m3 cache (792 MB) 138 + 4.9, 32 of 300 to 6000 in a window of 4096 with 16 kv heads (473 MB) 79 + 4.6.
 // Below some 50 MB the way to the first rows (length, page, row: three memory latencies) and the second launch bound it:
-// 1000 tokens, 8 kv heads (4 MB) 6.9 + 3.4 us.  A
-// (sequence, head group) that one workgroup has whole is written at once; the pieces of one that several share leave
-// fp32 sums in the workspace, and a second launch joins them.
+// 1000 tokens, 8 kv heads (4 MB) 6.9 + 3.4 us.  A (sequence, head group) that one workgroup has whole is written at once;
+// the pieces of one that several share leave fp32 sums in the workspace, and a second launch joins them.
 #include <algorithm>
 
 #include "tris_paged.h"
@@ -618,7 +617,8 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
       at += span - from;
       continue;
     }
-    if (a.owners != nullptr && from == 0 && thread == 0) a.owners[b * head_groups + hg] = make_int2(w, st.line.owner(at + tiles - 1));
+    if (a.owners != nullptr && from == 0 && thread == 0)
+      a.owners[b * head_groups + hg] = make_int2(w, st.line.owner(at + tiles - 1));
     const int count = min(tiles - from, stop - at), t0 = first / kTileKeys + from;
     // a piece that begins its (sequence, head group) and is not all of it ends its workgroup's stretch: the second slot
     const Piece p{b, n, first, hg, t0, t0 + count, at, 2 * w + (from == 0), count == tiles};

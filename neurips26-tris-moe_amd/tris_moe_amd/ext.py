@@ -2264,8 +2264,8 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
 
     q [batch, q_heads, head_dim] fp16 or bf16, q_heads a multiple of kv_heads (query head h reads kv head
     h // (q_heads / kv_heads)); the cache, block_table, seq_lens and scales as rotary_append_paged takes them.  An
-    idle sequence (length 0) gives zeros; slots outside a sequence may hold anything.  out may be q.  The launch depends on no value
-    on the device, so a captured call may be replayed with other lengths and tables.  No gradient."""
+    idle sequence (length 0) gives zeros; slots outside a sequence may hold anything.  out may be q.  The launch depends
+    on no value on the device, so a captured call may be replayed with other lengths and tables.  No gradient."""
     who = "paged_attention_decode"
     if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dtype in _ACT_DTYPES):
         _check_on(who, "q", q, 3, _ACT_DTYPES)
