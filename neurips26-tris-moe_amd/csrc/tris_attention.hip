@@ -21,10 +21,10 @@
 // block table is narrow there is no line: each workgroup has a (sequence, head group), in one launch.)
 //
 // Bound by memory: a (key, kv head) is 4 head_dim bytes in 16 bits and 4 flops a byte for each query head of the group.
-// One MI355X reads 6.2 TB/s; 131072 tokens with 4 kv heads of 128 (268 MB) take 46.5 + 4.5 us, 64 sequences of 4000 to
-// 8192 tokens on an e4m3 cache (792 MB) 138 + 4.9, 32 of 300 to 6000 in a window of 4096 with 16 kv heads (473 MB) 79 + 4.6.
+// One MI355X reads 6.2 TB/s; 131072 tokens with 4 kv heads of 128 (268 MB) take 46.0 + 4.7 us, 64 sequences of 4000 to
+// 8192 tokens on an e4m3 cache (792 MB) 136 + 4.8, 32 of 300 to 6000 in a window of 4096 with 16 kv heads (473 MB) 78 + 4.6.
 // Below some 50 MB the way to the first rows (length, page, row: three memory latencies) and the second launch bound it:
-// 1000 tokens, 8 kv heads (4 MB) 6.9 + 3.4 us.  A (sequence, head group) that one workgroup has whole is written at once;
+// 1000 tokens, 8 kv heads (4 MB) 6.2 + 3.5 us.  A (sequence, head group) that one workgroup has whole is written at once;
 // the pieces of one that several share leave fp32 sums in the workspace, and a second launch joins them.
 #include <algorithm>
 
