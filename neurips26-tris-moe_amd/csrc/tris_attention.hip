@@ -501,7 +501,8 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int k = j / 4 * 16 + g * 4 + j % 4;
-        valid[j] = key0 + k >= first && key0 + k < n && (kWhole ? cur.id[j / 4] : __shfl(cur.id[0], k)) >= 0;
+        const int id = kWhole ? cur.id[j / 4] : __shfl(cur.id[0], k);  // (from any lane: before the lane's own test)
+        valid[j] = key0 + k >= first && key0 + k < n && id >= 0;
         x[j] = valid[j] ? x[j] : -INFINITY;
       }
     }

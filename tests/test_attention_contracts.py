@@ -1,8 +1,10 @@
-"""What the append and the paged attention promise at their borders: the weights' bits."""
+"""What the append and the paged attention promise at their borders: the weights' bits, invalid pages beside a sequence's
+end and a window's beginning."""
 import pytest
 import torch
 
 from paged_cases import E4M3
+from test_paged_attention import _case, _check
 
 F16, BF16 = torch.float16, torch.bfloat16
 
@@ -47,3 +49,60 @@ def test_weights_keep_their_bits(tris, cuda, types, page):
     bound = half * rest.abs() + 41 * u * size + (2.0 ** -25 if dtype == F16 else 1e-38)
     worst = ((got - rest).abs() / bound).max().item()
     assert worst <= 1.0, f"off by {worst:.3f} of the bound"
+
+
+def _free_first_page(a, fill):
+    """Moves the sequences off page 0, which then holds `fill`: nothing may read it."""
+    table, pages = a["block_table"], a["k_cache"].shape[0]
+    spare = next(p for p in range(1, pages) if not bool((table == p).any()))
+    for name in ("k_cache", "v_cache", "k_scale", "v_scale"):
+        t = a[name]
+        if t is None:
+            continue
+        raw = t.view(torch.uint8) if t.dtype == E4M3 else t
+        raw[spare] = raw[0]
+        t[0].copy_(torch.full(t[0].shape, fill).to(t.dtype))
+    table[table == 0] = spare
+
+
+def _without_pages(tris, a, lengths, bad, page, window=0):
+    """Attention with the table's entries (sequence, index) in `bad` outside the pool."""
+    keep = [torch.ones(n, dtype=torch.bool) for n in lengths]
+    for i, (b, p) in enumerate(bad):
+        a["block_table"][b, p] = (-1, a["k_cache"].shape[0], 2 ** 31 - 1)[i % 3]
+        keep[b][p * page: (p + 1) * page] = False
+    got = tris["ext"].paged_attention_decode(**a, window=window)
+    a["block_table"] = a["block_table"].clamp(0, a["k_cache"].shape[0] - 1)   # only for the host's gather
+    _check(a, lengths, got, window=window, keep=keep)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", [(F16, F16), (BF16, BF16), (BF16, E4M3)], ids=str)
+@pytest.mark.parametrize("fill", [float("nan"), 1.0])
+@pytest.mark.parametrize("page", [10, 7, 3, 16])
+def test_invalid_pages_at_a_sequences_end(tris, cuda, types, fill, page):
+    """The last page, or every page, of sequences that end anywhere in a tile of 32 keys."""
+    lengths = list(range(17, 25)) + [50, 52, 55, 31, 33, 5]
+    for every in (False, True):
+        a = _case(cuda, 4, 2, 64, *types, page, lengths, seed=page)
+        _free_first_page(a, fill)
+        if types[1] == E4M3 and page == 16:           # scales that cannot be read four at a time
+            for name in ("k_scale", "v_scale"):
+                flat = torch.empty(a[name].numel() + 1, device=cuda)[1:]
+                a[name] = flat.view(a[name].shape).copy_(a[name])
+        last = [-(-n // page) - 1 for n in lengths]
+        bad = [(b, p) for b, top in enumerate(last) for p in (range(top + 1) if every else [top])]
+        _without_pages(tris, a, lengths, bad, page)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("types", [(F16, F16), (BF16, E4M3)], ids=str)
+@pytest.mark.parametrize("fill", [float("nan"), 1.0])
+@pytest.mark.parametrize("page", [10, 7, 16])
+def test_invalid_pages_where_a_window_begins(tris, cuda, types, fill, page):
+    lengths = [60, 64, 95, 200, 41]
+    for window in (3, 17, 25, 30):
+        a = _case(cuda, 4, 2, 64, *types, page, lengths, seed=window)
+        _free_first_page(a, fill)
+        bad = [(b, min((n - window) // page + 1, (n - 1) // page)) for b, n in enumerate(lengths)]
+        _without_pages(tris, a, lengths, bad, page, window)
