@@ -200,9 +200,59 @@ struct Piece {
 
 constexpr bool query_in_lds(int head_dim) { return head_dim == 256; }
 
+// element i of a row of 16-bit or e4m3 values
+template <bool kBf16, bool kE4m3>
+__device__ __forceinline__ float element(const void* rows, int64_t i) {
+  if constexpr (kE4m3) return __builtin_amdgcn_cvt_f32_fp8(static_cast<const uint8_t*>(rows)[i], 0);
+  else return load1(rows, i, kBf16 ? TRIS_DTYPE_BF16 : TRIS_DTYPE_F16);
+}
+
+// What a piece's sums at dimensions d and d + 1 are where they came out as NaN and the sum of its weights is a number
+// above zero: a weight's 16-bit part that is zero has made an infinite value NaN.  By the formula every finite score has a
+// weight above zero, so that the sum is infinite with the sign of its infinite values; NaN if they have both, if one has
+// a score of -infinity, or if a value is NaN itself.  (Such a score shows in the key alone: with an infinity or NaN in
+// the query no score is finite, and a score of infinity or NaN is one of the sum too.)  131072 tokens with one row of
+// infinities: the call 142 us, 50 without.  Calls without any pay 0 to 2 % (8.7 / 8.9 us for 1000 tokens in a graph,
+// 52.1 / 52.5 for 128k); a second pass over the tiles with all operands in registers cost them 1 to 5 %.
+template <int kDim, bool kBf16, bool kE4m3>
+__device__ __forceinline__ float2 infinite_sums(const AttentionArgs& a, const Piece& p, int kvh, int d) {
+  const auto& c = a.c;
+  const int32_t* table = c.block_table + p.b * c.table_stride;
+  bool up[2] = {false, false}, down[2] = {false, false}, nan[2] = {false, false};
+#pragma unroll 1
+  for (int key = max(p.first, p.t0 * kTileKeys), end = min(p.n, p.t1 * kTileKeys); key < end; ++key) {
+    const int i = a.page_of(key), slot = key - i * c.page_size;
+    const int64_t page = table[i];
+    if (page < 0 || page >= c.num_pages) continue;
+    const int64_t at = page * c.v_page_stride + kvh * c.v_head_stride + slot * c.v_slot_stride + d;
+    float scale = 1.0f;
+    if constexpr (kE4m3)
+      scale = c.v_scale[page * c.v_scale_page_stride + kvh * c.v_scale_head_stride + slot * c.v_scale_slot_stride];
+    const float v[2] = {element<kBf16, kE4m3>(c.v, at) * scale, element<kBf16, kE4m3>(c.v, at + 1) * scale};
+    if (fabsf(v[0]) < INFINITY && fabsf(v[1]) < INFINITY) continue;
+    bool finite = true;
+    if constexpr (kE4m3) {
+      finite = fabsf(c.k_scale[page * c.k_scale_page_stride + kvh * c.k_scale_head_stride +
+                               slot * c.k_scale_slot_stride]) < INFINITY;
+    } else {
+      const int64_t row = page * c.k_page_stride + kvh * c.k_head_stride + slot * c.k_slot_stride;
+#pragma unroll 1
+      for (int e = 0; e < kDim; ++e) finite &= fabsf(element<kBf16, false>(c.k, row + e)) < INFINITY;
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      up[t] |= v[t] == INFINITY;
+      down[t] |= v[t] == -INFINITY;
+      nan[t] |= v[t] != v[t] || (fabsf(v[t]) == INFINITY && !finite);
+    }
+  }
+  const auto sum = [&](int t) { return nan[t] || up[t] == down[t] ? __builtin_nanf("") : up[t] ? INFINITY : -INFINITY; };
+  return make_float2(sum(0), sum(1));
+}
+
 // The wavefronts' sums of a piece joined under the workgroup's maximum: to the output, or to the piece's slot.
 // lds: [kWaves][tile_heads][head_dim + 4] sums, then [kWaves][16] maxima and sums.
-template <int kDim, bool kBf16>
+template <int kDim, bool kBf16, bool kE4m3>
 __device__ __forceinline__ void write_piece(const AttentionArgs& a, const Piece& p, int thread, float m, float l,
                                             const f32x4* acc, float* lds) {
   constexpr int kRun = kDim < 128 ? kDim / 16 : 8;
@@ -236,6 +286,7 @@ __device__ __forceinline__ void write_piece(const AttentionArgs& a, const Piece&
   }
   __syncthreads();
   const int64_t row0 = static_cast<int64_t>(p.slot) * a.tile_heads;
+  uint32_t redo = 0;
   for (int i = thread * 2; i < heads * kDim; i += kWaves * kWave * 2) {
     const int h = i / kDim, d = i % kDim;
     float top = -INFINITY;
@@ -258,6 +309,24 @@ __device__ __forceinline__ void write_piece(const AttentionArgs& a, const Piece&
     } else {
       *reinterpret_cast<float2*>(a.part_o + (row0 + h) * kDim + d) = make_float2(y0, y1);
       if (d == 0) a.part_ml[row0 + h] = make_float2(top, sum);
+    }
+    if ((y0 != y0 || y1 != y1) && sum > 0.0f && sum < INFINITY) redo |= 1u << i / (kWaves * kWave * 2);
+  }
+  if (!__any(redo != 0)) return;
+#pragma unroll 1
+  for (int i = thread * 2; i < heads * kDim; i += kWaves * kWave * 2, redo >>= 1) {
+    if (!(redo & 1)) continue;
+    const int h = i / kDim, d = i % kDim;
+    const float2 y = infinite_sums<kDim, kBf16, kE4m3>(a, p, kvh, d);
+    if (p.whole) {
+      uint16_t* dst = a.out + p.b * a.out_seq + (kvh * a.group + head0 + h) * a.out_head + d;
+      const int32_t type = kBf16 ? TRIS_DTYPE_BF16 : TRIS_DTYPE_F16;
+      if (isnan(load1(dst, 0, type))) store1(dst, 0, y.x, type);
+      if (isnan(load1(dst, 1, type))) store1(dst, 1, y.y, type);
+    } else {
+      float* dst = a.part_o + (row0 + h) * kDim + d;
+      if (isnan(dst[0])) dst[0] = y.x;
+      if (isnan(dst[1])) dst[1] = y.y;
     }
   }
 }
@@ -591,7 +660,7 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
   }
 
   asm volatile("" : "+v"(thread));  // (what follows takes the lane's number anew too)
-  write_piece<kDim, kBf16>(a, p, thread, m, l, acc, lds);
+  write_piece<kDim, kBf16, kE4m3>(a, p, thread, m, l, acc, lds);
 }
 
 template <int kDim, bool kBf16, bool kE4m3, bool kWhole>
@@ -645,7 +714,9 @@ struct Part {
   f32x4 o;
   __device__ __forceinline__ void add(float m2, float l2, f32x4 o2) {
     const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top;
-    const float f = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
+    // (a factor is never zero, so that it leaves an infinite sum infinite; a share without keys has sums of zero)
+    const float f = fmaxf(__builtin_amdgcn_exp2f(m - base), 0x1p-126f);
+    const float f2 = fmaxf(__builtin_amdgcn_exp2f(m2 - base), 0x1p-126f);
     m = top;
     l = l * f + l2 * f2;
     o = o * f + o2 * f2;

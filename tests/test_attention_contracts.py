@@ -1,9 +1,9 @@
 """What the append and the paged attention promise at their borders: the weights' bits, invalid pages beside a sequence's
-end and a window's beginning."""
+end and a window's beginning, infinite values."""
 import pytest
 import torch
 
-from paged_cases import E4M3
+from paged_cases import E4M3, rows_of
 from test_paged_attention import _case, _check
 
 F16, BF16 = torch.float16, torch.bfloat16
@@ -106,3 +106,96 @@ def test_invalid_pages_where_a_window_begins(tris, cuda, types, fill, page):
         _free_first_page(a, fill)
         bad = [(b, min((n - window) // page + 1, (n - 1) // page)) for b, n in enumerate(lengths)]
         _without_pages(tris, a, lengths, bad, page, window)
+
+
+def _plant(a, b, h, key, column, value):
+    page = a["k_cache"].shape[2]
+    a["v_cache"][int(a["block_table"][b, key // page]), h, key % page, column] = value
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [16, 10])
+def test_infinite_values(tris, cuda, dtype, dim, page):
+    """An infinite value makes its column infinite, whatever its key's weight is (above zero for every finite score,
+    also where fp32 holds none so small): at the key with the largest weight and at that with the smallest, in sequences
+    of one token, a few, and so many that several workgroups share them; of both signs, not a number.  All else keeps
+    its bits."""
+    ext, inf = tris["ext"], float("inf")
+    lengths = [1, 40, 33, 5000]
+    a = _case(cuda, 4, 2, dim, dtype, dtype, page, lengths, seed=dim)
+    for scale in (dim ** -0.5, 0.0, 6 * dim ** -0.5, 60 * dim ** -0.5):   # the last: weights far below 2^-126
+        v = a["v_cache"].clone()
+        want = ext.paged_attention_decode(**a, scale=scale).float()
+        for b, n in enumerate(lengths):
+            k = rows_of(a["k_cache"], None, a["block_table"], b, n, page)
+            for h in range(2):
+                s = a["q"][b, 2 * h].cpu().double() @ k[h].T * scale
+                top, low = int(s.argmax()), int(s.argmin())
+                _plant(a, b, h, top, 7, inf)
+                _plant(a, b, h, low, 9, -inf)
+                _plant(a, b, h, top, 20, -inf)
+                _plant(a, b, h, 0, 21, inf)
+                _plant(a, b, h, n - 1, 21, inf if n == 1 else -inf)
+                _plant(a, b, h, n // 2, 40, float("nan"))
+                columns = (0, 1) if h == 0 else (2, 3)
+                want[b, columns, 7], want[b, columns, 9], want[b, columns, 20] = inf, -inf, -inf
+                want[b, columns, 21] = inf if n == 1 else float("nan")
+                want[b, columns, 40] = float("nan")
+        for given in (None, a["q"].clone()):              # and over the queries
+            q = a["q"] if given is None else given
+            got = ext.paged_attention_decode(**{**a, "q": q}, scale=scale, out=given).float()
+            assert torch.equal(torch.isnan(got), torch.isnan(want))
+            assert torch.equal(got[~torch.isnan(want)], want[~torch.isnan(want)])
+        a["v_cache"].copy_(v)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 10])
+def test_infinite_scales_of_an_8_bit_cache(tris, cuda, page):
+    """value = element * scale: an infinite scale makes its row's elements infinite, and zeros not a number."""
+    ext, lengths = tris["ext"], [1, 50, 4000]
+    a = _case(cuda, 4, 2, 128, BF16, E4M3, page, lengths)
+    want = ext.paged_attention_decode(**a).float()
+    for b, n in enumerate(lengths):
+        key = n // 2
+        at = int(a["block_table"][b, key // page]), 1, key % page
+        a["v_scale"][at] = float("inf")
+        a["v_cache"][at].view(torch.uint8)[5] = 0
+        want[b, 2:] = a["v_cache"][at].float() * float("inf")
+    got = ext.paged_attention_decode(**a).float()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and bool(torch.isnan(want[:, 2:, 5]).all())
+    assert torch.equal(got[~torch.isnan(want)], want[~torch.isnan(want)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 10])
+def test_infinite_values_under_special_weights(tris, cuda, page):
+    """A weight of exactly zero (a score of -infinity) or of NaN makes an infinite value NaN; keys that are left out do
+    not count, whatever they hold."""
+    ext, inf = tris["ext"], float("inf")
+    lengths = [50, 50, 50, 45]
+    a = _case(cuda, 4, 2, 64, BF16, BF16, page, lengths)
+    p = a["block_table"].cpu()
+    a["q"][0, :2] = -1.0
+    a["k_cache"][p[0, 0], 0, 1] = inf                 # key 1 of sequence 0: a score of -infinity
+    a["k_cache"][p[1, 0], 0, 1, 3] = float("nan")     # of sequence 1: NaN
+    a["k_cache"][p[2, 0], 0, 1] = inf                 # of sequence 2: +infinity
+    a["q"][2, :2] = 1.0
+    want = ext.paged_attention_decode(**a).float()
+    assert bool(torch.isfinite(want[0]).all()) and bool(torch.isnan(want[1:3, :2]).all())
+    for b in range(3):
+        _plant(a, b, 0, 1, 7, inf)
+        want[b, :2, 7] = float("nan")
+        _plant(a, b, 0, 2, 9, -inf)
+        want[b, :2, 9] = -inf if b == 0 else float("nan")
+    _plant(a, 3, 1, 0, 5, inf)                        # before a window of 40
+    for window, columns in ((0, inf), (40, None)):
+        got = ext.paged_attention_decode(**a, window=window).float()
+        if columns is None:
+            assert bool(torch.isfinite(got[3]).all())
+            continue
+        want[3, 2:, 5] = columns
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(got[~torch.isnan(want)], want[~torch.isnan(want)])
