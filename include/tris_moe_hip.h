@@ -939,7 +939,8 @@ int tris_rotary_append_paged(const void* q, int64_t q_token_stride, int64_t q_he
  *   out[b][h] = sum_j softmax_j(scale * q[b][h] . k_j) v_j,
  * scores, softmax statistics and sums in fp32, rounded once to q's type.  A sequence without keys (idle, or none of
  * its pages valid), and one whose scores are all -infinity, gives zeros.  An infinite value of a key with a finite score
- * makes its column infinite (values of both signs: NaN).  out may be q with the same strides.  Slots past the sequence's
+ * makes its column infinite (values of both signs: NaN); the weighted sums of an E4M3 cache, under weights up to one, pass
+ * fp32's range where its values come near it.  out may be q with the same strides.  Slots past the sequence's
  * end, before its window, or on invalid pages may hold anything.  q, out [batch][q_heads][head_dim] of q_type (F16 or BF16; a 16-bit cache has the same type), strides in
  * elements, rows 16-byte aligned; q_heads a multiple of kv_heads.  workspace: tris_paged_attention_workspace_bytes of
  * the same sizes (0: none needed), 16-byte aligned, no initial contents; calls that may overlap need one each.

@@ -589,10 +589,12 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
     // The probabilities enter the value product as three 16-bit parts, each what the one before left, which together
     // are their 24 bits (in fp16 down to 2^-39 of the head's largest): the result has one rounding to speak of, the
     // output's.  (Three parts / two, in a graph: 128k tokens 52.0 / 52.1 us, 32 windowed sequences 83.5 / 83.3, 64 on an
-    // e4m3 cache 142.4 / 141.6: the matrix cores wait for memory.)  In fp16 they are 2^15 times as large (the sum too, so
-    // that it cancels): a long tail far below the maximum would lose its bits to the subnormals otherwise.  An 8-bit
-    // cache's product runs in bf16, whose range takes any scale; its elements are exact in either type.
-    const float base = (m == -INFINITY ? 0.0f : m) - (kBf16V ? 0.0f : 15.0f);
+    // e4m3 cache 142.4 / 141.6: the matrix cores wait for memory.)  They are taken 2^kShift times as large, the sum too,
+    // so that it cancels: in fp16 a long tail far below the maximum would lose its bits to the subnormals otherwise, and
+    // of bf16 values near the type's largest two would pass fp32's range.  An 8-bit cache's product runs in bf16, whose
+    // range takes any scale; its elements are exact in either type, and a small scale leaves no room for a shift.
+    constexpr float kShift = kE4m3 ? 0.0f : kBf16 ? -16.0f : 15.0f;
+    const float base = (m == -INFINITY ? 0.0f : m) - kShift;
     float pr[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {

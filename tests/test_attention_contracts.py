@@ -1,5 +1,5 @@
 """What the append and the paged attention promise at their borders: the weights' bits, invalid pages beside a sequence's
-end and a window's beginning, infinite values."""
+end and a window's beginning, infinite and very large values."""
 import pytest
 import torch
 
@@ -199,3 +199,19 @@ def test_infinite_values_under_special_weights(tris, cuda, page):
         want[3, 2:, 5] = columns
         assert torch.equal(torch.isnan(got), torch.isnan(want))
         assert torch.equal(got[~torch.isnan(want)], want[~torch.isnan(want)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 10])
+def test_largest_finite_values(tris, cuda, page):
+    """Means of bf16 values near the type's largest: their weighted sum would pass fp32's range under weights up to one."""
+    lengths = [1, 2, 40, 5000]
+    a = _case(cuda, 4, 2, 128, BF16, BF16, page, lengths)
+    top = torch.finfo(BF16).max
+    v = a["v_cache"]
+    good = ~torch.isnan(v.float())
+    v[good] = (torch.rand(v.shape, device=cuda).sub_(0.5).sign_() * top).to(BF16)[good]
+    v[..., :64][good[..., :64]] = top
+    got = tris["ext"].paged_attention_decode(**a)
+    assert bool((got[..., :64] == top).all())
+    _check(a, lengths, got)
