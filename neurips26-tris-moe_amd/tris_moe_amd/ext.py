@@ -1992,7 +1992,7 @@ _DTYPE_IDS = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, to
 _ACT_DTYPES = (torch.float16, torch.bfloat16)
 _WEIGHT_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 _CACHE_DTYPES = (torch.float16, torch.bfloat16, torch.float8_e4m3fn)
-_CACHE_LAYOUT = struct.Struct("@6P13q7i")  # struct tris_paged_cache
+_CACHE_LAYOUT = struct.Struct("@6P13q7i0P")  # struct tris_paged_cache, with the padding at its end
 _NO_STRIDES = (0, 0, 0)
 _INT32_MAX = 2 ** 31 - 1
 RMS_NORM_MAX_WIDTH = 32768

@@ -1,5 +1,8 @@
 """What the append and the paged attention promise at their borders: the weights' bits, invalid pages beside a sequence's
-end and a window's beginning, infinite and very large values."""
+end and a window's beginning, infinite and very large values, the cache's descriptor."""
+import ctypes
+import struct
+
 import pytest
 import torch
 
@@ -215,3 +218,15 @@ def test_largest_finite_values(tris, cuda, page):
     got = tris["ext"].paged_attention_decode(**a)
     assert bool((got[..., :64] == top).all())
     _check(a, lengths, got)
+
+
+def test_cache_descriptor_is_the_c_struct(tris):
+    from tris_moe_amd import _lib
+
+    layout, fields = tris["ext"]._CACHE_LAYOUT, [n for n, _ in _lib.TrisPagedCache._fields_]
+    assert layout.size == ctypes.sizeof(_lib.TrisPagedCache)
+    values = [(7 * i + 3) << (20 if i < 19 else 0) for i in range(len(fields))]
+    c = _lib.TrisPagedCache.from_buffer_copy(layout.pack(*values))
+    assert [getattr(c, n) for n in fields] == values
+    with pytest.raises(struct.error):
+        layout.pack(*values[:-1], 1 << 31)
