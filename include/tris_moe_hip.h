@@ -922,7 +922,8 @@ typedef struct tris_paged_cache {
  * name the same page for a position being written race there.
  * q [tokens][q_heads][head_dim] (NULL with q_heads 0: keys and values only), k, v [tokens][kv_heads][head_dim] of
  * act_type (F16 or BF16; a 16-bit cache has the same type), strides in elements over tokens and heads, rows 16-byte
- * aligned.  rotary_dim a multiple of 16 up to head_dim; positions >= max_pages * page_size.
+ * aligned; rows of q_out, and of the cache, without shared memory.  rotary_dim a multiple of 16 up to head_dim;
+ * positions >= max_pages * page_size.
  */
 int tris_rotary_append_paged(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                              int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
@@ -938,12 +939,13 @@ int tris_rotary_append_paged(const void* q, int64_t q_token_stride, int64_t q_he
  * max(0, n - window):
  *   out[b][h] = sum_j softmax_j(scale * q[b][h] . k_j) v_j,
  * scores, softmax statistics and sums in fp32, rounded once to q's type.  A sequence without keys (idle, or none of
- * its pages valid), and one whose scores are all -infinity, gives zeros.  An infinite value of a key with a finite score
- * makes its column infinite (values of both signs: NaN); the weighted sums of an E4M3 cache, under weights up to one, pass
- * fp32's range where its values come near it.  out may be q with the same strides.  Slots past the sequence's
- * end, before its window, or on invalid pages may hold anything.  q, out [batch][q_heads][head_dim] of q_type (F16 or BF16; a 16-bit cache has the same type), strides in
- * elements, rows 16-byte aligned; q_heads a multiple of kv_heads.  workspace: tris_paged_attention_workspace_bytes of
- * the same sizes (0: none needed), 16-byte aligned, no initial contents; calls that may overlap need one each.
+ * its pages valid), and one whose scores are all -infinity, gives zeros.  An infinite value of a key with a finite
+ * score makes its column infinite (values of both signs: NaN); the weighted sums of an E4M3 cache, under weights up
+ * to one, pass fp32's range where its values come near it.  out may be q with the same strides.  Slots past the
+ * sequence's end, before its window, or on invalid pages may hold anything.  q, out [batch][q_heads][head_dim] of
+ * q_type (F16 or BF16; a 16-bit cache has the same type), strides in elements, rows 16-byte aligned, rows of out
+ * without shared memory; q_heads a multiple of kv_heads.  workspace: tris_paged_attention_workspace_bytes of the same
+ * sizes (0: none needed), 16-byte aligned, no initial contents; calls that may overlap need one each.
  */
 int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, int64_t q_head_stride, int32_t q_type,
                                 int32_t q_heads, const tris_paged_cache* cache, float scale, int32_t window, void* out,

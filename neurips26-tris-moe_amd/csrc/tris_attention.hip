@@ -876,6 +876,8 @@ extern "C" int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, 
   for (const int64_t s : {q_seq_stride, q_head_stride, out_seq_stride, out_head_stride})
     TRIS_REQUIRE(s >= 0 && s % 8 == 0, "%s: rows must be 16-byte aligned", who);
   TRIS_REQUIRE(aligned16(q) && aligned16(out), "%s: rows must be 16-byte aligned", who);
+  TRIS_REQUIRE(rows_apart<2>({{{cache->batch, out_seq_stride}, {q_heads, out_head_stride}}}, cache->head_dim),
+               "%s: output rows overlap", who);
   const int64_t rows = static_cast<int64_t>(cache->batch) * q_heads;
   const AttentionShape s =
       attention_shape(cache->batch, q_heads, cache->kv_heads, cache->head_dim, cache_positions(*cache));

@@ -206,6 +206,18 @@ extern "C" int tris_rotary_append_paged(const void* q, int64_t q_token_stride, i
                "%s: rows must be 16-byte aligned", who);
   const int64_t units = (static_cast<int64_t>(q_heads) + 2LL * cache->kv_heads) * (cache->head_dim / 16);
   TRIS_REQUIRE(units < (1 << 24), "%s: too many heads", who);
+  const tris_paged_cache& c = *cache;
+  const auto apart = [&c](int64_t page_stride, int64_t head_stride, int64_t slot_stride, int64_t row) {
+    return rows_apart<3>({{{c.num_pages, page_stride}, {c.kv_heads, head_stride}, {c.page_size, slot_stride}}}, row);
+  };
+  TRIS_REQUIRE(q_heads == 0 || rows_apart<2>({{{tokens, q_out_token_stride}, {q_heads, q_out_head_stride}}}, c.head_dim),
+               "%s: output rows overlap", who);
+  TRIS_REQUIRE(apart(c.k_page_stride, c.k_head_stride, c.k_slot_stride, c.head_dim) &&
+                   apart(c.v_page_stride, c.v_head_stride, c.v_slot_stride, c.head_dim),
+               "%s: cache rows overlap", who);
+  TRIS_REQUIRE(!c.k_scale || (apart(c.k_scale_page_stride, c.k_scale_head_stride, c.k_scale_slot_stride, 1) &&
+                              apart(c.v_scale_page_stride, c.v_scale_head_stride, c.v_scale_slot_stride, 1)),
+               "%s: cache scales overlap", who);
   const int64_t token_waves = (units + kUnits * kWave - 1) / (kUnits * kWave);
   const int64_t blocks = (tokens * token_waves + 3) / 4;
   TRIS_REQUIRE(blocks < (1LL << 32) / (4 * kWave), "%s: too many tokens", who);  // a launch has less than 2^32 threads

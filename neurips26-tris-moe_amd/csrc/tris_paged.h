@@ -1,6 +1,9 @@
 // The paged key / value cache: host checks and addressing shared by the append and the attention.
 #pragma once
 
+#include <algorithm>
+#include <array>
+
 #include "tris_dtype.h"
 
 namespace tris {
@@ -26,6 +29,23 @@ struct PageDivision {
     return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(x)) * magic) >> shift);
   }
 };
+
+// Whether rows of `dim` values over these dimensions (sizes and strides) share no memory: each dimension's stride is past
+// all that the ones of smaller strides span.
+struct RowDimension {
+  int64_t size, stride;
+};
+template <size_t kDims>
+bool rows_apart(std::array<RowDimension, kDims> dims, int64_t dim) {
+  std::sort(dims.begin(), dims.end(), [](const RowDimension& x, const RowDimension& y) { return x.stride < y.stride; });
+  __int128 span = dim;
+  for (const RowDimension& d : dims) {
+    if (d.size <= 1) continue;
+    if (d.stride < span) return false;
+    span += static_cast<__int128>(d.size - 1) * d.stride;
+  }
+  return true;
+}
 
 // The cache's own contract; `who` names the entry point in the message.
 inline int check_paged_cache(const char* who, const tris_paged_cache* c, int32_t act_type) {

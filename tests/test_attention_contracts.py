@@ -1,5 +1,5 @@
 """What the append and the paged attention promise at their borders: the weights' bits, invalid pages beside a sequence's
-end and a window's beginning, infinite and very large values, the cache's descriptor."""
+end and a window's beginning, infinite and very large values, the cache's descriptor, rows of outputs that overlap."""
 import ctypes
 import struct
 
@@ -8,6 +8,7 @@ import torch
 
 from paged_cases import E4M3, rows_of
 from test_paged_attention import _case, _check
+from test_paged_cache import _case as _append_case, c_cache
 
 F16, BF16 = torch.float16, torch.bfloat16
 
@@ -230,3 +231,72 @@ def test_cache_descriptor_is_the_c_struct(tris):
     assert [getattr(c, n) for n in fields] == values
     with pytest.raises(struct.error):
         layout.pack(*values[:-1], 1 << 31)
+
+
+def test_output_rows_that_overlap_are_refused(tris):
+    """Rows of an output that share memory would be written by several wavefronts at once."""
+    from tris_moe_amd import _lib
+
+    lib, p = _lib.load(), ctypes.c_void_p(4096)
+
+    def append(token, head, heads=4, tokens=2):
+        c = c_cache(batch=tokens)
+        return lib.tris_rotary_append_paged(p, 512, 128, p, 256, 128, p, 256, 128, 0, tokens, heads, p, p, 128, 48, None,
+                                            ctypes.byref(c), p, token, head, 0, None)
+
+    def attend(seq, head, heads=4, batch=2):
+        return lib.tris_paged_attention_decode(p, 512, 128, 0, heads, ctypes.byref(c_cache(batch=batch)), 0.1, 0, p, seq,
+                                               head, p, 1 << 40, None)
+
+    for call in (append, attend):
+        for strides in ((0, 128), (512, 0), (384, 128), (504, 128), (512, 120), (128, 248), (256, 128), (0, 0), (128, 128)):
+            assert call(*strides) == -1 and b"output rows overlap" in lib.tris_last_error(), strides
+        assert call(8, 120, 4, 1) == -1 and b"output rows overlap" in lib.tris_last_error()
+        assert call(120, 8, 2, 2) == -1 and b"output rows overlap" in lib.tris_last_error()
+
+
+def test_cache_rows_that_overlap_are_not_appended_to(tris):
+    """A cache whose heads, pages or slots share memory (an expanded pool) can be read, not written."""
+    from tris_moe_amd import _lib
+
+    lib, p = _lib.load(), ctypes.c_void_p(4096)
+
+    def append(**kw):
+        return lib.tris_rotary_append_paged(p, 512, 128, p, 256, 128, p, 256, 128, 0, 2, 4, p, p, 128, 48, None,
+                                            ctypes.byref(c_cache(**kw)), p, 512, 128, 0, None)
+
+    for kw in (dict(k_head_stride=0), dict(v_head_stride=0), dict(k_page_stride=0), dict(v_page_stride=2048),
+               dict(k_page_stride=4088), dict(v_head_stride=64)):
+        assert append(**kw) == -1 and b"cache rows overlap" in lib.tris_last_error(), kw
+    scales = dict(dtype=3, k_scale=4096, v_scale=4096)
+    for n in ("k", "v"):
+        scales.update({f"{n}_scale_page_stride": 32, f"{n}_scale_head_stride": 16, f"{n}_scale_slot_stride": 1})
+    for kw in (dict(k_scale_slot_stride=0), dict(v_scale_head_stride=0), dict(v_scale_page_stride=16)):
+        assert append(**{**scales, **kw}) == -1 and b"cache scales overlap" in lib.tris_last_error(), kw
+    # reading: refused for its window alone
+    for kw in (dict(k_head_stride=0, v_head_stride=0), dict(scales, k_scale_slot_stride=0)):
+        assert lib.tris_paged_attention_decode(p, 512, 128, 0, 4, ctypes.byref(c_cache(**kw)), 0.1, -1, p, 512, 128, p,
+                                               1 << 40, None) == -1 and b"window" in lib.tris_last_error()
+
+
+@pytest.mark.gpu
+def test_output_strides(tris, cuda):
+    """Expanded outputs are refused; ones whose heads are the outer dimension, and ones of one row, are taken."""
+    ext = tris["ext"]
+    lengths = [30, 3, 77]
+    a = _case(cuda, 4, 2, 64, F16, F16, 16, lengths)
+    want = ext.paged_attention_decode(**a)
+    new = _append_case(cuda, 4, 2, 64, 64, F16, F16, 16, [0, 4, 9], [1, 1, 1])
+    q = ext.rotary_append_paged(**new)
+    for shape, dims in (((1, 4, 64), (3, 4, 64)), ((3, 1, 64), (3, 4, 64))):
+        out = torch.zeros(shape, dtype=F16, device=cuda).expand(dims)
+        with pytest.raises(RuntimeError, match="output rows overlap"):
+            ext.paged_attention_decode(**a, out=out)
+        with pytest.raises(RuntimeError, match="output rows overlap"):
+            ext.rotary_append_paged(**new, q_out=out)
+    by_head = torch.zeros((4, 3, 64), dtype=F16, device=cuda).transpose(0, 1)
+    assert torch.equal(ext.paged_attention_decode(**a, out=by_head), want)
+    assert torch.equal(ext.rotary_append_paged(**new, q_out=by_head), q)
+    one = {**a, "q": a["q"][:1], "block_table": a["block_table"][:1], "seq_lens": a["seq_lens"][:1]}
+    out = torch.zeros((1, 4, 64), dtype=F16, device=cuda).as_strided((1, 4, 64), (0, 64, 1))
+    assert torch.equal(ext.paged_attention_decode(**one, out=out), want[:1])
