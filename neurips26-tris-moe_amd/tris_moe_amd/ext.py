@@ -23,6 +23,7 @@ import ctypes
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import TRIS_COMPACT3_KERNEL_ABI_VERSION, TrisPayload  # noqa: F401
@@ -2007,10 +2008,17 @@ def _launch(index, fn, *args):
     return fn(*args)
 
 
-def _refuse_gradient(who):
-    """These entries have no backward: an input that would need one is refused, not cut from its graph."""
+def _refuse_gradient(who, *tensors):
+    """These entries have no backward and no tangent: tensors (or None) of which one would need it, inputs, caches and
+    given outputs alike, are refused, not cut from their graph."""
     if torch.is_grad_enabled():
-        raise RuntimeError(f"{who}: no gradient is defined; call it under torch.no_grad()")
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{who}: no gradient is defined; call it under torch.no_grad()")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{who}: no gradient is defined, nor a forward-mode tangent")
 
 
 def _check_on(who, name, t, dims, dtypes, device=None):
@@ -2065,8 +2073,6 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.
             and weight.get_device() == index and weight.is_contiguous()):
         _check_on(who, "weight", weight, 1, _WEIGHT_DTYPES, x.device)
         raise RuntimeError(f"{who}: weight must be contiguous")
-    if x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad):
-        _refuse_gradient(who)
     width = weight.numel()
     if not 1 <= width <= RMS_NORM_MAX_WIDTH:
         raise RuntimeError(f"{who}: width must be 1 to {RMS_NORM_MAX_WIDTH}")
@@ -2099,6 +2105,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.
         r_ptr, ro_ptr = residual.data_ptr(), residual_out.data_ptr()
     elif residual_out is not None:
         raise RuntimeError(f"{who}: residual_out needs a residual")
+    _refuse_gradient(who, x, weight, residual, out, residual_out)
     rc = _launch(index, _lib.load().tris_rms_norm, x.data_ptr(), x_type, x_stride, r_ptr, r_type, r_stride,
                  weight.data_ptr(), _DTYPE_IDS[weight.dtype], weight_offset, eps, rows, width, out.data_ptr(), out_type,
                  out_stride, ro_ptr, ro_stride, torch._C._cuda_getCurrentRawStream(index))
@@ -2212,8 +2219,6 @@ def rotary_append_paged(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor
                                                     index)
     k, (tokens, k_heads, _), ks = _heads(who, "k", k, dt, index, dim)
     v, (v_tokens, v_heads, _), vs = _heads(who, "v", v, dt, index, dim)
-    if k.requires_grad or v.requires_grad or (q is not None and q.requires_grad):
-        _refuse_gradient(who)
     if k_heads != heads or v_heads != heads or v_tokens != tokens:
         raise RuntimeError(f"{who}: k and v must be [tokens, kv_heads, head_dim] of the cache's kv_heads")
     angles = getattr(cos, "shape", ())
@@ -2246,6 +2251,7 @@ def rotary_append_paged(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor
         q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise RuntimeError(f"{who}: q_out needs q")
+    _refuse_gradient(who, q, k, v, cos, sin, k_cache, v_cache, k_scale, v_scale, q_out)
     rc = _launch(index, _lib.load().tris_rotary_append_paged, q_ptr, qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
                  v.data_ptr(), vs[0], vs[1], _DTYPE_IDS[dt], tokens, q_heads, cos.data_ptr(), sin.data_ptr(), 2 * half,
                  positions, starts, cache, qo_ptr, qos[0], qos[1], zero, torch._C._cuda_getCurrentRawStream(index))
@@ -2273,8 +2279,6 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     cache, (batch, max_pages, page, heads, dim) = _paged_cache(who, k_cache, v_cache, block_table, seq_lens, k_scale,
                                                                v_scale, index)
     q, shape, qs = _heads(who, "q", q, dt, index, dim)
-    if q.requires_grad:
-        _refuse_gradient(who)
     tokens, q_heads, _ = shape
     if tokens != batch:
         raise RuntimeError(f"{who}: q must hold one token for each row of block_table")
@@ -2283,6 +2287,7 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         if window < 0:
             raise RuntimeError(f"{who}: negative window")
         window = _INT32_MAX  # no sequence is longer
+    _refuse_gradient(who, q, k_cache, v_cache, k_scale, v_scale, out)
     lib = _lib.load()
     need = lib.tris_paged_attention_workspace_bytes(batch, q_heads, heads, dim, max_pages, page)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # of this call alone

@@ -1,5 +1,6 @@
 """What the append and the paged attention promise at their borders: the weights' bits, invalid pages beside a sequence's
-end and a window's beginning, infinite and very large values, the cache's descriptor, rows of outputs that overlap."""
+end and a window's beginning, infinite and very large values, the cache's descriptor, rows of outputs that overlap,
+gradients (the norm's too)."""
 import ctypes
 import struct
 
@@ -300,3 +301,49 @@ def test_output_strides(tris, cuda):
     one = {**a, "q": a["q"][:1], "block_table": a["block_table"][:1], "seq_lens": a["seq_lens"][:1]}
     out = torch.zeros((1, 4, 64), dtype=F16, device=cuda).as_strided((1, 4, 64), (0, 64, 1))
     assert torch.equal(ext.paged_attention_decode(**one, out=out), want[:1])
+
+
+def test_gradients_are_refused_on_any_tensor(tris):
+    import torch.autograd.forward_ad as fwd
+
+    refuse = tris["ext"]._refuse_gradient
+    t, leaf = torch.ones(3), torch.ones(3, requires_grad=True)
+    refuse("op", t, None)
+    for tensors in ((leaf,), (t, None, leaf)):
+        with pytest.raises(RuntimeError, match="op: no gradient"):
+            refuse("op", *tensors)
+        with torch.no_grad():
+            refuse("op", *tensors)
+    with fwd.dual_level():
+        refuse("op", t, None)
+        dual = fwd.make_dual(t, torch.ones(3))
+        with pytest.raises(RuntimeError, match="op: no gradient"):
+            refuse("op", t, None, dual)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="op: no gradient"):   # tangents pass through no_grad
+            refuse("op", dual)
+
+
+@pytest.mark.gpu
+def test_calls_refuse_gradients_on_every_tensor(tris, cuda):
+    import torch.autograd.forward_ad as fwd
+
+    ext = tris["ext"]
+    x, w = torch.ones((4, 64), dtype=F16, device=cuda), torch.ones(64, dtype=F16, device=cuda)
+    norm = dict(x=x, weight=w, eps=1e-6, residual=x.clone(), out=x.clone(), residual_out=x.clone())
+    append = dict(_append_case(cuda, 4, 2, 64, 64, F16, F16, 16, [0, 3], [4, 2]))
+    append["q_out"] = torch.zeros_like(append["q"])
+    attend = _case(cuda, 4, 2, 64, F16, F16, 16, [10, 3])
+    attend["out"] = torch.zeros_like(attend["q"])
+    scaled = _case(cuda, 4, 2, 64, F16, E4M3, 16, [10, 3])
+    for call, args in ((ext.rms_norm, norm), (ext.rotary_append_paged, append), (ext.paged_attention_decode, attend),
+                       (ext.paged_attention_decode, scaled)):
+        names = [n for n, t in args.items() if isinstance(t, torch.Tensor) and t.dtype in (F16, torch.float32)]
+        assert len(names) > 3 or args is scaled
+        for n in names:
+            leaf = args[n].detach().clone().requires_grad_()
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call(**{**args, n: leaf})
+            with torch.no_grad():
+                call(**{**args, n: leaf})
+            with fwd.dual_level(), pytest.raises(RuntimeError, match="no gradient"):
+                call(**{**args, n: fwd.make_dual(args[n], torch.ones_like(args[n]))})
