@@ -70,8 +70,13 @@ inline int check_paged_cache(const char* who, const tris_paged_cache* c, int32_t
                           c->v_slot_stride})
     TRIS_REQUIRE(s >= 0 && s * size % 16 == 0, "%s: cache rows must be 16-byte aligned", who);
   TRIS_REQUIRE(aligned16(c->k) && aligned16(c->v), "%s: cache rows must be 16-byte aligned", who);
-  for (const int64_t s : {c->k_slot_stride, c->v_slot_stride, c->k_scale_slot_stride, c->v_scale_slot_stride})
-    TRIS_REQUIRE(s >= 0 && s < 2147483648LL && s * 4 * c->page_size < 2147483648LL, "%s: slot stride too large", who);
+  // (a page's bytes along its slots are int32 in the kernels)
+  const auto slots_fit = [&](int64_t stride, int bytes) {
+    return stride >= 0 && stride <= ((1LL << 31) - 1) / bytes / c->page_size;
+  };
+  TRIS_REQUIRE(slots_fit(c->k_slot_stride, size) && slots_fit(c->v_slot_stride, size) &&
+                   (!e4m3 || (slots_fit(c->k_scale_slot_stride, 4) && slots_fit(c->v_scale_slot_stride, 4))),
+               "%s: slot stride too large", who);
   TRIS_REQUIRE(c->page_size == 1 || (c->k_slot_stride >= c->head_dim && c->v_slot_stride >= c->head_dim),
                "%s: cache rows overlap", who);
   for (const int64_t s : {c->k_scale_page_stride, c->k_scale_head_stride, c->v_scale_page_stride,

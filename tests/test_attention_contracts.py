@@ -1,6 +1,6 @@
 """What the append and the paged attention promise at their borders: the weights' bits, invalid pages beside a sequence's
 end and a window's beginning, infinite and very large values, the cache's descriptor, rows of outputs that overlap,
-gradients (the norm's too)."""
+gradients (the norm's too), slot strides."""
 import ctypes
 import struct
 
@@ -347,3 +347,27 @@ def test_calls_refuse_gradients_on_every_tensor(tris, cuda):
                 call(**{**args, n: leaf})
             with fwd.dual_level(), pytest.raises(RuntimeError, match="no gradient"):
                 call(**{**args, n: fwd.make_dual(args[n], torch.ones_like(args[n]))})
+
+
+def test_slot_strides_are_bounded_in_bytes(tris):
+    """page_size * slot stride stays below 2^31 bytes, whatever the element's size; products that pass 64 bits are caught."""
+    from tris_moe_amd import _lib
+
+    lib, p = _lib.load(), ctypes.c_void_p(4096)
+
+    def call(**kw):
+        rc = lib.tris_paged_attention_decode(p, 512, 128, 0, 4, ctypes.byref(c_cache(**kw)), 0.1, -1, p, 512, 128, p, 1 << 40,
+                                             None)
+        return rc, lib.tris_last_error()      # (a negative window: nothing is launched)
+
+    e4m3 = dict(dtype=3, k_scale=4096, v_scale=4096)
+    most = (1 << 31) // 16
+    for kw in (dict(k_slot_stride=most // 2 - 8), dict(v_slot_stride=most // 2 - 8),
+               dict(e4m3, k_slot_stride=most - 16), dict(e4m3, k_scale_slot_stride=most // 4 - 1)):
+        assert call(**kw) == (-1, b"tris_paged_attention_decode: negative window"), kw
+    for kw in (dict(k_slot_stride=most // 2), dict(v_slot_stride=most // 2), dict(e4m3, v_slot_stride=most),
+               dict(e4m3, v_scale_slot_stride=most // 4), dict(k_slot_stride=1 << 40), dict(e4m3, k_scale_slot_stride=-1),
+               dict(page_size=(1 << 31) - (1 << 17), max_pages=1, k_slot_stride=(1 << 31) - 8),
+               dict(page_size=1 << 30, max_pages=1, k_slot_stride=1 << 62)):
+        rc, error = call(**kw)
+        assert rc == -1 and b"slot stride" in error, (kw, error)
