@@ -917,9 +917,9 @@ typedef struct tris_paged_cache {
  * fp32 with each product rounded, and y[i] = x[i] from rotary_dim on; values are not rotated.  q_out takes the rotated
  * queries (may be q itself with the same strides), the cache the keys and values, each rounded once.  E4M3:
  * scale = max(max_i |y[i]| * (1 / 448), 2^-126) and the element y[i] / scale rounded to nearest even; a row with an
- * infinity or NaN is stored as NaN.  Tokens past query_start[batch], and those of a negative position, are not
- * stored; their rows of q_out are left as they were, or set to zero with zero_unplaced.  Two sequences whose tables
- * name the same page for a position being written race there.
+ * infinity or NaN is stored as NaN.  Tokens past query_start[batch], and those of a position below zero or past the
+ * table's, are not stored; their rows of q_out are left as they were, or set to zero with zero_unplaced.  Two
+ * sequences whose tables name the same page for a position being written race there.
  * q [tokens][q_heads][head_dim] (NULL with q_heads 0: keys and values only), k, v [tokens][kv_heads][head_dim] of
  * act_type (F16 or BF16; a 16-bit cache has the same type), strides in elements over tokens and heads, rows 16-byte
  * aligned; rows of q_out, and of the cache, without shared memory.  rotary_dim a multiple of 16 up to head_dim;

@@ -13,7 +13,8 @@
 //                                 operand wants eight keys of one dimension in a lane; it loads eight keys' rows, a
 //                                 run of eight dimensions each, and turns that 8 x 8 block with one v_perm_b32 a word:
 //                                 product m of eight takes the m-th dimension of every lane's run.
-// No operand goes through LDS, the statistics of a head stay in its lanes, and rescaling is a product in a lane.
+// No operand but the query at 256 dimensions goes through LDS, the statistics of a head stay in its lanes, and rescaling
+// is a product in a lane.
 //
 // The work is split over the length: the tiles of all sequences and head groups form one line, and each workgroup takes
 // an equal stretch of it, so that a long sequence beside short ones is shared by the whole GPU and all workgroups end
@@ -21,11 +22,17 @@
 // block table is narrow there is no line: each workgroup has a (sequence, head group), in one launch.)
 //
 // Bound by memory: a (key, kv head) is 4 head_dim bytes in 16 bits and 4 flops a byte for each query head of the group.
-// One MI355X reads 6.2 TB/s; 131072 tokens with 4 kv heads of 128 (268 MB) take 46.0 + 4.7 us, 64 sequences of 4000 to
-// 8192 tokens on an e4m3 cache (792 MB) 136 + 4.8, 32 of 300 to 6000 in a window of 4096 with 16 kv heads (473 MB) 78 + 4.6.
-// Below some 50 MB the way to the first rows (length, page, row: three memory latencies) and the second launch bound it:
-// 1000 tokens, 8 kv heads (4 MB) 6.2 + 3.5 us.  A (sequence, head group) that one workgroup has whole is written at once;
-// the pieces of one that several share leave fp32 sums in the workspace, and a second launch joins them.
+// One MI355X reads 6.2 TB/s; 131072 tokens with 4 kv heads of 128 (268 MB) take 45.5 + 4.7 us, 64 sequences of 4000 to
+// 8192 tokens on an e4m3 cache (792 MB) 137 + 5.2, 32 of 300 to 6000 in a window of 4096 with 16 kv heads (473 MB) 78 +
+// 4.7. Below some 50 MB the way to the first rows (length, page, row: three memory latencies) and the second launch
+// bound it: 1000 tokens, 8 kv heads (4 MB) 6.6 + 3.3 us.  More than 16 query heads of a kv head read its rows once for
+// each 16: 16 sequences of 32768 with one kv head 56 us for 16 heads, 94 for 20.  A (sequence, head group) that one
+// workgroup has whole is written at once; the pieces of one that several share leave fp32 sums in the workspace, and a
+// second launch joins them.
+//
+// Times beside the choices below are of whole calls, kernels and join, in a graph over three states: "128k" and the
+// others are the calls named here, "ragged" is 16 sequences of 20 to 8000 tokens on fp16, "wide" 8 of 1000 to 16000 with
+// 256 dimensions and pages of 20.
 #include <algorithm>
 
 #include "tris_paged.h"
@@ -37,12 +44,12 @@ constexpr int kWaves = 4;          // wavefronts of a workgroup, taking its tile
 constexpr int kHeadTile = 16;      // query heads of a workgroup
 constexpr int kCus = 256;
 // Wavefronts a SIMD, and so workgroups a CU, that a head dimension's registers leave room for; a grid of as many runs in
-// one go (half as many / twice as many: 128k tokens 62 / 58 against 54 us, 32 windowed sequences 100 / 87 against 84).
+// one go (half as many / as many / twice: 128k 56.3 / 50.9 / 53.6 us, 64 on e4m3 163 / 138 / 142, windowed 99 / 83 / 83,
+// ragged 26.5 / 24.2 / 28.2, wide 29.3 / 30.0 / 40.2).
 __host__ __device__ constexpr int resident(int head_dim) { return head_dim == 64 ? 4 : head_dim == 128 ? 3 : 2; }
-// Cache policy of the rows, which are read once: non-temporal.  In a graph over four states, cached against not: 128k
-// tokens 59.6 / 52.4 us, 32 windowed sequences 94.5 / 83.5, 64 on an e4m3 cache 156 / 144, 16 ragged ones 25.9 / 25.7.
-// Where each lane has its row's address, a key row's quarters come by different instructions and may lie across lines:
-// there the keys are cached, the values not (pages of 20, head_dim 256: 31.0 with both cached, 33.8 with neither, 29.1).
+// Cache policy of the rows, which are read once: non-temporal (cached / not: 128k 57.2 / 50.9 us, windowed 92.9 / 83.8, 64
+// on e4m3 152 / 138, ragged 23.6 / 24.2).  Where each lane has its row's address, a key row's quarters come by different
+// instructions and may lie across lines: there the keys are cached (wide: 30.0, not cached 33.6), the values not (30.1).
 constexpr int kLoadOnce = 2;
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -92,8 +99,8 @@ __device__ __forceinline__ int range_tiles(int n, int first) {
 // places for what a piece costs whatever its length (its query, the first rows' way from memory, the sums' way out), so
 // that a stretch of short sequences is a short one.  Of `total` places workgroup w of `shares` has
 // [start(w), start(w + 1)), equal to within one.
-// (0, 2, 4, 8, 12 places: 16 ragged sequences 41.3, 28.2, 26.1, 26.0, 27.4 us, 32 windowed ones 86.5, 84.3, 84.0, 86.0,
-// 88.5; one or 64 long ones do not care.)
+// (0, 2, 4, 8, 12 places: ragged 38.1, 26.5, 24.2, 24.8, 25.8 us, wide 35.1, 31.3, 30.0, 29.3, 29.3, windowed 81 to 86
+// without an order; one or 64 long ones do not care.)
 constexpr int kPieceCost = 4;
 
 typedef const __attribute__((address_space(4))) AttentionArgs* KernelArgs;
@@ -155,7 +162,7 @@ __device__ __forceinline__ bool line_stretch(const AttentionArgs& a, int head_gr
 }
 
 // Without a line: workgroup w has one (sequence, head group), all of it.
-__device__ __forceinline__ bool whole_stretch(const AttentionArgs& a, int head_groups, int w, Stretch* s) {
+__device__ __forceinline__ bool own_stretch(const AttentionArgs& a, int head_groups, int w, Stretch* s) {
   s->b = w / head_groups;
   s->n = uniform(sequence_length(a, s->b));
   const int tiles = range_tiles(s->n, range_begin(a, s->n));
@@ -331,11 +338,11 @@ __device__ __forceinline__ void write_piece(const AttentionArgs& a, const Piece&
   }
 }
 
-// kWhole: every 16 keys of a tile lie in one page (page_size a multiple of 16; with e4m3, scale rows that can be read
+// kRowRuns: every 16 keys of a tile lie in one page (page_size a multiple of 16; with e4m3, scale rows that can be read
 // four at a time), so that page numbers and row addresses are the same for the whole wavefront; else each lane looks
-// up one key and hands its rows' addresses around (of the same calls, whole / by lanes: 52.4 / 57.1, 83.5 / 91.3,
-// 144 / 147 and 25.7 / 26.5 us).
-template <int kDim, bool kBf16, bool kE4m3, bool kWhole>
+// up one key and hands its rows' addresses around (of the same calls, with runs / by lanes: 128k 50.9 / 55.5 us, windowed
+// 83.8 / 86.4, 64 on e4m3 138 / 139, ragged 24.2 / 25.4).
+template <int kDim, bool kBf16, bool kE4m3, bool kRowRuns>
 __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece& p, int thread, u32x4 (*sh_q)[kWave],
                                              float* lds) {
   constexpr bool kBf16V = kBf16 || kE4m3;           // type of the value product (see the probabilities below)
@@ -357,8 +364,8 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
   const int ks_slot = static_cast<int>(a.c.k_scale_slot_stride) * 4, vs_slot = static_cast<int>(a.c.v_scale_slot_stride) * 4;
 
   // The query operand: head col, the dimensions that the K operand's lane has.  At 256 dimensions it would push the
-  // tiles' loads out of the registers (it is 32 of them), so there it stays in LDS, read when it is used (8 ragged
-  // sequences of up to 16000: 31.0 us, 39.4 with it in registers; at 128 dimensions both ways take the same time).
+  // tiles' loads out of the registers (it is 32 of them), so there it stays in LDS, read when it is used (wide: 30.0
+  // us, 36.2 with it in registers; at 128 dimensions both ways take the same time).
   u32x4 q[kQueryInLds ? 1 : kDim / 32];
   const auto query = [&](int i) {
     const int d = kE4m3 ? (i / 2) * 64 + g * 16 + (i % 2) * 8 : i * 32 + g * 8;
@@ -381,13 +388,13 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
   // wavefronts take the workgroup's tiles in turn, also over the pieces
   int tile = p.t0 + ((wave - p.at) & (kWaves - 1));
 
-  // Page numbers run ahead of the rows, so that no row waits for its page: whole, lane 2 i + t holds the block table's
-  // entry of half t of the wavefront's i-th tile from `ids0`, 32 tiles a load and the next 32 behind them; else lane
+  // Page numbers run ahead of the rows, so that no row waits for its page: with kRowRuns lane 2 i + t holds the block
+  // table's entry of half t of the wavefront's i-th tile from `ids0`, 32 tiles a load and the next 32 behind them; else lane
   // 32 i + k that of key k of the next tile.  Entries past the table's end read its last one; all are checked where
   // they are used.
   const auto entry = [&](int key) { return table[min(a.page_of(key), a.c.max_pages - 1)]; };
   const auto fetch_ids = [&](int from) {
-    if constexpr (kWhole) return entry((from + lane / 2 * kWaves) * kTileKeys + lane % 2 * 16);
+    if constexpr (kRowRuns) return entry((from + lane / 2 * kWaves) * kTileKeys + lane % 2 * 16);
     else return entry(from * kTileKeys + lane % kTileKeys);
   };
   // the pages of one tile: of its halves, or of the key that the lane looked up, -1 where there is none; and of that
@@ -402,7 +409,7 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
   };
   const auto pages_of = [&](int of_tile, int ids, int i) {
     Pages pg;
-    if constexpr (kWhole) {
+    if constexpr (kRowRuns) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
         pg.id[t] = checked(of_tile * kTileKeys + t * 16, __builtin_amdgcn_readlane(ids, 2 * i + t), of_tile);
@@ -419,7 +426,7 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
     }
     return pg;
   };
-  // Whole: one half's 16 rows as a buffer that ends with the sequence, empty without a page or past the workgroup's
+  // With kRowRuns: one half's 16 rows as a buffer that ends with the sequence, empty without a page or past the workgroup's
   // tiles: rows outside read as zeros, without a memory access and without a branch.
   const auto half_rows = [&](const char* base, int64_t page_stride, int slot_bytes, int of_tile, const Pages& pg, int t) {
     const int key = of_tile * kTileKeys + t * 16, page = pg.id[t];
@@ -439,7 +446,7 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
   const auto load_k = [&](int tile, const Pages& pg) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      if constexpr (kWhole) {
+      if constexpr (kRowRuns) {
         const __amdgpu_buffer_rsrc_t rows = half_rows(kbase, k_page, k_slot, tile, pg, t);
 #pragma unroll
         for (int i = 0; i < kKLoads; ++i)
@@ -462,17 +469,17 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       __amdgpu_buffer_rsrc_t rows, scales;
-      if constexpr (kWhole) rows = half_rows(vbase, v_page, v_slot, tile, pg, t);
+      if constexpr (kRowRuns) rows = half_rows(vbase, v_page, v_slot, tile, pg, t);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int j = t * 4 + r;
         const char* row = vbase;
-        if constexpr (!kWhole) row += of_key(pg.v, t * 16 + g * 4 + r);
+        if constexpr (!kRowRuns) row += of_key(pg.v, t * 16 + g * 4 + r);
 #pragma unroll
         for (int c = 0; c < kRuns; ++c) {
           uint32_t* dst = vr[j] + c * kVWords;
           const int in_row = col * kRun * kSize + c * 16 * kRun * kSize;
-          if constexpr (kWhole) {
+          if constexpr (kRowRuns) {
             const int at_row = (g * 4 + r) * v_slot + in_row;
             if constexpr (kVWords == 4)
               *reinterpret_cast<u32x4*>(dst) = __builtin_amdgcn_raw_buffer_load_b128(rows, at_row, 0, kLoadOnce);
@@ -488,7 +495,7 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
           }
         }
       }
-      if constexpr (kE4m3 && kWhole) {
+      if constexpr (kE4m3 && kRowRuns) {
         scales = half_rows(vsbase, vs_page, 4, tile, pg, t);
         const u32x4 s = __builtin_amdgcn_raw_buffer_load_b128(scales, g * 16, 0, 0);
 #pragma unroll
@@ -503,20 +510,20 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
   for (int i = 0; i < kRuns * kRun; ++i) acc[i] = f32x4{0, 0, 0, 0};
 
   // A tile's keys and values are loaded while the tile before it is computed: the next tile's keys are asked for when
-  // this one's have been used, the values likewise, without a branch (past the last tile from empty buffers): behind
-  // one, the compiler waits for every load in flight before it uses the values.
+  // this one's have been used, the values likewise, without a branch (past the last tile from empty buffers, by lanes
+  // rows of page 0): behind one, the compiler waits for every load in flight before it uses the values.
   const int tile0 = tile;
   Pages cur = {}, nxt = {};
   int ids = 0, ahead = 0;
   if (tile < t_end) {
     ids = fetch_ids(tile);
-    ahead = fetch_ids(tile + (kWhole ? kWave / 2 : 1) * kWaves);
+    ahead = fetch_ids(tile + (kRowRuns ? kWave / 2 : 1) * kWaves);
     cur = pages_of(tile, ids, 0);
     load_k(tile, cur);
     load_v(tile, cur);
   }
   for (int i = 1; tile < t_end; ++i, tile += kWaves) {
-    if constexpr (kWhole) {
+    if constexpr (kRowRuns) {
       if (i % (kWave / 2) == 0) {
         ids = ahead;
         ahead = fetch_ids(tile0 + (i + kWave / 2) * kWaves);
@@ -546,7 +553,7 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
         s[t] = mfma<kBf16>(k, kQueryInLds ? sh_q[i][q_lane] : q[kQueryInLds ? 0 : i], s[t]);
       }
     }
-    if constexpr (kE4m3 && !kWhole) {
+    if constexpr (kE4m3 && !kRowRuns) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int k = j / 4 * 16 + g * 4 + j % 4;
@@ -563,14 +570,14 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
     // keys outside the sequence, before its window or without a page
     const int key0 = tile * kTileKeys;
     bool edge = key0 < first || key0 + kTileKeys > n;
-    if constexpr (kWhole) edge = edge || cur.id[0] < 0 || cur.id[1] < 0;
+    if constexpr (kRowRuns) edge = edge || cur.id[0] < 0 || cur.id[1] < 0;
     else edge = edge || __any(cur.id[0] < 0);
     bool valid[8];
     if (edge) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int k = j / 4 * 16 + g * 4 + j % 4;
-        const int id = kWhole ? cur.id[j / 4] : __shfl(cur.id[0], k);  // (from any lane: before the lane's own test)
+        const int id = kRowRuns ? cur.id[j / 4] : __shfl(cur.id[0], k);  // (from any lane: before the lane's own test)
         valid[j] = key0 + k >= first && key0 + k < n && id >= 0;
         x[j] = valid[j] ? x[j] : -INFINITY;
       }
@@ -588,8 +595,8 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
     }
     // The probabilities enter the value product as three 16-bit parts, each what the one before left, which together
     // are their 24 bits (in fp16 down to 2^-39 of the head's largest): the result has one rounding to speak of, the
-    // output's.  (Three parts / two, in a graph: 128k tokens 52.0 / 52.1 us, 32 windowed sequences 83.5 / 83.3, 64 on an
-    // e4m3 cache 142.4 / 141.6: the matrix cores wait for memory.)  They are taken 2^kShift times as large, the sum too,
+    // output's.  (Three parts / two: 128k 52.0 / 52.1 us, windowed 83.5 / 83.3, 64 on e4m3 142.4 / 141.6: the matrix
+    // cores wait for memory.)  They are taken 2^kShift times as large, the sum too,
     // so that it cancels: in fp16 a long tail far below the maximum would lose its bits to the subnormals otherwise, and
     // of bf16 values near the type's largest two would pass fp32's range.  An 8-bit cache's product runs in bf16, whose
     // range takes any scale; its elements are exact in either type, and a small scale leaves no room for a shift.
@@ -607,7 +614,7 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
       for (int j = 0; j < 8; ++j) {
         pr[j] = valid[j] ? pr[j] : 0.0f;
         // (a buffer's end has done this for rows past the sequence)
-        if (!kWhole || key0 < first) {
+        if (!kRowRuns || key0 < first) {
 #pragma unroll
           for (int i = 0; i < kRuns * kVWords; ++i) vr[j][i] = valid[j] ? vr[j][i] : 0u;
         }
@@ -665,13 +672,13 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
   write_piece<kDim, kBf16, kE4m3>(a, p, thread, m, l, acc, lds);
 }
 
-template <int kDim, bool kBf16, bool kE4m3, bool kWhole>
+template <int kDim, bool kBf16, bool kE4m3, bool kRowRuns>
 __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_decode_kernel(const AttentionArgs args) {
   __shared__ u32x4 sh_q[query_in_lds(kDim) ? kDim / 32 : 1][kWave];
   extern __shared__ float lds[];
   const int head_groups = args.c.kv_heads * args.head_tiles, w = blockIdx.x;
   Stretch st;
-  if (!(args.owners == nullptr ? whole_stretch(args, head_groups, w, &st) : line_stretch(args, head_groups, w, &st)))
+  if (!(args.owners == nullptr ? own_stretch(args, head_groups, w, &st) : line_stretch(args, head_groups, w, &st)))
     return;
   int at = st.at, begin = st.begin, b = st.b, n = st.n;
   const int stop = st.stop;
@@ -699,15 +706,15 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
     const int count = min(tiles - from, stop - at), t0 = first / kTileKeys + from;
     // a piece that begins its (sequence, head group) and is not all of it ends its workgroup's stretch: the second slot
     const Piece p{b, n, first, hg, t0, t0 + count, at, 2 * w + (from == 0), count == tiles};
-    attend_piece<kDim, kBf16, kE4m3, kWhole>(a, p, thread, sh_q, lds);
+    attend_piece<kDim, kBf16, kE4m3, kRowRuns>(a, p, thread, sh_q, lds);
     at += count;
     __syncthreads();  // the next piece's sums go where this one's are read
   }
 }
 
-// Pieces of a (sequence, head group) on average, from which a join takes 16 or 4 wavefronts for the same dimensions
-// (192 pieces, 16 together: 4.5 us, an earlier form with 32 pieces at a time 5.9; 32 pieces, 4 together: the call 31.0
-// us, 16 together 34.5; 12 pieces, 1 / 4 together: 9.05 / 9.4; 1.5 pieces: the call 144 either way, 151 with 4 from 1).
+// Pieces of a (sequence, head group) on average, from which a join takes 16 or 4 wavefronts for the same dimensions (16 /
+// 4 / 1 together: 192 pieces, 128k, 50.8 / 51.0 / 54.4 us; 32 pieces, wide, 33.0 / 30.0 / 30.7; 9 pieces, 1000 tokens,
+// 9.7 / 9.4 / 9.1; 6 pieces, ragged, 30.6 / 24.5 / 24.2; 1.5 pieces, 64 on e4m3, 177 / 145 / 138).
 constexpr int kJoinMany = 64, kJoinSome = 16;
 
 // A lane's share of a join: the running maximum, sum and four dimensions' sums, and another's added to them.
@@ -785,10 +792,10 @@ __global__ __launch_bounds__(kTogether == 16 ? 1024 : 256) void attention_join_k
 // Positions times head_dim of a block table up to which a (sequence, head group) is one workgroup's: one launch, no
 // workspace, no line; twice as many where there is one for each CU.  Only the table's width is known here, not the lengths:
 // beyond, one long sequence would hold up the call.  In a graph, on the line / whole, us: one sequence of 128, 512, 1024
-// with 8 kv heads of 128: 7.0 / 4.9, 8.2 / 8.2, 8.5 / 12.4 (called eagerly 14.6 / 10.6, 14.7 / 10.5, 14.7 / 12.5); 64 of
-// 512, 1024 and 2048: 33 / 24, 51 / 45, 94 / 86; one of 128, 256 and 512 with 2 kv heads of 256: 10.5 / 8.9, 11.8 / 12.2,
-// 11.7 / 18.3.
-constexpr int64_t kWhole = 512 * 128;
+// with 8 kv heads of 128: 7.5 / 5.1, 8.6 / 8.4, 8.8 / 14.6 (called eagerly 14.1 / 10.1, 14.1 / 10.3, 14.4 / 14.5); 64 of
+// 512, 1024 and 2048: 33 / 24, 53 / 44, 95 / 83; one of 128, 256 and 512 with 2 kv heads of 256: 11.3 / 9.4, 12.3 / 11.3,
+// 12.2 / 16.1.
+constexpr int64_t kNarrow = 512 * 128;
 
 // The launch's sizes, from shapes alone.
 struct AttentionShape {
@@ -805,7 +812,7 @@ static AttentionShape attention_shape(int64_t batch, int q_heads, int kv_heads, 
   const int64_t head_groups = static_cast<int64_t>(kv_heads) * s.head_tiles;
   const int64_t most = positions / kTileKeys + 2;  // of one sequence: a window may begin and end inside a tile
   s.places = batch * (most + kPieceCost) * head_groups;
-  s.line = positions * head_dim > kWhole * (batch * head_groups >= kCus ? 2 : 1);
+  s.line = positions * head_dim > kNarrow * (batch * head_groups >= kCus ? 2 : 1);
   s.workgroups = static_cast<int>(s.line ? std::min<int64_t>(kCus * resident(head_dim), (s.places + kWaves - 1) / kWaves)
                                          : std::min<int64_t>(batch * head_groups, 2147483647LL));
   return s;
@@ -826,10 +833,10 @@ static AttentionSpace attention_space(const AttentionShape& s, int64_t batch, in
 }
 
 template <int kDim, bool kBf16, bool kE4m3>
-static void attention_launch(const AttentionArgs& a, const AttentionShape& s, bool whole, hipStream_t st) {
+static void attention_launch(const AttentionArgs& a, const AttentionShape& s, bool row_runs, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(s.workgroups)), block(kWaves * kWave);
   const size_t lds = (kWaves * a.tile_heads * (kDim + 4) + 2 * kWaves * kHeadTile) * sizeof(float);
-  if (whole) hipLaunchKernelGGL((attention_decode_kernel<kDim, kBf16, kE4m3, true>), grid, block, lds, st, a);
+  if (row_runs) hipLaunchKernelGGL((attention_decode_kernel<kDim, kBf16, kE4m3, true>), grid, block, lds, st, a);
   else hipLaunchKernelGGL((attention_decode_kernel<kDim, kBf16, kE4m3, false>), grid, block, lds, st, a);
   if (!s.line) return;
   // few sequences are cut into many pieces each, many into a few
@@ -842,13 +849,13 @@ static void attention_launch(const AttentionArgs& a, const AttentionShape& s, bo
 }
 
 template <int kDim>
-static void attention_by_type(const AttentionArgs& a, const AttentionShape& s, bool bf16, bool whole, hipStream_t st) {
+static void attention_by_type(const AttentionArgs& a, const AttentionShape& s, bool bf16, bool row_runs, hipStream_t st) {
   if (a.c.dtype == TRIS_DTYPE_E4M3) {
-    if (bf16) attention_launch<kDim, true, true>(a, s, whole, st);
-    else attention_launch<kDim, false, true>(a, s, whole, st);
+    if (bf16) attention_launch<kDim, true, true>(a, s, row_runs, st);
+    else attention_launch<kDim, false, true>(a, s, row_runs, st);
   } else {
-    if (bf16) attention_launch<kDim, true, false>(a, s, whole, st);
-    else attention_launch<kDim, false, false>(a, s, whole, st);
+    if (bf16) attention_launch<kDim, true, false>(a, s, row_runs, st);
+    else attention_launch<kDim, false, false>(a, s, row_runs, st);
   }
 }
 
@@ -913,18 +920,18 @@ extern "C" int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, 
     a.part_ml = reinterpret_cast<float2*>(at + w.ml);
     a.part_o = reinterpret_cast<float*>(at + w.o);
   }
-  bool whole = cache->page_size % 16 == 0;
+  bool row_runs = cache->page_size % 16 == 0;
   if (cache->dtype == TRIS_DTYPE_E4M3) {  // four scales a load
-    whole = whole && cache->k_scale_slot_stride == 1 && cache->v_scale_slot_stride == 1 && aligned16(cache->k_scale) &&
+    row_runs = row_runs && cache->k_scale_slot_stride == 1 && cache->v_scale_slot_stride == 1 && aligned16(cache->k_scale) &&
             aligned16(cache->v_scale);
     for (const int64_t t : {cache->k_scale_page_stride, cache->k_scale_head_stride, cache->v_scale_page_stride,
                             cache->v_scale_head_stride})
-      whole = whole && t % 4 == 0;
+      row_runs = row_runs && t % 4 == 0;
   }
   const bool bf16 = q_type == TRIS_DTYPE_BF16;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (cache->head_dim == 64) attention_by_type<64>(a, s, bf16, whole, st);
-  else if (cache->head_dim == 128) attention_by_type<128>(a, s, bf16, whole, st);
-  else attention_by_type<256>(a, s, bf16, whole, st);
+  if (cache->head_dim == 64) attention_by_type<64>(a, s, bf16, row_runs, st);
+  else if (cache->head_dim == 128) attention_by_type<128>(a, s, bf16, row_runs, st);
+  else attention_by_type<256>(a, s, bf16, row_runs, st);
   return check_launch(who);
 }

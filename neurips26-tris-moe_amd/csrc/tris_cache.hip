@@ -53,7 +53,7 @@ __device__ __forceinline__ int token_sequence(const AppendArgs& a, int t, int64_
   return -1;
 }
 
-// 16 values of one row as e4m3 pairs: v / scale, round to nearest even
+// eight values of one row as e4m3: v / scale, round to nearest even
 __device__ __forceinline__ uint2 e4m3x8(const float v[8], float scale) {
   uint32_t w[2];
 #pragma unroll

@@ -55,10 +55,14 @@ __device__ __forceinline__ void store_run(void* p, int64_t at, int i, int width,
 }
 
 // kLanes threads a row, each with kChunks runs of eight columns in registers, so that a row is read once.  Up to 64
-// lanes a row a workgroup has 256 / kLanes rows and a row's sum stays in its wavefront; above, a row has the workgroup.
+// lanes a row, so to 1024 columns, a workgroup has 256 / kLanes rows and a row's sum stays in its wavefront; above, a row
+// has the workgroup.
 // Measured with the residual: 10656 x 64 and x 128, as many lanes as runs 3.06 / 3.76 us, a wavefront a row 5.25 / 5.44;
 // 4096 columns, a workgroup of 256 for 8192 rows 42.2 us and for one 2.7, a wavefront a row 44.2 and 4.4, 128 threads
-// 43.0 and 3.3; 8192 columns, 512 threads 42.1 / 2.95, 1024 44.5 / 3.05, 256 42.9 / 3.4.
+// 43.0 and 3.3; 8192 columns, 512 threads 42.1 / 2.95, 1024 44.5 / 3.05, 256 42.9 / 3.4.  1024 columns, a wavefront for
+// 8192 rows 11.2 and for one 2.5, 128 threads 12.4 and 2.35; 2048, 256 threads 23.5 and 2.4, 128 23.5 and 2.65, a wavefront
+// 23.8 and 3.4; 16384, 1024 threads for 2048 rows 45.6 and for one 3.6, 512 46.3 and 4.1; 32768, 1024 threads for 1024 rows
+// 51.8 and for one 5.1, 512 54.5 and 6.1.
 template <int kLanes, int kChunks, bool kTail>
 __global__ __launch_bounds__(kLanes > 256 ? kLanes : 256) void rms_norm_kernel(const RmsNormArgs a) {
   constexpr int kRows = kLanes <= kWave ? 256 / kLanes : 1;

@@ -32,8 +32,10 @@ def rotary_tables(rotary_dim: int, positions: int, theta: float = 10000.0, devic
 
 class PagedKVCache:
     """One layer's pool of pages: k and v [pages, kv_heads, page_size, head_dim] of dtype (float16, bfloat16, or
-    float8_e4m3fn with k_scale and v_scale fp32 [pages, kv_heads, page_size]).  Which pages a sequence has is the block
-    table's matter; a page's contents count only below the lengths given with it."""
+    float8_e4m3fn with k_scale and v_scale fp32 [pages, kv_heads, page_size]).  A 16-bit cache takes activations of
+    its own type: under ``TrisPagedAttention``, whose projections are fp16, a cache is float16 or float8_e4m3fn.
+    Which pages a sequence has is the block table's matter; a page's contents count only below the lengths given with
+    it."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.float16,
                  device="cuda"):

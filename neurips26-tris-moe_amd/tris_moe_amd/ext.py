@@ -1985,8 +1985,8 @@ def swiglu_mul(gate: torch.Tensor, up: torch.Tensor, out: torch.Tensor | None = 
 
 # ------------------------------------------------------------------ attention side of a decoder layer
 # One decode step makes a handful of these calls a layer, each a few microseconds on the GPU, so their host path is kept
-# short (measured on the host of an MI355X node, us a call: rms_norm with a residual 13.7 -> 8.7, rotary_append_paged
-# 18.7 -> 12.2, paged_attention_decode 18.7 -> 13.5 and 10.2 in one launch): each check is one condition over attribute
+# short (measured on the host of an MI355X node, us a call: rms_norm with a residual 13.7 -> 8.9, rotary_append_paged
+# 18.7 -> 12.4, paged_attention_decode 18.7 -> 14.1 and 10.1 in one launch): each check is one condition over attribute
 # reads, and a call that fails one goes through the named checks below for its message.
 _DTYPE_IDS = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32,
               torch.float8_e4m3fn: _lib.DTYPE_E4M3}
