@@ -88,7 +88,7 @@ class TrisPagedAttention(nn.Module):
         """x [tokens, heads, head_dim] under a norm of each head or of the whole row."""
         if weight is None:
             return x
-        rows = x if weight.numel() == self.head_dim else x.view(x.size(0), -1)
+        rows = x if weight.numel() == self.head_dim else x.view(x.size(0), x.size(1) * x.size(2))
         return ext.rms_norm(rows, weight, self.norm_eps).view(x.shape)
 
     @torch.no_grad()
@@ -98,7 +98,7 @@ class TrisPagedAttention(nn.Module):
         and values and returns the rotated queries [tokens, num_heads, head_dim]."""
         fused = run_compact3_qkv_block_gr_forward(self.q_proj, self.k_proj, self.v_proj, x16)
         q, k, v = fused if fused is not None else (self.q_proj(x16), self.k_proj(x16), self.v_proj(x16))
-        q, k, v = (t.view(t.size(0), -1, self.head_dim) for t in (q, k, v))
+        q, k, v = (t.view(t.size(0), t.size(1) // self.head_dim, self.head_dim) for t in (q, k, v))
         q, k = self._normed(q, self.q_norm), self._normed(k, self.k_norm)
         return cache.append(q, k, v, self.cos, self.sin, block_table, seq_lens, query_start)
 
@@ -109,7 +109,7 @@ class TrisPagedAttention(nn.Module):
         [batch, hidden]."""
         q = self.append(x16, cache, block_table, seq_lens)
         y = cache.attend(q, block_table, seq_lens, self.scale, self.window)
-        return self.o_proj(y.view(y.size(0), -1))
+        return self.o_proj(y.view(y.size(0), self.num_heads * self.head_dim))
 
 
 class TrisDecoderLayer(nn.Module):

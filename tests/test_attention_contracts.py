@@ -1,6 +1,6 @@
 """What the append and the paged attention promise at their borders: the weights' bits, invalid pages beside a sequence's
 end and a window's beginning, infinite and very large values, the cache's descriptor, rows of outputs that overlap,
-gradients (the norm's too), slot strides."""
+gradients (the norm's too), slot strides, steps without tokens."""
 import ctypes
 import struct
 
@@ -371,3 +371,24 @@ def test_slot_strides_are_bounded_in_bytes(tris):
                dict(page_size=1 << 30, max_pages=1, k_slot_stride=1 << 62)):
         rc, error = call(**kw)
         assert rc == -1 and b"slot stride" in error, (kw, error)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("norms", [None, (64, 64), (512, 128)])
+def test_steps_without_tokens(tris, cuda, norms):
+    """An empty batch, and prompts of which none has a new token, as the linears and the MoE block take them."""
+    from test_attention_layer import _layer
+    from tris_moe_amd import attention
+
+    layer = _layer(tris, cuda, 64, 31, norms)
+    cache = attention.PagedKVCache(6, 16, 2, 64, F16, cuda)
+    cache.k.fill_(3.0), cache.v.fill_(5.0)
+    table, lens = torch.zeros((2, 4), dtype=torch.int32, device=cuda), torch.full((2,), 5, dtype=torch.int32, device=cuda)
+    x = torch.zeros((0, 512), dtype=F16, device=cuda)
+    starts = torch.zeros(3, dtype=torch.int32, device=cuda)
+    assert layer.attention.append(x, cache, table, lens, starts).shape == (0, 8, 64)
+    assert layer.attention.decode(x, cache, table[:0], lens[:0]).shape == (0, 512)
+    for residual in (None, x.to(BF16)):
+        out, stream = layer.decode(x.to(BF16), residual, cache, table[:0], lens[:0])
+        assert out.shape == stream.shape == (0, 512) and out.dtype == stream.dtype == BF16
+    assert bool((cache.k == 3).all()) and bool((cache.v == 5).all())
