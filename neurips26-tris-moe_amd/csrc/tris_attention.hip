@@ -593,13 +593,13 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
 #pragma unroll
       for (int i = 0; i < kRuns * kRun; ++i) acc[i] *= f;
     }
-    // The probabilities enter the value product as three 16-bit parts, each what the one before left, which together
-    // are their 24 bits (in fp16 down to 2^-39 of the head's largest): the result has one rounding to speak of, the
-    // output's.  (Three parts / two: 128k 52.0 / 52.1 us, windowed 83.5 / 83.3, 64 on e4m3 142.4 / 141.6: the matrix
-    // cores wait for memory.)  They are taken 2^kShift times as large, the sum too,
-    // so that it cancels: in fp16 a long tail far below the maximum would lose its bits to the subnormals otherwise, and
-    // of bf16 values near the type's largest two would pass fp32's range.  An 8-bit cache's product runs in bf16, whose
-    // range takes any scale; its elements are exact in either type, and a small scale leaves no room for a shift.
+    // The probabilities enter the value product as three 16-bit parts, each what the one before left, which together are
+    // their 24 bits (in fp16 down to 2^-39 of the head's largest): the result has one rounding to speak of, the output's.
+    // (Three parts / two: 128k 52.0 / 52.1 us, windowed 83.5 / 83.3, 64 on e4m3 142.4 / 141.6: the matrix cores wait for
+    // memory.)  They are taken 2^kShift times as large, the sum too, so that it cancels: in fp16 a long tail far below
+    // the maximum would lose its bits to the subnormals otherwise, and of bf16 values near the type's largest two would
+    // pass fp32's range.  An 8-bit cache's product runs in bf16, whose range takes any scale; its elements are exact in
+    // either type, and a small scale leaves no room for a shift.
     constexpr float kShift = kE4m3 ? 0.0f : kBf16 ? -16.0f : 15.0f;
     const float base = (m == -INFINITY ? 0.0f : m) - kShift;
     float pr[8];
@@ -723,9 +723,7 @@ struct Part {
   f32x4 o;
   __device__ __forceinline__ void add(float m2, float l2, f32x4 o2) {
     const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top;
-    // (a factor is never zero, so that it leaves an infinite sum infinite; a share without keys has sums of zero)
-    const float f = fmaxf(__builtin_amdgcn_exp2f(m - base), 0x1p-126f);
-    const float f2 = fmaxf(__builtin_amdgcn_exp2f(m2 - base), 0x1p-126f);
+    const float f = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
     m = top;
     l = l * f + l2 * f2;
     o = o * f + o2 * f2;
@@ -783,6 +781,21 @@ __global__ __launch_bounds__(kTogether == 16 ? 1024 : 256) void attention_join_k
     p.across();
   }
   if (lane >= 8) return;
+  // A factor of zero has made a piece's infinite sum NaN: the weights that it stands for are above zero, so that the whole
+  // is that of the infinite sums alone.
+  const bool lost = p.o[0] != p.o[0] || p.o[1] != p.o[1] || p.o[2] != p.o[2] || p.o[3] != p.o[3];
+  if (lost && p.l > 0.0f && p.l < INFINITY) {
+    f32x4 infinite = {0, 0, 0, 0};
+#pragma unroll 1
+    for (int w = owners.x; w <= owners.y; ++w) {
+      const int64_t r = static_cast<int64_t>(2 * w + (w == owners.x)) * a.tile_heads + in;
+      const f32x4 o = *reinterpret_cast<const f32x4*>(a.part_o + r * kDim + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) infinite[i] += fabsf(o[i]) < INFINITY ? 0.0f : o[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p.o[i] = p.o[i] != p.o[i] && infinite[i] != 0.0f ? infinite[i] : p.o[i];
+  }
   const f32x4 y = p.o * (p.l == 0.0f ? 0.0f : 1.0f / p.l);
   const uint2 packed = kBf16 ? make_uint2(pack_bf16_rne(y[0], y[1]), pack_bf16_rne(y[2], y[3]))
                              : make_uint2(pack_f16_rne(y[0], y[1]), pack_f16_rne(y[2], y[3]));

@@ -392,3 +392,18 @@ def test_steps_without_tokens(tris, cuda, norms):
         out, stream = layer.decode(x.to(BF16), residual, cache, table[:0], lens[:0])
         assert out.shape == stream.shape == (0, 512) and out.dtype == stream.dtype == BF16
     assert bool((cache.k == 3).all()) and bool((cache.v == 5).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_large_values_under_vanishing_weights(tris, cuda, dim):
+    """Keys whose weights fp32 does not hold (2^-1000 and less of the others') do not count, however large their values,
+    in pieces of their own too."""
+    n, page = 6000, 16
+    a = _case(cuda, 4, 2, dim, BF16, BF16, page, [n])
+    table = a["block_table"][0].long()
+    a["q"].fill_(1.0)
+    a["k_cache"][table[: n // page]], a["v_cache"][table[: n // page]] = 0.0, 1.0
+    a["k_cache"][table[: n // 2 // page]] = -1000.0 / dim
+    a["v_cache"][table[: n // 2 // page]] = torch.finfo(BF16).max
+    assert bool((tris["ext"].paged_attention_decode(**a, scale=1.0) == 1.0).all())
