@@ -934,6 +934,26 @@ int tris_rotary_append_paged(const void* q, int64_t q_token_stride, int64_t q_he
                              void* stream);
 
 /*
+ * tris_rotary_append_paged with rotary positions of their own, one for each of 1 to TRIS_MAX_ROTARY_AXES axes (time,
+ * height and width of an image's patches; or one axis, where a token's place in the cache is no longer its position):
+ * pair i of token t is turned by row token_positions[axis(i)][t] of cos and sin, while where the token is stored goes by
+ * seq_lens as there.  sections [axes] (host memory) say how many of the rotary_dim / 2 pairs each axis has: its section
+ * of them in a row, or, interleaved, pair i has axis i % axes as long as that axis has pairs left
+ * (i / axes < sections[i % axes]), then axis 0.  token_positions [axes][tokens], rows axis_stride apart.  A token one of
+ * whose positions is outside [0, positions) is treated as one without a place: not stored, its row of q_out as
+ * zero_unplaced says.  positions >= 1 need not cover the block table.
+ */
+#define TRIS_MAX_ROTARY_AXES 4
+int tris_rotary_axes_append_paged(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                                  int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                                  int64_t v_head_stride, int32_t act_type, int32_t tokens, int32_t q_heads,
+                                  const float* cos, const float* sin, int32_t rotary_dim, int32_t positions,
+                                  const int32_t* query_start, const tris_paged_cache* cache, void* q_out,
+                                  int64_t q_out_token_stride, int64_t q_out_head_stride, int32_t zero_unplaced,
+                                  const int32_t* token_positions, int64_t axis_stride, int32_t axes,
+                                  const int32_t* sections, int32_t interleaved, void* stream);
+
+/*
  * Attention of one new token a sequence over the paged cache: with n = seq_lens[b] (cut as above), query head h of
  * sequence b reads kv head h / (q_heads / kv_heads) and keys j in [first, n), first = 0 or, with window > 0,
  * max(0, n - window):
@@ -953,6 +973,42 @@ int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, int64_t q_h
                                 int64_t workspace_bytes, void* stream);
 int64_t tris_paged_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
                                              int32_t max_pages, int32_t page_size);
+
+/*
+ * tris_paged_attention_decode that adds each key's attention weights to a running sum:
+ *   weight_sum[b][g][j] += sum over the query heads h of kv head g of softmax_j(scale * q[b][h] . k_j)
+ * for the keys j that sequence b's token attends to; the sums of all other positions, those on invalid pages among
+ * them, stay as they were.  fp32, in an order that depends on the sizes alone.  A head whose scores hold an infinity of
+ * positive sign or a NaN makes the sums of all its keys NaN, as its softmax is; one whose scores are all -infinity adds
+ * zeros.  out is tris_paged_attention_decode's.  weight_sum [batch][kv_heads][>= max_pages * page_size] fp32, strides in
+ * elements over sequences and heads, positions contiguous, rows without shared memory.  workspace:
+ * tris_paged_attention_weights_workspace_bytes, as above (the scores, 4 bytes for each query head and position of the
+ * table, among it).
+ */
+int tris_paged_attention_decode_weights(const void* q, int64_t q_seq_stride, int64_t q_head_stride, int32_t q_type,
+                                        int32_t q_heads, const tris_paged_cache* cache, float scale, int32_t window,
+                                        void* out, int64_t out_seq_stride, int64_t out_head_stride, float* weight_sum,
+                                        int64_t sum_seq_stride, int64_t sum_head_stride, void* workspace,
+                                        int64_t workspace_bytes, void* stream);
+int64_t tris_paged_attention_weights_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads,
+                                                     int32_t head_dim, int32_t max_pages, int32_t page_size);
+
+/*
+ * Eviction from the paged cache by accumulated attention weight.  A sequence of n > limit positions (n = seq_lens[b], cut
+ * as above) keeps `budget` of them, each kv head its own: the first `sink`, the last `recent`, and of those between the
+ * budget - sink - recent with the largest weight_sum (NaN above all numbers, -0 equal to 0; of equal ones the lowest
+ * position).  In order, their keys, values, scales and sums move to positions 0 .. budget - 1, the sums of positions
+ * budget .. n - 1 become zero, new_lens[b] is budget, and kept[b][g][i] is the position that i's token had.  A sequence
+ * of limit positions or fewer, and one of which a page below n is outside the pool, stays as it is: new_lens[b] is
+ * seq_lens[b], and kept[b] is -1 throughout.  The keys and values of positions budget .. n - 1 stay in the cache's memory.
+ * No page below an evicted sequence's length may be another sequence's, or its own twice.
+ * 0 <= sink, 0 <= recent, sink + recent <= budget, 1 <= budget <= limit.  weight_sum as
+ * tris_paged_attention_decode_weights takes it; new_lens [batch], apart from seq_lens; kept
+ * [batch][kv_heads][budget], contiguous.  The cache's rows, scales and sums without shared memory.
+ */
+int tris_paged_cache_evict(const tris_paged_cache* cache, float* weight_sum, int64_t sum_seq_stride,
+                           int64_t sum_head_stride, int32_t budget, int32_t limit, int32_t sink, int32_t recent,
+                           int32_t* new_lens, int32_t* kept, void* stream);
 
 #ifdef __cplusplus
 }

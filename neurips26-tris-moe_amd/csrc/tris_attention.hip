@@ -69,6 +69,12 @@ struct AttentionArgs {
   float2* part_ml;                   // [2 * workgroups][tile_heads]: maximum and sum of a piece
   float* part_o;                     // the same rows of head_dim sums
   tris_paged_cache c;
+  // of the calls that sum the weights
+  float* scores;                     // [batch][q_heads][score_row]: scale_log2 * q . k, -infinity for a key left out
+  int64_t score_row;
+  float2* whole_ml;                  // [batch][q_heads]: maximum and sum of what one workgroup had whole
+  float* weight_sum;
+  int64_t sum_seq, sum_head;
 };
 
 // a value that every lane holds alike, moved to a scalar register
@@ -257,9 +263,12 @@ __device__ __forceinline__ float2 infinite_sums(const AttentionArgs& a, const Pi
   return make_float2(sum(0), sum(1));
 }
 
+// The powers of two that the weights and their sum are taken larger by (see the probabilities below).
+__host__ __device__ constexpr float weight_shift(bool bf16, bool e4m3) { return e4m3 ? 0.0f : bf16 ? -16.0f : 15.0f; }
+
 // The wavefronts' sums of a piece joined under the workgroup's maximum: to the output, or to the piece's slot.
 // lds: [kWaves][tile_heads][head_dim + 4] sums, then [kWaves][16] maxima and sums.
-template <int kDim, bool kBf16, bool kE4m3>
+template <int kDim, bool kBf16, bool kE4m3, bool kWeights>
 __device__ __forceinline__ void write_piece(const AttentionArgs& a, const Piece& p, int thread, float m, float l,
                                             const f32x4* acc, float* lds) {
   constexpr int kRun = kDim < 128 ? kDim / 16 : 8;
@@ -310,6 +319,8 @@ __device__ __forceinline__ void write_piece(const AttentionArgs& a, const Piece&
       y1 += o[1] * f;
     }
     if (p.whole) {
+      if (kWeights && d == 0)
+        a.whole_ml[static_cast<int64_t>(p.b) * a.q_heads + kvh * a.group + head0 + h] = make_float2(top, sum);
       const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
       uint16_t* dst = a.out + p.b * a.out_seq + (kvh * a.group + head0 + h) * a.out_head + d;
       *reinterpret_cast<uint32_t*>(dst) = kBf16 ? pack_bf16_rne(y0 * f, y1 * f) : pack_f16_rne(y0 * f, y1 * f);
@@ -342,7 +353,7 @@ __device__ __forceinline__ void write_piece(const AttentionArgs& a, const Piece&
 // four at a time), so that page numbers and row addresses are the same for the whole wavefront; else each lane looks
 // up one key and hands its rows' addresses around (of the same calls, with runs / by lanes: 128k 50.9 / 55.5 us, windowed
 // 83.8 / 86.4, 64 on e4m3 138 / 139, ragged 24.2 / 25.4).
-template <int kDim, bool kBf16, bool kE4m3, bool kRowRuns>
+template <int kDim, bool kBf16, bool kE4m3, bool kRowRuns, bool kWeights>
 __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece& p, int thread, u32x4 (*sh_q)[kWave],
                                              float* lds) {
   constexpr bool kBf16V = kBf16 || kE4m3;           // type of the value product (see the probabilities below)
@@ -504,6 +515,10 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
     }
   };
 
+  float* scores = nullptr;  // of the lane's head, from its four keys on
+  if constexpr (kWeights)
+    scores = a.scores + (static_cast<int64_t>(p.b) * a.q_heads + kvh * a.group + head0 + col) * a.score_row + g * 4;
+
   float m = -INFINITY, l = 0.0f;
   f32x4 acc[kRuns * kRun];
 #pragma unroll
@@ -582,6 +597,12 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
         x[j] = valid[j] ? x[j] : -INFINITY;
       }
     }
+    if constexpr (kWeights) {
+      if (col < heads) {
+        *reinterpret_cast<f32x4*>(scores + key0) = f32x4{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<f32x4*>(scores + key0 + 16) = f32x4{x[4], x[5], x[6], x[7]};
+      }
+    }
     load_k(tile + kWaves, nxt);
 
     float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
@@ -600,7 +621,7 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
     // the maximum would lose its bits to the subnormals otherwise, and of bf16 values near the type's largest two would
     // pass fp32's range.  An 8-bit cache's product runs in bf16, whose range takes any scale; its elements are exact in
     // either type, and a small scale leaves no room for a shift.
-    constexpr float kShift = kE4m3 ? 0.0f : kBf16 ? -16.0f : 15.0f;
+    constexpr float kShift = weight_shift(kBf16, kE4m3);
     const float base = (m == -INFINITY ? 0.0f : m) - kShift;
     float pr[8];
 #pragma unroll
@@ -669,10 +690,10 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
   }
 
   asm volatile("" : "+v"(thread));  // (what follows takes the lane's number anew too)
-  write_piece<kDim, kBf16, kE4m3>(a, p, thread, m, l, acc, lds);
+  write_piece<kDim, kBf16, kE4m3, kWeights>(a, p, thread, m, l, acc, lds);
 }
 
-template <int kDim, bool kBf16, bool kE4m3, bool kRowRuns>
+template <int kDim, bool kBf16, bool kE4m3, bool kRowRuns, bool kWeights>
 __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_decode_kernel(const AttentionArgs args) {
   __shared__ u32x4 sh_q[query_in_lds(kDim) ? kDim / 32 : 1][kWave];
   extern __shared__ float lds[];
@@ -706,7 +727,7 @@ __global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_deco
     const int count = min(tiles - from, stop - at), t0 = first / kTileKeys + from;
     // a piece that begins its (sequence, head group) and is not all of it ends its workgroup's stretch: the second slot
     const Piece p{b, n, first, hg, t0, t0 + count, at, 2 * w + (from == 0), count == tiles};
-    attend_piece<kDim, kBf16, kE4m3, kRowRuns>(a, p, thread, sh_q, lds);
+    attend_piece<kDim, kBf16, kE4m3, kRowRuns, kWeights>(a, p, thread, sh_q, lds);
     at += count;
     __syncthreads();  // the next piece's sums go where this one's are read
   }
@@ -802,6 +823,80 @@ __global__ __launch_bounds__(kTogether == 16 ? 1024 : 256) void attention_join_k
   *reinterpret_cast<uint2*>(a.out + b * a.out_seq + h * a.out_head + d) = packed;
 }
 
+// Adds the keys' weights to their sums, from the scores that the attention left: a workgroup takes the stretch that the
+// workgroup of its number took there, and of its pieces those of each kv head's first head group, for all of them.
+// shift: weight_shift of the types; sums4: the sums' rows can be read four at a time.
+__global__ __launch_bounds__(kWaves * kWave) void attention_weights_kernel(const AttentionArgs a, const float shift,
+                                                                          const bool sums4) {
+  extern __shared__ float2 stats[];  // of each query head: the maximum (less the shift) and the inverse sum
+  const int head_groups = a.c.kv_heads * a.head_tiles;
+  Stretch st;
+  if (!(a.owners == nullptr ? own_stretch(a, head_groups, blockIdx.x, &st)
+                            : line_stretch(a, head_groups, blockIdx.x, &st)))
+    return;
+  const int thread = threadIdx.x, wave = uniform(thread / kWave), lane = thread % kWave;
+  int at = st.at, begin = st.begin, b = st.b, n = st.n;
+  while (at < st.stop && b < a.c.batch) {
+    const int first = range_begin(a, n), tiles = range_tiles(n, first), span = tiles + kPieceCost;
+    const int hg = (at - begin) / span, from = at - begin - hg * span;
+    if (hg == head_groups) {
+      begin = at;
+      n = uniform(sequence_length(a, ++b));
+      continue;
+    }
+    const int count = min(tiles - from, st.stop - at);
+    at += from >= tiles ? span - from : count;
+    if (from >= tiles || n == 0 || hg % a.head_tiles != 0) continue;
+    const int kvh = hg / a.head_tiles;
+    const int64_t row0 = static_cast<int64_t>(b) * a.q_heads + kvh * a.group;
+    __syncthreads();  // the piece before has read its statistics
+    for (int h = wave; h < a.group; h += kWaves) {
+      float2 ml = {-INFINITY, 0.0f};
+      const int2 own = a.owners == nullptr ? make_int2(0, 0) : a.owners[b * head_groups + hg + h / kHeadTile];
+      if (own.x == own.y) {
+        ml = a.whole_ml[row0 + h];
+      } else {
+        for (int w = own.x + lane; w <= own.y; w += kWave) {
+          const float2 part = a.part_ml[static_cast<int64_t>(2 * w + (w == own.x)) * a.tile_heads + h % kHeadTile];
+          const float top = fmaxf(ml.x, part.x), base = top == -INFINITY ? 0.0f : top;
+          ml = make_float2(top, ml.y * __builtin_amdgcn_exp2f(ml.x - base) + part.y * __builtin_amdgcn_exp2f(part.x - base));
+        }
+        const float top = wave_max_f32(ml.x), base = top == -INFINITY ? 0.0f : top;
+        ml = make_float2(top, wave_sum_f32(ml.y * __builtin_amdgcn_exp2f(ml.x - base)));
+      }
+      if (lane == 0) stats[h] = make_float2((ml.x == -INFINITY ? 0.0f : ml.x) - shift, ml.y == 0.0f ? 0.0f : 1.0f / ml.y);
+    }
+    __syncthreads();
+    const int32_t* table = a.c.block_table + b * a.c.table_stride;
+    float* sums = a.weight_sum + b * a.sum_seq + kvh * a.sum_head;
+    const float* scores = a.scores + row0 * a.score_row;
+    const int t0 = first / kTileKeys + from, end = min(n, (t0 + count) * kTileKeys);
+    for (int key = t0 * kTileKeys + thread * 4; key < end; key += kWaves * kWave * 4) {
+      f32x4 weight = {0, 0, 0, 0};
+#pragma unroll 4
+      for (int h = 0; h < a.group; ++h) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(scores + h * a.score_row + key);
+        const float2 of = stats[h];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) weight[i] += __builtin_amdgcn_exp2f(x[i] - of.x) * of.y;
+      }
+      const auto valid = [&](int k) {
+        return k >= first && k < n &&
+               static_cast<uint32_t>(table[a.page_of(k)]) < static_cast<uint32_t>(a.c.num_pages);
+      };
+      const bool use[4] = {valid(key), valid(key + 1), valid(key + 2), valid(key + 3)};
+      if (sums4 && use[0] && use[1] && use[2] && use[3]) {
+        f32x4* dst = reinterpret_cast<f32x4*>(sums + key);
+        *dst = *dst + weight;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (use[i]) sums[key + i] += weight[i];
+      }
+    }
+  }
+}
+
 // Positions times head_dim of a block table up to which a (sequence, head group) is one workgroup's: one launch, no
 // workspace, no line; twice as many where there is one for each CU.  Only the table's width is known here, not the lengths:
 // beyond, one long sequence would hold up the call.  In a graph, on the line / whole, us: one sequence of 128, 512, 1024
@@ -845,12 +940,17 @@ static AttentionSpace attention_space(const AttentionShape& s, int64_t batch, in
   return w;
 }
 
-template <int kDim, bool kBf16, bool kE4m3>
+template <int kDim, bool kBf16, bool kE4m3, bool kWeights>
 static void attention_launch(const AttentionArgs& a, const AttentionShape& s, bool row_runs, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(s.workgroups)), block(kWaves * kWave);
   const size_t lds = (kWaves * a.tile_heads * (kDim + 4) + 2 * kWaves * kHeadTile) * sizeof(float);
-  if (row_runs) hipLaunchKernelGGL((attention_decode_kernel<kDim, kBf16, kE4m3, true>), grid, block, lds, st, a);
-  else hipLaunchKernelGGL((attention_decode_kernel<kDim, kBf16, kE4m3, false>), grid, block, lds, st, a);
+  if (row_runs) hipLaunchKernelGGL((attention_decode_kernel<kDim, kBf16, kE4m3, true, kWeights>), grid, block, lds, st, a);
+  else hipLaunchKernelGGL((attention_decode_kernel<kDim, kBf16, kE4m3, false, kWeights>), grid, block, lds, st, a);
+  if constexpr (kWeights) {
+    const bool sums4 = aligned16(a.weight_sum) && a.sum_seq % 4 == 0 && a.sum_head % 4 == 0;
+    hipLaunchKernelGGL(attention_weights_kernel, grid, block, a.group * sizeof(float2), st, a, weight_shift(kBf16, kE4m3),
+                       sums4);
+  }
   if (!s.line) return;
   // few sequences are cut into many pieces each, many into a few
   const int64_t units = static_cast<int64_t>(a.c.batch) * a.q_heads * (kDim / 32);
@@ -861,33 +961,53 @@ static void attention_launch(const AttentionArgs& a, const AttentionShape& s, bo
   else hipLaunchKernelGGL((attention_join_kernel<kDim, kBf16, 1>), fourth, dim3(256), 0, st, a);
 }
 
-template <int kDim>
+template <int kDim, bool kWeights>
 static void attention_by_type(const AttentionArgs& a, const AttentionShape& s, bool bf16, bool row_runs, hipStream_t st) {
   if (a.c.dtype == TRIS_DTYPE_E4M3) {
-    if (bf16) attention_launch<kDim, true, true>(a, s, row_runs, st);
-    else attention_launch<kDim, false, true>(a, s, row_runs, st);
+    if (bf16) attention_launch<kDim, true, true, kWeights>(a, s, row_runs, st);
+    else attention_launch<kDim, false, true, kWeights>(a, s, row_runs, st);
   } else {
-    if (bf16) attention_launch<kDim, true, false>(a, s, row_runs, st);
-    else attention_launch<kDim, false, false>(a, s, row_runs, st);
+    if (bf16) attention_launch<kDim, true, false, kWeights>(a, s, row_runs, st);
+    else attention_launch<kDim, false, false, kWeights>(a, s, row_runs, st);
   }
 }
 
-}  // namespace tris
-
-using namespace tris;
-
-extern "C" int64_t tris_paged_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads,
-                                                        int32_t head_dim, int32_t max_pages, int32_t page_size) {
-  if (batch < 1 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1 || max_pages < 0 || page_size < 1) return 0;
-  const int64_t positions = static_cast<int64_t>(max_pages) * page_size;
-  return attention_space(attention_shape(batch, q_heads, kv_heads, head_dim, positions), batch, kv_heads, head_dim).bytes;
+template <bool kWeights>
+static void attention_by_dim(const AttentionArgs& a, const AttentionShape& s, bool bf16, bool row_runs, hipStream_t st) {
+  if (a.c.head_dim == 64) attention_by_type<64, kWeights>(a, s, bf16, row_runs, st);
+  else if (a.c.head_dim == 128) attention_by_type<128, kWeights>(a, s, bf16, row_runs, st);
+  else attention_by_type<256, kWeights>(a, s, bf16, row_runs, st);
 }
 
-extern "C" int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, int64_t q_head_stride, int32_t q_type,
-                                           int32_t q_heads, const tris_paged_cache* cache, float scale, int32_t window,
-                                           void* out, int64_t out_seq_stride, int64_t out_head_stride, void* workspace,
-                                           int64_t workspace_bytes, void* stream) {
-  const char* who = "tris_paged_attention_decode";
+// What the weights' sums need behind the workspace of the attention alone, in bytes from its beginning; -1: more than 2^62.
+struct WeightsSpace {
+  int64_t whole_ml, scores, score_row, bytes;
+};
+
+static WeightsSpace weights_space(const AttentionSpace& a, int64_t batch, int64_t q_heads, int64_t positions) {
+  const auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+  WeightsSpace w;
+  w.score_row = (positions + kTileKeys - 1) / kTileKeys * kTileKeys;
+  w.whole_ml = up(a.bytes);
+  w.scores = w.whole_ml + up(batch * q_heads * static_cast<int64_t>(sizeof(float2)));
+  const __int128 end = static_cast<__int128>(batch) * q_heads * w.score_row * static_cast<int64_t>(sizeof(float)) + w.scores;
+  w.bytes = end < (static_cast<__int128>(1) << 62) ? static_cast<int64_t>(end) : -1;
+  return w;
+}
+
+// Query heads of a kv head that the weights' sums take: their statistics are in LDS.
+constexpr int kMostGroup = 4096;
+
+// Where the weights are summed.
+struct WeightSums {
+  float* sums;
+  int64_t seq_stride, head_stride;
+};
+
+static int attention_decode(const char* who, const void* q, int64_t q_seq_stride, int64_t q_head_stride, int32_t q_type,
+                            int32_t q_heads, const tris_paged_cache* cache, float scale, int32_t window, void* out,
+                            int64_t out_seq_stride, int64_t out_head_stride, const WeightSums* weights, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
   if (const int rc = check_paged_cache(who, cache, q_type)) return rc;
   TRIS_REQUIRE(q_heads >= 1 && q_heads % cache->kv_heads == 0, "%s: q_heads must be a multiple of kv_heads", who);
   TRIS_REQUIRE(window >= 0, "%s: negative window", who);
@@ -898,6 +1018,11 @@ extern "C" int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, 
   TRIS_REQUIRE(aligned16(q) && aligned16(out), "%s: rows must be 16-byte aligned", who);
   TRIS_REQUIRE(rows_apart<2>({{{cache->batch, out_seq_stride}, {q_heads, out_head_stride}}}, cache->head_dim),
                "%s: output rows overlap", who);
+  if (weights) {
+    TRIS_REQUIRE(weights->sums || cache->max_pages == 0, "%s: null pointer", who);
+    TRIS_REQUIRE(sum_rows_apart(*cache, weights->seq_stride, weights->head_stride), "%s: rows of weight_sum overlap", who);
+    TRIS_REQUIRE(q_heads / cache->kv_heads <= kMostGroup, "%s: more than %d query heads for a kv head", who, kMostGroup);
+  }
   const int64_t rows = static_cast<int64_t>(cache->batch) * q_heads;
   const AttentionShape s =
       attention_shape(cache->batch, q_heads, cache->kv_heads, cache->head_dim, cache_positions(*cache));
@@ -907,8 +1032,11 @@ extern "C" int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, 
                "%s: too many rows", who);
   TRIS_REQUIRE(s.places < (1LL << 31) - (1 << 16), "%s: too many positions", who);
   const AttentionSpace w = attention_space(s, cache->batch, cache->kv_heads, cache->head_dim);
-  TRIS_REQUIRE(!s.line || (workspace && aligned16(workspace) && workspace_bytes >= w.bytes),
-               "%s: workspace of %lld bytes needed", who, static_cast<long long>(w.bytes));
+  const WeightsSpace ww = weights_space(w, cache->batch, q_heads, cache_positions(*cache));
+  const int64_t need = weights ? ww.bytes : w.bytes;
+  TRIS_REQUIRE(need >= 0, "%s: too many positions", who);
+  TRIS_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),
+               "%s: workspace of %lld bytes needed", who, static_cast<long long>(need));
   AttentionArgs a{static_cast<const uint16_t*>(q),
                   static_cast<uint16_t*>(out),
                   q_seq_stride,
@@ -926,12 +1054,26 @@ extern "C" int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, 
                   nullptr,
                   nullptr,
                   nullptr,
-                  *cache};
+                  *cache,
+                  nullptr,
+                  0,
+                  nullptr,
+                  nullptr,
+                  0,
+                  0};
+  char* at = static_cast<char*>(workspace);
   if (s.line) {
-    char* at = static_cast<char*>(workspace);
     a.owners = reinterpret_cast<int2*>(at);
     a.part_ml = reinterpret_cast<float2*>(at + w.ml);
     a.part_o = reinterpret_cast<float*>(at + w.o);
+  }
+  if (weights) {
+    a.scores = reinterpret_cast<float*>(at + ww.scores);
+    a.score_row = ww.score_row;
+    a.whole_ml = reinterpret_cast<float2*>(at + ww.whole_ml);
+    a.weight_sum = weights->sums;
+    a.sum_seq = weights->seq_stride;
+    a.sum_head = weights->head_stride;
   }
   bool row_runs = cache->page_size % 16 == 0;
   if (cache->dtype == TRIS_DTYPE_E4M3) {  // four scales a load
@@ -943,8 +1085,46 @@ extern "C" int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, 
   }
   const bool bf16 = q_type == TRIS_DTYPE_BF16;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (cache->head_dim == 64) attention_by_type<64>(a, s, bf16, row_runs, st);
-  else if (cache->head_dim == 128) attention_by_type<128>(a, s, bf16, row_runs, st);
-  else attention_by_type<256>(a, s, bf16, row_runs, st);
+  if (weights) attention_by_dim<true>(a, s, bf16, row_runs, st);
+  else attention_by_dim<false>(a, s, bf16, row_runs, st);
   return check_launch(who);
+}
+
+}  // namespace tris
+
+using namespace tris;
+
+extern "C" int64_t tris_paged_attention_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads,
+                                                        int32_t head_dim, int32_t max_pages, int32_t page_size) {
+  if (batch < 1 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1 || max_pages < 0 || page_size < 1) return 0;
+  const int64_t positions = static_cast<int64_t>(max_pages) * page_size;
+  return attention_space(attention_shape(batch, q_heads, kv_heads, head_dim, positions), batch, kv_heads, head_dim).bytes;
+}
+
+extern "C" int tris_paged_attention_decode(const void* q, int64_t q_seq_stride, int64_t q_head_stride, int32_t q_type,
+                                           int32_t q_heads, const tris_paged_cache* cache, float scale, int32_t window,
+                                           void* out, int64_t out_seq_stride, int64_t out_head_stride, void* workspace,
+                                           int64_t workspace_bytes, void* stream) {
+  return attention_decode("tris_paged_attention_decode", q, q_seq_stride, q_head_stride, q_type, q_heads, cache, scale,
+                          window, out, out_seq_stride, out_head_stride, nullptr, workspace, workspace_bytes, stream);
+}
+
+extern "C" int64_t tris_paged_attention_weights_workspace_bytes(int32_t batch, int32_t q_heads, int32_t kv_heads,
+                                                                int32_t head_dim, int32_t max_pages,
+                                                                int32_t page_size) {
+  if (batch < 1 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1 || max_pages < 0 || page_size < 1) return 0;
+  const int64_t positions = static_cast<int64_t>(max_pages) * page_size;
+  const AttentionShape s = attention_shape(batch, q_heads, kv_heads, head_dim, positions);
+  return weights_space(attention_space(s, batch, kv_heads, head_dim), batch, q_heads, positions).bytes;
+}
+
+extern "C" int tris_paged_attention_decode_weights(const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+                                                   int32_t q_type, int32_t q_heads, const tris_paged_cache* cache,
+                                                   float scale, int32_t window, void* out, int64_t out_seq_stride,
+                                                   int64_t out_head_stride, float* weight_sum, int64_t sum_seq_stride,
+                                                   int64_t sum_head_stride, void* workspace, int64_t workspace_bytes,
+                                                   void* stream) {
+  const WeightSums weights{weight_sum, sum_seq_stride, sum_head_stride};
+  return attention_decode("tris_paged_attention_decode_weights", q, q_seq_stride, q_head_stride, q_type, q_heads, cache,
+                          scale, window, out, out_seq_stride, out_head_stride, &weights, workspace, workspace_bytes, stream);
 }

@@ -17,6 +17,8 @@
 
 namespace tris {
 
+constexpr int kMaxAxes = TRIS_MAX_ROTARY_AXES;
+
 struct AppendArgs {
   const uint16_t* q;
   const uint16_t* k;
@@ -28,8 +30,25 @@ struct AppendArgs {
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, qo_token, qo_head;
   int32_t act_bf16, tokens, q_heads, rotary_dim, zero_unplaced, token_waves;
   PageDivision page_of;
+  const int32_t* token_positions;  // [axes][tokens], rows axis_stride apart
+  int64_t axis_stride;
+  int32_t axes, interleaved, table_rows;
+  int32_t ends[kMaxAxes];  // of the axes' pairs: the first pair past them
   tris_paged_cache c;
 };
+
+// The axis whose position turns pair i: sections one after the other, or, interleaved, the axes in turn while they have
+// pairs left and then the first.
+__device__ __forceinline__ int pair_axis(const AppendArgs& a, int i) {
+  if (a.interleaved) {
+    const int axis = i % a.axes;
+    return i < a.ends[axis] ? axis : 0;
+  }
+  int axis = 0;
+#pragma unroll
+  for (int n = 0; n < kMaxAxes - 1; ++n) axis += n < a.axes - 1 && i >= a.ends[n];
+  return axis;
+}
 
 // The sequence whose new tokens hold token t, or -1; *pos: the token's position.  The wavefront reads 64 boundaries and
 // lengths at a time and takes the first boundary past t.
@@ -69,7 +88,7 @@ __device__ __forceinline__ uint2 e4m3x8(const float v[8], float scale) {
 // 6.0.
 constexpr int kUnits = 2;
 
-template <bool kE4m3>
+template <bool kE4m3, bool kAxes>
 __global__ __launch_bounds__(256) void rotary_append_kernel(const AppendArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x) / kWave);
   const int t = wave / a.token_waves;
@@ -97,16 +116,41 @@ __global__ __launch_bounds__(256) void rotary_append_kernel(const AppendArgs a) 
     ys[i] = *reinterpret_cast<const uint4*>(src + (is_q || is_k ? hi_qk : hi_v));
   }
 
+  // the table rows of the token's angles
+  int64_t at_row[kAxes ? kMaxAxes : 1];
+  bool turnable = true;
+  if constexpr (kAxes) {
+#pragma unroll
+    for (int n = 0; n < kMaxAxes; ++n) {
+      at_row[n] = 0;
+      if (n < a.axes) {
+        const int32_t row = a.token_positions[n * a.axis_stride + t];
+        turnable = turnable && row >= 0 && row < a.table_rows;
+        at_row[n] = row;
+      }
+    }
+  }
+
   int64_t place = -1;
   const int seq = token_sequence(a, t, &place);
-  const int pos = seq >= 0 && place >= 0 && place < cache_positions(a.c) ? static_cast<int>(place) : -1;
+  const int pos = seq >= 0 && place >= 0 && place < cache_positions(a.c) && turnable ? static_cast<int>(place) : -1;
   int page = -1, slot = 0;
   float cs[8], sn[8];
   if (pos >= 0) {
     const int i = a.page_of(pos);
     page = a.c.block_table[seq * a.c.table_stride + i];
     slot = pos - i * a.c.page_size;
-    if (turning) {
+    if (kAxes && turning) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int axis = pair_axis(a, lo_qk + e);
+        int64_t row = at_row[0];
+#pragma unroll
+        for (int n = 1; n < kMaxAxes; ++n) row = axis == n ? at_row[kAxes ? n : 0] : row;
+        cs[e] = a.cos[row * half + lo_qk + e];
+        sn[e] = a.sin[row * half + lo_qk + e];
+      }
+    } else if (turning) {
       const float* c = a.cos + static_cast<int64_t>(pos) * half + lo_qk;
       const float* s = a.sin + static_cast<int64_t>(pos) * half + lo_qk;
 #pragma unroll
@@ -180,23 +224,48 @@ __global__ __launch_bounds__(256) void rotary_append_kernel(const AppendArgs a) 
 
 using namespace tris;
 
-extern "C" int tris_rotary_append_paged(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
-                                        int64_t k_token_stride, int64_t k_head_stride, const void* v,
-                                        int64_t v_token_stride, int64_t v_head_stride, int32_t act_type,
-                                        int32_t tokens, int32_t q_heads, const float* cos, const float* sin,
-                                        int32_t rotary_dim, int32_t positions, const int32_t* query_start,
-                                        const tris_paged_cache* cache, void* q_out, int64_t q_out_token_stride,
-                                        int64_t q_out_head_stride, int32_t zero_unplaced, void* stream) {
-  const char* who = "tris_rotary_append_paged";
+namespace {
+
+// The rotary positions of tokens whose places in the cache do not give them.
+struct TokenPositions {
+  const int32_t* positions;
+  int64_t axis_stride;
+  int32_t axes, interleaved;
+  const int32_t* sections;
+};
+
+int append(const char* who, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+           int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+           int32_t act_type, int32_t tokens, int32_t q_heads, const float* cos, const float* sin, int32_t rotary_dim,
+           int32_t positions, const int32_t* query_start, const tris_paged_cache* cache, void* q_out,
+           int64_t q_out_token_stride, int64_t q_out_head_stride, int32_t zero_unplaced, const TokenPositions* given,
+           void* stream) {
   if (const int rc = check_paged_cache(who, cache, act_type)) return rc;
   TRIS_REQUIRE(tokens >= 0 && q_heads >= 0, "%s: negative shape", who);
   TRIS_REQUIRE(query_start || tokens == cache->batch, "%s: without query_start there is one token a sequence", who);
   TRIS_REQUIRE(rotary_dim >= 16 && rotary_dim % 16 == 0 && rotary_dim <= cache->head_dim,
                "%s: rotary_dim must be a multiple of 16 up to head_dim", who);
-  TRIS_REQUIRE(positions >= cache_positions(*cache), "%s: cos and sin must cover max_pages * page_size positions", who);
+  if (given) {
+    TRIS_REQUIRE(given->axes >= 1 && given->axes <= kMaxAxes && given->sections && given->axis_stride >= 0,
+                 "%s: positions have 1 to %d axes, a section for each", who, kMaxAxes);
+    int64_t pairs = 0;
+    for (int i = 0; i < given->axes; ++i) {
+      TRIS_REQUIRE(given->sections[i] >= 0, "%s: negative section", who);
+      pairs += given->sections[i];
+    }
+    TRIS_REQUIRE(pairs == rotary_dim / 2, "%s: the sections must add up to rotary_dim / 2 pairs", who);
+    for (int i = 1; i < given->axes && given->interleaved; ++i)
+      TRIS_REQUIRE(given->sections[i] == 0 || (given->sections[i] - 1) * given->axes + i < rotary_dim / 2,
+                   "%s: interleaved sections that do not fit", who);
+    TRIS_REQUIRE(positions >= 1, "%s: cos and sin without rows", who);
+  } else {
+    TRIS_REQUIRE(positions >= cache_positions(*cache), "%s: cos and sin must cover max_pages * page_size positions",
+                 who);
+  }
   if (tokens == 0) return TRIS_OK;
   TRIS_REQUIRE(cache->batch > 0, "%s: tokens without sequences", who);
-  TRIS_REQUIRE(k && v && cos && sin && (q_heads == 0 || (q && q_out)), "%s: null pointer", who);
+  TRIS_REQUIRE(k && v && cos && sin && (q_heads == 0 || (q && q_out)) && (!given || given->positions),
+               "%s: null pointer", who);
   for (const int64_t s : {q_heads ? q_token_stride : 0, q_heads ? q_head_stride : 0, k_token_stride, k_head_stride,
                           v_token_stride, v_head_stride, q_heads ? q_out_token_stride : 0,
                           q_heads ? q_out_head_stride : 0})
@@ -207,17 +276,10 @@ extern "C" int tris_rotary_append_paged(const void* q, int64_t q_token_stride, i
   const int64_t units = (static_cast<int64_t>(q_heads) + 2LL * cache->kv_heads) * (cache->head_dim / 16);
   TRIS_REQUIRE(units < (1 << 24), "%s: too many heads", who);
   const tris_paged_cache& c = *cache;
-  const auto apart = [&c](int64_t page_stride, int64_t head_stride, int64_t slot_stride, int64_t row) {
-    return rows_apart<3>({{{c.num_pages, page_stride}, {c.kv_heads, head_stride}, {c.page_size, slot_stride}}}, row);
-  };
   TRIS_REQUIRE(q_heads == 0 || rows_apart<2>({{{tokens, q_out_token_stride}, {q_heads, q_out_head_stride}}}, c.head_dim),
                "%s: output rows overlap", who);
-  TRIS_REQUIRE(apart(c.k_page_stride, c.k_head_stride, c.k_slot_stride, c.head_dim) &&
-                   apart(c.v_page_stride, c.v_head_stride, c.v_slot_stride, c.head_dim),
-               "%s: cache rows overlap", who);
-  TRIS_REQUIRE(!c.k_scale || (apart(c.k_scale_page_stride, c.k_scale_head_stride, c.k_scale_slot_stride, 1) &&
-                              apart(c.v_scale_page_stride, c.v_scale_head_stride, c.v_scale_slot_stride, 1)),
-               "%s: cache scales overlap", who);
+  TRIS_REQUIRE(cache_rows_apart(c), "%s: cache rows overlap", who);
+  TRIS_REQUIRE(cache_scales_apart(c), "%s: cache scales overlap", who);
   const int64_t token_waves = (units + kUnits * kWave - 1) / (kUnits * kWave);
   const int64_t blocks = (tokens * token_waves + 3) / 4;
   TRIS_REQUIRE(blocks < (1LL << 32) / (4 * kWave), "%s: too many tokens", who);  // a launch has less than 2^32 threads
@@ -225,10 +287,56 @@ extern "C" int tris_rotary_append_paged(const void* q, int64_t q_token_stride, i
                static_cast<uint16_t*>(q_out), cos, sin, query_start, q_token_stride, q_head_stride, k_token_stride,
                k_head_stride, v_token_stride, v_head_stride, q_out_token_stride, q_out_head_stride,
                act_type == TRIS_DTYPE_BF16, tokens, q_heads, rotary_dim, zero_unplaced,
-               static_cast<int32_t>(token_waves), PageDivision(cache->page_size), *cache};
+               static_cast<int32_t>(token_waves), PageDivision(cache->page_size), nullptr, 0, 0, 0, 0, {}, *cache};
+  if (given) {
+    a.token_positions = given->positions;
+    a.axis_stride = given->axis_stride;
+    a.axes = given->axes;
+    a.interleaved = given->interleaved;
+    a.table_rows = positions;
+    for (int i = 0, end = 0; i < given->axes; ++i) {
+      end += given->sections[i];
+      a.ends[i] = given->interleaved ? given->axes * given->sections[i] : end;
+    }
+  }
   const dim3 grid(static_cast<unsigned>(blocks)), block(4 * kWave);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (cache->dtype == TRIS_DTYPE_E4M3) hipLaunchKernelGGL(rotary_append_kernel<true>, grid, block, 0, st, a);
-  else hipLaunchKernelGGL(rotary_append_kernel<false>, grid, block, 0, st, a);
+  if (cache->dtype == TRIS_DTYPE_E4M3) {
+    if (given) hipLaunchKernelGGL((rotary_append_kernel<true, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((rotary_append_kernel<true, false>), grid, block, 0, st, a);
+  } else {
+    if (given) hipLaunchKernelGGL((rotary_append_kernel<false, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((rotary_append_kernel<false, false>), grid, block, 0, st, a);
+  }
   return check_launch(who);
+}
+
+}  // namespace
+
+extern "C" int tris_rotary_append_paged(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                                        int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                                        int64_t v_token_stride, int64_t v_head_stride, int32_t act_type,
+                                        int32_t tokens, int32_t q_heads, const float* cos, const float* sin,
+                                        int32_t rotary_dim, int32_t positions, const int32_t* query_start,
+                                        const tris_paged_cache* cache, void* q_out, int64_t q_out_token_stride,
+                                        int64_t q_out_head_stride, int32_t zero_unplaced, void* stream) {
+  return append("tris_rotary_append_paged", q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, v,
+                v_token_stride, v_head_stride, act_type, tokens, q_heads, cos, sin, rotary_dim, positions, query_start,
+                cache, q_out, q_out_token_stride, q_out_head_stride, zero_unplaced, nullptr, stream);
+}
+
+extern "C" int tris_rotary_axes_append_paged(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                             const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                                             const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                                             int32_t act_type, int32_t tokens, int32_t q_heads, const float* cos,
+                                             const float* sin, int32_t rotary_dim, int32_t positions,
+                                             const int32_t* query_start, const tris_paged_cache* cache, void* q_out,
+                                             int64_t q_out_token_stride, int64_t q_out_head_stride,
+                                             int32_t zero_unplaced, const int32_t* token_positions,
+                                             int64_t axis_stride, int32_t axes, const int32_t* sections,
+                                             int32_t interleaved, void* stream) {
+  const TokenPositions given{token_positions, axis_stride, axes, interleaved != 0, sections};
+  return append("tris_rotary_axes_append_paged", q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, v,
+                v_token_stride, v_head_stride, act_type, tokens, q_heads, cos, sin, rotary_dim, positions, query_start,
+                cache, q_out, q_out_token_stride, q_out_head_stride, zero_unplaced, &given, stream);
 }

@@ -85,4 +85,23 @@ inline int check_paged_cache(const char* who, const tris_paged_cache* c, int32_t
   return TRIS_OK;
 }
 
+// What a cache that is written to has to be: pages, heads and slots without shared memory; its scales likewise.
+inline bool cache_rows_apart(const tris_paged_cache& c, int64_t page, int64_t head, int64_t slot, int64_t row) {
+  return rows_apart<3>({{{c.num_pages, page}, {c.kv_heads, head}, {c.page_size, slot}}}, row);
+}
+inline bool cache_rows_apart(const tris_paged_cache& c) {
+  return cache_rows_apart(c, c.k_page_stride, c.k_head_stride, c.k_slot_stride, c.head_dim) &&
+         cache_rows_apart(c, c.v_page_stride, c.v_head_stride, c.v_slot_stride, c.head_dim);
+}
+inline bool cache_scales_apart(const tris_paged_cache& c) {
+  return !c.k_scale || (cache_rows_apart(c, c.k_scale_page_stride, c.k_scale_head_stride, c.k_scale_slot_stride, 1) &&
+                        cache_rows_apart(c, c.v_scale_page_stride, c.v_scale_head_stride, c.v_scale_slot_stride, 1));
+}
+
+// Sums of attention weights, a row of all positions for each (sequence, kv head): strides that keep the rows apart.
+inline bool sum_rows_apart(const tris_paged_cache& c, int64_t seq_stride, int64_t head_stride) {
+  return seq_stride >= 0 && head_stride >= 0 &&
+         rows_apart<2>({{{c.batch, seq_stride}, {c.kv_heads, head_stride}}}, cache_positions(c));
+}
+
 }  // namespace tris

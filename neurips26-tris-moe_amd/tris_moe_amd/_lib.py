@@ -238,6 +238,13 @@ SIGNATURES = {
     "tris_paged_attention_decode": (ctypes.c_int, [_P, _I64, _I64, _I32, _I32, _PPC, ctypes.c_float, _I32, _P, _I64,
                                                    _I64, _P, _I64, _P]),
     "tris_paged_attention_workspace_bytes": (_I64, [_I32] * 6),
+    "tris_rotary_axes_append_paged": (ctypes.c_int, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _I32, _I32,
+                                                     _P, _P, _I32, _I32, _P, _PPC, _P, _I64, _I64, _I32, _P, _I64, _I32,
+                                                     _P, _I32, _P]),
+    "tris_paged_attention_decode_weights": (ctypes.c_int, [_P, _I64, _I64, _I32, _I32, _PPC, ctypes.c_float, _I32, _P,
+                                                           _I64, _I64, _P, _I64, _I64, _P, _I64, _P]),
+    "tris_paged_attention_weights_workspace_bytes": (_I64, [_I32] * 6),
+    "tris_paged_cache_evict": (ctypes.c_int, [_PPC, _P, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P, _P]),
 }
 
 _lib = None

@@ -20,6 +20,7 @@ unavailable" (convert it to block-GR at load).
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 
 import torch
@@ -1998,6 +1999,7 @@ _NO_STRIDES = (0, 0, 0)
 _INT32_MAX = 2 ** 31 - 1
 RMS_NORM_MAX_WIDTH = 32768
 PAGED_HEAD_DIMS = (64, 128, 256)
+MAX_ROTARY_AXES = 4
 
 
 def _launch(index, fn, *args):
@@ -2190,13 +2192,34 @@ def _paged_cache(who, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale,
             batch, max_pages, page, heads, dim)
 
 
+def _token_positions(who, positions, tokens, index):
+    """The number of axes of a positions tensor, and the stride between its rows."""
+    shape = getattr(positions, "shape", ())
+    if not (isinstance(positions, torch.Tensor) and positions.dtype is torch.int32 and positions.get_device() == index
+            and len(shape) in (1, 2)):
+        _check_on(who, "positions", positions, None, (torch.int32,), torch.device("cuda", index))
+        raise RuntimeError(f"{who}: positions must be [tokens] or [axes, tokens]")
+    if shape[-1] != tokens:
+        raise RuntimeError(f"{who}: positions must hold one for each token")
+    if tokens > 1 and positions.stride(-1) != 1:
+        raise RuntimeError(f"{who}: the rows of positions must be contiguous")
+    return (1, 0) if len(shape) == 1 else (shape[0], positions.stride(0))
+
+
+@functools.lru_cache(64)
+def _sections(sections):
+    """A C array of the sections."""
+    return (ctypes.c_int32 * len(sections))(*sections)
+
+
 def rotary_append_paged(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                         k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                         seq_lens: torch.Tensor, query_start: torch.Tensor | None = None,
                         k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
-                        q_out: torch.Tensor | None = None):
+                        q_out: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+                        sections: tuple | None = None, interleaved: bool = False):
     """Rotates queries and keys by their positions and appends keys and values to the paged cache, in one launch
-    (tris_rotary_append_paged).  Returns the rotated queries (None without q).
+    (tris_rotary_append_paged, tris_rotary_axes_append_paged).  Returns the rotated queries (None without q).
 
     q [tokens, q_heads, head_dim], k and v [tokens, kv_heads, head_dim], fp16 or bf16 (rows that are not 16-byte
     aligned are copied first).  cos, sin fp32 [positions, rotary_dim / 2] (``attention.rotary_tables``), covering
@@ -2209,8 +2232,15 @@ def rotary_append_paged(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor
     the lengths with the new tokens.  query_start int32 [batch + 1]: sequence b's new tokens are rows
     query_start[b] to query_start[b + 1], its last ones; None: one new token a sequence, token b is sequence b's.
 
-    A row past query_start[-1], or of an idle sequence (length 0), is not stored and its rotated query is zero (left
-    as it was in a given q_out).  A page number outside the pool is skipped.  q_out may be q.  No gradient."""
+    positions int32 [tokens] or [axes, tokens]: rotary positions other than the tokens' places in the cache, on up to
+    MAX_ROTARY_AXES axes (time, height and width of an image's patches; one axis after an eviction).  Pair i of the
+    rotary_dim / 2 is turned by positions[axis(i)]: sections, one count of pairs for each axis, lie in a row, or with
+    ``interleaved`` pair i has axis i % axes while that axis has pairs left, then axis 0 (None: one axis).  cos and sin
+    then need rows for these positions only.
+
+    A row past query_start[-1], of an idle sequence (length 0), or with one of its positions outside cos and sin, is not
+    stored and its rotated query is zero (left as it was in a given q_out).  A page number outside the pool is skipped.
+    q_out may be q.  No gradient."""
     who = "rotary_append_paged"
     if not (isinstance(k, torch.Tensor) and k.is_cuda and k.dtype in _ACT_DTYPES):
         _check_on(who, "k", k, 3, _ACT_DTYPES)
@@ -2228,7 +2258,7 @@ def rotary_append_paged(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor
         for name, t in (("cos", cos), ("sin", sin)):
             _check_cuda(name, t, torch.float32, 2, k.device)
         raise RuntimeError(f"{who}: cos and sin must have one shape")
-    positions, half = angles
+    rows, half = angles
     starts = None
     if query_start is not None:
         _check_cuda("query_start", query_start, torch.int32, 1, k.device)
@@ -2252,26 +2282,55 @@ def rotary_append_paged(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor
     elif q_out is not None:
         raise RuntimeError(f"{who}: q_out needs q")
     _refuse_gradient(who, q, k, v, cos, sin, k_cache, v_cache, k_scale, v_scale, q_out)
-    rc = _launch(index, _lib.load().tris_rotary_append_paged, q_ptr, qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
-                 v.data_ptr(), vs[0], vs[1], _DTYPE_IDS[dt], tokens, q_heads, cos.data_ptr(), sin.data_ptr(), 2 * half,
-                 positions, starts, cache, qo_ptr, qos[0], qos[1], zero, torch._C._cuda_getCurrentRawStream(index))
+    args = (q_ptr, qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _DTYPE_IDS[dt], tokens, q_heads,
+            cos.data_ptr(), sin.data_ptr(), 2 * half, rows, starts, cache, qo_ptr, qos[0], qos[1], zero)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if positions is None:
+        if sections is not None or interleaved:
+            raise RuntimeError(f"{who}: sections need positions")
+        name, rc = "tris_rotary_append_paged", _launch(index, _lib.load().tris_rotary_append_paged, *args, stream)
+    else:
+        name = "tris_rotary_axes_append_paged"
+        axes, stride = _token_positions(who, positions, tokens, index)
+        split = _sections((half,) if sections is None else tuple(sections))
+        if len(split) != axes:
+            raise RuntimeError(f"{who}: positions must have a row for each of the sections")
+        rc = _launch(index, _lib.load().tris_rotary_axes_append_paged, *args, positions.data_ptr(), stride, axes, split,
+                     interleaved, stream)
     if rc:
-        _lib.check(rc, "tris_rotary_append_paged")
+        _lib.check(rc, name)
     return q_out
+
+
+def _weight_sum(who, t, batch, heads, positions, index):
+    """(pointer, strides) of sums of attention weights, a contiguous row of positions for each (sequence, kv head)."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.get_device() == index and t.ndim == 3):
+        _check_on(who, "weight_sum", t, 3, (torch.float32,), torch.device("cuda", index))
+    b, h, n = t.shape
+    if b != batch or h != heads or n < positions:
+        raise RuntimeError(f"{who}: weight_sum must be [batch, kv_heads, at least {positions} positions]")
+    s0, s1, s2 = t.stride()
+    if s2 != 1 and n > 1:
+        raise RuntimeError(f"{who}: the rows of weight_sum must be contiguous")
+    return t.data_ptr(), s0, s1
 
 
 def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                            seq_lens: torch.Tensor, scale: float | None = None, window: int = 0,
                            k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
-                           out: torch.Tensor | None = None) -> torch.Tensor:
-    """Attention of one new token a sequence over the paged cache (tris_paged_attention_decode): out[b, h] =
-    sum_j softmax_j(scale * q[b, h] . k_j) v_j over sequence b's seq_lens[b] positions, or its last ``window`` of
-    them; fp32 inside, rounded once.  scale: head_dim ** -0.5 by default.
+                           out: torch.Tensor | None = None, weight_sum: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one new token a sequence over the paged cache (tris_paged_attention_decode,
+    tris_paged_attention_decode_weights): out[b, h] = sum_j softmax_j(scale * q[b, h] . k_j) v_j over sequence b's
+    seq_lens[b] positions, or its last ``window`` of them; fp32 inside, rounded once.  scale: head_dim ** -0.5 by default.
 
     q [batch, q_heads, head_dim] fp16 or bf16, q_heads a multiple of kv_heads (query head h reads kv head
     h // (q_heads / kv_heads)); the cache, block_table, seq_lens and scales as rotary_append_paged takes them.  An
     idle sequence (length 0) gives zeros; slots outside a sequence may hold anything.  out may be q.  The launch depends
-    on no value on the device, so a captured call may be replayed with other lengths and tables.  No gradient."""
+    on no value on the device, so a captured call may be replayed with other lengths and tables.  No gradient.
+
+    weight_sum fp32 [batch, kv_heads, positions], positions at least the block table's: each position that the token
+    attends to gets its weights of the kv head's query heads added, weight_sum[b, g, j] += sum_h softmax_j(...); all
+    others stay as they were.  It is what ``paged_cache_evict`` chooses by; a sequence begins with zeros there."""
     who = "paged_attention_decode"
     if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dtype in _ACT_DTYPES):
         _check_on(who, "q", q, 3, _ACT_DTYPES)
@@ -2287,16 +2346,65 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         if window < 0:
             raise RuntimeError(f"{who}: negative window")
         window = _INT32_MAX  # no sequence is longer
-    _refuse_gradient(who, q, k_cache, v_cache, k_scale, v_scale, out)
+    sums = () if weight_sum is None else _weight_sum(who, weight_sum, batch, heads, max_pages * page, index)
+    _refuse_gradient(who, q, k_cache, v_cache, k_scale, v_scale, out, weight_sum)
     lib = _lib.load()
-    need = lib.tris_paged_attention_workspace_bytes(batch, q_heads, heads, dim, max_pages, page)
+    args = (q.data_ptr(), qs[0], qs[1], _DTYPE_IDS[dt], q_heads, cache, dim ** -0.5 if scale is None else scale, window,
+            out.data_ptr(), outs[0], outs[1])
+    if weight_sum is None:
+        name, fn = "tris_paged_attention_decode", lib.tris_paged_attention_decode
+        need = lib.tris_paged_attention_workspace_bytes(batch, q_heads, heads, dim, max_pages, page)
+    else:
+        name, fn = "tris_paged_attention_decode_weights", lib.tris_paged_attention_decode_weights
+        need = lib.tris_paged_attention_weights_workspace_bytes(batch, q_heads, heads, dim, max_pages, page)
+        if need < 0:
+            raise RuntimeError(f"{who}: too many positions")
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # of this call alone
-    rc = _launch(index, lib.tris_paged_attention_decode, q.data_ptr(), qs[0], qs[1], _DTYPE_IDS[dt], q_heads, cache,
-                 dim ** -0.5 if scale is None else scale, window, out.data_ptr(), outs[0], outs[1], _ptr(ws), need,
-                 torch._C._cuda_getCurrentRawStream(index))
+    rc = _launch(index, fn, *args, *sums, _ptr(ws), need, torch._C._cuda_getCurrentRawStream(index))
     if rc:
-        _lib.check(rc, "tris_paged_attention_decode")
+        _lib.check(rc, name)
     return out
+
+
+def paged_cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                      weight_sum: torch.Tensor, budget: int, limit: int | None = None, sink: int = 0, recent: int = 0,
+                      k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None):
+    """Eviction from the paged cache by accumulated attention weight (tris_paged_cache_evict).  Each sequence of more
+    than ``limit`` positions (budget by default) keeps ``budget`` of them, each kv head its own: the first ``sink``, the
+    last ``recent``, and between them those of the largest weight_sum (as ``paged_attention_decode`` adds them up; NaN
+    above all numbers, of equal ones the lowest position).  What stays moves, in order, to the positions from 0 on, in
+    the sequence's own pages: keys, values, scales and sums; the sums behind become zero.  So a window counts what
+    stayed, and the pages past budget positions are free.
+
+    Returns (new_lens int32 [batch], kept int32 [batch, kv_heads, budget]): the lengths now (budget, or as they were), and
+    the position that each place's token had, -1 throughout for a sequence left alone: one of limit positions or fewer, or
+    with a page outside the pool.  seq_lens is not changed: with one pair of tables for all layers, every layer evicts by
+    the old lengths before the new ones are copied there.
+
+    The cache, block_table and seq_lens as rotary_append_paged takes them, weight_sum as paged_attention_decode does.  No
+    page of an evicted sequence may be another sequence's too.  Rotary positions go on from the sequence's true length
+    (``positions`` of rotary_append_paged).  The launch depends on no value on the device, so a captured decode step may
+    evict in every replay, with a limit above the budget every limit - budget + 1 steps.  No gradient."""
+    who = "paged_cache_evict"
+    if not (isinstance(k_cache, torch.Tensor) and k_cache.is_cuda):
+        _check_on(who, "k_cache", k_cache, 4, _CACHE_DTYPES)
+    index = k_cache.get_device()
+    cache, (batch, max_pages, page, heads, _) = _paged_cache(who, k_cache, v_cache, block_table, seq_lens, k_scale, v_scale,
+                                                             index)
+    sums = _weight_sum(who, weight_sum, batch, heads, max_pages * page, index)
+    limit = budget if limit is None else limit
+    if not 1 <= budget <= limit or budget > _INT32_MAX:
+        raise RuntimeError(f"{who}: 1 <= budget <= limit")
+    if sink < 0 or recent < 0 or sink + recent > budget:
+        raise RuntimeError(f"{who}: sink and recent must be within the budget")
+    _refuse_gradient(who, k_cache, v_cache, k_scale, v_scale, weight_sum)
+    new_lens = torch.empty_like(seq_lens)
+    kept = torch.empty((batch, heads, budget), dtype=torch.int32, device=k_cache.device)
+    rc = _launch(index, _lib.load().tris_paged_cache_evict, cache, *sums, budget, min(limit, _INT32_MAX), sink, recent,
+                 new_lens.data_ptr(), kept.data_ptr(), torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc, "tris_paged_cache_evict")
+    return new_lens, kept
 
 
 def gr_encode(packed, k_min: int = 0, k_max: int = 7, force_raw: bool = False):
