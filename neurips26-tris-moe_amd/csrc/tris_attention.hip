@@ -70,8 +70,8 @@ struct AttentionArgs {
   float* part_o;                     // the same rows of head_dim sums
   tris_paged_cache c;
   // of the calls that sum the weights
-  float* scores;                     // [batch][q_heads][score_row]: scale_log2 * q . k, -infinity for a key left out
-  int64_t score_row;
+  float* scores;                     // scale_log2 * q . k, see score_block
+  int64_t score_row;                 // keys of a (sequence, query head) there
   float2* whole_ml;                  // [batch][q_heads]: maximum and sum of what one workgroup had whole
   float* weight_sum;
   int64_t sum_seq, sum_head;
@@ -261,6 +261,12 @@ __device__ __forceinline__ float2 infinite_sums(const AttentionArgs& a, const Pi
   }
   const auto sum = [&](int t) { return nan[t] || up[t] == down[t] ? __builtin_nanf("") : up[t] ? INFINITY : -INFINITY; };
   return make_float2(sum(0), sum(1));
+}
+
+// The scores of a (sequence, head group): tile by tile, in each its halves of 16 keys, in each the group's heads, so that
+// a wavefront's store is one stretch of memory.  (64 on e4m3 201 us with each head's scores in a row of its own, xx.)
+__device__ __forceinline__ float* score_block(const AttentionArgs& a, int b, int kvh, int head0) {
+  return a.scores + ((static_cast<int64_t>(b) * a.c.kv_heads + kvh) * a.group + head0) * a.score_row;
 }
 
 // The powers of two that the weights and their sum are taken larger by (see the probabilities below).
@@ -515,9 +521,8 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
     }
   };
 
-  float* scores = nullptr;  // of the lane's head, from its four keys on
-  if constexpr (kWeights)
-    scores = a.scores + (static_cast<int64_t>(p.b) * a.q_heads + kvh * a.group + head0 + col) * a.score_row + g * 4;
+  float* const scores = kWeights ? score_block(a, p.b, kvh, head0) : nullptr;
+  const int score_at = col < heads ? (col * 16 + g * 4) * 4 : INT32_MAX;  // the lane's four keys of its head, in bytes
 
   float m = -INFINITY, l = 0.0f;
   f32x4 acc[kRuns * kRun];
@@ -597,11 +602,11 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
         x[j] = valid[j] ? x[j] : -INFINITY;
       }
     }
-    if constexpr (kWeights) {
-      if (col < heads) {
-        *reinterpret_cast<f32x4*>(scores + key0) = f32x4{x[0], x[1], x[2], x[3]};
-        *reinterpret_cast<f32x4*>(scores + key0 + 16) = f32x4{x[4], x[5], x[6], x[7]};
-      }
+    if constexpr (kWeights) {  // (a lane without a head: outside the buffer, without a branch)
+      const __amdgpu_buffer_rsrc_t rows = make_rsrc(scores + static_cast<int64_t>(key0) * heads, heads * 128);
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{x[0], x[1], x[2], x[3]}), rows, score_at, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{x[4], x[5], x[6], x[7]}), rows, score_at,
+                                             heads * 64, 0);
     }
     load_k(tile + kWaves, nxt);
 
@@ -768,44 +773,53 @@ struct Part {
 };
 
 // Joins the pieces of one (sequence, query head), 32 dimensions a wavefront: eight lanes a piece, eight pieces at a time.
-// kTogether: 16 or 4 wavefronts on the same dimensions, or (1) four on dimensions of their own.
-template <int kDim, bool kBf16, int kTogether>
-__global__ __launch_bounds__(kTogether == 16 ? 1024 : 256) void attention_join_kernel(const AttentionArgs a) {
+// kTogether: 16 or 4 shares of the pieces for the same dimensions, by kJoinWaves wavefronts, or (1) four wavefronts on
+// dimensions of their own.
+template <int kDim, bool kBf16, int kTogether, int kJoinWaves>
+__device__ __forceinline__ void join_pieces(const AttentionArgs& a, int block) {
   constexpr int kParts = kDim / 32;
   constexpr bool kMany = kTogether > 1;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const int unit = static_cast<int>(blockIdx.x) * (kMany ? 1 : 4) + (kMany ? 0 : wave);
+  const int unit = block * (kMany ? 1 : 4) + (kMany ? 0 : wave);
   const int row = unit / kParts, d = unit % kParts * 32 + lane % 8 * 4;
   const int b = row / a.q_heads, h = row % a.q_heads;
   if (b >= a.c.batch) return;
   const int hg = h / a.group * a.head_tiles + h % a.group / kHeadTile, in = h % a.group % kHeadTile;
   const int2 owners = a.owners[b * (a.c.kv_heads * a.head_tiles) + hg];
   if (owners.x == owners.y) return;
-  Part p{-INFINITY, 0.0f, f32x4{0, 0, 0, 0}};
+  constexpr int kShares = kMany ? kTogether / kJoinWaves : 1;  // of a wavefront
+  Part p[kShares];
+#pragma unroll
+  for (int u = 0; u < kShares; ++u) {
+    p[u] = Part{-INFINITY, 0.0f, f32x4{0, 0, 0, 0}};
 #pragma unroll 2
-  for (int w = owners.x + (kMany ? wave * 8 : 0) + lane / 8; w <= owners.y; w += 8 * kTogether) {
-    const int64_t r = static_cast<int64_t>(2 * w + (w == owners.x)) * a.tile_heads + in;
-    const float2 ml = a.part_ml[r];
-    p.add(ml.x, ml.y, *reinterpret_cast<const f32x4*>(a.part_o + r * kDim + d));
+    for (int w = owners.x + (kMany ? (wave + u * kJoinWaves) * 8 : 0) + lane / 8; w <= owners.y; w += 8 * kTogether) {
+      const int64_t r = static_cast<int64_t>(2 * w + (w == owners.x)) * a.tile_heads + in;
+      const float2 ml = a.part_ml[r];
+      p[u].add(ml.x, ml.y, *reinterpret_cast<const f32x4*>(a.part_o + r * kDim + d));
+    }
+    p[u].across();
   }
-  p.across();
   if constexpr (kMany) {
     __shared__ Part sh[kTogether][8];
-    if (lane < 8) sh[wave][lane] = p;
+#pragma unroll
+    for (int u = 0; u < kShares; ++u)
+      if (lane < 8) sh[wave + u * kJoinWaves][lane] = p[u];
     __syncthreads();
     if (wave != 0) return;
-    p = lane / 8 < kTogether ? sh[lane / 8 % kTogether][lane % 8] : Part{-INFINITY, 0.0f, f32x4{0, 0, 0, 0}};
+    p[0] = lane / 8 < kTogether ? sh[lane / 8 % kTogether][lane % 8] : Part{-INFINITY, 0.0f, f32x4{0, 0, 0, 0}};
     if constexpr (kTogether > 8) {
       const Part q = sh[lane / 8 + 8][lane % 8];
-      p.add(q.m, q.l, q.o);
+      p[0].add(q.m, q.l, q.o);
     }
-    p.across();
+    p[0].across();
   }
   if (lane >= 8) return;
+  Part& sum = p[0];
   // A factor of zero has made a piece's infinite sum NaN: the weights that it stands for are above zero, so that the whole
   // is that of the infinite sums alone.
-  const bool lost = p.o[0] != p.o[0] || p.o[1] != p.o[1] || p.o[2] != p.o[2] || p.o[3] != p.o[3];
-  if (lost && p.l > 0.0f && p.l < INFINITY) {
+  const bool lost = sum.o[0] != sum.o[0] || sum.o[1] != sum.o[1] || sum.o[2] != sum.o[2] || sum.o[3] != sum.o[3];
+  if (lost && sum.l > 0.0f && sum.l < INFINITY) {
     f32x4 infinite = {0, 0, 0, 0};
 #pragma unroll 1
     for (int w = owners.x; w <= owners.y; ++w) {
@@ -815,26 +829,116 @@ __global__ __launch_bounds__(kTogether == 16 ? 1024 : 256) void attention_join_k
       for (int i = 0; i < 4; ++i) infinite[i] += fabsf(o[i]) < INFINITY ? 0.0f : o[i];
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p.o[i] = p.o[i] != p.o[i] && infinite[i] != 0.0f ? infinite[i] : p.o[i];
+    for (int i = 0; i < 4; ++i) sum.o[i] = sum.o[i] != sum.o[i] && infinite[i] != 0.0f ? infinite[i] : sum.o[i];
   }
-  const f32x4 y = p.o * (p.l == 0.0f ? 0.0f : 1.0f / p.l);
+  const f32x4 y = sum.o * (sum.l == 0.0f ? 0.0f : 1.0f / sum.l);
   const uint2 packed = kBf16 ? make_uint2(pack_bf16_rne(y[0], y[1]), pack_bf16_rne(y[2], y[3]))
                              : make_uint2(pack_f16_rne(y[0], y[1]), pack_f16_rne(y[2], y[3]));
   *reinterpret_cast<uint2*>(a.out + b * a.out_seq + h * a.out_head + d) = packed;
 }
 
-// Adds the keys' weights to their sums, from the scores that the attention left: a workgroup takes the stretch that the
-// workgroup of its number took there, and of its pieces those of each kv head's first head group, for all of them.
-// shift: weight_shift of the types; sums4: the sums' rows can be read four at a time.
+template <int kDim, bool kBf16, int kTogether>
+__global__ __launch_bounds__(kTogether == 16 ? 1024 : 256) void attention_join_kernel(const AttentionArgs a) {
+  join_pieces<kDim, kBf16, kTogether, (kTogether == 16 ? 16 : 4)>(a, static_cast<int>(blockIdx.x));
+}
+
+// Adds the weights of a piece's keys (tiles [t0, t1) of sequence b's n positions from `first` on) to the sums of their kv
+// head, from the scores that the attention left, for all query heads of the kv head.  stats: LDS for a float2 of each.
+// A thread has four keys; the scores of eight heads and the sums are asked for a step ahead of their use, the first ones
+// before the statistics are known.
+__device__ __forceinline__ void sum_weights(const AttentionArgs& a, int b, int kvh, int n, int first, int t0, int t1,
+                                            float shift, bool sums4, float2* stats) {
+  constexpr int kStep = 8;
+  const int thread = threadIdx.x, wave = uniform(thread / kWave), lane = thread % kWave;
+  const int32_t* table = a.c.block_table + b * a.c.table_stride;
+  float* const sums = a.weight_sum + b * a.sum_seq + kvh * a.sum_head;
+  const float* const scores = score_block(a, b, kvh, 0);
+  const int end = min(n, t1 * kTileKeys);
+  int key = t0 * kTileKeys + thread * 4, h0 = 0;
+  f32x4 x[kStep], ahead[kStep];
+  // the scores of four keys and heads from h on, of the kv head's last ones again past them
+  const auto load = [&](int k, int h, f32x4* to) {
+    const int head0 = h / kHeadTile * kHeadTile, heads = min(kHeadTile, a.group - head0);
+    const float* from = scores + head0 * a.score_row + static_cast<int64_t>(k / kTileKeys * kTileKeys) * heads +
+                        k / 16 % 2 * heads * 16 + k % 16;
+#pragma unroll
+    for (int i = 0; i < kStep; ++i)
+      to[i] = *reinterpret_cast<const f32x4*>(from + min(h - head0 + i, heads - 1) * 16);
+  };
+  if (key < end) load(key, 0, x);
+
+  for (int h = wave; h < a.group; h += kWaves) {
+    float2 ml = {-INFINITY, 0.0f};
+    const int2 own = a.owners == nullptr
+                         ? make_int2(0, 0)
+                         : a.owners[b * (a.c.kv_heads * a.head_tiles) + kvh * a.head_tiles + h / kHeadTile];
+    if (own.x == own.y) {
+      ml = a.whole_ml[static_cast<int64_t>(b) * a.q_heads + kvh * a.group + h];
+    } else {
+      for (int w = own.x + lane; w <= own.y; w += kWave) {
+        const float2 part = a.part_ml[static_cast<int64_t>(2 * w + (w == own.x)) * a.tile_heads + h % kHeadTile];
+        const float top = fmaxf(ml.x, part.x), base = top == -INFINITY ? 0.0f : top;
+        ml = make_float2(top, ml.y * __builtin_amdgcn_exp2f(ml.x - base) + part.y * __builtin_amdgcn_exp2f(part.x - base));
+      }
+      const float top = wave_max_f32(ml.x), base = top == -INFINITY ? 0.0f : top;
+      ml = make_float2(top, wave_sum_f32(ml.y * __builtin_amdgcn_exp2f(ml.x - base)));
+    }
+    if (lane == 0) stats[h] = make_float2((ml.x == -INFINITY ? 0.0f : ml.x) - shift, ml.y == 0.0f ? 0.0f : 1.0f / ml.y);
+  }
+  __syncthreads();
+
+  f32x4 weight = {0, 0, 0, 0};
+  while (key < end) {
+    const bool last = h0 + kStep >= a.group;
+    const int key2 = last ? key + kWaves * kWave * 4 : key, h2 = last ? 0 : h0 + kStep;
+    if (key2 < end) load(key2, h2, ahead);
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) {
+      if (h0 + i < a.group) {
+        const float2 of = stats[h0 + i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) weight[e] += __builtin_amdgcn_exp2f(x[i][e] - of.x) * of.y;
+      }
+    }
+    if (last) {
+      const auto valid = [&](int k) {
+        return k >= first && k < n && static_cast<uint32_t>(table[a.page_of(k)]) < static_cast<uint32_t>(a.c.num_pages);
+      };
+      const bool use[4] = {valid(key), valid(key + 1), valid(key + 2), valid(key + 3)};
+      if (sums4 && use[0] && use[1] && use[2] && use[3]) {
+        f32x4* to = reinterpret_cast<f32x4*>(sums + key);
+        *to = *to + weight;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (use[e]) sums[key + e] += weight[e];
+      }
+      weight = f32x4{0, 0, 0, 0};
+    }
+    key = key2;
+    h0 = h2;
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) x[i] = ahead[i];
+  }
+}
+
+// The second launch of the calls that sum the weights: a.workgroups workgroups add the weights, each those of the stretch
+// that the workgroup of its number took in the first launch (of its pieces the first head group of each kv head, for all of
+// them), and behind them the join's, where there is a line.  shift: weight_shift of the types; sums4: the sums' rows can
+// be read four at a time.
+template <int kDim, bool kBf16, int kTogether>
 __global__ __launch_bounds__(kWaves * kWave) void attention_weights_kernel(const AttentionArgs a, const float shift,
                                                                           const bool sums4) {
-  extern __shared__ float2 stats[];  // of each query head: the maximum (less the shift) and the inverse sum
+  extern __shared__ float2 stats[];
+  if (blockIdx.x >= static_cast<uint32_t>(a.workgroups)) {
+    join_pieces<kDim, kBf16, kTogether, kWaves>(a, static_cast<int>(blockIdx.x) - a.workgroups);
+    return;
+  }
   const int head_groups = a.c.kv_heads * a.head_tiles;
   Stretch st;
   if (!(a.owners == nullptr ? own_stretch(a, head_groups, blockIdx.x, &st)
                             : line_stretch(a, head_groups, blockIdx.x, &st)))
     return;
-  const int thread = threadIdx.x, wave = uniform(thread / kWave), lane = thread % kWave;
   int at = st.at, begin = st.begin, b = st.b, n = st.n;
   while (at < st.stop && b < a.c.batch) {
     const int first = range_begin(a, n), tiles = range_tiles(n, first), span = tiles + kPieceCost;
@@ -847,53 +951,9 @@ __global__ __launch_bounds__(kWaves * kWave) void attention_weights_kernel(const
     const int count = min(tiles - from, st.stop - at);
     at += from >= tiles ? span - from : count;
     if (from >= tiles || n == 0 || hg % a.head_tiles != 0) continue;
-    const int kvh = hg / a.head_tiles;
-    const int64_t row0 = static_cast<int64_t>(b) * a.q_heads + kvh * a.group;
-    __syncthreads();  // the piece before has read its statistics
-    for (int h = wave; h < a.group; h += kWaves) {
-      float2 ml = {-INFINITY, 0.0f};
-      const int2 own = a.owners == nullptr ? make_int2(0, 0) : a.owners[b * head_groups + hg + h / kHeadTile];
-      if (own.x == own.y) {
-        ml = a.whole_ml[row0 + h];
-      } else {
-        for (int w = own.x + lane; w <= own.y; w += kWave) {
-          const float2 part = a.part_ml[static_cast<int64_t>(2 * w + (w == own.x)) * a.tile_heads + h % kHeadTile];
-          const float top = fmaxf(ml.x, part.x), base = top == -INFINITY ? 0.0f : top;
-          ml = make_float2(top, ml.y * __builtin_amdgcn_exp2f(ml.x - base) + part.y * __builtin_amdgcn_exp2f(part.x - base));
-        }
-        const float top = wave_max_f32(ml.x), base = top == -INFINITY ? 0.0f : top;
-        ml = make_float2(top, wave_sum_f32(ml.y * __builtin_amdgcn_exp2f(ml.x - base)));
-      }
-      if (lane == 0) stats[h] = make_float2((ml.x == -INFINITY ? 0.0f : ml.x) - shift, ml.y == 0.0f ? 0.0f : 1.0f / ml.y);
-    }
-    __syncthreads();
-    const int32_t* table = a.c.block_table + b * a.c.table_stride;
-    float* sums = a.weight_sum + b * a.sum_seq + kvh * a.sum_head;
-    const float* scores = a.scores + row0 * a.score_row;
-    const int t0 = first / kTileKeys + from, end = min(n, (t0 + count) * kTileKeys);
-    for (int key = t0 * kTileKeys + thread * 4; key < end; key += kWaves * kWave * 4) {
-      f32x4 weight = {0, 0, 0, 0};
-#pragma unroll 4
-      for (int h = 0; h < a.group; ++h) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(scores + h * a.score_row + key);
-        const float2 of = stats[h];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) weight[i] += __builtin_amdgcn_exp2f(x[i] - of.x) * of.y;
-      }
-      const auto valid = [&](int k) {
-        return k >= first && k < n &&
-               static_cast<uint32_t>(table[a.page_of(k)]) < static_cast<uint32_t>(a.c.num_pages);
-      };
-      const bool use[4] = {valid(key), valid(key + 1), valid(key + 2), valid(key + 3)};
-      if (sums4 && use[0] && use[1] && use[2] && use[3]) {
-        f32x4* dst = reinterpret_cast<f32x4*>(sums + key);
-        *dst = *dst + weight;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (use[i]) sums[key + i] += weight[i];
-      }
-    }
+    const int t0 = first / kTileKeys + from;
+    sum_weights(a, b, hg / a.head_tiles, n, first, t0, t0 + count, shift, sums4, stats);
+    __syncthreads();  // the statistics have been read
   }
 }
 
@@ -946,16 +1006,24 @@ static void attention_launch(const AttentionArgs& a, const AttentionShape& s, bo
   const size_t lds = (kWaves * a.tile_heads * (kDim + 4) + 2 * kWaves * kHeadTile) * sizeof(float);
   if (row_runs) hipLaunchKernelGGL((attention_decode_kernel<kDim, kBf16, kE4m3, true, kWeights>), grid, block, lds, st, a);
   else hipLaunchKernelGGL((attention_decode_kernel<kDim, kBf16, kE4m3, false, kWeights>), grid, block, lds, st, a);
-  if constexpr (kWeights) {
-    const bool sums4 = aligned16(a.weight_sum) && a.sum_seq % 4 == 0 && a.sum_head % 4 == 0;
-    hipLaunchKernelGGL(attention_weights_kernel, grid, block, a.group * sizeof(float2), st, a, weight_shift(kBf16, kE4m3),
-                       sums4);
-  }
-  if (!s.line) return;
   // few sequences are cut into many pieces each, many into a few
   const int64_t units = static_cast<int64_t>(a.c.batch) * a.q_heads * (kDim / 32);
   const int64_t pieces = a.workgroups / (static_cast<int64_t>(a.c.batch) * a.c.kv_heads * a.head_tiles);
   const dim3 each(static_cast<unsigned>(units)), fourth(static_cast<unsigned>((units + 3) / 4));
+  if constexpr (kWeights) {
+    const bool sums4 = aligned16(a.weight_sum) && a.sum_seq % 4 == 0 && a.sum_head % 4 == 0;
+    const float shift = weight_shift(kBf16, kE4m3);
+    const size_t stats = a.group * sizeof(float2);
+    const dim3 many(grid.x + each.x), few(grid.x + (s.line ? fourth.x : 0));
+    if (s.line && pieces >= kJoinMany)
+      hipLaunchKernelGGL((attention_weights_kernel<kDim, kBf16, 16>), many, block, stats, st, a, shift, sums4);
+    else if (s.line && pieces >= kJoinSome)
+      hipLaunchKernelGGL((attention_weights_kernel<kDim, kBf16, 4>), many, block, stats, st, a, shift, sums4);
+    else
+      hipLaunchKernelGGL((attention_weights_kernel<kDim, kBf16, 1>), few, block, stats, st, a, shift, sums4);
+    return;
+  }
+  if (!s.line) return;
   if (pieces >= kJoinMany) hipLaunchKernelGGL((attention_join_kernel<kDim, kBf16, 16>), each, dim3(1024), 0, st, a);
   else if (pieces >= kJoinSome) hipLaunchKernelGGL((attention_join_kernel<kDim, kBf16, 4>), each, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((attention_join_kernel<kDim, kBf16, 1>), fourth, dim3(256), 0, st, a);
@@ -1027,7 +1095,7 @@ static int attention_decode(const char* who, const void* q, int64_t q_seq_stride
   const AttentionShape s =
       attention_shape(cache->batch, q_heads, cache->kv_heads, cache->head_dim, cache_positions(*cache));
   // a launch has less than 2^32 threads
-  TRIS_REQUIRE(rows * (cache->head_dim / 32) < (1LL << 32) / kWave - 4 &&
+  TRIS_REQUIRE(rows * (cache->head_dim / 32) < (1LL << 32) / kWave - 4 - (weights && s.line ? 4LL * s.workgroups : 0) &&
                    s.workgroups < (1LL << 32) / (kWaves * kWave),
                "%s: too many rows", who);
   TRIS_REQUIRE(s.places < (1LL << 31) - (1 << 16), "%s: too many positions", who);
