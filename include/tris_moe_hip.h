@@ -981,8 +981,8 @@ int64_t tris_paged_attention_workspace_bytes(int32_t batch, int32_t q_heads, int
  * them, stay as they were.  fp32, in an order that depends on the sizes alone.  A head whose scores hold an infinity of
  * positive sign or a NaN makes the sums of all its keys NaN, as its softmax is; one whose scores are all -infinity adds
  * zeros.  out is tris_paged_attention_decode's.  weight_sum [batch][kv_heads][>= max_pages * page_size] fp32, strides in
- * elements over sequences and heads, positions contiguous, rows without shared memory.  workspace:
- * tris_paged_attention_weights_workspace_bytes, as above (the scores, 4 bytes for each query head and position of the
+ * elements over sequences and heads, positions contiguous, rows without shared memory; up to 1024 query heads for a kv
+ * head.  workspace: tris_paged_attention_weights_workspace_bytes, as above (the scores, 4 bytes for each query head and position of the
  * table, among it).
  */
 int tris_paged_attention_decode_weights(const void* q, int64_t q_seq_stride, int64_t q_head_stride, int32_t q_type,

@@ -842,8 +842,14 @@ __global__ __launch_bounds__(kTogether == 16 ? 1024 : 256) void attention_join_k
   join_pieces<kDim, kBf16, kTogether, (kTogether == 16 ? 16 : 4)>(a, static_cast<int>(blockIdx.x));
 }
 
+// The maximum and sum of two sets of keys together.
+__device__ __forceinline__ float2 joined(float2 x, float2 y) {
+  const float top = fmaxf(x.x, y.x), base = top == -INFINITY ? 0.0f : top;
+  return make_float2(top, x.y * __builtin_amdgcn_exp2f(x.x - base) + y.y * __builtin_amdgcn_exp2f(y.x - base));
+}
+
 // Adds the weights of a piece's keys (tiles [t0, t1) of sequence b's n positions from `first` on) to the sums of their kv
-// head, from the scores that the attention left, for all query heads of the kv head.  stats: LDS for a float2 of each.
+// head, from the scores that the attention left, for all query heads of the kv head.  stats: LDS for 1 + kWaves float2 of each.
 // A thread has four keys; the scores of eight heads and the sums are asked for a step ahead of their use, the first ones
 // before the statistics are known.
 __device__ __forceinline__ void sum_weights(const AttentionArgs& a, int b, int kvh, int n, int first, int t0, int t1,
@@ -867,23 +873,59 @@ __device__ __forceinline__ void sum_weights(const AttentionArgs& a, int b, int k
   };
   if (key < end) load(key, 0, x);
 
-  for (int h = wave; h < a.group; h += kWaves) {
-    float2 ml = {-INFINITY, 0.0f};
-    const int2 own = a.owners == nullptr
-                         ? make_int2(0, 0)
-                         : a.owners[b * (a.c.kv_heads * a.head_tiles) + kvh * a.head_tiles + h / kHeadTile];
-    if (own.x == own.y) {
-      ml = a.whole_ml[static_cast<int64_t>(b) * a.q_heads + kvh * a.group + h];
-    } else {
-      for (int w = own.x + lane; w <= own.y; w += kWave) {
-        const float2 part = a.part_ml[static_cast<int64_t>(2 * w + (w == own.x)) * a.tile_heads + h % kHeadTile];
-        const float top = fmaxf(ml.x, part.x), base = top == -INFINITY ? 0.0f : top;
-        ml = make_float2(top, ml.y * __builtin_amdgcn_exp2f(ml.x - base) + part.y * __builtin_amdgcn_exp2f(part.x - base));
+  // Each head's maximum and sum over the pieces.  Of few pieces a wavefront takes a head, a lane a piece; of many a lane takes
+  // one head and every sixteenth piece (131072 tokens, 192 pieces: the launch 11.6 us, 13.3 the other way; 16 ragged, 6
+  // pieces, 8.3, 8.9 the other way).
+  const auto owners = [&](int tile) {
+    return a.owners == nullptr ? make_int2(0, 0) : a.owners[(b * a.c.kv_heads + kvh) * a.head_tiles + tile];
+  };
+  const auto part = [&](int w, int2 own, int col) {
+    return a.part_ml[static_cast<int64_t>(2 * w + (w == own.x)) * a.tile_heads + col];
+  };
+  const float2* const whole = a.whole_ml + static_cast<int64_t>(b) * a.q_heads + kvh * a.group;
+  const auto to_stats = [&](int h, float top, float l) {
+    stats[h] = make_float2((top == -INFINITY ? 0.0f : top) - shift, l == 0.0f ? 0.0f : 1.0f / l);
+  };
+  const int2 own0 = owners(0);
+  if (own0.y - own0.x < kWave) {
+    for (int h = wave; h < a.group; h += kWaves) {
+      const int2 own = h < kHeadTile ? own0 : owners(h / kHeadTile);
+      if (own.x == own.y) {
+        const float2 ml = whole[h];
+        if (lane == 0) to_stats(h, ml.x, ml.y);
+      } else {
+        float2 ml = {-INFINITY, 0.0f};
+        for (int w = own.x + lane; w <= own.y; w += kWave) ml = joined(ml, part(w, own, h % kHeadTile));
+        const float top = wave_max_f32(ml.x);
+        const float l = wave_sum_f32(ml.y * __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.0f : top)));
+        if (lane == 0) to_stats(h, top, l);
       }
-      const float top = wave_max_f32(ml.x), base = top == -INFINITY ? 0.0f : top;
-      ml = make_float2(top, wave_sum_f32(ml.y * __builtin_amdgcn_exp2f(ml.x - base)));
     }
-    if (lane == 0) stats[h] = make_float2((ml.x == -INFINITY ? 0.0f : ml.x) - shift, ml.y == 0.0f ? 0.0f : 1.0f / ml.y);
+  } else {
+    float2* const shares = stats + a.group;  // [kWaves][group]
+    for (int tile = 0; tile < a.head_tiles; ++tile) {
+      const int col = lane % kHeadTile, heads = min(kHeadTile, a.group - tile * kHeadTile);
+      const int2 own = owners(tile);
+      float2 ml = {-INFINITY, 0.0f};
+      if (col < heads && own.x == own.y) {
+        if (thread < kHeadTile) ml = whole[tile * kHeadTile + col];
+      } else if (col < heads) {
+#pragma unroll 4
+        for (int w = own.x + thread / kHeadTile; w <= own.y; w += kWaves * kWave / kHeadTile)
+          ml = joined(ml, part(w, own, col));
+      }
+      const float top = across_groups(ml.x, [](float u, float v) { return fmaxf(u, v); });
+      const float l = across_groups(ml.y * __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.0f : top)),
+                                    [](float u, float v) { return u + v; });
+      if (lane < heads) shares[wave * a.group + tile * kHeadTile + lane] = make_float2(top, l);
+    }
+    __syncthreads();
+    for (int h = thread; h < a.group; h += kWaves * kWave) {
+      float2 ml = shares[h];
+#pragma unroll
+      for (int u = 1; u < kWaves; ++u) ml = joined(ml, shares[u * a.group + h]);
+      to_stats(h, ml.x, ml.y);
+    }
   }
   __syncthreads();
 
@@ -1013,7 +1055,7 @@ static void attention_launch(const AttentionArgs& a, const AttentionShape& s, bo
   if constexpr (kWeights) {
     const bool sums4 = aligned16(a.weight_sum) && a.sum_seq % 4 == 0 && a.sum_head % 4 == 0;
     const float shift = weight_shift(kBf16, kE4m3);
-    const size_t stats = a.group * sizeof(float2);
+    const size_t stats = (1 + kWaves) * a.group * sizeof(float2);
     const dim3 many(grid.x + each.x), few(grid.x + (s.line ? fourth.x : 0));
     if (s.line && pieces >= kJoinMany)
       hipLaunchKernelGGL((attention_weights_kernel<kDim, kBf16, 16>), many, block, stats, st, a, shift, sums4);
@@ -1064,7 +1106,7 @@ static WeightsSpace weights_space(const AttentionSpace& a, int64_t batch, int64_
 }
 
 // Query heads of a kv head that the weights' sums take: their statistics are in LDS.
-constexpr int kMostGroup = 4096;
+constexpr int kMostGroup = 1024;
 
 // Where the weights are summed.
 struct WeightSums {

@@ -288,7 +288,7 @@ def test_refusals_without_gpu(tris):
                      (dict(seq=95), b"overlap"), (dict(head=47), b"overlap"), (dict(head=0), b"overlap"),
                      (dict(seq=-96), b"overlap"), (dict(ws=None), b"workspace"), (dict(space=need - 1), b"workspace"),
                      (dict(ws=ctypes.c_void_p(4104)), b"workspace"),
-                     (dict(q_heads=2 * 4097, stride=2 * 4097 * 128), b"4096 query heads"),
+                     (dict(q_heads=2 * 1025, stride=2 * 1025 * 128), b"1024 query heads"),
                      (dict(cache=c_cache(max_pages=most, table_stride=most, k_slot_stride=128), q_heads=8, stride=1024,
                            seq=1 << 40, head=1 << 30, space=1 << 33), b"workspace")):
         assert call(**kw) == -1 and word in lib.tris_last_error(), kw
