@@ -1004,11 +1004,15 @@ int64_t tris_paged_attention_weights_workspace_bytes(int32_t batch, int32_t q_he
  * No page below an evicted sequence's length may be another sequence's, or its own twice.
  * 0 <= sink, 0 <= recent, sink + recent <= budget, 1 <= budget <= limit.  weight_sum as
  * tris_paged_attention_decode_weights takes it; new_lens [batch], apart from seq_lens; kept
- * [batch][kv_heads][budget], contiguous.  The cache's rows, scales and sums without shared memory.
+ * [batch][kv_heads][budget], contiguous.  The cache's rows, scales and sums without shared memory.  workspace:
+ * tris_paged_cache_evict_workspace_bytes of the same sizes (0: none needed), 16-byte aligned, no initial contents; calls
+ * that may overlap need one each.
  */
 int tris_paged_cache_evict(const tris_paged_cache* cache, float* weight_sum, int64_t sum_seq_stride,
                            int64_t sum_head_stride, int32_t budget, int32_t limit, int32_t sink, int32_t recent,
-                           int32_t* new_lens, int32_t* kept, void* stream);
+                           int32_t* new_lens, int32_t* kept, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t tris_paged_cache_evict_workspace_bytes(int32_t batch, int32_t kv_heads, int32_t max_pages, int32_t page_size,
+                                               int32_t budget);
 
 #ifdef __cplusplus
 }

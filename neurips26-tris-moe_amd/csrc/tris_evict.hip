@@ -1,11 +1,29 @@
 // Eviction from the paged cache by accumulated attention weight: which positions stay, and the move of what they hold.
 //
-// Two launches.  The first has a workgroup for each (sequence, kv head): it finds the weight at the border, the
-// (budget - sink - recent)-th largest between the first `sink` and the last `recent` positions, digit by digit of a key that
-// orders the weights, and lists the positions that stay, in order.  The second moves their rows down in place.
+// Which: for each (sequence, kv head) the want-th largest weight w* of those between the first `sink` and the last
+// `recent` positions, want = budget - sink - recent; above w* all stay, of those equal to it the lowest positions.  w* is
+// found digit by digit of a 32-bit key that orders the weights: 11, 11 and 10 bits, each by a histogram in LDS of the keys
+// that share the digits before.  The first digit is the sign, the exponent and two bits more, so that weights over many
+// powers of two spread over its bins (8-bit digits put two powers of two into one, and the additions wait for each other).
+//
+// Up to kSelectMost positions one workgroup has a row, its weights in registers, read once; it lists the positions that
+// stay and moves the sums as well.  Longer rows are cut into segments of a workgroup each, in three launches: histograms of
+// the first digit; the keys in the border's bin, gathered; and, in every workgroup alike, the border among those, by which
+// it places its segment.
+//
+// The move is bound by memory, 2 row reads and 2 row writes a position and kv head.
 #include "tris_paged.h"
 
 namespace tris {
+
+constexpr int kThreads = 1024;
+constexpr int kBlockWaves = kThreads / kWave;
+constexpr int kRowKeys = 16;                        // of a thread, where a workgroup has a row
+constexpr int kSelectMost = kThreads * kRowKeys;
+constexpr int kBins = 2048, kFirstShift = 21, kSecondShift = 10;
+constexpr int kMostSegments = 64;  // a lane each
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct EvictArgs {
   float* sums;
@@ -15,10 +33,17 @@ struct EvictArgs {
   int32_t* kept;
   PageDivision page_of;
   tris_paged_cache c;
+  // of rows in segments
+  int32_t segments, segment;  // how many, and positions of one
+  int32_t* state;             // [rows][kState]
+  int32_t* counts;            // [rows][segments][2]: keys above the bin; keys in it of the segments before
+  uint32_t* hist;             // [rows][segments][kBins]
+  uint32_t* found;            // [rows][segments * segment]: the keys in the bin, in order
+  float* moved;               // [rows][budget]: the sums of what stays
 };
 
-constexpr int kSelectThreads = 1024;
-constexpr int kSelectWaves = kSelectThreads / kWave;
+// Of a row in segments: whether it is left alone, the border's first digit, how many keys of its bin stay, how many it has.
+constexpr int kState = 4, kAlone = 0, kDigit = 1, kWanted = 2, kTotal = 3;
 
 // A weight as an unsigned number of the same order: NaN above all, the zeros equal.
 __device__ __forceinline__ uint32_t order_key(float w) {
@@ -31,176 +56,600 @@ __device__ __forceinline__ int evict_length(const EvictArgs& a, int b) {
   return min(max(a.c.seq_lens[b], 0), cache_positions(a.c));
 }
 
-__global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const EvictArgs a) {
-  __shared__ int hist[256];
-  __shared__ int totals[kSelectWaves];
-  __shared__ int pick, above;
+// Whether all pages of a sequence of n > 0 positions are in the pool (for the whole workgroup).
+__device__ __forceinline__ bool pages_good(const EvictArgs& a, int b, int n) {
+  const int32_t* table = a.c.block_table + b * a.c.table_stride;
+  const int last = a.page_of(n - 1);
+  bool good = true;
+  for (int i = threadIdx.x; i <= last; i += kThreads)
+    good = good && static_cast<uint32_t>(table[i]) < static_cast<uint32_t>(a.c.num_pages);
+  return __syncthreads_and(good);
+}
+
+// The bin, of kBins counted from the largest down, that holds the left-th largest key: *pick, and how many are above it.
+// count(bin): the keys in a bin.  For the whole workgroup; totals: LDS.
+struct Pick {
+  int bin, above;
+  int totals[kBlockWaves];
+};
+template <typename Count>
+__device__ __forceinline__ void pick_bin(Count count, int left, Pick* sh) {
+  const int thread = threadIdx.x, lane = thread % kWave, wave = thread / kWave;
+  const int high = kBins - 1 - 2 * thread, c0 = count(high), c1 = count(high - 1);
+  const int end = wave_incl_sum_i32(c0 + c1);
+  if (lane == kWave - 1) sh->totals[wave] = end;
+  __syncthreads();
+  int before = end - c0 - c1;
+  for (int w = 0; w < kBlockWaves; ++w) before += w < wave ? sh->totals[w] : 0;
+  if (before < left && left <= before + c0 + c1) {
+    const bool first = left <= before + c0;
+    sh->bin = first ? high : high - 1;
+    sh->above = first ? before : before + c0;
+  }
+  __syncthreads();
+}
+
+// Exclusive prefixes of kRowKeys * kBlockWaves numbers in LDS, in place, by the first wavefront.
+__device__ __forceinline__ void scan_counts(int* counts) {
+  constexpr int kEach = kRowKeys * kBlockWaves / kWave;
+  const int lane = threadIdx.x;
+  int c[kEach], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) sum += c[i] = counts[lane * kEach + i];
+  int before = wave_incl_sum_i32(sum) - sum;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    counts[lane * kEach + i] = before;
+    before += c[i];
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void evict_select_kernel(const EvictArgs a) {
+  __shared__ int hist[kBins];
+  __shared__ int counts[kRowKeys * kBlockWaves];
+  __shared__ Pick pick;
   const int row = blockIdx.x, b = row / a.c.kv_heads, h = row - b * a.c.kv_heads;
   const int thread = threadIdx.x, lane = thread % kWave, wave = thread / kWave;
   const int n = evict_length(a, b);
   int32_t* kept = a.kept + static_cast<int64_t>(row) * a.budget;
+  float* sums = a.sums + b * a.sum_seq + h * a.sum_head;
+  float w[kRowKeys];
   bool due = n > a.limit;
   if (due) {
-    const int32_t* table = a.c.block_table + b * a.c.table_stride;
-    bool good = true;
-    for (int i = thread; i <= a.page_of(n - 1); i += kSelectThreads)
-      good = good && static_cast<uint32_t>(table[i]) < static_cast<uint32_t>(a.c.num_pages);
-    due = __syncthreads_and(good);
+#pragma unroll
+    for (int j = 0; j < kRowKeys; ++j) w[j] = j * kThreads + thread < n ? sums[j * kThreads + thread] : 0.0f;
+    due = pages_good(a, b, n);
   }
   if (h == 0 && thread == 0) a.new_lens[b] = due ? a.budget : a.c.seq_lens[b];
   if (!due) {
-    for (int i = thread; i < a.budget; i += kSelectThreads) kept[i] = -1;
+    for (int i = thread; i < a.budget; i += kThreads) kept[i] = -1;
     return;
   }
-  const float* sums = a.sums + b * a.sum_seq + h * a.sum_head;
   const int lo = a.sink, hi = n - a.recent, want = a.budget - a.sink - a.recent;
-  // the key of the want-th largest between lo and hi, and how many of those equal to it stay
   uint32_t border = 0xFFFFFFFFu;
-  int equal = 0;
+  int equal = 0;  // of the keys equal to the border, how many stay
   if (want > 0) {
     uint32_t prefix = 0;
-    int left = want;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (thread < 256) hist[thread] = 0;
-      __syncthreads();
-      for (int i = lo + thread; i < hi; i += kSelectThreads) {
-        const uint32_t key = order_key(sums[i]);
-        if (shift == 24 || key >> (shift + 8) == prefix) atomicAdd(&hist[key >> shift & 255], 1);
-      }
-      __syncthreads();
-      if (wave == 0) {
-        // four digits a lane, from the largest down
-        int c[4], sum = 0;
+    equal = want;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum += c[i] = hist[255 - (lane * 4 + i)];
-        int before = wave_incl_sum_i32(sum) - sum;
+    for (int digit = 0; digit < 3; ++digit) {
+      const int shift = digit == 0 ? kFirstShift : digit == 1 ? kSecondShift : 0;
+      const int bits = digit == 2 ? 10 : 11;
+      hist[thread] = hist[thread + kThreads] = 0;
+      __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (before < left && before + c[i] >= left) {
-            pick = 255 - (lane * 4 + i);
-            above = before;
-          }
-          before += c[i];
+      for (int j = 0; j < kRowKeys; ++j) {
+        const int i = j * kThreads + thread;
+        if (j * kThreads < n && i >= lo && i < hi) {
+          const uint32_t key = order_key(w[j]);
+          if (digit == 0 || key >> (shift + bits) == prefix) atomicAdd(&hist[key >> shift & ((1 << bits) - 1)], 1);
         }
       }
       __syncthreads();
-      prefix = prefix << 8 | static_cast<uint32_t>(pick);
-      left -= above;
-      __syncthreads();
+      pick_bin([&](int bin) { return hist[bin]; }, equal, &pick);
+      prefix = prefix << bits | static_cast<uint32_t>(pick.bin);
+      equal -= pick.above;
     }
     border = prefix;
-    equal = left;
   }
-  // the positions in order: each thread's flags, the waves' counts, the places before
-  int placed = 0, ties = 0;
-  for (int i0 = 0; i0 < n; i0 += kSelectThreads) {
-    const int i = i0 + thread;
-    const bool held = i < n && (i < lo || i >= hi);
-    bool stays = held, tie = false;
-    if (want > 0 && i < n && !held) {
-      const uint32_t key = order_key(sums[i]);
-      stays = key > border;
-      tie = key == border;
+  // Of each 64 positions: how many stay for certain, and (from bit 16 on) how many are equal to the border.
+#pragma unroll
+  for (int j = 0; j < kRowKeys; ++j) {
+    const int i = j * kThreads + thread;
+    const bool middle = i >= lo && i < hi && want > 0;
+    const uint32_t key = order_key(w[j]);
+    const int sure = __popcll(__ballot(i < n && (i < lo || i >= hi || (middle && key > border))));
+    const int ties = __popcll(__ballot(middle && key == border));
+    if (lane == 0) counts[j * kBlockWaves + wave] = sure | ties << 16;
+  }
+  __syncthreads();
+  if (wave == 0) scan_counts(counts);
+  __syncthreads();
+  const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+  for (int j = 0; j < kRowKeys; ++j) {
+    if (j * kThreads >= n) break;
+    const int i = j * kThreads + thread;
+    const bool middle = i >= lo && i < hi && want > 0;
+    const uint32_t key = order_key(w[j]);
+    const bool sure = i < n && (i < lo || i >= hi || (middle && key > border)), tie = middle && key == border;
+    const int before = counts[j * kBlockWaves + wave];
+    const int sures = (before & 0xFFFF) + __popcll(__ballot(sure) & below);
+    const int ties = (before >> 16) + __popcll(__ballot(tie) & below);
+    if (sure || (tie && ties < equal)) {
+      const int place = sures + min(ties, equal);
+      kept[place] = i;
+      sums[place] = w[j];  // (every weight of the row is in registers)
     }
-    const uint64_t tied = __ballot(tie), below = (1ull << lane) - 1;
-    if (lane == 0) totals[wave] = __popcll(tied);
-    __syncthreads();
-    int rank = ties + __popcll(tied & below);
-    for (int w = 0; w < kSelectWaves; ++w) {
-      const int t = totals[w];
-      rank += w < wave ? t : 0;
-      ties += t;
+  }
+  for (int i = a.budget + thread; i < n; i += kThreads) sums[i] = 0.0f;
+}
+
+// ------------------------------------------------------------------------------------------------ rows in segments
+
+struct Segment {
+  int row, s, b, h, n, begin, end;
+  __device__ explicit Segment(const EvictArgs& a) {
+    row = blockIdx.x / a.segments;
+    s = blockIdx.x - row * a.segments;
+    b = row / a.c.kv_heads;
+    h = row - b * a.c.kv_heads;
+    n = evict_length(a, b);
+    begin = static_cast<int>(min(static_cast<int64_t>(s) * a.segment, static_cast<int64_t>(n)));
+    end = min(n, begin + a.segment);
+  }
+  __device__ int64_t index(const EvictArgs& a) const { return static_cast<int64_t>(row) * a.segments + s; }
+};
+
+// Four positions of a thread from i0 on, kThreads apart, and their weights.
+constexpr int kTileKeys = 4;
+constexpr int kTile = kTileKeys * kThreads;
+
+struct Weights {
+  float w[kTileKeys];
+  __device__ Weights(const EvictArgs& a, const Segment& g, int i0) {
+    const float* sums = a.sums + g.b * a.sum_seq + g.h * a.sum_head;
+#pragma unroll
+    for (int j = 0; j < kTileKeys; ++j) {
+      const int i = i0 + j * kThreads + static_cast<int>(threadIdx.x);
+      w[j] = i < g.end ? sums[i] : 0.0f;
+    }
+  }
+};
+
+__global__ __launch_bounds__(kThreads) void evict_histogram_kernel(const EvictArgs a) {
+  __shared__ uint32_t hist[kBins];
+  const Segment g(a);
+  const int thread = threadIdx.x;
+  hist[thread] = hist[thread + kThreads] = 0;
+  Weights now(a, g, g.begin);
+  const bool due = g.n > a.limit && pages_good(a, g.b, g.n);
+  if (g.s == 0 && thread == 0) {
+    if (g.h == 0) a.new_lens[g.b] = due ? a.budget : a.c.seq_lens[g.b];
+    a.state[kState * g.row + kAlone] = !due;
+  }
+  if (!due) {
+    int32_t* kept = a.kept + static_cast<int64_t>(g.row) * a.budget;
+    for (int i = g.s * kThreads + thread; i < a.budget; i += a.segments * kThreads) kept[i] = -1;
+    return;
+  }
+  const int lo = max(g.begin, a.sink), hi = min(g.end, g.n - a.recent);
+  for (int i0 = g.begin; i0 < hi; i0 += kTile) {
+    if (i0 > g.begin) now = Weights(a, g, i0);
+#pragma unroll
+    for (int j = 0; j < kTileKeys; ++j) {
+      const int i = i0 + j * kThreads + thread;
+      if (i >= lo && i < hi) atomicAdd(&hist[order_key(now.w[j]) >> kFirstShift], 1u);
+    }
+  }
+  __syncthreads();
+  uint32_t* out = a.hist + g.index(a) * kBins;
+  out[thread] = hist[thread];
+  out[thread + kThreads] = hist[thread + kThreads];
+}
+
+__global__ __launch_bounds__(kThreads) void evict_gather_kernel(const EvictArgs a) {
+  __shared__ Pick pick;
+  __shared__ int counts[kTileKeys * kBlockWaves];
+  __shared__ int above, offset, total;
+  const Segment g(a);
+  if (a.state[kState * g.row + kAlone]) return;
+  const int thread = threadIdx.x, lane = thread % kWave, wave = thread / kWave;
+  const int want = a.budget - a.sink - a.recent;
+  Weights now(a, g, g.begin);
+  // the row's histogram: two bins a thread, from the largest down
+  const uint32_t* row_hist = a.hist + static_cast<int64_t>(g.row) * a.segments * kBins;
+  const uint32_t* hist = row_hist + kBins - 2 - 2 * thread;
+  int c0 = 0, c1 = 0, mine0 = 0, mine1 = 0;
+#pragma unroll 8
+  for (int s = 0; s < a.segments; ++s) {
+    const uint2 c = *reinterpret_cast<const uint2*>(hist + static_cast<int64_t>(s) * kBins);
+    c0 += c.y;
+    c1 += c.x;
+    mine0 = s == g.s ? c.y : mine0;
+    mine1 = s == g.s ? c.x : mine1;
+  }
+  if (thread == 0) {
+    pick.bin = kBins;  // where nothing is wanted: no key is above it, none in it
+    pick.above = above = 0;
+  }
+  __syncthreads();
+  if (want > 0) pick_bin([&](int bin) { return bin & 1 ? c0 : c1; }, want, &pick);
+  const int bin = pick.bin, high = kBins - 1 - 2 * thread;
+  const int mine = wave_incl_sum_i32((high > bin ? mine0 : 0) + (high - 1 > bin ? mine1 : 0));
+  if (lane == kWave - 1 && mine) atomicAdd(&above, mine);
+  // the keys in the bin, of the segments before and of all
+  if (wave == 0) {
+    const int in = lane < a.segments && bin < kBins ? row_hist[static_cast<int64_t>(lane) * kBins + bin] : 0;
+    const int end = wave_incl_sum_i32(in);
+    if (lane == g.s) offset = end - in;
+    if (lane == kWave - 1) total = end;
+  }
+  __syncthreads();
+  if (thread == 0) {
+    a.counts[2 * g.index(a)] = above;
+    a.counts[2 * g.index(a) + 1] = offset;
+    if (g.s == 0) {
+      a.state[kState * g.row + kDigit] = bin;
+      a.state[kState * g.row + kWanted] = want - pick.above;
+      a.state[kState * g.row + kTotal] = total;
+    }
+  }
+  // its keys, in order
+  uint32_t* found = a.found + static_cast<int64_t>(g.row) * a.segments * a.segment;
+  const int lo = max(g.begin, a.sink), hi = min(g.end, g.n - a.recent);
+  int placed = offset;
+  for (int i0 = g.begin; i0 < hi; i0 += kTile) {
+    if (i0 > g.begin) now = Weights(a, g, i0);
+    uint64_t in[kTileKeys];
+#pragma unroll
+    for (int j = 0; j < kTileKeys; ++j) {
+      const int i = i0 + j * kThreads + thread;
+      in[j] = __ballot(i >= lo && i < hi && static_cast<int>(order_key(now.w[j]) >> kFirstShift) == bin);
+      if (lane == 0) counts[j * kBlockWaves + wave] = __popcll(in[j]);
     }
     __syncthreads();
-    stays = stays || (tie && rank < equal);
-    const uint64_t staying = __ballot(stays);
-    if (lane == 0) totals[wave] = __popcll(staying);
-    __syncthreads();
-    int place = placed + __popcll(staying & below);
-    for (int w = 0; w < kSelectWaves; ++w) {
-      const int t = totals[w];
-      place += w < wave ? t : 0;
-      placed += t;
+    const int c = counts[lane], end = wave_incl_sum_i32(c);  // (each wavefront: the tile's 64 counts)
+#pragma unroll
+    for (int j = 0; j < kTileKeys; ++j) {
+      const int before = __shfl(end - c, j * kBlockWaves + wave);
+      if (in[j] >> lane & 1) found[placed + before + __popcll(in[j] & ((1ull << lane) - 1))] = order_key(now.w[j]);
     }
+    placed += __builtin_amdgcn_readlane(end, kWave - 1);
     __syncthreads();
-    if (stays) kept[place] = i;
   }
 }
 
-// Moves the units of the positions that stay to their places, in place: a workgroup has a slice of every row of one
-// (sequence, kv head), so that no other reads what it writes.  It takes them in runs from the first place on: a place is
-// never past where its unit comes from, so what a run writes no later run reads, and its own units are in registers
-// before any is written.  at(position): a unit's address.
-constexpr int kMoveThreads = 1024;
+__global__ __launch_bounds__(kThreads) void evict_place_kernel(const EvictArgs a) {
+  __shared__ int hist[kBins];
+  __shared__ Pick pick;
+  __shared__ int before[2];      // of the segments before: positions that stay for certain, keys equal to the border
+  __shared__ int counts[kTileKeys * kBlockWaves];
+  const Segment g(a);
+  const int32_t* state = a.state + kState * g.row;
+  if (state[kAlone]) return;
+  const int thread = threadIdx.x, lane = thread % kWave, wave = thread / kWave;
+  const int first = state[kDigit], total = state[kTotal], lo = a.sink, hi = g.n - a.recent;
+  Weights now(a, g, g.begin);
+  const int2* row_counts = reinterpret_cast<const int2*>(a.counts) + static_cast<int64_t>(g.row) * a.segments;
+  const int offset = row_counts[g.s].y;
+  // every key of the row's bin, the first of a thread's in registers
+  const uint32_t* found = a.found + static_cast<int64_t>(g.row) * a.segments * a.segment;
+  uint32_t key[kTileKeys];
+#pragma unroll
+  for (int j = 0; j < kTileKeys; ++j) key[j] = j * kThreads + thread < total ? found[j * kThreads + thread] : 0u;
+  const auto each = [&](auto&& f) {
+#pragma unroll
+    for (int j = 0; j < kTileKeys; ++j)
+      if (j * kThreads + thread < total) f(j * kThreads + thread, key[j]);
+#pragma unroll 4
+    for (int i = kTile + thread; i < total; i += kThreads) f(i, found[i]);
+  };
+  if (thread < 2) before[thread] = 0;
+  __syncthreads();
+  if (thread < g.s) {
+    const int begin = static_cast<int>(min(static_cast<int64_t>(thread) * a.segment, static_cast<int64_t>(g.n)));
+    const int end = min(g.n, begin + a.segment);
+    // (and the first and last positions, which are held)
+    atomicAdd(&before[0], row_counts[thread].x + max(0, min(end, lo) - begin) + max(0, end - max(begin, hi)));
+  }
+  const bool some = first < kBins;
+  uint32_t border = 0xFFFFFFFFu;
+  int equal = 0;
+  if (some) {
+    border = static_cast<uint32_t>(first);
+    equal = state[kWanted];
+#pragma unroll
+    for (int digit = 1; digit < 3; ++digit) {
+      const int shift = digit == 1 ? kSecondShift : 0, bits = digit == 1 ? 11 : 10;
+      hist[thread] = hist[thread + kThreads] = 0;
+      __syncthreads();
+      each([&](int, uint32_t k) {
+        if (k >> (shift + bits) == border) atomicAdd(&hist[k >> shift & ((1 << bits) - 1)], 1);
+      });
+      __syncthreads();
+      pick_bin([&](int bin) { return hist[bin]; }, equal, &pick);
+      border = border << bits | static_cast<uint32_t>(pick.bin);
+      equal -= pick.above;
+    }
+    int sure = 0, ties = 0;
+    each([&](int i, uint32_t k) {
+      sure += i < offset && k > border;
+      ties += i < offset && k == border;
+    });
+    sure = wave_incl_sum_i32(sure);
+    ties = wave_incl_sum_i32(ties);
+    if (lane == kWave - 1) {
+      atomicAdd(&before[0], sure);
+      atomicAdd(&before[1], ties);
+    }
+  }
+  __syncthreads();
+  int sures = before[0], tied = before[1];
+  int32_t* kept = a.kept + static_cast<int64_t>(g.row) * a.budget;
+  float* moved = a.moved + static_cast<int64_t>(g.row) * a.budget;
+  for (int i0 = g.begin; i0 < g.end; i0 += kTile) {
+    if (i0 > g.begin) now = Weights(a, g, i0);
+    uint64_t sure[kTileKeys], tie[kTileKeys];
+#pragma unroll
+    for (int j = 0; j < kTileKeys; ++j) {
+      const int i = i0 + j * kThreads + thread;
+      const uint32_t k = order_key(now.w[j]);
+      const bool middle = some && i >= lo && i < hi;
+      sure[j] = __ballot(i < g.end && (i < lo || i >= hi || (middle && k > border)));
+      tie[j] = __ballot(i < g.end && middle && k == border);
+      if (lane == 0) counts[j * kBlockWaves + wave] = __popcll(sure[j]) | __popcll(tie[j]) << 16;
+    }
+    __syncthreads();
+    const int c = counts[lane], end = wave_incl_sum_i32(c);
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (int j = 0; j < kTileKeys; ++j) {
+      const int past = __shfl(end - c, j * kBlockWaves + wave);
+      const int t = tied + (past >> 16) + __popcll(tie[j] & below);
+      const int place = sures + (past & 0xFFFF) + __popcll(sure[j] & below) + min(t, equal);
+      const bool stays = (sure[j] >> lane & 1) || ((tie[j] >> lane & 1) && t < equal);
+      if (stays && place < a.budget) {  // (past it only if the sums change meanwhile)
+        kept[place] = i0 + j * kThreads + thread;
+        moved[place] = now.w[j];
+      }
+    }
+    const int all = __builtin_amdgcn_readlane(end, kWave - 1);
+    sures += all & 0xFFFF;
+    tied += all >> 16;
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ the move
+
+// A row of bytes or one 4-byte number of each position of one kv head: where a position's is.  Positions and pages are
+// checked again here, so that tables, lengths or sums that change meanwhile lead nowhere else.
+struct Units {
+  char* base;
+  const int32_t* table;
+  int64_t page_bytes;
+  int32_t slot_bytes, page_size, num_pages, positions;
+  PageDivision page_of;
+  __device__ bool valid(int page) const { return static_cast<uint32_t>(page) < static_cast<uint32_t>(num_pages); }
+  __device__ char* at(int i, int page) const {
+    return base + page * page_bytes + static_cast<int64_t>(i - page_of(i) * page_size) * slot_bytes;
+  }
+};
+
+// What a move's workgroup of part number `part` has of kv head h's cache: slices of the rows of keys, then of values, then
+// the scales.
+__device__ __forceinline__ Units part_units(const EvictArgs& a, int b, int h, int part, int slices, int slice_bytes) {
+  const tris_paged_cache& c = a.c;
+  const int32_t* table = c.block_table + b * c.table_stride;
+  if (part < 2 * slices) {
+    const bool v = part >= slices;
+    const int size = c.dtype == TRIS_DTYPE_E4M3 ? 1 : 2;
+    return Units{static_cast<char*>(v ? c.v : c.k) + (v ? c.v_head_stride : c.k_head_stride) * size * h +
+                     (v ? part - slices : part) * slice_bytes,
+                 table,
+                 (v ? c.v_page_stride : c.k_page_stride) * size,
+                 static_cast<int32_t>(v ? c.v_slot_stride : c.k_slot_stride) * size,
+                 c.page_size,
+                 c.num_pages,
+                 cache_positions(c),
+                 a.page_of};
+  }
+  const bool v = part > 2 * slices;
+  return Units{reinterpret_cast<char*>(v ? c.v_scale : c.k_scale) + (v ? c.v_scale_head_stride : c.k_scale_head_stride) * 4 * h,
+               table,
+               (v ? c.v_scale_page_stride : c.k_scale_page_stride) * 4,
+               static_cast<int32_t>(v ? c.v_scale_slot_stride : c.k_scale_slot_stride) * 4,
+               c.page_size,
+               c.num_pages,
+               cache_positions(c),
+               a.page_of};
+}
+
+// In place: a workgroup has a slice of every row of one (sequence, kv head), so that no other reads what it writes.  It
+// takes the rows in runs from the first place on: a place is never past where its row comes from, so what a run writes no
+// later run reads, and its own rows are in registers before any is written.  So a run's rows are asked for before the one
+// before it is stored, their pages before that, and the list before that.  Rows from `end` on are left to the second move.
 constexpr int kMoveUnits = 4;
 
-template <typename T, typename At>
-__device__ __forceinline__ void move_units(const int32_t* kept, int budget, int lanes, At at) {
-  const int thread = threadIdx.x, rows = kMoveThreads / lanes, unit = thread % lanes;
-  for (int i0 = 0; i0 < budget; i0 += rows * kMoveUnits) {
-    T x[kMoveUnits];
+template <typename T>
+__device__ __forceinline__ void shift_units(const int32_t* kept, int budget, int end, int lanes, const Units& u) {
+  const int thread = threadIdx.x, rows = kThreads / lanes, unit = thread % lanes, first = thread / lanes;
+  const int run = rows * kMoveUnits;
+  int last = budget;  // no row from here on comes from before `end`
+  if (end < INT32_MAX) {
+    const int each = (budget + kThreads - 1) / kThreads;
+    last = min(budget, each * __syncthreads_count(thread * each < budget && kept[thread * each] < end));
+  }
+  // of a unit: where its row comes from and goes (its own place: nowhere), their pages, the row
+  struct Listed {
     int from[kMoveUnits];
+  };
+  struct Paged {
+    int from[kMoveUnits], from_page[kMoveUnits], to_page[kMoveUnits];
+  };
+  const auto list = [&](int i0) {
+    Listed l;
 #pragma unroll
-    for (int u = 0; u < kMoveUnits; ++u) {
-      const int i = i0 + u * rows + thread / lanes;
-      from[u] = i < budget ? kept[i] : -1;
-      if (from[u] >= 0) x[u] = at(from[u])[unit];
+    for (int k = 0; k < kMoveUnits; ++k) {
+      const int i = i0 + k * rows + first;
+      l.from[k] = i < last ? kept[i] : i;
     }
-    // every load of the run has arrived before any wavefront stores
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+    return l;
+  };
+  const auto pages = [&](int i0, const Listed& l) {
+    Paged p;
 #pragma unroll
-    for (int u = 0; u < kMoveUnits; ++u) {
-      const int i = i0 + u * rows + thread / lanes;
-      if (from[u] >= 0 && from[u] != i) at(i)[unit] = x[u];
+    for (int k = 0; k < kMoveUnits; ++k) {
+      const int i = i0 + k * rows + first;
+      const bool moves = l.from[k] > i && l.from[k] < min(end, u.positions);
+      p.from[k] = l.from[k];
+      p.from_page[k] = moves ? u.table[u.page_of(l.from[k])] : -1;
+      p.to_page[k] = moves ? u.table[u.page_of(i)] : -1;
     }
+    return p;
+  };
+  struct Rows {
+    T x[kMoveUnits];
+    char* to[kMoveUnits];
+  };
+  const auto load = [&](int i0, const Paged& p) {
+    Rows r;
+#pragma unroll
+    for (int k = 0; k < kMoveUnits; ++k) {
+      const bool moves = u.valid(p.from_page[k]) && u.valid(p.to_page[k]);
+      r.x[k] = T{};
+      if (moves) r.x[k] = reinterpret_cast<const T*>(u.at(p.from[k], p.from_page[k]))[unit];
+      r.to[k] = moves ? u.at(i0 + k * rows + first, p.to_page[k]) : nullptr;
+    }
+    return r;
+  };
+  Listed listed = list(run);
+  Paged paged = pages(0, list(0));
+  Rows now = load(0, paged);
+  paged = pages(run, listed);
+  listed = list(2 * run);
+  for (int i0 = 0; i0 < last; i0 += run) {
+    const Paged next = pages(i0 + 2 * run, listed);
+    listed = list(i0 + 3 * run);
+    Rows ahead = load(i0 + run, paged);
+    paged = next;
+    // the run's rows have arrived in every wavefront before any stores
+#pragma unroll
+    for (int k = 0; k < kMoveUnits; ++k) asm volatile("" : "+v"(now.x[k])::"memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int k = 0; k < kMoveUnits; ++k)
+      if (now.to[k]) reinterpret_cast<T*>(now.to[k])[unit] = now.x[k];
+    now = ahead;
   }
 }
 
-constexpr int kSliceBytes = 64;
-
-__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(const EvictArgs a, int slices, int parts) {
+__global__ __launch_bounds__(kThreads) void evict_shift_kernel(const EvictArgs a, int slices, int slice_bytes, int parts,
+                                                               int end) {
   const int row = blockIdx.x / parts, part = blockIdx.x - row * parts;
   const int b = row / a.c.kv_heads, h = row - b * a.c.kv_heads;
   const int32_t* kept = a.kept + static_cast<int64_t>(row) * a.budget;
   if (kept[0] < 0) return;
-  const tris_paged_cache& c = a.c;
-  const int32_t* table = c.block_table + b * c.table_stride;
-  if (part < 2 * slices) {
-    const bool is_v = part >= slices;
-    const int size = c.dtype == TRIS_DTYPE_E4M3 ? 1 : 2;
-    const int64_t page_bytes = (is_v ? c.v_page_stride : c.k_page_stride) * size;
-    const int64_t slot_bytes = (is_v ? c.v_slot_stride : c.k_slot_stride) * size;
-    char* base = static_cast<char*>(is_v ? c.v : c.k) + (is_v ? c.v_head_stride : c.k_head_stride) * size * h +
-                 (part - (is_v ? slices : 0)) * kSliceBytes;
-    move_units<uint4>(kept, a.budget, kSliceBytes / 16, [&](int i) {
-      const int p = a.page_of(i);
-      return reinterpret_cast<uint4*>(base + table[p] * page_bytes + (i - p * c.page_size) * slot_bytes);
-    });
-  } else if (part == 2 * slices) {
-    float* sums = a.sums + b * a.sum_seq + h * a.sum_head;
-    move_units<float>(kept, a.budget, 1, [&](int i) { return sums + i; });
-    __syncthreads();
-    for (int i = a.budget + threadIdx.x, n = evict_length(a, b); i < n; i += kMoveThreads) sums[i] = 0.0f;
-  } else {
-    const bool is_v = part == 2 * slices + 2;
-    const int64_t page_stride = is_v ? c.v_scale_page_stride : c.k_scale_page_stride;
-    const int64_t slot_stride = is_v ? c.v_scale_slot_stride : c.k_scale_slot_stride;
-    float* base = is_v ? c.v_scale + h * c.v_scale_head_stride : c.k_scale + h * c.k_scale_head_stride;
-    move_units<float>(kept, a.budget, 1, [&](int i) {
-      const int p = a.page_of(i);
-      return base + table[p] * page_stride + (i - p * c.page_size) * slot_stride;
-    });
+  const Units u = part_units(a, b, h, part, slices, slice_bytes);
+  if (part < 2 * slices) shift_units<u32x4>(kept, a.budget, end, slice_bytes / 16, u);
+  else shift_units<uint32_t>(kept, a.budget, end, 1, u);
+}
+
+// From positions past the budget, which no move writes: after the first move in any order, by any number of workgroups.
+// And the sums of rows in segments.
+constexpr int kFetchUnits = 2;
+
+template <typename T>
+__device__ __forceinline__ void fetch_units(const int32_t* kept, int budget, int lanes, int i0, int step, const Units& u) {
+  const int unit = threadIdx.x % lanes;
+  for (int i = i0; i < budget; i += step * kFetchUnits) {
+    T x[kFetchUnits] = {};
+    char* to[kFetchUnits];
+    int from[kFetchUnits], from_page[kFetchUnits], to_page[kFetchUnits];
+#pragma unroll
+    for (int k = 0; k < kFetchUnits; ++k) from[k] = i + k * step < budget ? kept[i + k * step] : -1;
+#pragma unroll
+    for (int k = 0; k < kFetchUnits; ++k) {
+      const bool moves = from[k] >= budget && from[k] < u.positions;
+      from_page[k] = moves ? u.table[u.page_of(from[k])] : -1;
+      to_page[k] = moves ? u.table[u.page_of(i + k * step)] : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < kFetchUnits; ++k) {
+      const bool moves = u.valid(from_page[k]) && u.valid(to_page[k]);
+      if (moves) x[k] = reinterpret_cast<const T*>(u.at(from[k], from_page[k]))[unit];
+      to[k] = moves ? u.at(i + k * step, to_page[k]) : nullptr;
+    }
+#pragma unroll
+    for (int k = 0; k < kFetchUnits; ++k)
+      if (to[k]) reinterpret_cast<T*>(to[k])[unit] = x[k];
   }
+}
+
+constexpr int kCus = 256;
+constexpr int kFetchThreads = 256;
+constexpr int kFetchBlocks = 2048;  // of keys and values, at least, where there is work for them
+
+__global__ __launch_bounds__(kFetchThreads, 8) void evict_fetch_kernel(const EvictArgs a, int row_bytes, int parts, int splits,
+                                                                   bool rows_too) {
+  const int split = blockIdx.x % splits, unit = blockIdx.x / splits, row = unit / parts, part = unit - row * parts;
+  const int b = row / a.c.kv_heads, h = row - b * a.c.kv_heads;
+  const int32_t* kept = a.kept + static_cast<int64_t>(row) * a.budget;
+  if (kept[0] < 0) return;
+  const int thread = threadIdx.x;
+  if (part == parts - 1) {
+    if (a.segments == 0) return;
+    float* sums = a.sums + b * a.sum_seq + h * a.sum_head;
+    const float* moved = a.moved + static_cast<int64_t>(row) * a.budget;
+    const int n = evict_length(a, b);
+    for (int i = split * kFetchThreads + thread; i < n; i += splits * kFetchThreads) sums[i] = i < a.budget ? moved[i] : 0.0f;
+    return;
+  }
+  if (!rows_too) return;
+  const Units u = part_units(a, b, h, part, 1, row_bytes);
+  const int lanes = part < 2 ? row_bytes / 16 : 1, rows = kFetchThreads / lanes;
+  const int i0 = split * rows + thread / lanes, step = splits * rows;
+  if (part < 2) fetch_units<u32x4>(kept, a.budget, lanes, i0, step, u);
+  else fetch_units<uint32_t>(kept, a.budget, lanes, i0, step, u);
+}
+
+struct EvictSpace {
+  int64_t counts, hist, found, moved, bytes;
+  int segments, segment;
+};
+
+static EvictSpace evict_space(int64_t rows, int64_t positions, int64_t budget) {
+  EvictSpace s{};
+  if (positions <= kSelectMost) return s;
+  const auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+  s.segments = static_cast<int>(std::min<int64_t>(kMostSegments, (positions + kTile - 1) / kTile));
+  const int64_t each = (positions + s.segments - 1) / s.segments;
+  s.segment = static_cast<int>((each + kTile - 1) / kTile * kTile);
+  s.counts = up(rows * kState * 4);
+  s.hist = s.counts + up(rows * 2LL * s.segments * 4);
+  s.found = s.hist + rows * s.segments * kBins * 4;
+  s.moved = s.found + rows * s.segments * s.segment * 4;
+  s.bytes = s.moved + rows * budget * 4;
+  return s;
 }
 
 }  // namespace tris
 
 using namespace tris;
 
+extern "C" int64_t tris_paged_cache_evict_workspace_bytes(int32_t batch, int32_t kv_heads, int32_t max_pages,
+                                                          int32_t page_size, int32_t budget) {
+  if (batch < 1 || kv_heads < 1 || max_pages < 0 || page_size < 1 || budget < 1) return 0;
+  if (static_cast<int64_t>(batch) * kv_heads >= (1LL << 32) / kThreads) return 0;  // refused
+  return evict_space(static_cast<int64_t>(batch) * kv_heads, static_cast<int64_t>(max_pages) * page_size, budget).bytes;
+}
+
 extern "C" int tris_paged_cache_evict(const tris_paged_cache* cache, float* weight_sum, int64_t sum_seq_stride,
                                       int64_t sum_head_stride, int32_t budget, int32_t limit, int32_t sink,
-                                      int32_t recent, int32_t* new_lens, int32_t* kept, void* stream) {
+                                      int32_t recent, int32_t* new_lens, int32_t* kept, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
   const char* who = "tris_paged_cache_evict";
   if (const int rc = check_paged_cache(who, cache, cache && is_16bit(cache->dtype) ? cache->dtype : TRIS_DTYPE_F16))
     return rc;
@@ -214,15 +663,44 @@ extern "C" int tris_paged_cache_evict(const tris_paged_cache* cache, float* weig
   TRIS_REQUIRE(cache_rows_apart(c), "%s: cache rows overlap", who);
   TRIS_REQUIRE(cache_scales_apart(c), "%s: cache scales overlap", who);
   TRIS_REQUIRE(sum_rows_apart(c, sum_seq_stride, sum_head_stride), "%s: rows of weight_sum overlap", who);
-  const int slices = c.head_dim * (c.dtype == TRIS_DTYPE_E4M3 ? 1 : 2) / kSliceBytes;
-  const int parts = 2 * slices + (c.dtype == TRIS_DTYPE_E4M3 ? 3 : 1);
-  const int64_t rows = static_cast<int64_t>(c.batch) * c.kv_heads;
-  TRIS_REQUIRE(rows * parts < (1LL << 32) / kMoveThreads, "%s: too many rows", who);  // a launch has less than 2^32 threads
-  const EvictArgs a{weight_sum, sum_seq_stride, sum_head_stride, budget, limit, sink, recent, new_lens, kept,
-                    PageDivision(c.page_size), c};
+  const int64_t rows = static_cast<int64_t>(c.batch) * c.kv_heads, positions = cache_positions(c);
+  const bool e4m3 = c.dtype == TRIS_DTYPE_E4M3;
+  const int row_bytes = c.head_dim * (e4m3 ? 1 : 2);
+  // slices of 128 bytes where they occupy the GPU, else of 64
+  const int slice_bytes = row_bytes >= 128 && rows * 2 * (row_bytes / 128) >= kCus ? 128 : 64;
+  const int slices = row_bytes / slice_bytes, parts = 2 * slices + (e4m3 ? 2 : 0);
+  const EvictSpace s = evict_space(rows, positions, budget);
+  // rows may come from past the budget in numbers, and one workgroup a slice leaves the GPU idle
+  const bool far = positions >= 2LL * budget && rows * 2 * slices < 2 * kCus;
+  const int fetch_parts = (e4m3 ? 4 : 2) + 1;
+  const int splits = static_cast<int>(std::min<int64_t>(256, std::max<int64_t>(1, kFetchBlocks / (rows * 2))));
+  // a launch has less than 2^32 threads
+  TRIS_REQUIRE(rows * std::max(parts, s.segments) < (1LL << 32) / kThreads &&
+                   rows * fetch_parts * splits < (1LL << 32) / kFetchThreads,
+               "%s: too many rows", who);
+  TRIS_REQUIRE(s.bytes == 0 || (workspace && aligned16(workspace) && workspace_bytes >= s.bytes),
+               "%s: workspace of %lld bytes needed", who, static_cast<long long>(s.bytes));
+  EvictArgs a{weight_sum, sum_seq_stride, sum_head_stride, budget, limit, sink, recent, new_lens, kept,
+              PageDivision(c.page_size), c, s.segments, s.segment, nullptr, nullptr, nullptr, nullptr, nullptr};
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(evict_select_kernel, dim3(static_cast<unsigned>(rows)), dim3(kSelectThreads), 0, st, a);
-  hipLaunchKernelGGL(evict_move_kernel, dim3(static_cast<unsigned>(rows * parts)), dim3(kMoveThreads), 0, st, a, slices,
-                     parts);
+  if (s.segments == 0) {
+    hipLaunchKernelGGL(evict_select_kernel, dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, st, a);
+  } else {
+    char* at = static_cast<char*>(workspace);
+    a.state = reinterpret_cast<int32_t*>(at);
+    a.counts = reinterpret_cast<int32_t*>(at + s.counts);
+    a.hist = reinterpret_cast<uint32_t*>(at + s.hist);
+    a.found = reinterpret_cast<uint32_t*>(at + s.found);
+    a.moved = reinterpret_cast<float*>(at + s.moved);
+    const dim3 grid(static_cast<unsigned>(rows * s.segments)), block(kThreads);
+    hipLaunchKernelGGL(evict_histogram_kernel, grid, block, 0, st, a);
+    hipLaunchKernelGGL(evict_gather_kernel, grid, block, 0, st, a);
+    hipLaunchKernelGGL(evict_place_kernel, grid, block, 0, st, a);
+  }
+  hipLaunchKernelGGL(evict_shift_kernel, dim3(static_cast<unsigned>(rows * parts)), dim3(kThreads), 0, st, a, slices,
+                     slice_bytes, parts, far ? budget : INT32_MAX);
+  if (far || s.segments)
+    hipLaunchKernelGGL(evict_fetch_kernel, dim3(static_cast<unsigned>(rows * fetch_parts * splits)), dim3(kFetchThreads), 0,
+                       st, a, row_bytes, fetch_parts, splits, far);
   return check_launch(who);
 }

@@ -244,7 +244,8 @@ SIGNATURES = {
     "tris_paged_attention_decode_weights": (ctypes.c_int, [_P, _I64, _I64, _I32, _I32, _PPC, ctypes.c_float, _I32, _P,
                                                            _I64, _I64, _P, _I64, _I64, _P, _I64, _P]),
     "tris_paged_attention_weights_workspace_bytes": (_I64, [_I32] * 6),
-    "tris_paged_cache_evict": (ctypes.c_int, [_PPC, _P, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P, _P]),
+    "tris_paged_cache_evict": (ctypes.c_int, [_PPC, _P, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _I64, _P]),
+    "tris_paged_cache_evict_workspace_bytes": (_I64, [_I32] * 5),
 }
 
 _lib = None

@@ -2400,8 +2400,11 @@ def paged_cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table:
     _refuse_gradient(who, k_cache, v_cache, k_scale, v_scale, weight_sum)
     new_lens = torch.empty_like(seq_lens)
     kept = torch.empty((batch, heads, budget), dtype=torch.int32, device=k_cache.device)
-    rc = _launch(index, _lib.load().tris_paged_cache_evict, cache, *sums, budget, min(limit, _INT32_MAX), sink, recent,
-                 new_lens.data_ptr(), kept.data_ptr(), torch._C._cuda_getCurrentRawStream(index))
+    lib = _lib.load()
+    need = lib.tris_paged_cache_evict_workspace_bytes(batch, heads, max_pages, page, budget)
+    ws = torch.empty(need, dtype=torch.uint8, device=k_cache.device) if need else None  # of this call alone
+    rc = _launch(index, lib.tris_paged_cache_evict, cache, *sums, budget, min(limit, _INT32_MAX), sink, recent,
+                 new_lens.data_ptr(), kept.data_ptr(), _ptr(ws), need, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, "tris_paged_cache_evict")
     return new_lens, kept

@@ -110,12 +110,40 @@ def test_long_sequences(tris, cuda, heads, lengths, budget):
 
 
 @pytest.mark.gpu
-def test_special_weights_and_ties(tris, cuda):
+@pytest.mark.parametrize("lengths,budget,limit,sink,recent", [
+    ([20000, 16385, 15000, 0, 18000], 15000, 16000, 4, 3000), ([40000], 4096, None, 0, 0), ([33000, 40], 9000, None, 4500, 4500),
+    ([300000], 20000, None, 64, 1000), ([16384, 16383], 16380, None, 1, 1), ([20000], 19999, None, 9000, 9000)], ids=str)
+def test_rows_in_segments(tris, cuda, lengths, budget, limit, sink, recent):
+    """Tables of more positions than one workgroup takes; budgets beside and below half of them."""
+    for cache, page in ((BF16, 64), (E4M3, 7)):
+        print(f"[gpu-case] evict segments {cache} {lengths} budget={budget}", flush=True)
+        a = evict_case(cuda, 1, 64, cache, page, lengths, seed=budget, extra=1)
+        run_and_check(tris, a, budget, limit, sink, recent)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [16384, 30000])
+def test_ties_over_segments(tris, cuda, n):
+    """The border among equal weights that lie in every segment, one segment, or are all there is."""
+    a = evict_case(cuda, 4, 64, F16, 16, [n], extra_pages=0)
+    w = a["weight_sum"]
+    w[0, 0] = 0.5
+    w[0, 1] = 0.0
+    w[0, 1, 9000:9100] = 1.0
+    w[0, 2, ::3], w[0, 2, 1::3], w[0, 2, 2::3] = 2.0, 1.0, 3.0
+    w[0, 3] = float("nan")
+    w[0, 3, 5::5] = float("inf")
+    run_and_check(tris, a, n // 2 + 77, None, 3, 500)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("extra_pages", [1, 1100])
+def test_special_weights_and_ties(tris, cuda, extra_pages):
     """All equal, zeros of both signs, subnormals, negative ones, infinities and NaN of either sign; ties at the border go
-    to the lowest positions."""
+    to the lowest positions.  The same in a table wide enough for rows in segments."""
     inf, nan = float("inf"), float("nan")
     lengths = [3000, 500, 300, 64, 200, 400]
-    a = evict_case(cuda, 2, 64, F16, 16, lengths)
+    a = evict_case(cuda, 2, 64, F16, 16, lengths, extra_pages=extra_pages)
     w = a["weight_sum"]
     w[0] = 0.25
     w[1, :, ::2], w[1, :, 1::2] = 0.0, -0.0
@@ -273,20 +301,28 @@ def test_refusals_without_gpu(tris):
 
     lib, p = _lib.load(), ctypes.c_void_p(4096)
 
-    def call(cache=None, sums=p, seq=96, head=48, budget=8, limit=8, sink=1, recent=2, lens=ctypes.c_void_p(8192), kept=p):
+    def call(cache=None, sums=p, seq=96, head=48, budget=8, limit=8, sink=1, recent=2, lens=ctypes.c_void_p(8192), kept=p,
+             ws=None, space=0):
         return lib.tris_paged_cache_evict(ctypes.byref(cache or c_cache()), sums, seq, head, budget, limit, sink, recent, lens,
-                                          kept, None)
+                                          kept, ws, space, None)
 
     for kw, word in BAD_CACHES:
         if "dtype" not in kw or kw["dtype"] == 3:
             assert call(c_cache(**kw)) == -1 and word in lib.tris_last_error(), kw
     most = 2 ** 31 - 1
+    need = lib.tris_paged_cache_evict_workspace_bytes(2, 2, 1025, 16, 8)
+    assert need > 4 * 16400 * 4 and lib.tris_paged_cache_evict_workspace_bytes(2, 2, 1024, 16, 8) == 0
+    wide = dict(cache=c_cache(max_pages=1025, table_stride=1025), seq=32800, head=16400, ws=p, space=need)
+    for bad in ((0, 2, 1025, 16, 8), (2, 0, 1025, 16, 8), (2, 2, -1, 16, 8), (2, 2, 1025, 0, 8), (2, 2, 1025, 16, 0)):
+        assert lib.tris_paged_cache_evict_workspace_bytes(*bad) == 0
     for kw, word in ((dict(budget=0, limit=0), b"budget"), (dict(limit=7), b"budget"), (dict(sink=-1), b"within"),
                      (dict(recent=-1), b"within"), (dict(sink=7), b"within"), (dict(sink=most, recent=most), b"within"),
                      (dict(sums=None), b"null"), (dict(lens=None), b"null"), (dict(kept=None), b"null"),
                      (dict(lens=p), b"seq_lens"), (dict(seq=95), b"overlap"), (dict(head=47), b"overlap"),
                      (dict(seq=-96), b"overlap"), (dict(cache=c_cache(dtype=2)), b"e4m3"),
                      (dict(cache=c_cache(k_head_stride=0)), b"rows overlap"), (dict(cache=c_cache(v_page_stride=2048)), b"rows overlap"),
-                     (dict(cache=c_cache(batch=1 << 26)), b"too many rows")):
+                     (dict(cache=c_cache(batch=1 << 26)), b"too many rows"),
+                     (dict(wide, ws=None), b"workspace"), (dict(wide, space=need - 1), b"workspace"),
+                     (dict(wide, ws=ctypes.c_void_p(4104)), b"workspace")):
         assert call(**kw) == -1 and word in lib.tris_last_error(), (kw, lib.tris_last_error())
     assert call(c_cache(batch=0)) == 0
