@@ -18,6 +18,7 @@
 namespace tris {
 
 constexpr int kMaxAxes = TRIS_MAX_ROTARY_AXES;
+constexpr int kMostPairs = 128;  // of the widest head
 
 struct AppendArgs {
   const uint16_t* q;
@@ -116,6 +117,7 @@ __global__ __launch_bounds__(256) void rotary_append_kernel(const AppendArgs a) 
     ys[i] = *reinterpret_cast<const uint4*>(src + (is_q || is_k ? hi_qk : hi_v));
   }
 
+  __shared__ float sh_cos[kAxes ? 4 : 1][kAxes ? kMostPairs : 1], sh_sin[kAxes ? 4 : 1][kAxes ? kMostPairs : 1];
   // the table rows of the token's angles
   int64_t at_row[kAxes ? kMaxAxes : 1];
   bool turnable = true;
@@ -140,15 +142,29 @@ __global__ __launch_bounds__(256) void rotary_append_kernel(const AppendArgs a) 
     const int i = a.page_of(pos);
     page = a.c.block_table[seq * a.c.table_stride + i];
     slot = pos - i * a.c.page_size;
-    if (kAxes && turning) {
+    if constexpr (kAxes) {
+      // each pair's angle once for the wavefront, handed to the lanes that turn it through LDS
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int axis = pair_axis(a, lo_qk + e);
-        int64_t row = at_row[0];
+      for (int u = 0; u < kMostPairs / kWave; ++u) {
+        const int pair = u * kWave + lane;
+        if (pair < half) {
+          const int axis = pair_axis(a, pair);
+          int64_t row = at_row[0];
 #pragma unroll
-        for (int n = 1; n < kMaxAxes; ++n) row = axis == n ? at_row[kAxes ? n : 0] : row;
-        cs[e] = a.cos[row * half + lo_qk + e];
-        sn[e] = a.sin[row * half + lo_qk + e];
+          for (int n = 1; n < kMaxAxes; ++n) row = axis == n ? at_row[n] : row;
+          sh_cos[threadIdx.x / kWave][pair] = a.cos[row * half + pair];
+          sh_sin[threadIdx.x / kWave][pair] = a.sin[row * half + pair];
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      if (turning) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          cs[e] = sh_cos[threadIdx.x / kWave][lo_qk + e];
+          sn[e] = sh_sin[threadIdx.x / kWave][lo_qk + e];
+        }
       }
     } else if (turning) {
       const float* c = a.cos + static_cast<int64_t>(pos) * half + lo_qk;
