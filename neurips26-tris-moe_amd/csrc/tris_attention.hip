@@ -75,7 +75,12 @@ struct AttentionArgs {
   float2* whole_ml;                  // [batch][q_heads]: maximum and sum of what one workgroup had whole
   float* weight_sum;
   int64_t sum_seq, sum_head;
+  int32_t sums4;                     // the sums' rows can be read four at a time
 };
+
+// Whether a workgroup of the attention adds the weights of what it has itself: it has a kv head's keys and query heads
+// whole.
+__host__ __device__ inline bool own_weights(const AttentionArgs& a) { return a.owners == nullptr && a.head_tiles == 1; }
 
 // a value that every lane holds alike, moved to a scalar register
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -698,150 +703,6 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
   write_piece<kDim, kBf16, kE4m3, kWeights>(a, p, thread, m, l, acc, lds);
 }
 
-template <int kDim, bool kBf16, bool kE4m3, bool kRowRuns, bool kWeights>
-__global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_decode_kernel(const AttentionArgs args) {
-  __shared__ u32x4 sh_q[query_in_lds(kDim) ? kDim / 32 : 1][kWave];
-  extern __shared__ float lds[];
-  const int head_groups = args.c.kv_heads * args.head_tiles, w = blockIdx.x;
-  Stretch st;
-  if (!(args.owners == nullptr ? own_stretch(args, head_groups, w, &st) : line_stretch(args, head_groups, w, &st)))
-    return;
-  int at = st.at, begin = st.begin, b = st.b, n = st.n;
-  const int stop = st.stop;
-  // one piece of a (sequence, head group) after the other
-  while (at < stop && b < args.c.batch) {
-    // What a piece needs of the arguments and of the lane's number is taken anew for each: kept in registers from piece
-    // to piece, it would cost the tiles' loop a third of its wavefronts.
-    int thread = threadIdx.x;
-    KernelArgs fresh = (KernelArgs)__builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+v"(thread), "+s"(fresh));
-    const AttentionArgs& a = *(const AttentionArgs*)fresh;
-    const int first = range_begin(a, n), tiles = range_tiles(n, first), span = tiles + kPieceCost;
-    const int hg = (at - begin) / span, from = at - begin - hg * span;
-    if (hg == head_groups) {  // the next sequence
-      begin = at;
-      n = uniform(sequence_length(a, ++b));
-      continue;
-    }
-    if (from >= tiles) {  // between two head groups
-      at += span - from;
-      continue;
-    }
-    if (a.owners != nullptr && from == 0 && thread == 0)
-      a.owners[b * head_groups + hg] = make_int2(w, st.line.owner(at + tiles - 1));
-    const int count = min(tiles - from, stop - at), t0 = first / kTileKeys + from;
-    // a piece that begins its (sequence, head group) and is not all of it ends its workgroup's stretch: the second slot
-    const Piece p{b, n, first, hg, t0, t0 + count, at, 2 * w + (from == 0), count == tiles};
-    attend_piece<kDim, kBf16, kE4m3, kRowRuns, kWeights>(a, p, thread, sh_q, lds);
-    at += count;
-    __syncthreads();  // the next piece's sums go where this one's are read
-  }
-}
-
-// Pieces of a (sequence, head group) on average, from which a join takes 16 or 4 wavefronts for the same dimensions (16 /
-// 4 / 1 together: 192 pieces, 128k, 50.8 / 51.0 / 54.4 us; 32 pieces, wide, 33.0 / 30.0 / 30.7; 9 pieces, 1000 tokens,
-// 9.7 / 9.4 / 9.1; 6 pieces, ragged, 30.6 / 24.5 / 24.2; 1.5 pieces, 64 on e4m3, 177 / 145 / 138).
-constexpr int kJoinMany = 64, kJoinSome = 16;
-
-// A lane's share of a join: the running maximum, sum and four dimensions' sums, and another's added to them.
-struct Part {
-  float m, l;
-  f32x4 o;
-  __device__ __forceinline__ void add(float m2, float l2, f32x4 o2) {
-    const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top;
-    const float f = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
-    m = top;
-    l = l * f + l2 * f2;
-    o = o * f + o2 * f2;
-  }
-  // over the wavefront's lanes of the same dimensions
-  __device__ __forceinline__ void across() {
-#pragma unroll
-    for (int d = 8; d < kWave; d *= 2) {
-      const f32x4 o2 = {__shfl_xor(o[0], d), __shfl_xor(o[1], d), __shfl_xor(o[2], d), __shfl_xor(o[3], d)};
-      const float m2 = __shfl_xor(m, d), l2 = __shfl_xor(l, d);
-      // (in the same order on both sides, so that both get the same bits)
-      if (threadIdx.x & d) {
-        Part other{m2, l2, o2};
-        other.add(m, l, o);
-        *this = other;
-      } else {
-        add(m2, l2, o2);
-      }
-    }
-  }
-};
-
-// Joins the pieces of one (sequence, query head), 32 dimensions a wavefront: eight lanes a piece, eight pieces at a time.
-// kTogether: 16 or 4 shares of the pieces for the same dimensions, by kJoinWaves wavefronts, or (1) four wavefronts on
-// dimensions of their own.
-template <int kDim, bool kBf16, int kTogether, int kJoinWaves>
-__device__ __forceinline__ void join_pieces(const AttentionArgs& a, int block) {
-  constexpr int kParts = kDim / 32;
-  constexpr bool kMany = kTogether > 1;
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const int unit = block * (kMany ? 1 : 4) + (kMany ? 0 : wave);
-  const int row = unit / kParts, d = unit % kParts * 32 + lane % 8 * 4;
-  const int b = row / a.q_heads, h = row % a.q_heads;
-  if (b >= a.c.batch) return;
-  const int hg = h / a.group * a.head_tiles + h % a.group / kHeadTile, in = h % a.group % kHeadTile;
-  const int2 owners = a.owners[b * (a.c.kv_heads * a.head_tiles) + hg];
-  if (owners.x == owners.y) return;
-  constexpr int kShares = kMany ? kTogether / kJoinWaves : 1;  // of a wavefront
-  Part p[kShares];
-#pragma unroll
-  for (int u = 0; u < kShares; ++u) {
-    p[u] = Part{-INFINITY, 0.0f, f32x4{0, 0, 0, 0}};
-#pragma unroll 2
-    for (int w = owners.x + (kMany ? (wave + u * kJoinWaves) * 8 : 0) + lane / 8; w <= owners.y; w += 8 * kTogether) {
-      const int64_t r = static_cast<int64_t>(2 * w + (w == owners.x)) * a.tile_heads + in;
-      const float2 ml = a.part_ml[r];
-      p[u].add(ml.x, ml.y, *reinterpret_cast<const f32x4*>(a.part_o + r * kDim + d));
-    }
-    p[u].across();
-  }
-  if constexpr (kMany) {
-    __shared__ Part sh[kTogether][8];
-#pragma unroll
-    for (int u = 0; u < kShares; ++u)
-      if (lane < 8) sh[wave + u * kJoinWaves][lane] = p[u];
-    __syncthreads();
-    if (wave != 0) return;
-    p[0] = lane / 8 < kTogether ? sh[lane / 8 % kTogether][lane % 8] : Part{-INFINITY, 0.0f, f32x4{0, 0, 0, 0}};
-    if constexpr (kTogether > 8) {
-      const Part q = sh[lane / 8 + 8][lane % 8];
-      p[0].add(q.m, q.l, q.o);
-    }
-    p[0].across();
-  }
-  if (lane >= 8) return;
-  Part& sum = p[0];
-  // A factor of zero has made a piece's infinite sum NaN: the weights that it stands for are above zero, so that the whole
-  // is that of the infinite sums alone.
-  const bool lost = sum.o[0] != sum.o[0] || sum.o[1] != sum.o[1] || sum.o[2] != sum.o[2] || sum.o[3] != sum.o[3];
-  if (lost && sum.l > 0.0f && sum.l < INFINITY) {
-    f32x4 infinite = {0, 0, 0, 0};
-#pragma unroll 1
-    for (int w = owners.x; w <= owners.y; ++w) {
-      const int64_t r = static_cast<int64_t>(2 * w + (w == owners.x)) * a.tile_heads + in;
-      const f32x4 o = *reinterpret_cast<const f32x4*>(a.part_o + r * kDim + d);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) infinite[i] += fabsf(o[i]) < INFINITY ? 0.0f : o[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sum.o[i] = sum.o[i] != sum.o[i] && infinite[i] != 0.0f ? infinite[i] : sum.o[i];
-  }
-  const f32x4 y = sum.o * (sum.l == 0.0f ? 0.0f : 1.0f / sum.l);
-  const uint2 packed = kBf16 ? make_uint2(pack_bf16_rne(y[0], y[1]), pack_bf16_rne(y[2], y[3]))
-                             : make_uint2(pack_f16_rne(y[0], y[1]), pack_f16_rne(y[2], y[3]));
-  *reinterpret_cast<uint2*>(a.out + b * a.out_seq + h * a.out_head + d) = packed;
-}
-
-template <int kDim, bool kBf16, int kTogether>
-__global__ __launch_bounds__(kTogether == 16 ? 1024 : 256) void attention_join_kernel(const AttentionArgs a) {
-  join_pieces<kDim, kBf16, kTogether, (kTogether == 16 ? 16 : 4)>(a, static_cast<int>(blockIdx.x));
-}
-
 // The maximum and sum of two sets of keys together.
 __device__ __forceinline__ float2 joined(float2 x, float2 y) {
   const float top = fmaxf(x.x, y.x), base = top == -INFINITY ? 0.0f : top;
@@ -853,7 +714,8 @@ __device__ __forceinline__ float2 joined(float2 x, float2 y) {
 // A thread has four keys; the scores of eight heads and the sums are asked for a step ahead of their use, the first ones
 // before the statistics are known.
 __device__ __forceinline__ void sum_weights(const AttentionArgs& a, int b, int kvh, int n, int first, int t0, int t1,
-                                            float shift, bool sums4, float2* stats) {
+                                            float shift, float2* stats) {
+  const bool sums4 = a.sums4 != 0;
   constexpr int kStep = 8;
   const int thread = threadIdx.x, wave = uniform(thread / kWave), lane = thread % kWave;
   const int32_t* table = a.c.block_table + b * a.c.table_stride;
@@ -964,13 +826,159 @@ __device__ __forceinline__ void sum_weights(const AttentionArgs& a, int b, int k
   }
 }
 
+template <int kDim, bool kBf16, bool kE4m3, bool kRowRuns, bool kWeights>
+__global__ __launch_bounds__(kWaves * kWave, resident(kDim)) void attention_decode_kernel(const AttentionArgs args) {
+  __shared__ u32x4 sh_q[query_in_lds(kDim) ? kDim / 32 : 1][kWave];
+  extern __shared__ float lds[];
+  const int head_groups = args.c.kv_heads * args.head_tiles, w = blockIdx.x;
+  Stretch st;
+  if (!(args.owners == nullptr ? own_stretch(args, head_groups, w, &st) : line_stretch(args, head_groups, w, &st)))
+    return;
+  int at = st.at, begin = st.begin, b = st.b, n = st.n;
+  const int stop = st.stop;
+  // one piece of a (sequence, head group) after the other
+  while (at < stop && b < args.c.batch) {
+    // What a piece needs of the arguments and of the lane's number is taken anew for each: kept in registers from piece
+    // to piece, it would cost the tiles' loop a third of its wavefronts.
+    int thread = threadIdx.x;
+    KernelArgs fresh = (KernelArgs)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+v"(thread), "+s"(fresh));
+    const AttentionArgs& a = *(const AttentionArgs*)fresh;
+    const int first = range_begin(a, n), tiles = range_tiles(n, first), span = tiles + kPieceCost;
+    const int hg = (at - begin) / span, from = at - begin - hg * span;
+    if (hg == head_groups) {  // the next sequence
+      begin = at;
+      n = uniform(sequence_length(a, ++b));
+      continue;
+    }
+    if (from >= tiles) {  // between two head groups
+      at += span - from;
+      continue;
+    }
+    if (a.owners != nullptr && from == 0 && thread == 0)
+      a.owners[b * head_groups + hg] = make_int2(w, st.line.owner(at + tiles - 1));
+    const int count = min(tiles - from, stop - at), t0 = first / kTileKeys + from;
+    // a piece that begins its (sequence, head group) and is not all of it ends its workgroup's stretch: the second slot
+    const Piece p{b, n, first, hg, t0, t0 + count, at, 2 * w + (from == 0), count == tiles};
+    attend_piece<kDim, kBf16, kE4m3, kRowRuns, kWeights>(a, p, thread, sh_q, lds);
+    at += count;
+    __syncthreads();  // the next piece's sums go where this one's are read
+    if constexpr (kWeights) {
+      if (own_weights(a) && n > 0)
+        sum_weights(a, b, hg, n, first, t0, t0 + count, weight_shift(kBf16, kE4m3), reinterpret_cast<float2*>(lds));
+    }
+  }
+}
+
+// Pieces of a (sequence, head group) on average, from which a join takes 16 or 4 wavefronts for the same dimensions (16 /
+// 4 / 1 together: 192 pieces, 128k, 50.8 / 51.0 / 54.4 us; 32 pieces, wide, 33.0 / 30.0 / 30.7; 9 pieces, 1000 tokens,
+// 9.7 / 9.4 / 9.1; 6 pieces, ragged, 30.6 / 24.5 / 24.2; 1.5 pieces, 64 on e4m3, 177 / 145 / 138).
+constexpr int kJoinMany = 64, kJoinSome = 16;
+
+// A lane's share of a join: the running maximum, sum and four dimensions' sums, and another's added to them.
+struct Part {
+  float m, l;
+  f32x4 o;
+  __device__ __forceinline__ void add(float m2, float l2, f32x4 o2) {
+    const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top;
+    const float f = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
+    m = top;
+    l = l * f + l2 * f2;
+    o = o * f + o2 * f2;
+  }
+  // over the wavefront's lanes of the same dimensions
+  __device__ __forceinline__ void across() {
+#pragma unroll
+    for (int d = 8; d < kWave; d *= 2) {
+      const f32x4 o2 = {__shfl_xor(o[0], d), __shfl_xor(o[1], d), __shfl_xor(o[2], d), __shfl_xor(o[3], d)};
+      const float m2 = __shfl_xor(m, d), l2 = __shfl_xor(l, d);
+      // (in the same order on both sides, so that both get the same bits)
+      if (threadIdx.x & d) {
+        Part other{m2, l2, o2};
+        other.add(m, l, o);
+        *this = other;
+      } else {
+        add(m2, l2, o2);
+      }
+    }
+  }
+};
+
+// Joins the pieces of one (sequence, query head), 32 dimensions a wavefront: eight lanes a piece, eight pieces at a time.
+// kTogether: 16 or 4 shares of the pieces for the same dimensions, by kJoinWaves wavefronts, or (1) four wavefronts on
+// dimensions of their own.
+template <int kDim, bool kBf16, int kTogether, int kJoinWaves>
+__device__ __forceinline__ void join_pieces(const AttentionArgs& a, int block) {
+  constexpr int kParts = kDim / 32;
+  constexpr bool kMany = kTogether > 1;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int unit = block * (kMany ? 1 : 4) + (kMany ? 0 : wave);
+  const int row = unit / kParts, d = unit % kParts * 32 + lane % 8 * 4;
+  const int b = row / a.q_heads, h = row % a.q_heads;
+  if (b >= a.c.batch) return;
+  const int hg = h / a.group * a.head_tiles + h % a.group / kHeadTile, in = h % a.group % kHeadTile;
+  const int2 owners = a.owners[b * (a.c.kv_heads * a.head_tiles) + hg];
+  if (owners.x == owners.y) return;
+  constexpr int kShares = kMany ? kTogether / kJoinWaves : 1;  // of a wavefront
+  Part p[kShares];
+#pragma unroll
+  for (int u = 0; u < kShares; ++u) {
+    p[u] = Part{-INFINITY, 0.0f, f32x4{0, 0, 0, 0}};
+#pragma unroll 2
+    for (int w = owners.x + (kMany ? (wave + u * kJoinWaves) * 8 : 0) + lane / 8; w <= owners.y; w += 8 * kTogether) {
+      const int64_t r = static_cast<int64_t>(2 * w + (w == owners.x)) * a.tile_heads + in;
+      const float2 ml = a.part_ml[r];
+      p[u].add(ml.x, ml.y, *reinterpret_cast<const f32x4*>(a.part_o + r * kDim + d));
+    }
+    p[u].across();
+  }
+  if constexpr (kMany) {
+    __shared__ Part sh[kTogether][8];
+#pragma unroll
+    for (int u = 0; u < kShares; ++u)
+      if (lane < 8) sh[wave + u * kJoinWaves][lane] = p[u];
+    __syncthreads();
+    if (wave != 0) return;
+    p[0] = lane / 8 < kTogether ? sh[lane / 8 % kTogether][lane % 8] : Part{-INFINITY, 0.0f, f32x4{0, 0, 0, 0}};
+    if constexpr (kTogether > 8) {
+      const Part q = sh[lane / 8 + 8][lane % 8];
+      p[0].add(q.m, q.l, q.o);
+    }
+    p[0].across();
+  }
+  if (lane >= 8) return;
+  Part& sum = p[0];
+  // A factor of zero has made a piece's infinite sum NaN: the weights that it stands for are above zero, so that the whole
+  // is that of the infinite sums alone.
+  const bool lost = sum.o[0] != sum.o[0] || sum.o[1] != sum.o[1] || sum.o[2] != sum.o[2] || sum.o[3] != sum.o[3];
+  if (lost && sum.l > 0.0f && sum.l < INFINITY) {
+    f32x4 infinite = {0, 0, 0, 0};
+#pragma unroll 1
+    for (int w = owners.x; w <= owners.y; ++w) {
+      const int64_t r = static_cast<int64_t>(2 * w + (w == owners.x)) * a.tile_heads + in;
+      const f32x4 o = *reinterpret_cast<const f32x4*>(a.part_o + r * kDim + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) infinite[i] += fabsf(o[i]) < INFINITY ? 0.0f : o[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum.o[i] = sum.o[i] != sum.o[i] && infinite[i] != 0.0f ? infinite[i] : sum.o[i];
+  }
+  const f32x4 y = sum.o * (sum.l == 0.0f ? 0.0f : 1.0f / sum.l);
+  const uint2 packed = kBf16 ? make_uint2(pack_bf16_rne(y[0], y[1]), pack_bf16_rne(y[2], y[3]))
+                             : make_uint2(pack_f16_rne(y[0], y[1]), pack_f16_rne(y[2], y[3]));
+  *reinterpret_cast<uint2*>(a.out + b * a.out_seq + h * a.out_head + d) = packed;
+}
+
+template <int kDim, bool kBf16, int kTogether>
+__global__ __launch_bounds__(kTogether == 16 ? 1024 : 256) void attention_join_kernel(const AttentionArgs a) {
+  join_pieces<kDim, kBf16, kTogether, (kTogether == 16 ? 16 : 4)>(a, static_cast<int>(blockIdx.x));
+}
+
 // The second launch of the calls that sum the weights: a.workgroups workgroups add the weights, each those of the stretch
 // that the workgroup of its number took in the first launch (of its pieces the first head group of each kv head, for all of
-// them), and behind them the join's, where there is a line.  shift: weight_shift of the types; sums4: the sums' rows can
-// be read four at a time.
+// them), and behind them the join's, where there is a line.  shift: weight_shift of the types.
 template <int kDim, bool kBf16, int kTogether>
-__global__ __launch_bounds__(kWaves * kWave) void attention_weights_kernel(const AttentionArgs a, const float shift,
-                                                                          const bool sums4) {
+__global__ __launch_bounds__(kWaves * kWave) void attention_weights_kernel(const AttentionArgs a, const float shift) {
   extern __shared__ float2 stats[];
   if (blockIdx.x >= static_cast<uint32_t>(a.workgroups)) {
     join_pieces<kDim, kBf16, kTogether, kWaves>(a, static_cast<int>(blockIdx.x) - a.workgroups);
@@ -994,7 +1002,7 @@ __global__ __launch_bounds__(kWaves * kWave) void attention_weights_kernel(const
     at += from >= tiles ? span - from : count;
     if (from >= tiles || n == 0 || hg % a.head_tiles != 0) continue;
     const int t0 = first / kTileKeys + from;
-    sum_weights(a, b, hg / a.head_tiles, n, first, t0, t0 + count, shift, sums4, stats);
+    sum_weights(a, b, hg / a.head_tiles, n, first, t0, t0 + count, shift, stats);
     __syncthreads();  // the statistics have been read
   }
 }
@@ -1053,16 +1061,16 @@ static void attention_launch(const AttentionArgs& a, const AttentionShape& s, bo
   const int64_t pieces = a.workgroups / (static_cast<int64_t>(a.c.batch) * a.c.kv_heads * a.head_tiles);
   const dim3 each(static_cast<unsigned>(units)), fourth(static_cast<unsigned>((units + 3) / 4));
   if constexpr (kWeights) {
-    const bool sums4 = aligned16(a.weight_sum) && a.sum_seq % 4 == 0 && a.sum_head % 4 == 0;
+    if (own_weights(a)) return;
     const float shift = weight_shift(kBf16, kE4m3);
     const size_t stats = (1 + kWaves) * a.group * sizeof(float2);
     const dim3 many(grid.x + each.x), few(grid.x + (s.line ? fourth.x : 0));
     if (s.line && pieces >= kJoinMany)
-      hipLaunchKernelGGL((attention_weights_kernel<kDim, kBf16, 16>), many, block, stats, st, a, shift, sums4);
+      hipLaunchKernelGGL((attention_weights_kernel<kDim, kBf16, 16>), many, block, stats, st, a, shift);
     else if (s.line && pieces >= kJoinSome)
-      hipLaunchKernelGGL((attention_weights_kernel<kDim, kBf16, 4>), many, block, stats, st, a, shift, sums4);
+      hipLaunchKernelGGL((attention_weights_kernel<kDim, kBf16, 4>), many, block, stats, st, a, shift);
     else
-      hipLaunchKernelGGL((attention_weights_kernel<kDim, kBf16, 1>), few, block, stats, st, a, shift, sums4);
+      hipLaunchKernelGGL((attention_weights_kernel<kDim, kBf16, 1>), few, block, stats, st, a, shift);
     return;
   }
   if (!s.line) return;
@@ -1170,6 +1178,7 @@ static int attention_decode(const char* who, const void* q, int64_t q_seq_stride
                   nullptr,
                   nullptr,
                   0,
+                  0,
                   0};
   char* at = static_cast<char*>(workspace);
   if (s.line) {
@@ -1184,6 +1193,7 @@ static int attention_decode(const char* who, const void* q, int64_t q_seq_stride
     a.weight_sum = weights->sums;
     a.sum_seq = weights->seq_stride;
     a.sum_head = weights->head_stride;
+    a.sums4 = aligned16(a.weight_sum) && a.sum_seq % 4 == 0 && a.sum_head % 4 == 0;
   }
   bool row_runs = cache->page_size % 16 == 0;
   if (cache->dtype == TRIS_DTYPE_E4M3) {  // four scales a load
