@@ -7,21 +7,24 @@
 // powers of two spread over its bins (8-bit digits put two powers of two into one, and the additions wait for each other).
 //
 // Up to kSelectMost positions one workgroup has a row, its weights in registers, read once; it lists the positions that
-// stay and moves the sums as well.  Longer rows are cut into segments of a workgroup each, in three launches: histograms of
-// the first digit; the keys in the border's bin, gathered; and, in every workgroup alike, the border among those, by which
-// it places its segment.
+// stay and moves the sums as well, and keys and values too where rows are many or small.  Longer rows are cut into segments
+// of a workgroup each, in three launches: histograms of the first digit; the keys in the border's bin, gathered; and, in
+// every workgroup alike, the border among those, by which it places its segment.
 //
 // The move is bound by memory, 2 row reads and 2 row writes a position and kv head.
 #include "tris_paged.h"
 
 namespace tris {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 1024;  // of the workgroups of long rows, and of the moves
 constexpr int kBlockWaves = kThreads / kWave;
-constexpr int kRowKeys = 16;                        // of a thread, where a workgroup has a row
-constexpr int kSelectMost = kThreads * kRowKeys;
-constexpr int kBins = 2048, kFirstShift = 21, kSecondShift = 10;
+constexpr int kSelectMost = 32 * kThreads;
+// bits of the digits, first to last, of rows in one workgroup and in segments (whose histograms of the first every workgroup
+// of the row reads)
+constexpr int kRowBits[3] = {11, 11, 10}, kSegmentBits[3] = {10, 11, 11};
+constexpr int kBins = 1 << 11, kFirstBins = 1 << kSegmentBits[0], kFirstShift = 32 - kSegmentBits[0];
 constexpr int kMostSegments = 64;  // a lane each
+constexpr int kCus = 256;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -37,7 +40,7 @@ struct EvictArgs {
   int32_t segments, segment;  // how many, and positions of one
   int32_t* state;             // [rows][kState]
   int32_t* counts;            // [rows][segments][2]: keys above the bin; keys in it of the segments before
-  uint32_t* hist;             // [rows][segments][kBins]
+  uint32_t* hist;             // [rows][segments][kFirstBins]
   uint32_t* found;            // [rows][segments * segment]: the keys in the bin, in order
   float* moved;               // [rows][budget]: the sums of what stays
 };
@@ -57,371 +60,52 @@ __device__ __forceinline__ int evict_length(const EvictArgs& a, int b) {
 }
 
 // Whether all pages of a sequence of n > 0 positions are in the pool (for the whole workgroup).
+template <int kBlock>
 __device__ __forceinline__ bool pages_good(const EvictArgs& a, int b, int n) {
   const int32_t* table = a.c.block_table + b * a.c.table_stride;
   const int last = a.page_of(n - 1);
   bool good = true;
-  for (int i = threadIdx.x; i <= last; i += kThreads)
+  for (int i = threadIdx.x; i <= last; i += kBlock)
     good = good && static_cast<uint32_t>(table[i]) < static_cast<uint32_t>(a.c.num_pages);
   return __syncthreads_and(good);
 }
 
-// The bin, of kBins counted from the largest down, that holds the left-th largest key: *pick, and how many are above it.
-// count(bin): the keys in a bin.  For the whole workgroup; totals: LDS.
+// The bin, of kCount counted from the largest down, that holds the left-th largest key, how many are above it and in it.
+// count(bin): the keys in a bin; a thread asks for kCount / kBlock of them, from kCount - 1 - thread * kCount / kBlock down.
+// For the whole workgroup.
+template <int kBlock>
 struct Pick {
-  int bin, above;
-  int totals[kBlockWaves];
+  int bin, above, in;
+  int totals[kBlock / kWave];
 };
-template <typename Count>
-__device__ __forceinline__ void pick_bin(Count count, int left, Pick* sh) {
-  const int thread = threadIdx.x, lane = thread % kWave, wave = thread / kWave;
-  const int high = kBins - 1 - 2 * thread, c0 = count(high), c1 = count(high - 1);
-  const int end = wave_incl_sum_i32(c0 + c1);
-  if (lane == kWave - 1) sh->totals[wave] = end;
-  __syncthreads();
-  int before = end - c0 - c1;
-  for (int w = 0; w < kBlockWaves; ++w) before += w < wave ? sh->totals[w] : 0;
-  if (before < left && left <= before + c0 + c1) {
-    const bool first = left <= before + c0;
-    sh->bin = first ? high : high - 1;
-    sh->above = first ? before : before + c0;
-  }
-  __syncthreads();
-}
-
-// Exclusive prefixes of kRowKeys * kBlockWaves numbers in LDS, in place, by the first wavefront.
-__device__ __forceinline__ void scan_counts(int* counts) {
-  constexpr int kEach = kRowKeys * kBlockWaves / kWave;
-  const int lane = threadIdx.x;
+template <int kBlock, int kCount, typename Count>
+__device__ __forceinline__ void pick_bin(Count count, int left, Pick<kBlock>* sh) {
+  constexpr int kEach = kCount / kBlock;
+  const int thread = threadIdx.x, lane = thread % kWave, wave = thread / kWave, high = kCount - 1 - kEach * thread;
   int c[kEach], sum = 0;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) sum += c[i] = counts[lane * kEach + i];
-  int before = wave_incl_sum_i32(sum) - sum;
+  for (int i = 0; i < kEach; ++i) sum += c[i] = count(high - i);
+  const int end = wave_incl_sum_i32(sum);
+  if (lane == kWave - 1) sh->totals[wave] = end;
+  __syncthreads();
+  int before = end - sum;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    counts[lane * kEach + i] = before;
-    before += c[i];
-  }
-}
-
-__global__ __launch_bounds__(kThreads) void evict_select_kernel(const EvictArgs a) {
-  __shared__ int hist[kBins];
-  __shared__ int counts[kRowKeys * kBlockWaves];
-  __shared__ Pick pick;
-  const int row = blockIdx.x, b = row / a.c.kv_heads, h = row - b * a.c.kv_heads;
-  const int thread = threadIdx.x, lane = thread % kWave, wave = thread / kWave;
-  const int n = evict_length(a, b);
-  int32_t* kept = a.kept + static_cast<int64_t>(row) * a.budget;
-  float* sums = a.sums + b * a.sum_seq + h * a.sum_head;
-  float w[kRowKeys];
-  bool due = n > a.limit;
-  if (due) {
+  for (int w = 0; w < kBlock / kWave; ++w) before += w < wave ? sh->totals[w] : 0;
+  if (before < left && left <= before + sum) {
 #pragma unroll
-    for (int j = 0; j < kRowKeys; ++j) w[j] = j * kThreads + thread < n ? sums[j * kThreads + thread] : 0.0f;
-    due = pages_good(a, b, n);
-  }
-  if (h == 0 && thread == 0) a.new_lens[b] = due ? a.budget : a.c.seq_lens[b];
-  if (!due) {
-    for (int i = thread; i < a.budget; i += kThreads) kept[i] = -1;
-    return;
-  }
-  const int lo = a.sink, hi = n - a.recent, want = a.budget - a.sink - a.recent;
-  uint32_t border = 0xFFFFFFFFu;
-  int equal = 0;  // of the keys equal to the border, how many stay
-  if (want > 0) {
-    uint32_t prefix = 0;
-    equal = want;
-#pragma unroll
-    for (int digit = 0; digit < 3; ++digit) {
-      const int shift = digit == 0 ? kFirstShift : digit == 1 ? kSecondShift : 0;
-      const int bits = digit == 2 ? 10 : 11;
-      hist[thread] = hist[thread + kThreads] = 0;
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < kRowKeys; ++j) {
-        const int i = j * kThreads + thread;
-        if (j * kThreads < n && i >= lo && i < hi) {
-          const uint32_t key = order_key(w[j]);
-          if (digit == 0 || key >> (shift + bits) == prefix) atomicAdd(&hist[key >> shift & ((1 << bits) - 1)], 1);
-        }
+    for (int i = 0; i < kEach; ++i) {
+      if (before < left && left <= before + c[i]) {
+        sh->bin = high - i;
+        sh->above = before;
+        sh->in = c[i];
       }
-      __syncthreads();
-      pick_bin([&](int bin) { return hist[bin]; }, equal, &pick);
-      prefix = prefix << bits | static_cast<uint32_t>(pick.bin);
-      equal -= pick.above;
-    }
-    border = prefix;
-  }
-  // Of each 64 positions: how many stay for certain, and (from bit 16 on) how many are equal to the border.
-#pragma unroll
-  for (int j = 0; j < kRowKeys; ++j) {
-    const int i = j * kThreads + thread;
-    const bool middle = i >= lo && i < hi && want > 0;
-    const uint32_t key = order_key(w[j]);
-    const int sure = __popcll(__ballot(i < n && (i < lo || i >= hi || (middle && key > border))));
-    const int ties = __popcll(__ballot(middle && key == border));
-    if (lane == 0) counts[j * kBlockWaves + wave] = sure | ties << 16;
-  }
-  __syncthreads();
-  if (wave == 0) scan_counts(counts);
-  __syncthreads();
-  const uint64_t below = (1ull << lane) - 1;
-#pragma unroll
-  for (int j = 0; j < kRowKeys; ++j) {
-    if (j * kThreads >= n) break;
-    const int i = j * kThreads + thread;
-    const bool middle = i >= lo && i < hi && want > 0;
-    const uint32_t key = order_key(w[j]);
-    const bool sure = i < n && (i < lo || i >= hi || (middle && key > border)), tie = middle && key == border;
-    const int before = counts[j * kBlockWaves + wave];
-    const int sures = (before & 0xFFFF) + __popcll(__ballot(sure) & below);
-    const int ties = (before >> 16) + __popcll(__ballot(tie) & below);
-    if (sure || (tie && ties < equal)) {
-      const int place = sures + min(ties, equal);
-      kept[place] = i;
-      sums[place] = w[j];  // (every weight of the row is in registers)
+      before += c[i];
     }
   }
-  for (int i = a.budget + thread; i < n; i += kThreads) sums[i] = 0.0f;
+  __syncthreads();
 }
 
-// ------------------------------------------------------------------------------------------------ rows in segments
-
-struct Segment {
-  int row, s, b, h, n, begin, end;
-  __device__ explicit Segment(const EvictArgs& a) {
-    row = blockIdx.x / a.segments;
-    s = blockIdx.x - row * a.segments;
-    b = row / a.c.kv_heads;
-    h = row - b * a.c.kv_heads;
-    n = evict_length(a, b);
-    begin = static_cast<int>(min(static_cast<int64_t>(s) * a.segment, static_cast<int64_t>(n)));
-    end = min(n, begin + a.segment);
-  }
-  __device__ int64_t index(const EvictArgs& a) const { return static_cast<int64_t>(row) * a.segments + s; }
-};
-
-// Four positions of a thread from i0 on, kThreads apart, and their weights.
-constexpr int kTileKeys = 4;
-constexpr int kTile = kTileKeys * kThreads;
-
-struct Weights {
-  float w[kTileKeys];
-  __device__ Weights(const EvictArgs& a, const Segment& g, int i0) {
-    const float* sums = a.sums + g.b * a.sum_seq + g.h * a.sum_head;
-#pragma unroll
-    for (int j = 0; j < kTileKeys; ++j) {
-      const int i = i0 + j * kThreads + static_cast<int>(threadIdx.x);
-      w[j] = i < g.end ? sums[i] : 0.0f;
-    }
-  }
-};
-
-__global__ __launch_bounds__(kThreads) void evict_histogram_kernel(const EvictArgs a) {
-  __shared__ uint32_t hist[kBins];
-  const Segment g(a);
-  const int thread = threadIdx.x;
-  hist[thread] = hist[thread + kThreads] = 0;
-  Weights now(a, g, g.begin);
-  const bool due = g.n > a.limit && pages_good(a, g.b, g.n);
-  if (g.s == 0 && thread == 0) {
-    if (g.h == 0) a.new_lens[g.b] = due ? a.budget : a.c.seq_lens[g.b];
-    a.state[kState * g.row + kAlone] = !due;
-  }
-  if (!due) {
-    int32_t* kept = a.kept + static_cast<int64_t>(g.row) * a.budget;
-    for (int i = g.s * kThreads + thread; i < a.budget; i += a.segments * kThreads) kept[i] = -1;
-    return;
-  }
-  const int lo = max(g.begin, a.sink), hi = min(g.end, g.n - a.recent);
-  for (int i0 = g.begin; i0 < hi; i0 += kTile) {
-    if (i0 > g.begin) now = Weights(a, g, i0);
-#pragma unroll
-    for (int j = 0; j < kTileKeys; ++j) {
-      const int i = i0 + j * kThreads + thread;
-      if (i >= lo && i < hi) atomicAdd(&hist[order_key(now.w[j]) >> kFirstShift], 1u);
-    }
-  }
-  __syncthreads();
-  uint32_t* out = a.hist + g.index(a) * kBins;
-  out[thread] = hist[thread];
-  out[thread + kThreads] = hist[thread + kThreads];
-}
-
-__global__ __launch_bounds__(kThreads) void evict_gather_kernel(const EvictArgs a) {
-  __shared__ Pick pick;
-  __shared__ int counts[kTileKeys * kBlockWaves];
-  __shared__ int above, offset, total;
-  const Segment g(a);
-  if (a.state[kState * g.row + kAlone]) return;
-  const int thread = threadIdx.x, lane = thread % kWave, wave = thread / kWave;
-  const int want = a.budget - a.sink - a.recent;
-  Weights now(a, g, g.begin);
-  // the row's histogram: two bins a thread, from the largest down
-  const uint32_t* row_hist = a.hist + static_cast<int64_t>(g.row) * a.segments * kBins;
-  const uint32_t* hist = row_hist + kBins - 2 - 2 * thread;
-  int c0 = 0, c1 = 0, mine0 = 0, mine1 = 0;
-#pragma unroll 8
-  for (int s = 0; s < a.segments; ++s) {
-    const uint2 c = *reinterpret_cast<const uint2*>(hist + static_cast<int64_t>(s) * kBins);
-    c0 += c.y;
-    c1 += c.x;
-    mine0 = s == g.s ? c.y : mine0;
-    mine1 = s == g.s ? c.x : mine1;
-  }
-  if (thread == 0) {
-    pick.bin = kBins;  // where nothing is wanted: no key is above it, none in it
-    pick.above = above = 0;
-  }
-  __syncthreads();
-  if (want > 0) pick_bin([&](int bin) { return bin & 1 ? c0 : c1; }, want, &pick);
-  const int bin = pick.bin, high = kBins - 1 - 2 * thread;
-  const int mine = wave_incl_sum_i32((high > bin ? mine0 : 0) + (high - 1 > bin ? mine1 : 0));
-  if (lane == kWave - 1 && mine) atomicAdd(&above, mine);
-  // the keys in the bin, of the segments before and of all
-  if (wave == 0) {
-    const int in = lane < a.segments && bin < kBins ? row_hist[static_cast<int64_t>(lane) * kBins + bin] : 0;
-    const int end = wave_incl_sum_i32(in);
-    if (lane == g.s) offset = end - in;
-    if (lane == kWave - 1) total = end;
-  }
-  __syncthreads();
-  if (thread == 0) {
-    a.counts[2 * g.index(a)] = above;
-    a.counts[2 * g.index(a) + 1] = offset;
-    if (g.s == 0) {
-      a.state[kState * g.row + kDigit] = bin;
-      a.state[kState * g.row + kWanted] = want - pick.above;
-      a.state[kState * g.row + kTotal] = total;
-    }
-  }
-  // its keys, in order
-  uint32_t* found = a.found + static_cast<int64_t>(g.row) * a.segments * a.segment;
-  const int lo = max(g.begin, a.sink), hi = min(g.end, g.n - a.recent);
-  int placed = offset;
-  for (int i0 = g.begin; i0 < hi; i0 += kTile) {
-    if (i0 > g.begin) now = Weights(a, g, i0);
-    uint64_t in[kTileKeys];
-#pragma unroll
-    for (int j = 0; j < kTileKeys; ++j) {
-      const int i = i0 + j * kThreads + thread;
-      in[j] = __ballot(i >= lo && i < hi && static_cast<int>(order_key(now.w[j]) >> kFirstShift) == bin);
-      if (lane == 0) counts[j * kBlockWaves + wave] = __popcll(in[j]);
-    }
-    __syncthreads();
-    const int c = counts[lane], end = wave_incl_sum_i32(c);  // (each wavefront: the tile's 64 counts)
-#pragma unroll
-    for (int j = 0; j < kTileKeys; ++j) {
-      const int before = __shfl(end - c, j * kBlockWaves + wave);
-      if (in[j] >> lane & 1) found[placed + before + __popcll(in[j] & ((1ull << lane) - 1))] = order_key(now.w[j]);
-    }
-    placed += __builtin_amdgcn_readlane(end, kWave - 1);
-    __syncthreads();
-  }
-}
-
-__global__ __launch_bounds__(kThreads) void evict_place_kernel(const EvictArgs a) {
-  __shared__ int hist[kBins];
-  __shared__ Pick pick;
-  __shared__ int before[2];      // of the segments before: positions that stay for certain, keys equal to the border
-  __shared__ int counts[kTileKeys * kBlockWaves];
-  const Segment g(a);
-  const int32_t* state = a.state + kState * g.row;
-  if (state[kAlone]) return;
-  const int thread = threadIdx.x, lane = thread % kWave, wave = thread / kWave;
-  const int first = state[kDigit], total = state[kTotal], lo = a.sink, hi = g.n - a.recent;
-  Weights now(a, g, g.begin);
-  const int2* row_counts = reinterpret_cast<const int2*>(a.counts) + static_cast<int64_t>(g.row) * a.segments;
-  const int offset = row_counts[g.s].y;
-  // every key of the row's bin, the first of a thread's in registers
-  const uint32_t* found = a.found + static_cast<int64_t>(g.row) * a.segments * a.segment;
-  uint32_t key[kTileKeys];
-#pragma unroll
-  for (int j = 0; j < kTileKeys; ++j) key[j] = j * kThreads + thread < total ? found[j * kThreads + thread] : 0u;
-  const auto each = [&](auto&& f) {
-#pragma unroll
-    for (int j = 0; j < kTileKeys; ++j)
-      if (j * kThreads + thread < total) f(j * kThreads + thread, key[j]);
-#pragma unroll 4
-    for (int i = kTile + thread; i < total; i += kThreads) f(i, found[i]);
-  };
-  if (thread < 2) before[thread] = 0;
-  __syncthreads();
-  if (thread < g.s) {
-    const int begin = static_cast<int>(min(static_cast<int64_t>(thread) * a.segment, static_cast<int64_t>(g.n)));
-    const int end = min(g.n, begin + a.segment);
-    // (and the first and last positions, which are held)
-    atomicAdd(&before[0], row_counts[thread].x + max(0, min(end, lo) - begin) + max(0, end - max(begin, hi)));
-  }
-  const bool some = first < kBins;
-  uint32_t border = 0xFFFFFFFFu;
-  int equal = 0;
-  if (some) {
-    border = static_cast<uint32_t>(first);
-    equal = state[kWanted];
-#pragma unroll
-    for (int digit = 1; digit < 3; ++digit) {
-      const int shift = digit == 1 ? kSecondShift : 0, bits = digit == 1 ? 11 : 10;
-      hist[thread] = hist[thread + kThreads] = 0;
-      __syncthreads();
-      each([&](int, uint32_t k) {
-        if (k >> (shift + bits) == border) atomicAdd(&hist[k >> shift & ((1 << bits) - 1)], 1);
-      });
-      __syncthreads();
-      pick_bin([&](int bin) { return hist[bin]; }, equal, &pick);
-      border = border << bits | static_cast<uint32_t>(pick.bin);
-      equal -= pick.above;
-    }
-    int sure = 0, ties = 0;
-    each([&](int i, uint32_t k) {
-      sure += i < offset && k > border;
-      ties += i < offset && k == border;
-    });
-    sure = wave_incl_sum_i32(sure);
-    ties = wave_incl_sum_i32(ties);
-    if (lane == kWave - 1) {
-      atomicAdd(&before[0], sure);
-      atomicAdd(&before[1], ties);
-    }
-  }
-  __syncthreads();
-  int sures = before[0], tied = before[1];
-  int32_t* kept = a.kept + static_cast<int64_t>(g.row) * a.budget;
-  float* moved = a.moved + static_cast<int64_t>(g.row) * a.budget;
-  for (int i0 = g.begin; i0 < g.end; i0 += kTile) {
-    if (i0 > g.begin) now = Weights(a, g, i0);
-    uint64_t sure[kTileKeys], tie[kTileKeys];
-#pragma unroll
-    for (int j = 0; j < kTileKeys; ++j) {
-      const int i = i0 + j * kThreads + thread;
-      const uint32_t k = order_key(now.w[j]);
-      const bool middle = some && i >= lo && i < hi;
-      sure[j] = __ballot(i < g.end && (i < lo || i >= hi || (middle && k > border)));
-      tie[j] = __ballot(i < g.end && middle && k == border);
-      if (lane == 0) counts[j * kBlockWaves + wave] = __popcll(sure[j]) | __popcll(tie[j]) << 16;
-    }
-    __syncthreads();
-    const int c = counts[lane], end = wave_incl_sum_i32(c);
-    const uint64_t below = (1ull << lane) - 1;
-#pragma unroll
-    for (int j = 0; j < kTileKeys; ++j) {
-      const int past = __shfl(end - c, j * kBlockWaves + wave);
-      const int t = tied + (past >> 16) + __popcll(tie[j] & below);
-      const int place = sures + (past & 0xFFFF) + __popcll(sure[j] & below) + min(t, equal);
-      const bool stays = (sure[j] >> lane & 1) || ((tie[j] >> lane & 1) && t < equal);
-      if (stays && place < a.budget) {  // (past it only if the sums change meanwhile)
-        kept[place] = i0 + j * kThreads + thread;
-        moved[place] = now.w[j];
-      }
-    }
-    const int all = __builtin_amdgcn_readlane(end, kWave - 1);
-    sures += all & 0xFFFF;
-    tied += all >> 16;
-    __syncthreads();
-  }
-}
-
-// ------------------------------------------------------------------------------------------------ the move
+// ------------------------------------------------------------------------------------------------ the move in place
 
 // A row of bytes or one 4-byte number of each position of one kv head: where a position's is.  Positions and pages are
 // checked again here, so that tables, lengths or sums that change meanwhile lead nowhere else.
@@ -472,13 +156,13 @@ __device__ __forceinline__ Units part_units(const EvictArgs& a, int b, int h, in
 // before it is stored, their pages before that, and the list before that.  Rows from `end` on are left to the second move.
 constexpr int kMoveUnits = 4;
 
-template <typename T>
-__device__ __forceinline__ void shift_units(const int32_t* kept, int budget, int end, int lanes, const Units& u) {
-  const int thread = threadIdx.x, rows = kThreads / lanes, unit = thread % lanes, first = thread / lanes;
+template <typename T, int kBlock>
+__device__ __forceinline__ void shift_units(const int32_t* kept, int budget, int end, int lanes, int unit, const Units& u) {
+  const int thread = threadIdx.x, rows = kBlock / lanes, first = thread / lanes;
   const int run = rows * kMoveUnits;
   int last = budget;  // no row from here on comes from before `end`
   if (end < INT32_MAX) {
-    const int each = (budget + kThreads - 1) / kThreads;
+    const int each = (budget + kBlock - 1) / kBlock;
     last = min(budget, each * __syncthreads_count(thread * each < budget && kept[thread * each] < end));
   }
   // of a unit: where its row comes from and goes (its own place: nowhere), their pages, the row
@@ -546,19 +230,389 @@ __device__ __forceinline__ void shift_units(const int32_t* kept, int budget, int
   }
 }
 
+// ------------------------------------------------------------------------------------------------ a row in one workgroup
+
+// kMove: the workgroup moves its row's keys and values as well.
+template <int kBlock, int kKeys, bool kMove>
+__global__ __launch_bounds__(kBlock) void evict_select_kernel(const EvictArgs a) {
+  constexpr int kWaves = kBlock / kWave, kCounts = kKeys * kWaves;
+  __shared__ int hist[kBins];
+  __shared__ uint32_t counts[kCounts];
+  __shared__ Pick<kBlock> pick;
+  const int row = blockIdx.x, b = row / a.c.kv_heads, h = row - b * a.c.kv_heads;
+  const int thread = threadIdx.x, lane = thread % kWave, wave = thread / kWave;
+  const int n = evict_length(a, b);
+  int32_t* kept = a.kept + static_cast<int64_t>(row) * a.budget;
+  float* sums = a.sums + b * a.sum_seq + h * a.sum_head;
+  float w[kKeys];
+  bool due = n > a.limit;
+  if (due) {
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j) w[j] = j * kBlock + thread < n ? sums[j * kBlock + thread] : 0.0f;
+    due = pages_good<kBlock>(a, b, n);
+  }
+  if (h == 0 && thread == 0) a.new_lens[b] = due ? a.budget : a.c.seq_lens[b];
+  if (!due) {
+    for (int i = thread; i < a.budget; i += kBlock) kept[i] = -1;
+    return;
+  }
+  const int lo = a.sink, hi = n - a.recent, want = a.budget - a.sink - a.recent;
+  uint32_t border = 0xFFFFFFFFu;
+  int equal = 0;  // of the keys equal to the border, how many stay
+  if (want > 0) {
+    uint32_t prefix = 0;
+    equal = want;
+#pragma unroll
+    for (int digit = 0; digit < 3; ++digit) {
+      const int bits = kRowBits[digit], shift = digit == 0 ? kRowBits[1] + kRowBits[2] : digit == 1 ? kRowBits[2] : 0;
+#pragma unroll
+      for (int i = thread; i < kBins; i += kBlock) hist[i] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kKeys; ++j) {
+        const int i = j * kBlock + thread;
+        if (j * kBlock < n && i >= lo && i < hi) {
+          const uint32_t key = order_key(w[j]);
+          if (digit == 0 || key >> (shift + bits) == prefix) atomicAdd(&hist[key >> shift & ((1 << bits) - 1)], 1);
+        }
+      }
+      __syncthreads();
+      pick_bin<kBlock, kBins>([&](int bin) { return hist[bin]; }, equal, &pick);
+      prefix = prefix << bits | static_cast<uint32_t>(pick.bin);
+      equal -= pick.above;
+      border = prefix;
+      if (digit < 2 && equal == pick.in) {
+        // the whole bin stays: the border is the largest key below it (there is one: no key is below 2^22)
+        border = (prefix << shift) - 1;
+        equal = 0;
+        break;
+      }
+    }
+  }
+  // Of each 64 positions: how many stay for certain, and (from bit 16 on) how many are equal to the border.
+  const auto classes = [&](int j, uint64_t* sure, uint64_t* tie) {
+    const int i = j * kBlock + thread;
+    const bool middle = i >= lo && i < hi && want > 0;
+    const uint32_t key = order_key(w[j]);
+    *sure = __ballot(i < n && (i < lo || i >= hi || (middle && key > border)));
+    *tie = __ballot(middle && key == border);
+  };
+#pragma unroll
+  for (int j = 0; j < kKeys; ++j) {
+    uint64_t sure, tie;
+    classes(j, &sure, &tie);
+    if (lane == 0) counts[j * kWaves + wave] = __popcll(sure) | __popcll(tie) << 16;
+  }
+  __syncthreads();
+  if (wave == 0) {  // the numbers before each
+    constexpr int kEach = kCounts / kWave;
+    uint32_t c[kEach], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) sum += c[i] = counts[lane * kEach + i];
+    uint32_t before = static_cast<uint32_t>(wave_incl_sum_i32(static_cast<int>(sum))) - sum;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      counts[lane * kEach + i] = before;
+      before += c[i];
+    }
+  }
+  __syncthreads();
+  const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+  for (int j = 0; j < kKeys; ++j) {
+    if (j * kBlock >= n) break;
+    uint64_t sure, tie;
+    classes(j, &sure, &tie);
+    const uint32_t before = counts[j * kWaves + wave];
+    const int ties = static_cast<int>(before >> 16) + __popcll(tie & below);
+    if ((sure >> lane & 1) || ((tie >> lane & 1) && ties < equal)) {
+      const int place = static_cast<int>(before & 0xFFFF) + __popcll(sure & below) + min(ties, equal);
+      kept[place] = j * kBlock + thread;
+      sums[place] = w[j];  // (every weight of the row is in registers)
+    }
+  }
+  for (int i = a.budget + thread; i < n; i += kBlock) sums[i] = 0.0f;
+  if constexpr (kMove) {
+    __syncthreads();
+    const bool e4m3 = a.c.dtype == TRIS_DTYPE_E4M3;
+    const int lanes = a.c.head_dim * (e4m3 ? 1 : 2) / 16;  // of a row; the values beside the keys
+    const bool v = thread % (2 * lanes) >= lanes;
+    shift_units<u32x4, kBlock>(kept, a.budget, INT32_MAX, 2 * lanes, thread % lanes, part_units(a, b, h, v, 1, 0));
+    if (e4m3) shift_units<uint32_t, kBlock>(kept, a.budget, INT32_MAX, 2, 0, part_units(a, b, h, 2 + thread % 2, 1, 0));
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ rows in segments
+
+struct Segment {
+  int row, s, b, h, n, begin, end;
+  __device__ explicit Segment(const EvictArgs& a) {
+    row = blockIdx.x / a.segments;
+    s = blockIdx.x - row * a.segments;
+    b = row / a.c.kv_heads;
+    h = row - b * a.c.kv_heads;
+    n = evict_length(a, b);
+    begin = static_cast<int>(min(static_cast<int64_t>(s) * a.segment, static_cast<int64_t>(n)));
+    end = min(n, begin + a.segment);
+  }
+  __device__ int64_t index(const EvictArgs& a) const { return static_cast<int64_t>(row) * a.segments + s; }
+};
+
+// Four positions of a thread from i0 on, kThreads apart, and their weights.
+constexpr int kTileKeys = 4;
+constexpr int kTile = kTileKeys * kThreads;
+
+struct Weights {
+  float w[kTileKeys];
+  __device__ Weights(const EvictArgs& a, const Segment& g, int i0) {
+    const float* sums = a.sums + g.b * a.sum_seq + g.h * a.sum_head;
+#pragma unroll
+    for (int j = 0; j < kTileKeys; ++j) {
+      const int i = i0 + j * kThreads + static_cast<int>(threadIdx.x);
+      w[j] = i < g.end ? sums[i] : 0.0f;
+    }
+  }
+};
+
+__global__ __launch_bounds__(kThreads) void evict_histogram_kernel(const EvictArgs a) {
+  static_assert(kFirstBins == kThreads, "a bin for each thread");
+  __shared__ uint32_t hist[kFirstBins];
+  const Segment g(a);
+  const int thread = threadIdx.x;
+  hist[thread] = 0;
+  Weights now(a, g, g.begin);
+  const bool due = g.n > a.limit && pages_good<kThreads>(a, g.b, g.n);
+  if (g.s == 0 && thread == 0) {
+    if (g.h == 0) a.new_lens[g.b] = due ? a.budget : a.c.seq_lens[g.b];
+    a.state[kState * g.row + kAlone] = !due;
+  }
+  if (!due) {
+    int32_t* kept = a.kept + static_cast<int64_t>(g.row) * a.budget;
+    for (int i = g.s * kThreads + thread; i < a.budget; i += a.segments * kThreads) kept[i] = -1;
+    return;
+  }
+  const int lo = max(g.begin, a.sink), hi = min(g.end, g.n - a.recent);
+  for (int i0 = g.begin; i0 < hi; i0 += kTile) {
+    if (i0 > g.begin) now = Weights(a, g, i0);
+#pragma unroll
+    for (int j = 0; j < kTileKeys; ++j) {
+      const int i = i0 + j * kThreads + thread;
+      if (i >= lo && i < hi) atomicAdd(&hist[order_key(now.w[j]) >> kFirstShift], 1u);
+    }
+  }
+  __syncthreads();
+  a.hist[g.index(a) * kFirstBins + thread] = hist[thread];
+}
+
+__global__ __launch_bounds__(kThreads) void evict_gather_kernel(const EvictArgs a) {
+  __shared__ Pick<kThreads> pick;
+  __shared__ int counts[kTileKeys * kBlockWaves];
+  __shared__ int above, offset, total;
+  const Segment g(a);
+  if (a.state[kState * g.row + kAlone]) return;
+  const int thread = threadIdx.x, lane = thread % kWave, wave = thread / kWave;
+  const int want = a.budget - a.sink - a.recent;
+  Weights now(a, g, g.begin);
+  // the row's histogram: a bin a thread, from the largest down
+  const uint32_t* row_hist = a.hist + static_cast<int64_t>(g.row) * a.segments * kFirstBins;
+  const int own = kFirstBins - 1 - thread;
+  int count = 0, mine = 0;
+#pragma unroll 16
+  for (int s = 0; s < a.segments; ++s) {
+    const int c = row_hist[static_cast<int64_t>(s) * kFirstBins + own];
+    count += c;
+    mine = s == g.s ? c : mine;
+  }
+  if (thread == 0) {
+    pick.bin = kFirstBins;  // where nothing is wanted: no key is above it, none in it
+    pick.above = above = 0;
+  }
+  __syncthreads();
+  if (want > 0) pick_bin<kThreads, kFirstBins>([&](int) { return count; }, want, &pick);
+  const int bin = pick.bin;
+  mine = wave_incl_sum_i32(own > bin ? mine : 0);
+  if (lane == kWave - 1 && mine) atomicAdd(&above, mine);
+  // the keys in the bin, of the segments before and of all
+  if (wave == 0) {
+    const int in = lane < a.segments && bin < kFirstBins ? row_hist[static_cast<int64_t>(lane) * kFirstBins + bin] : 0;
+    const int end = wave_incl_sum_i32(in);
+    if (lane == g.s) offset = end - in;
+    if (lane == kWave - 1) total = end;
+  }
+  __syncthreads();
+  if (thread == 0) {
+    a.counts[2 * g.index(a)] = above;
+    a.counts[2 * g.index(a) + 1] = offset;
+    if (g.s == 0) {
+      a.state[kState * g.row + kDigit] = bin;
+      a.state[kState * g.row + kWanted] = want - pick.above;
+      a.state[kState * g.row + kTotal] = total;
+    }
+  }
+  // its keys, in order
+  uint32_t* found = a.found + static_cast<int64_t>(g.row) * a.segments * a.segment;
+  const int lo = max(g.begin, a.sink), hi = min(g.end, g.n - a.recent);
+  int placed = offset;
+  for (int i0 = g.begin; i0 < hi; i0 += kTile) {
+    if (i0 > g.begin) now = Weights(a, g, i0);
+    uint64_t in[kTileKeys];
+#pragma unroll
+    for (int j = 0; j < kTileKeys; ++j) {
+      const int i = i0 + j * kThreads + thread;
+      in[j] = __ballot(i >= lo && i < hi && static_cast<int>(order_key(now.w[j]) >> kFirstShift) == bin);
+      if (lane == 0) counts[j * kBlockWaves + wave] = __popcll(in[j]);
+    }
+    __syncthreads();
+    const int c = counts[lane], end = wave_incl_sum_i32(c);  // (each wavefront: the tile's 64 counts)
+#pragma unroll
+    for (int j = 0; j < kTileKeys; ++j) {
+      const int before = __shfl(end - c, j * kBlockWaves + wave);
+      if (in[j] >> lane & 1) found[placed + before + __popcll(in[j] & ((1ull << lane) - 1))] = order_key(now.w[j]);
+    }
+    placed += __builtin_amdgcn_readlane(end, kWave - 1);
+    __syncthreads();
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void evict_place_kernel(const EvictArgs a) {
+  __shared__ int hist[kBins];
+  __shared__ Pick<kThreads> pick;
+  __shared__ int before[2];      // of the segments before: positions that stay for certain, keys equal to the border
+  __shared__ int counts[kTileKeys * kBlockWaves];
+  const Segment g(a);
+  const int32_t* state = a.state + kState * g.row;
+  if (state[kAlone]) return;
+  const int thread = threadIdx.x, lane = thread % kWave, wave = thread / kWave;
+  const int first = state[kDigit], total = state[kTotal], lo = a.sink, hi = g.n - a.recent;
+  Weights now(a, g, g.begin);
+  const int2* row_counts = reinterpret_cast<const int2*>(a.counts) + static_cast<int64_t>(g.row) * a.segments;
+  const int offset = row_counts[g.s].y;
+  // every key of the row's bin, the first of a thread's in registers
+  const uint32_t* found = a.found + static_cast<int64_t>(g.row) * a.segments * a.segment;
+  uint32_t key[kTileKeys];
+#pragma unroll
+  for (int j = 0; j < kTileKeys; ++j) key[j] = j * kThreads + thread < total ? found[j * kThreads + thread] : 0u;
+  const auto each = [&](auto&& f) {
+#pragma unroll
+    for (int j = 0; j < kTileKeys; ++j)
+      if (j * kThreads + thread < total) f(j * kThreads + thread, key[j]);
+#pragma unroll 4
+    for (int i = kTile + thread; i < total; i += kThreads) f(i, found[i]);
+  };
+  if (thread < 2) before[thread] = 0;
+  __syncthreads();
+  if (thread < g.s) {
+    const int begin = static_cast<int>(min(static_cast<int64_t>(thread) * a.segment, static_cast<int64_t>(g.n)));
+    const int end = min(g.n, begin + a.segment);
+    // (and the first and last positions, which are held)
+    atomicAdd(&before[0], row_counts[thread].x + max(0, min(end, lo) - begin) + max(0, end - max(begin, hi)));
+  }
+  const bool some = first < kFirstBins;
+  uint32_t border = 0xFFFFFFFFu;
+  int equal = 0;
+  if (some) {
+    border = static_cast<uint32_t>(first);
+    equal = state[kWanted];
+#pragma unroll
+    for (int digit = 1; digit < 3; ++digit) {
+      constexpr int kLast = kSegmentBits[2];
+      const int shift = digit == 1 ? kLast : 0, bits = kSegmentBits[digit];
+      hist[thread] = hist[thread + kThreads] = 0;
+      __syncthreads();
+      each([&](int, uint32_t k) {
+        if (k >> (shift + bits) == border) atomicAdd(&hist[k >> shift & ((1 << bits) - 1)], 1);
+      });
+      __syncthreads();
+      pick_bin<kThreads, kBins>([&](int bin) { return hist[bin]; }, equal, &pick);
+      border = border << bits | static_cast<uint32_t>(pick.bin);
+      equal -= pick.above;
+      if (digit == 1 && equal == pick.in) {  // (as above)
+        border = (border << shift) - 1;
+        equal = 0;
+        break;
+      }
+    }
+    int sure = 0, ties = 0;
+    each([&](int i, uint32_t k) {
+      sure += i < offset && k > border;
+      ties += i < offset && k == border;
+    });
+    sure = wave_incl_sum_i32(sure);
+    ties = wave_incl_sum_i32(ties);
+    if (lane == kWave - 1) {
+      atomicAdd(&before[0], sure);
+      atomicAdd(&before[1], ties);
+    }
+  }
+  __syncthreads();
+  int sures = before[0], tied = before[1];
+  int32_t* kept = a.kept + static_cast<int64_t>(g.row) * a.budget;
+  float* moved = a.moved + static_cast<int64_t>(g.row) * a.budget;
+  float* sums = a.sums + g.b * a.sum_seq + g.h * a.sum_head;
+  for (int i0 = g.begin; i0 < g.end; i0 += kTile) {
+    if (i0 > g.begin) now = Weights(a, g, i0);
+    uint64_t sure[kTileKeys], tie[kTileKeys];
+#pragma unroll
+    for (int j = 0; j < kTileKeys; ++j) {
+      const int i = i0 + j * kThreads + thread;
+      const uint32_t k = order_key(now.w[j]);
+      const bool middle = some && i >= lo && i < hi;
+      sure[j] = __ballot(i < g.end && (i < lo || i >= hi || (middle && k > border)));
+      tie[j] = __ballot(i < g.end && middle && k == border);
+      if (lane == 0) counts[j * kBlockWaves + wave] = __popcll(sure[j]) | __popcll(tie[j]) << 16;
+    }
+    __syncthreads();
+    const int c = counts[lane], end = wave_incl_sum_i32(c);
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (int j = 0; j < kTileKeys; ++j) {
+      const int past = __shfl(end - c, j * kBlockWaves + wave);
+      const int t = tied + (past >> 16) + __popcll(tie[j] & below);
+      const int place = sures + (past & 0xFFFF) + __popcll(sure[j] & below) + min(t, equal);
+      const bool stays = (sure[j] >> lane & 1) || ((tie[j] >> lane & 1) && t < equal);
+      if (stays && place < a.budget) {  // (past it only if the sums change meanwhile)
+        kept[place] = i0 + j * kThreads + thread;
+        moved[place] = now.w[j];
+      }
+    }
+    const int all = __builtin_amdgcn_readlane(end, kWave - 1);
+    sures += all & 0xFFFF;
+    tied += all >> 16;
+    // (no other workgroup reads this segment's sums, and what stays is in `moved`)
+#pragma unroll
+    for (int j = 0; j < kTileKeys; ++j) {
+      const int i = i0 + j * kThreads + thread;
+      if (i >= a.budget && i < g.end) sums[i] = 0.0f;
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ the moves
+
+// parts: of a row: slices of keys, then of values, the scales, and where the row is in segments the sums.
 __global__ __launch_bounds__(kThreads) void evict_shift_kernel(const EvictArgs a, int slices, int slice_bytes, int parts,
                                                                int end) {
   const int row = blockIdx.x / parts, part = blockIdx.x - row * parts;
   const int b = row / a.c.kv_heads, h = row - b * a.c.kv_heads;
   const int32_t* kept = a.kept + static_cast<int64_t>(row) * a.budget;
   if (kept[0] < 0) return;
+  const int thread = threadIdx.x;
+  if (a.segments > 0 && part == parts - 1) {
+    float* sums = a.sums + b * a.sum_seq + h * a.sum_head;
+    const float* moved = a.moved + static_cast<int64_t>(row) * a.budget;
+    const int n = min(a.budget, evict_length(a, b));
+#pragma unroll 4
+    for (int i = thread; i < n; i += kThreads) sums[i] = moved[i];
+    return;
+  }
   const Units u = part_units(a, b, h, part, slices, slice_bytes);
-  if (part < 2 * slices) shift_units<u32x4>(kept, a.budget, end, slice_bytes / 16, u);
-  else shift_units<uint32_t>(kept, a.budget, end, 1, u);
+  const int lanes = slice_bytes / 16;
+  if (part < 2 * slices) shift_units<u32x4, kThreads>(kept, a.budget, end, lanes, thread % lanes, u);
+  else shift_units<uint32_t, kThreads>(kept, a.budget, end, 1, 0, u);
 }
 
 // From positions past the budget, which no move writes: after the first move in any order, by any number of workgroups.
-// And the sums of rows in segments.
 constexpr int kFetchUnits = 2;
 
 template <typename T>
@@ -588,32 +642,35 @@ __device__ __forceinline__ void fetch_units(const int32_t* kept, int budget, int
   }
 }
 
-constexpr int kCus = 256;
 constexpr int kFetchThreads = 256;
 constexpr int kFetchBlocks = 2048;  // of keys and values, at least, where there is work for them
 
-__global__ __launch_bounds__(kFetchThreads, 8) void evict_fetch_kernel(const EvictArgs a, int row_bytes, int parts, int splits,
-                                                                   bool rows_too) {
+__global__ __launch_bounds__(kFetchThreads, 8) void evict_fetch_kernel(const EvictArgs a, int row_bytes, int parts,
+                                                                       int splits) {
   const int split = blockIdx.x % splits, unit = blockIdx.x / splits, row = unit / parts, part = unit - row * parts;
   const int b = row / a.c.kv_heads, h = row - b * a.c.kv_heads;
   const int32_t* kept = a.kept + static_cast<int64_t>(row) * a.budget;
   if (kept[0] < 0) return;
-  const int thread = threadIdx.x;
-  if (part == parts - 1) {
-    if (a.segments == 0) return;
-    float* sums = a.sums + b * a.sum_seq + h * a.sum_head;
-    const float* moved = a.moved + static_cast<int64_t>(row) * a.budget;
-    const int n = evict_length(a, b);
-    for (int i = split * kFetchThreads + thread; i < n; i += splits * kFetchThreads) sums[i] = i < a.budget ? moved[i] : 0.0f;
-    return;
-  }
-  if (!rows_too) return;
   const Units u = part_units(a, b, h, part, 1, row_bytes);
   const int lanes = part < 2 ? row_bytes / 16 : 1, rows = kFetchThreads / lanes;
-  const int i0 = split * rows + thread / lanes, step = splits * rows;
+  const int i0 = split * rows + static_cast<int>(threadIdx.x) / lanes, step = splits * rows;
   if (part < 2) fetch_units<u32x4>(kept, a.budget, lanes, i0, step, u);
   else fetch_units<uint32_t>(kept, a.budget, lanes, i0, step, u);
 }
+
+template <bool kMove>
+static void select_launch(const EvictArgs& a, int64_t rows, int64_t positions, bool small, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(rows));
+  if (positions <= 16 * 256 && small)
+    hipLaunchKernelGGL((evict_select_kernel<256, 16, kMove>), grid, dim3(256), 0, st, a);
+  else if (positions <= 16 * kThreads)
+    hipLaunchKernelGGL((evict_select_kernel<kThreads, 16, kMove>), grid, dim3(kThreads), 0, st, a);
+  else
+    hipLaunchKernelGGL((evict_select_kernel<kThreads, 32, kMove>), grid, dim3(kThreads), 0, st, a);
+}
+
+constexpr int64_t kSmallMove = 128 << 10;
+constexpr int kFarBudget = 4096;
 
 struct EvictSpace {
   int64_t counts, hist, found, moved, bytes;
@@ -629,7 +686,7 @@ static EvictSpace evict_space(int64_t rows, int64_t positions, int64_t budget) {
   s.segment = static_cast<int>((each + kTile - 1) / kTile * kTile);
   s.counts = up(rows * kState * 4);
   s.hist = s.counts + up(rows * 2LL * s.segments * 4);
-  s.found = s.hist + rows * s.segments * kBins * 4;
+  s.found = s.hist + rows * s.segments * kFirstBins * 4;
   s.moved = s.found + rows * s.segments * s.segment * 4;
   s.bytes = s.moved + rows * budget * 4;
   return s;
@@ -666,13 +723,16 @@ extern "C" int tris_paged_cache_evict(const tris_paged_cache* cache, float* weig
   const int64_t rows = static_cast<int64_t>(c.batch) * c.kv_heads, positions = cache_positions(c);
   const bool e4m3 = c.dtype == TRIS_DTYPE_E4M3;
   const int row_bytes = c.head_dim * (e4m3 ? 1 : 2);
+  const EvictSpace s = evict_space(rows, positions, budget);
+  const int64_t row_move = static_cast<int64_t>(budget) * row_bytes * 2;
+  const bool small = row_move <= kSmallMove;
+  const bool together = s.segments == 0 && (small || rows >= kCus);  // the selecting workgroups move
   // slices of 128 bytes where they occupy the GPU, else of 64
   const int slice_bytes = row_bytes >= 128 && rows * 2 * (row_bytes / 128) >= kCus ? 128 : 64;
-  const int slices = row_bytes / slice_bytes, parts = 2 * slices + (e4m3 ? 2 : 0);
-  const EvictSpace s = evict_space(rows, positions, budget);
+  const int slices = row_bytes / slice_bytes, parts = 2 * slices + (e4m3 ? 2 : 0) + (s.segments ? 1 : 0);
   // rows may come from past the budget in numbers, and one workgroup a slice leaves the GPU idle
-  const bool far = positions >= 2LL * budget && rows * 2 * slices < 2 * kCus;
-  const int fetch_parts = (e4m3 ? 4 : 2) + 1;
+  const bool far = positions >= 2LL * budget && rows * 2 * slices < 2 * kCus && budget > kFarBudget;
+  const int fetch_parts = e4m3 ? 4 : 2;
   const int splits = static_cast<int>(std::min<int64_t>(256, std::max<int64_t>(1, kFetchBlocks / (rows * 2))));
   // a launch has less than 2^32 threads
   TRIS_REQUIRE(rows * std::max(parts, s.segments) < (1LL << 32) / kThreads &&
@@ -683,8 +743,12 @@ extern "C" int tris_paged_cache_evict(const tris_paged_cache* cache, float* weig
   EvictArgs a{weight_sum, sum_seq_stride, sum_head_stride, budget, limit, sink, recent, new_lens, kept,
               PageDivision(c.page_size), c, s.segments, s.segment, nullptr, nullptr, nullptr, nullptr, nullptr};
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (together) {
+    select_launch<true>(a, rows, positions, small, st);
+    return check_launch(who);
+  }
   if (s.segments == 0) {
-    hipLaunchKernelGGL(evict_select_kernel, dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, st, a);
+    select_launch<false>(a, rows, positions, true, st);
   } else {
     char* at = static_cast<char*>(workspace);
     a.state = reinterpret_cast<int32_t*>(at);
@@ -699,8 +763,8 @@ extern "C" int tris_paged_cache_evict(const tris_paged_cache* cache, float* weig
   }
   hipLaunchKernelGGL(evict_shift_kernel, dim3(static_cast<unsigned>(rows * parts)), dim3(kThreads), 0, st, a, slices,
                      slice_bytes, parts, far ? budget : INT32_MAX);
-  if (far || s.segments)
+  if (far)
     hipLaunchKernelGGL(evict_fetch_kernel, dim3(static_cast<unsigned>(rows * fetch_parts * splits)), dim3(kFetchThreads), 0,
-                       st, a, row_bytes, fetch_parts, splits, far);
+                       st, a, row_bytes, fetch_parts, splits);
   return check_launch(who);
 }

@@ -101,7 +101,7 @@ def test_lengths_and_budgets(tris, cuda, cache, dim, page, order):
 @pytest.mark.gpu
 @pytest.mark.parametrize("heads", [1, 3, 8])
 @pytest.mark.parametrize("lengths,budget", [([5000, 4097, 4096, 3], 4096), ([9000, 1030], 1025), ([20000], 1500),
-                                            ([3000] * 5, 2999), ([2000], 1)], ids=str)
+                                            ([3000] * 5, 2999), ([2000], 1), ([1500] * 33, 1400)], ids=str)
 def test_long_sequences(tris, cuda, heads, lengths, budget):
     for cache, page in ((F16, 16), (E4M3, 5)):
         print(f"[gpu-case] evict long {cache} heads={heads} {lengths} budget={budget}", flush=True)
@@ -112,9 +112,10 @@ def test_long_sequences(tris, cuda, heads, lengths, budget):
 @pytest.mark.gpu
 @pytest.mark.parametrize("lengths,budget,limit,sink,recent", [
     ([20000, 16385, 15000, 0, 18000], 15000, 16000, 4, 3000), ([40000], 4096, None, 0, 0), ([33000, 40], 9000, None, 4500, 4500),
-    ([300000], 20000, None, 64, 1000), ([16384, 16383], 16380, None, 1, 1), ([20000], 19999, None, 9000, 9000)], ids=str)
-def test_rows_in_segments(tris, cuda, lengths, budget, limit, sink, recent):
-    """Tables of more positions than one workgroup takes; budgets beside and below half of them."""
+    ([300000], 20000, None, 64, 1000), ([16384, 16383], 16380, None, 1, 1), ([32768], 20000, None, 9000, 9000),
+    ([50000, 49000, 7], 49000, 49500, 100, 100), ([33000], 4097, None, 0, 4097)], ids=str)
+def test_long_rows(tris, cuda, lengths, budget, limit, sink, recent):
+    """Tables of as many positions as one workgroup takes and more; budgets beside and below half of them."""
     for cache, page in ((BF16, 64), (E4M3, 7)):
         print(f"[gpu-case] evict segments {cache} {lengths} budget={budget}", flush=True)
         a = evict_case(cuda, 1, 64, cache, page, lengths, seed=budget, extra=1)
@@ -122,7 +123,7 @@ def test_rows_in_segments(tris, cuda, lengths, budget, limit, sink, recent):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("n", [16384, 30000])
+@pytest.mark.parametrize("n", [16384, 30000, 40000])
 def test_ties_over_segments(tris, cuda, n):
     """The border among equal weights that lie in every segment, one segment, or are all there is."""
     a = evict_case(cuda, 4, 64, F16, 16, [n], extra_pages=0)
@@ -137,10 +138,10 @@ def test_ties_over_segments(tris, cuda, n):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("extra_pages", [1, 1100])
+@pytest.mark.parametrize("extra_pages", [1, 300, 1100, 2100])
 def test_special_weights_and_ties(tris, cuda, extra_pages):
     """All equal, zeros of both signs, subnormals, negative ones, infinities and NaN of either sign; ties at the border go
-    to the lowest positions.  The same in a table wide enough for rows in segments."""
+    to the lowest positions.  The same in tables of other widths."""
     inf, nan = float("inf"), float("nan")
     lengths = [3000, 500, 300, 64, 200, 400]
     a = evict_case(cuda, 2, 64, F16, 16, lengths, extra_pages=extra_pages)
@@ -310,10 +311,10 @@ def test_refusals_without_gpu(tris):
         if "dtype" not in kw or kw["dtype"] == 3:
             assert call(c_cache(**kw)) == -1 and word in lib.tris_last_error(), kw
     most = 2 ** 31 - 1
-    need = lib.tris_paged_cache_evict_workspace_bytes(2, 2, 1025, 16, 8)
-    assert need > 4 * 16400 * 4 and lib.tris_paged_cache_evict_workspace_bytes(2, 2, 1024, 16, 8) == 0
-    wide = dict(cache=c_cache(max_pages=1025, table_stride=1025), seq=32800, head=16400, ws=p, space=need)
-    for bad in ((0, 2, 1025, 16, 8), (2, 0, 1025, 16, 8), (2, 2, -1, 16, 8), (2, 2, 1025, 0, 8), (2, 2, 1025, 16, 0)):
+    need = lib.tris_paged_cache_evict_workspace_bytes(2, 2, 2049, 16, 8)
+    assert need > 4 * 32784 * 4 and lib.tris_paged_cache_evict_workspace_bytes(2, 2, 2048, 16, 8) == 0
+    wide = dict(cache=c_cache(max_pages=2049, table_stride=2049), seq=65568, head=32784, ws=p, space=need)
+    for bad in ((0, 2, 2049, 16, 8), (2, 0, 2049, 16, 8), (2, 2, -1, 16, 8), (2, 2, 2049, 0, 8), (2, 2, 2049, 16, 0)):
         assert lib.tris_paged_cache_evict_workspace_bytes(*bad) == 0
     for kw, word in ((dict(budget=0, limit=0), b"budget"), (dict(limit=7), b"budget"), (dict(sink=-1), b"within"),
                      (dict(recent=-1), b"within"), (dict(sink=7), b"within"), (dict(sink=most, recent=most), b"within"),
