@@ -6,7 +6,7 @@
 // that share the digits before.  The first digit is the sign, the exponent and two bits more, so that weights over many
 // powers of two spread over its bins (8-bit digits put two powers of two into one, and the additions wait for each other).
 //
-// Up to kSelectMost positions one workgroup has a row, its weights in registers, read once; it lists the positions that
+// Up to kSelectMost positions one workgroup has a row, its weights in LDS, read once; it lists the positions that
 // stay and moves the sums as well, and keys and values too where rows are many or small.  Longer rows are cut into segments
 // of a workgroup each, in three launches: histograms of the first digit; the keys in the border's bin, gathered; and, in
 // every workgroup alike, the border among those, by which it places its segment.
@@ -50,9 +50,9 @@ constexpr int kState = 4, kAlone = 0, kDigit = 1, kWanted = 2, kTotal = 3;
 
 // A weight as an unsigned number of the same order: NaN above all, the zeros equal.
 __device__ __forceinline__ uint32_t order_key(float w) {
-  if (w != w) return 0xFFFFFFFFu;
-  const uint32_t u = __float_as_uint(w == 0.0f ? 0.0f : w);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t u = __float_as_uint(w + 0.0f);  // (-0 + 0 is 0)
+  const uint32_t key = u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+  return w != w ? 0xFFFFFFFFu : key;
 }
 
 __device__ __forceinline__ int evict_length(const EvictArgs& a, int b) {
@@ -88,9 +88,8 @@ __device__ __forceinline__ void pick_bin(Count count, int left, Pick<kBlock>* sh
   const int end = wave_incl_sum_i32(sum);
   if (lane == kWave - 1) sh->totals[wave] = end;
   __syncthreads();
-  int before = end - sum;
-#pragma unroll
-  for (int w = 0; w < kBlock / kWave; ++w) before += w < wave ? sh->totals[w] : 0;
+  const int total = lane < kBlock / kWave ? sh->totals[lane] : 0, ends = wave_incl_sum_i32(total);
+  int before = end - sum + __builtin_amdgcn_readlane(ends - total, wave);
   if (before < left && left <= before + sum) {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
@@ -236,6 +235,7 @@ __device__ __forceinline__ void shift_units(const int32_t* kept, int budget, int
 template <int kBlock, int kKeys, bool kMove>
 __global__ __launch_bounds__(kBlock) void evict_select_kernel(const EvictArgs a) {
   constexpr int kWaves = kBlock / kWave, kCounts = kKeys * kWaves;
+  __shared__ float weights[kBlock * kKeys];  // (a position is read by the thread that wrote it)
   __shared__ int hist[kBins];
   __shared__ uint32_t counts[kCounts];
   __shared__ Pick<kBlock> pick;
@@ -244,11 +244,17 @@ __global__ __launch_bounds__(kBlock) void evict_select_kernel(const EvictArgs a)
   const int n = evict_length(a, b);
   int32_t* kept = a.kept + static_cast<int64_t>(row) * a.budget;
   float* sums = a.sums + b * a.sum_seq + h * a.sum_head;
-  float w[kKeys];
   bool due = n > a.limit;
   if (due) {
+    constexpr int kAtOnce = 8;
+#pragma unroll 1
+    for (int i0 = thread; i0 < n; i0 += kAtOnce * kBlock) {
+      float w[kAtOnce];
 #pragma unroll
-    for (int j = 0; j < kKeys; ++j) w[j] = j * kBlock + thread < n ? sums[j * kBlock + thread] : 0.0f;
+      for (int u = 0; u < kAtOnce; ++u) w[u] = i0 + u * kBlock < n ? sums[i0 + u * kBlock] : 0.0f;
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) weights[i0 + u * kBlock] = w[u];
+    }
     due = pages_good<kBlock>(a, b, n);
   }
   if (h == 0 && thread == 0) a.new_lens[b] = due ? a.budget : a.c.seq_lens[b];
@@ -262,26 +268,26 @@ __global__ __launch_bounds__(kBlock) void evict_select_kernel(const EvictArgs a)
   if (want > 0) {
     uint32_t prefix = 0;
     equal = want;
-#pragma unroll
-    for (int digit = 0; digit < 3; ++digit) {
-      const int bits = kRowBits[digit], shift = digit == 0 ? kRowBits[1] + kRowBits[2] : digit == 1 ? kRowBits[2] : 0;
+#pragma unroll 1
+    for (int shift = 32, bits; shift > 0;) {
+      bits = shift > kRowBits[2] ? kRowBits[0] : kRowBits[2];
+      shift -= bits;
 #pragma unroll
       for (int i = thread; i < kBins; i += kBlock) hist[i] = 0;
       __syncthreads();
-#pragma unroll
-      for (int j = 0; j < kKeys; ++j) {
-        const int i = j * kBlock + thread;
-        if (j * kBlock < n && i >= lo && i < hi) {
-          const uint32_t key = order_key(w[j]);
-          if (digit == 0 || key >> (shift + bits) == prefix) atomicAdd(&hist[key >> shift & ((1 << bits) - 1)], 1);
-        }
+      // (64-bit shifts: the first digit has nothing before it)
+#pragma unroll 2
+      for (int i = thread; i < hi; i += kBlock) {
+        const uint32_t key = order_key(weights[i]);
+        if (i >= lo && static_cast<uint64_t>(key) >> (shift + bits) == prefix)
+          atomicAdd(&hist[key >> shift & ((1u << bits) - 1)], 1);
       }
       __syncthreads();
       pick_bin<kBlock, kBins>([&](int bin) { return hist[bin]; }, equal, &pick);
       prefix = prefix << bits | static_cast<uint32_t>(pick.bin);
       equal -= pick.above;
       border = prefix;
-      if (digit < 2 && equal == pick.in) {
+      if (equal == pick.in) {
         // the whole bin stays: the border is the largest key below it (there is one: no key is below 2^22)
         border = (prefix << shift) - 1;
         equal = 0;
@@ -290,19 +296,20 @@ __global__ __launch_bounds__(kBlock) void evict_select_kernel(const EvictArgs a)
     }
   }
   // Of each 64 positions: how many stay for certain, and (from bit 16 on) how many are equal to the border.
-  const auto classes = [&](int j, uint64_t* sure, uint64_t* tie) {
+  uint32_t mine = 0;                  // lane j: of the wavefront's 64 from j * kBlock on
+  uint32_t sure_bits = 0, tie_bits = 0;  // bit j: of the thread's own
+#pragma unroll 1
+  for (int j = 0; j * kBlock < n; ++j) {
     const int i = j * kBlock + thread;
-    const bool middle = i >= lo && i < hi && want > 0;
-    const uint32_t key = order_key(w[j]);
-    *sure = __ballot(i < n && (i < lo || i >= hi || (middle && key > border)));
-    *tie = __ballot(middle && key == border);
-  };
-#pragma unroll
-  for (int j = 0; j < kKeys; ++j) {
-    uint64_t sure, tie;
-    classes(j, &sure, &tie);
-    if (lane == 0) counts[j * kWaves + wave] = __popcll(sure) | __popcll(tie) << 16;
+    const uint32_t key = order_key(weights[i]);
+    const bool middle = i >= lo && i < hi, decides = middle && want > 0;
+    const bool sure = decides ? key > border : !middle && i < n, tie = decides && key == border;
+    sure_bits |= static_cast<uint32_t>(sure) << j;
+    tie_bits |= static_cast<uint32_t>(tie) << j;
+    const uint32_t both = __popcll(__ballot(sure)) | __popcll(__ballot(tie)) << 16;
+    mine = lane == j ? both : mine;
   }
+  if (lane < kKeys) counts[lane * kWaves + wave] = mine;
   __syncthreads();
   if (wave == 0) {  // the numbers before each
     constexpr int kEach = kCounts / kWave;
@@ -318,17 +325,17 @@ __global__ __launch_bounds__(kBlock) void evict_select_kernel(const EvictArgs a)
   }
   __syncthreads();
   const uint64_t below = (1ull << lane) - 1;
-#pragma unroll
-  for (int j = 0; j < kKeys; ++j) {
-    if (j * kBlock >= n) break;
-    uint64_t sure, tie;
-    classes(j, &sure, &tie);
+#pragma unroll 1
+  for (int j = 0; j * kBlock < n; ++j) {
+    const int i = j * kBlock + thread;
+    const bool sure = sure_bits >> j & 1, tie = tie_bits >> j & 1;
     const uint32_t before = counts[j * kWaves + wave];
-    const int ties = static_cast<int>(before >> 16) + __popcll(tie & below);
-    if ((sure >> lane & 1) || ((tie >> lane & 1) && ties < equal)) {
-      const int place = static_cast<int>(before & 0xFFFF) + __popcll(sure & below) + min(ties, equal);
-      kept[place] = j * kBlock + thread;
-      sums[place] = w[j];  // (every weight of the row is in registers)
+    const int sures = static_cast<int>(before & 0xFFFF) + __popcll(__ballot(sure) & below);
+    const int ties = static_cast<int>(before >> 16) + __popcll(__ballot(tie) & below);
+    if (sure || (tie && ties < equal)) {
+      const int place = sures + min(ties, equal);
+      kept[place] = i;
+      sums[place] = weights[i];  // (the row's weights are all in LDS)
     }
   }
   for (int i = a.budget + thread; i < n; i += kBlock) sums[i] = 0.0f;
