@@ -24,7 +24,7 @@ constexpr int kSelectMost = 32 * kThreads;
 constexpr int kRowBits[3] = {11, 11, 10}, kSegmentBits[3] = {10, 11, 11};
 constexpr int kBins = 1 << 11, kFirstBins = 1 << kSegmentBits[0], kFirstShift = 32 - kSegmentBits[0];
 constexpr int kMostSegments = 64;  // a lane each
-constexpr int kCus = 256;
+constexpr int kCus = 256, kXcds = 8;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -600,7 +600,10 @@ __global__ __launch_bounds__(kThreads) void evict_place_kernel(const EvictArgs a
 // parts: of a row: slices of keys, then of values, the scales, and where the row is in segments the sums.
 __global__ __launch_bounds__(kThreads) void evict_shift_kernel(const EvictArgs a, int slices, int slice_bytes, int parts,
                                                                int end) {
-  const int row = blockIdx.x / parts, part = blockIdx.x - row * parts;
+  // a row's parts on one XCD, whose cache then has a line for both of its slices
+  const int group = blockIdx.x / (kXcds * parts), in = blockIdx.x - group * (kXcds * parts);
+  const int row = group * kXcds + in % kXcds, part = in / kXcds;
+  if (row >= a.c.batch * a.c.kv_heads) return;
   const int b = row / a.c.kv_heads, h = row - b * a.c.kv_heads;
   const int32_t* kept = a.kept + static_cast<int64_t>(row) * a.budget;
   if (kept[0] < 0) return;
@@ -676,7 +679,12 @@ static void select_launch(const EvictArgs& a, int64_t rows, int64_t positions, b
     hipLaunchKernelGGL((evict_select_kernel<kThreads, 32, kMove>), grid, dim3(kThreads), 0, st, a);
 }
 
+// Slices of 128 bytes from as many workgroups on, else of 64 (the call in a graph, 128 / 64: 64 workgroups of 128 bytes 29.9
+// / 23.9 us, 128 33.3 / 29.9, 184 68.0 / 75.3, 512 101.9 / 107.7).
+constexpr int kWideSlices = 160;
+// Bytes of a row's keys and values up to which the selecting workgroup moves them (xx).
 constexpr int64_t kSmallMove = 128 << 10;
+// Budget from which on the rows past it are moved by a launch of their own (xx).
 constexpr int kFarBudget = 4096;
 
 struct EvictSpace {
@@ -734,15 +742,14 @@ extern "C" int tris_paged_cache_evict(const tris_paged_cache* cache, float* weig
   const int64_t row_move = static_cast<int64_t>(budget) * row_bytes * 2;
   const bool small = row_move <= kSmallMove;
   const bool together = s.segments == 0 && (small || rows >= kCus);  // the selecting workgroups move
-  // slices of 128 bytes where they occupy the GPU, else of 64
-  const int slice_bytes = row_bytes >= 128 && rows * 2 * (row_bytes / 128) >= kCus ? 128 : 64;
+  const int slice_bytes = row_bytes >= 128 && rows * 2 * (row_bytes / 128) >= kWideSlices ? 128 : 64;
   const int slices = row_bytes / slice_bytes, parts = 2 * slices + (e4m3 ? 2 : 0) + (s.segments ? 1 : 0);
   // rows may come from past the budget in numbers, and one workgroup a slice leaves the GPU idle
   const bool far = positions >= 2LL * budget && rows * 2 * slices < 2 * kCus && budget > kFarBudget;
   const int fetch_parts = e4m3 ? 4 : 2;
   const int splits = static_cast<int>(std::min<int64_t>(256, std::max<int64_t>(1, kFetchBlocks / (rows * 2))));
   // a launch has less than 2^32 threads
-  TRIS_REQUIRE(rows * std::max(parts, s.segments) < (1LL << 32) / kThreads &&
+  TRIS_REQUIRE((rows + kXcds) * std::max(parts, s.segments) < (1LL << 32) / kThreads &&
                    rows * fetch_parts * splits < (1LL << 32) / kFetchThreads,
                "%s: too many rows", who);
   TRIS_REQUIRE(s.bytes == 0 || (workspace && aligned16(workspace) && workspace_bytes >= s.bytes),
@@ -768,7 +775,7 @@ extern "C" int tris_paged_cache_evict(const tris_paged_cache* cache, float* weig
     hipLaunchKernelGGL(evict_gather_kernel, grid, block, 0, st, a);
     hipLaunchKernelGGL(evict_place_kernel, grid, block, 0, st, a);
   }
-  hipLaunchKernelGGL(evict_shift_kernel, dim3(static_cast<unsigned>(rows * parts)), dim3(kThreads), 0, st, a, slices,
+  hipLaunchKernelGGL(evict_shift_kernel, dim3(static_cast<unsigned>((rows + kXcds - 1) / kXcds * kXcds * parts)), dim3(kThreads), 0, st, a, slices,
                      slice_bytes, parts, far ? budget : INT32_MAX);
   if (far)
     hipLaunchKernelGGL(evict_fetch_kernel, dim3(static_cast<unsigned>(rows * fetch_parts * splits)), dim3(kFetchThreads), 0,

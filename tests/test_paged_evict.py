@@ -236,8 +236,8 @@ def test_again_and_again(tris, cuda):
 
 
 @pytest.mark.gpu
-def test_streams_and_graphs(tris, cuda):
-    """Beside another call on another stream, and from a graph replayed over lengths that grow past the limit."""
+def test_streams(tris, cuda):
+    """Beside another call on another stream."""
     ext = tris["ext"]
     a, b = (evict_case(cuda, 2, 64, BF16, 16, [600, 300], seed=s) for s in (1, 2))
     want = [expected(x, 256, None, 4, 100) for x in (a, b)]
@@ -250,8 +250,17 @@ def test_streams_and_graphs(tris, cuda):
     for x, (out, sums, new, kept), got in ((a, want[0], got_a), (b, want[1], got_b)):
         assert torch.equal(got[0].cpu(), new) and torch.equal(got[1].cpu(), kept)
         assert torch.equal(x["weight_sum"].cpu(), sums) and torch.equal(_bits(x["k_cache"]), _bits(out["k_cache"]))
-    a = evict_case(cuda, 2, 64, BF16, 16, [600, 300], seed=3)
-    args = dict(budget=250, limit=290, sink=4, recent=40)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("extra_pages,budget", [(1, 250), (2100, 250), (1, 40)])
+def test_graph_replays(tris, cuda, extra_pages, budget):
+    """A captured call over lengths that grow past the limit, with eager calls and other work between its replays; a table
+    of one workgroup a row and of several, a move of its own and with the choice."""
+    ext = tris["ext"]
+    a = evict_case(cuda, 2, 64, BF16, 16, [600, 300], seed=3, extra_pages=extra_pages)
+    other = evict_case(cuda, 2, 64, BF16, 16, [500, 450], seed=4, extra_pages=extra_pages)
+    args = dict(budget=budget, limit=290, sink=4, recent=20)
     a["seq_lens"].zero_()
     ext.paged_cache_evict(**a, **args)
     graph = torch.cuda.CUDAGraph()
@@ -267,7 +276,8 @@ def test_streams_and_graphs(tris, cuda):
         assert torch.equal(a["weight_sum"].cpu(), sums)
         for n in ("k_cache", "v_cache"):
             assert torch.equal(_bits(a[n]), _bits(out[n]))
-        lens = [n + 1 for n in want_new.tolist()]
+        ext.paged_cache_evict(**other, budget=300 + step)
+        lens = [n + 1 if n > 250 else 289 + i for i, n in enumerate(want_new.tolist())]
         a["weight_sum"].add_(torch.rand_like(a["weight_sum"]))
 
 
