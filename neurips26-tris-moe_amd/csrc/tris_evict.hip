@@ -6,7 +6,7 @@
 // that share the digits before.  The first digit is the sign, the exponent and two bits more, so that weights over many
 // powers of two spread over its bins (8-bit digits put two powers of two into one, and the additions wait for each other).
 //
-// Up to kSelectMost positions one workgroup has a row, its weights in LDS, read once; it lists the positions that
+// Up to 16384 or 32768 positions one workgroup has a row, its weights in LDS, read once; it lists the positions that
 // stay and moves the sums as well, and keys and values too where rows are many or small.  Longer rows are cut into segments
 // of a workgroup each, in three launches: histograms of the first digit; the keys in the border's bin, gathered; and, in
 // every workgroup alike, the border among those, by which it places its segment.
@@ -18,7 +18,6 @@ namespace tris {
 
 constexpr int kThreads = 1024;  // of the workgroups of long rows, and of the moves
 constexpr int kBlockWaves = kThreads / kWave;
-constexpr int kSelectMost = 32 * kThreads;
 // bits of the digits, first to last, of rows in one workgroup and in segments (whose histograms of the first every workgroup
 // of the row reads)
 constexpr int kRowBits[3] = {11, 11, 10}, kSegmentBits[3] = {10, 11, 11};
@@ -668,10 +667,14 @@ __global__ __launch_bounds__(kFetchThreads, 8) void evict_fetch_kernel(const Evi
   else fetch_units<uint32_t>(kept, a.budget, lanes, i0, step, u);
 }
 
+// A row's workgroup has 1024 threads, or 256 where the table is so narrow (256 / 1024: 4 rows of 900 positions 11.7 / 10.4
+// us, 320 rows 13.6 / 18.3, of 3000 positions 19.7 / 22.4).
+constexpr int kShort = 256, kShortManyRows = 16 * 256;
+
 template <bool kMove>
-static void select_launch(const EvictArgs& a, int64_t rows, int64_t positions, bool small, hipStream_t st) {
+static void select_launch(const EvictArgs& a, int64_t rows, int64_t positions, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(rows));
-  if (positions <= 16 * 256 && small)
+  if (positions <= (rows > kCus ? kShortManyRows : kShort))
     hipLaunchKernelGGL((evict_select_kernel<256, 16, kMove>), grid, dim3(256), 0, st, a);
   else if (positions <= 16 * kThreads)
     hipLaunchKernelGGL((evict_select_kernel<kThreads, 16, kMove>), grid, dim3(kThreads), 0, st, a);
@@ -682,9 +685,15 @@ static void select_launch(const EvictArgs& a, int64_t rows, int64_t positions, b
 // Slices of 128 bytes from as many workgroups on, else of 64 (the call in a graph, 128 / 64: 64 workgroups of 128 bytes 29.9
 // / 23.9 us, 128 33.3 / 29.9, 184 68.0 / 75.3, 512 101.9 / 107.7).
 constexpr int kWideSlices = 160;
-// Bytes of a row's keys and values up to which the selecting workgroup moves them (xx).
-constexpr int64_t kSmallMove = 128 << 10;
-// Budget from which on the rows past it are moved by a launch of their own (xx).
+// The selecting workgroups move what their rows keep, in one launch, where that is up to so many bytes of a row, and, up to
+// four times as many or one workgroup a CU, from so many rows on (together / in two launches: 8 rows of 32, 128 and 256
+// positions of 512 bytes 8.9 / 10.9, 11.7 / 10.9, 16.1 / 11.7 us in a graph, and a launch less for the host; 192 rows of
+// 512 and 2048 23.4 / 32.3, 78 / 85; 320 rows of 512, 1024 and 2048 40 / 44, 86 / 84, 155 / 138).
+constexpr int64_t kSmallMove = 64 << 10;
+constexpr int kManyRows = 160;
+// Budgets from which on the rows past them are moved by a launch of their own, where slices are few and the table has
+// twice as many positions (with it / without: 4 rows of 4096 of 32768 positions 43.5 / 46.1 us, 8192 of 65536 35.4 / 42.5;
+// 16 rows 53.5 / 51.1 and 56.8 / 67.7; 32 rows of 8192 of 32768 102.5 / 96.1).
 constexpr int kFarBudget = 4096;
 
 struct EvictSpace {
@@ -692,9 +701,14 @@ struct EvictSpace {
   int segments, segment;
 };
 
+// Positions of a table up to which a row is one workgroup's: more where rows are many (in segments / in one workgroup: 4 rows
+// of 12000 positions 25.7 / 23.8 us, 20000 26.3 / 29.0; 32 rows of 20000 32.0 / 36.0; 128 rows of 32000 93 / 83).
+constexpr int kFewRows = 64;
+static int64_t one_workgroup(int64_t rows) { return (rows <= kFewRows ? 16 : 32) * kThreads; }
+
 static EvictSpace evict_space(int64_t rows, int64_t positions, int64_t budget) {
   EvictSpace s{};
-  if (positions <= kSelectMost) return s;
+  if (positions <= one_workgroup(rows)) return s;
   const auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
   s.segments = static_cast<int>(std::min<int64_t>(kMostSegments, (positions + kTile - 1) / kTile));
   const int64_t each = (positions + s.segments - 1) / s.segments;
@@ -741,11 +755,11 @@ extern "C" int tris_paged_cache_evict(const tris_paged_cache* cache, float* weig
   const EvictSpace s = evict_space(rows, positions, budget);
   const int64_t row_move = static_cast<int64_t>(budget) * row_bytes * 2;
   const bool small = row_move <= kSmallMove;
-  const bool together = s.segments == 0 && (small || rows >= kCus);  // the selecting workgroups move
+  const bool together =
+      s.segments == 0 && (small || (rows >= kManyRows && (rows <= kCus || row_move <= 4 * kSmallMove)));
   const int slice_bytes = row_bytes >= 128 && rows * 2 * (row_bytes / 128) >= kWideSlices ? 128 : 64;
   const int slices = row_bytes / slice_bytes, parts = 2 * slices + (e4m3 ? 2 : 0) + (s.segments ? 1 : 0);
-  // rows may come from past the budget in numbers, and one workgroup a slice leaves the GPU idle
-  const bool far = positions >= 2LL * budget && rows * 2 * slices < 2 * kCus && budget > kFarBudget;
+  const bool far = positions >= 2LL * budget && rows * 2 * slices <= kCus / 2 && budget > kFarBudget;
   const int fetch_parts = e4m3 ? 4 : 2;
   const int splits = static_cast<int>(std::min<int64_t>(256, std::max<int64_t>(1, kFetchBlocks / (rows * 2))));
   // a launch has less than 2^32 threads
@@ -758,11 +772,11 @@ extern "C" int tris_paged_cache_evict(const tris_paged_cache* cache, float* weig
               PageDivision(c.page_size), c, s.segments, s.segment, nullptr, nullptr, nullptr, nullptr, nullptr};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (together) {
-    select_launch<true>(a, rows, positions, small, st);
+    select_launch<true>(a, rows, positions, st);
     return check_launch(who);
   }
   if (s.segments == 0) {
-    select_launch<false>(a, rows, positions, true, st);
+    select_launch<false>(a, rows, positions, st);
   } else {
     char* at = static_cast<char*>(workspace);
     a.state = reinterpret_cast<int32_t*>(at);

@@ -322,7 +322,7 @@ def test_refusals_without_gpu(tris):
             assert call(c_cache(**kw)) == -1 and word in lib.tris_last_error(), kw
     most = 2 ** 31 - 1
     need = lib.tris_paged_cache_evict_workspace_bytes(2, 2, 2049, 16, 8)
-    assert need > 4 * 32784 * 4 and lib.tris_paged_cache_evict_workspace_bytes(2, 2, 2048, 16, 8) == 0
+    assert need > 4 * 32784 * 4 and lib.tris_paged_cache_evict_workspace_bytes(2, 2, 16, 16, 8) == 0
     wide = dict(cache=c_cache(max_pages=2049, table_stride=2049), seq=65568, head=32784, ws=p, space=need)
     for bad in ((0, 2, 2049, 16, 8), (2, 0, 2049, 16, 8), (2, 2, -1, 16, 8), (2, 2, 2049, 0, 8), (2, 2, 2049, 16, 0)):
         assert lib.tris_paged_cache_evict_workspace_bytes(*bad) == 0
