@@ -691,6 +691,10 @@ constexpr int kWideSlices = 160;
 // 512 and 2048 23.4 / 32.3, 78 / 85; 320 rows of 512, 1024 and 2048 40 / 44, 86 / 84, 155 / 138).
 constexpr int64_t kSmallMove = 64 << 10;
 constexpr int kManyRows = 160;
+// In a decode loop a sequence is due in one of limit - budget + 1 steps, and in the others a launch less is what counts: so
+// they move too where all sequences' moves come to so many bytes of a row a step (one sequence of 8 heads, 2048 positions of
+// 512 bytes, limit 2176: 3.9 / 5.5 us with nothing due, 40 / 20 when it is).
+constexpr int64_t kRareMove = 16 << 10;
 // Budgets from which on the rows past them are moved by a launch of their own, where slices are few and the table has
 // twice as many positions (with it / without: 4 rows of 4096 of 32768 positions 43.5 / 46.1 us, 8192 of 65536 35.4 / 42.5;
 // 16 rows 53.5 / 51.1 and 56.8 / 67.7; 32 rows of 8192 of 32768 102.5 / 96.1).
@@ -754,7 +758,8 @@ extern "C" int tris_paged_cache_evict(const tris_paged_cache* cache, float* weig
   const int row_bytes = c.head_dim * (e4m3 ? 1 : 2);
   const EvictSpace s = evict_space(rows, positions, budget);
   const int64_t row_move = static_cast<int64_t>(budget) * row_bytes * 2;
-  const bool small = row_move <= kSmallMove;
+  const bool small = row_move <= kSmallMove ||
+                     static_cast<__int128>(row_move) * c.batch <= kRareMove * (static_cast<__int128>(limit) - budget + 1);
   const bool together =
       s.segments == 0 && (small || (rows >= kManyRows && (rows <= kCus || row_move <= 4 * kSmallMove)));
   const int slice_bytes = row_bytes >= 128 && rows * 2 * (row_bytes / 128) >= kWideSlices ? 128 : 64;
@@ -789,7 +794,8 @@ extern "C" int tris_paged_cache_evict(const tris_paged_cache* cache, float* weig
     hipLaunchKernelGGL(evict_gather_kernel, grid, block, 0, st, a);
     hipLaunchKernelGGL(evict_place_kernel, grid, block, 0, st, a);
   }
-  hipLaunchKernelGGL(evict_shift_kernel, dim3(static_cast<unsigned>((rows + kXcds - 1) / kXcds * kXcds * parts)), dim3(kThreads), 0, st, a, slices,
+  const int64_t shift_blocks = (rows + kXcds - 1) / kXcds * kXcds * parts;
+  hipLaunchKernelGGL(evict_shift_kernel, dim3(static_cast<unsigned>(shift_blocks)), dim3(kThreads), 0, st, a, slices,
                      slice_bytes, parts, far ? budget : INT32_MAX);
   if (far)
     hipLaunchKernelGGL(evict_fetch_kernel, dim3(static_cast<unsigned>(rows * fetch_parts * splits)), dim3(kFetchThreads), 0,

@@ -2399,7 +2399,7 @@ def paged_cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table:
         raise RuntimeError(f"{who}: sink and recent must be within the budget")
     _refuse_gradient(who, k_cache, v_cache, k_scale, v_scale, weight_sum)
     new_lens = torch.empty_like(seq_lens)
-    kept = torch.empty((batch, heads, budget), dtype=torch.int32, device=k_cache.device)
+    kept = seq_lens.new_empty((batch, heads, budget))
     lib = _lib.load()
     need = lib.tris_paged_cache_evict_workspace_bytes(batch, heads, max_pages, page, budget)
     ws = torch.empty(need, dtype=torch.uint8, device=k_cache.device) if need else None  # of this call alone
