@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 import struct
 
 import torch
@@ -2207,9 +2208,19 @@ def _token_positions(who, positions, tokens, index):
 
 
 @functools.lru_cache(64)
-def _sections(sections):
+def _int32_array(counts):
+    return (ctypes.c_int32 * len(counts))(*counts)
+
+
+def _sections(who, sections):
     """A C array of the sections."""
-    return (ctypes.c_int32 * len(sections))(*sections)
+    try:
+        counts = tuple(map(operator.index, sections))
+    except TypeError:
+        counts = None
+    if counts is None or any(not -_INT32_MAX <= n <= _INT32_MAX for n in counts):
+        raise RuntimeError(f"{who}: sections must be counts of pairs")
+    return _int32_array(counts)
 
 
 def rotary_append_paged(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
@@ -2292,7 +2303,7 @@ def rotary_append_paged(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor
     else:
         name = "tris_rotary_axes_append_paged"
         axes, stride = _token_positions(who, positions, tokens, index)
-        split = _sections((half,) if sections is None else tuple(sections))
+        split = _int32_array((half,)) if sections is None else _sections(who, sections)
         if len(split) != axes:
             raise RuntimeError(f"{who}: positions must have a row for each of the sections")
         rc = _launch(index, _lib.load().tris_rotary_axes_append_paged, *args, positions.data_ptr(), stride, axes, split,
