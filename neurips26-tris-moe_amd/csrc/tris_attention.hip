@@ -30,6 +30,15 @@
 // workgroup has whole is written at once; the pieces of one that several share leave fp32 sums in the workspace, and a
 // second launch joins them.
 //
+// The keys' weights (weight_sum[kv head][j] += sum_h exp(s_hj - m_h) / l_h, over the kv head's query heads) need every
+// head's m and l before the first of them is known, so the first launch leaves the scaled scores, 4 bytes for each query
+// head and key, and the second, beside the join, takes the weights from them: 8 group bytes a key and kv head more than
+// 4 head_dim, and 8 for the sum.  What they cost over the call without them: 131072 tokens with 4 kv heads of 8 query heads
+// 51 -> 69 us, 64 sequences on e4m3 of 4 query heads a kv head 137 -> 196, 16 ragged 23 -> 29, 1000 tokens 8.8 -> 10.2.  The
+// scores' way to memory is most of it: 47 MB of stores cost the second of these 44 us beside its 5.9 TB/s of loads, 1 TB/s
+// (a large copy writes at 2.6), in stretches of 64 bytes to 4 KB, cached or written through alike, and nothing where they
+// fall on lines that stay in the L2.  Reading the keys again instead would take 23 and 67 us.
+//
 // Times beside the choices below are of whole calls, kernels and join, in a graph over three states: "128k" and the
 // others are the calls named here, "ragged" is 16 sequences of 20 to 8000 tokens on fp16, "wide" 8 of 1000 to 16000 with
 // 256 dimensions and pages of 20.
@@ -79,7 +88,7 @@ struct AttentionArgs {
 };
 
 // Whether a workgroup of the attention adds the weights of what it has itself: it has a kv head's keys and query heads
-// whole.
+// whole, so that there is no second launch (128 tokens 7.3 us, 9.0 with one; 64 of 100 to 500 21.3, 23.6).
 __host__ __device__ inline bool own_weights(const AttentionArgs& a) { return a.owners == nullptr && a.head_tiles == 1; }
 
 // a value that every lane holds alike, moved to a scalar register
@@ -269,7 +278,7 @@ __device__ __forceinline__ float2 infinite_sums(const AttentionArgs& a, const Pi
 }
 
 // The scores of a (sequence, head group): tile by tile, in each its halves of 16 keys, in each the group's heads, so that
-// a wavefront's store is one stretch of memory.  (64 on e4m3 201 us with each head's scores in a row of its own, xx.)
+// a wavefront's store is one stretch of memory (64 on e4m3 199 us, 202 with a row for each head).
 __device__ __forceinline__ float* score_block(const AttentionArgs& a, int b, int kvh, int head0) {
   return a.scores + ((static_cast<int64_t>(b) * a.c.kv_heads + kvh) * a.group + head0) * a.score_row;
 }
@@ -607,7 +616,9 @@ __device__ __forceinline__ void attend_piece(const AttentionArgs& a, const Piece
         x[j] = valid[j] ? x[j] : -INFINITY;
       }
     }
-    if constexpr (kWeights) {  // (a lane without a head: outside the buffer, without a branch)
+    // (a lane without a head: outside the buffer, without a branch, which would make the loads in flight wait: wide 37.9 us,
+    // 39.1 with one)
+    if constexpr (kWeights) {
       const __amdgpu_buffer_rsrc_t rows = make_rsrc(scores + static_cast<int64_t>(key0) * heads, heads * 128);
       __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{x[0], x[1], x[2], x[3]}), rows, score_at, 0, 0);
       __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{x[4], x[5], x[6], x[7]}), rows, score_at,
@@ -711,8 +722,8 @@ __device__ __forceinline__ float2 joined(float2 x, float2 y) {
 
 // Adds the weights of a piece's keys (tiles [t0, t1) of sequence b's n positions from `first` on) to the sums of their kv
 // head, from the scores that the attention left, for all query heads of the kv head.  stats: LDS for 1 + kWaves float2 of each.
-// A thread has four keys; the scores of eight heads and the sums are asked for a step ahead of their use, the first ones
-// before the statistics are known.
+// A thread has four keys; the scores of eight heads are asked for a step ahead of their use, the first ones before the
+// statistics are known.  (The sums and pages asked for with them: no difference.)
 __device__ __forceinline__ void sum_weights(const AttentionArgs& a, int b, int kvh, int n, int first, int t0, int t1,
                                             float shift, float2* stats) {
   const bool sums4 = a.sums4 != 0;
@@ -736,8 +747,8 @@ __device__ __forceinline__ void sum_weights(const AttentionArgs& a, int b, int k
   if (key < end) load(key, 0, x);
 
   // Each head's maximum and sum over the pieces.  Of few pieces a wavefront takes a head, a lane a piece; of many a lane takes
-  // one head and every sixteenth piece (131072 tokens, 192 pieces: the launch 11.6 us, 13.3 the other way; 16 ragged, 6
-  // pieces, 8.3, 8.9 the other way).
+  // one head and every sixteenth piece (131072 tokens, 192 pieces: the launch 12.0 us, 13.3 the other way; 16 ragged, 6
+  // pieces, 8.5, 8.9 the other way).
   const auto owners = [&](int tile) {
     return a.owners == nullptr ? make_int2(0, 0) : a.owners[(b * a.c.kv_heads + kvh) * a.head_tiles + tile];
   };
