@@ -86,7 +86,7 @@ def test_ragged_lengths(tris, cuda, types, dim, page, order):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("heads", [(1, 1), (4, 4), (6, 2), (7, 1), (16, 1), (17, 1), (40, 2), (33, 3), (64, 1)], ids=str)
+@pytest.mark.parametrize("heads", [(1, 1), (4, 4), (6, 2), (7, 1), (16, 1), (17, 1), (40, 2), (33, 3), (64, 1), (1024, 1)], ids=str)
 @pytest.mark.parametrize("types", [(BF16, BF16), (F16, E4M3)], ids=str)
 @pytest.mark.parametrize("lengths", [[300, 1, 0, 77], [3000, 1, 0, 77, 1500], [12000]], ids=str)
 def test_head_layouts(tris, cuda, heads, types, lengths):
