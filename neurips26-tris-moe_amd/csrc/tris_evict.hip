@@ -264,7 +264,7 @@ __global__ __launch_bounds__(kBlock) void evict_select_kernel(const EvictArgs a)
   }
   if (h == 0 && thread == 0) a.new_lens[b] = due ? a.budget : a.c.seq_lens[b];
   if (!due) {
-    for (int i = thread; i < a.budget; i += kBlock) kept[i] = -1;
+    for (uint32_t i = thread; i < static_cast<uint32_t>(a.budget); i += kBlock) kept[i] = -1;  // (a step past 2^31 at most)
     return;
   }
   const int lo = a.sink, hi = n - a.recent, want = a.budget - a.sink - a.recent;
@@ -365,7 +365,7 @@ struct Segment {
     h = row - b * a.c.kv_heads;
     n = evict_length(a, b);
     begin = static_cast<int>(min(static_cast<int64_t>(s) * a.segment, static_cast<int64_t>(n)));
-    end = min(n, begin + a.segment);
+    end = static_cast<int>(min(static_cast<int64_t>(n), static_cast<int64_t>(begin) + a.segment));
   }
   __device__ int64_t index(const EvictArgs& a) const { return static_cast<int64_t>(row) * a.segments + s; }
 };
@@ -400,7 +400,8 @@ __global__ __launch_bounds__(kThreads) void evict_histogram_kernel(const EvictAr
   }
   if (!due) {
     int32_t* kept = a.kept + static_cast<int64_t>(g.row) * a.budget;
-    for (int i = g.s * kThreads + thread; i < a.budget; i += a.segments * kThreads) kept[i] = -1;
+    const uint32_t step = a.segments * kThreads;
+    for (uint32_t i = g.s * kThreads + thread; i < static_cast<uint32_t>(a.budget); i += step) kept[i] = -1;
     return;
   }
   const int lo = max(g.begin, a.sink), hi = min(g.end, g.n - a.recent);
@@ -515,7 +516,7 @@ __global__ __launch_bounds__(kThreads) void evict_place_kernel(const EvictArgs a
   __syncthreads();
   if (thread < g.s) {
     const int begin = static_cast<int>(min(static_cast<int64_t>(thread) * a.segment, static_cast<int64_t>(g.n)));
-    const int end = min(g.n, begin + a.segment);
+    const int end = static_cast<int>(min(static_cast<int64_t>(g.n), static_cast<int64_t>(begin) + a.segment));
     // (and the first and last positions, which are held)
     atomicAdd(&before[0], row_counts[thread].x + max(0, min(end, lo) - begin) + max(0, end - max(begin, hi)));
   }
@@ -727,7 +728,7 @@ static EvictSpace evict_space(int64_t rows, int64_t positions, int64_t budget) {
   s.hist = s.counts + up(rows * 2LL * s.segments * 4);
   s.found = s.hist + rows * s.segments * kFirstBins * 4;
   s.moved = s.found + rows * s.segments * s.segment * 4;
-  s.bytes = s.moved + rows * budget * 4;
+  s.bytes = s.moved + (budget < positions ? rows * budget * 4 : 0);  // (no sequence is due from there on)
   return s;
 }
 

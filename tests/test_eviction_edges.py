@@ -125,3 +125,27 @@ def test_evicted_cache_is_read_and_appended_to(tris, cuda):
             for h in range(2):
                 assert torch.equal(now[h], before[h][kept[b, h].cpu().long()])
     assert not bool(sums[0, :, budget:150].any()) and not bool(sums[1, :, budget:90].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("extra_pages", [1, 1200], ids=["one workgroup", "segments"])
+def test_the_largest_budget(tris, cuda, extra_pages):
+    """A budget of 2^31 - 1: no sequence is due, nothing moves, and every one of its places says so."""
+    a = evict_case(cuda, 1, 64, F16, 16, [200], seed=3, extra_pages=extra_pages)
+    before = {n: a[n].clone() for n in ("k_cache", "v_cache", "weight_sum")}
+    new, kept = tris["ext"].paged_cache_evict(**a, budget=2 ** 31 - 1)
+    assert new.tolist() == [200] and kept.shape == (1, 1, 2 ** 31 - 1)
+    for part in kept[0, 0].split(1 << 28):
+        assert bool((part == -1).all())
+    for n, t in before.items():
+        raw = torch.int16 if t.element_size() == 2 else torch.int32
+        assert torch.equal(t.view(raw), a[n].view(raw)), n
+
+
+def test_workspace_of_budgets_past_the_table(tris):
+    """No sums move where no sequence can be due."""
+    from tris_moe_amd import _lib
+
+    need = _lib.load().tris_paged_cache_evict_workspace_bytes
+    assert need(1, 1, 1213, 16, 1213 * 16) == need(1, 1, 1213, 16, 2 ** 31 - 1)
+    assert need(1, 1, 1213, 16, 1213 * 16 - 1) == need(1, 1, 1213, 16, 1213 * 16) + 4 * (1213 * 16 - 1)
