@@ -982,8 +982,8 @@ int64_t tris_paged_attention_workspace_bytes(int32_t batch, int32_t q_heads, int
  * positive sign or a NaN makes the sums of all its keys NaN, as its softmax is; one whose scores are all -infinity adds
  * zeros.  out is tris_paged_attention_decode's.  weight_sum [batch][kv_heads][>= max_pages * page_size] fp32, strides in
  * elements over sequences and heads, positions contiguous, rows without shared memory; up to 1024 query heads for a kv
- * head.  workspace: tris_paged_attention_weights_workspace_bytes, as above (the scores, 4 bytes for each query head and position of the
- * table, among it).
+ * head.  workspace: tris_paged_attention_weights_workspace_bytes, as above (the scores, 4 bytes for each query head and
+ * position of the table, among it).
  */
 int tris_paged_attention_decode_weights(const void* q, int64_t q_seq_stride, int64_t q_head_stride, int32_t q_type,
                                         int32_t q_heads, const tris_paged_cache* cache, float scale, int32_t window,
@@ -1004,7 +1004,8 @@ int64_t tris_paged_attention_weights_workspace_bytes(int32_t batch, int32_t q_he
  * No page below an evicted sequence's length may be another sequence's, or its own twice.
  * 0 <= sink, 0 <= recent, sink + recent <= budget, 1 <= budget <= limit.  weight_sum as
  * tris_paged_attention_decode_weights takes it; new_lens [batch], apart from seq_lens; kept
- * [batch][kv_heads][budget], contiguous.  The cache's rows, scales and sums without shared memory.  workspace:
+ * [batch][kv_heads][budget], contiguous.  The cache's rows, scales and sums without shared memory, keys and values apart
+ * (both move, at the same time).  workspace:
  * tris_paged_cache_evict_workspace_bytes of the same sizes (0: none needed), 16-byte aligned, no initial contents; calls
  * that may overlap need one each.
  */

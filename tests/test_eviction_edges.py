@@ -149,3 +149,29 @@ def test_workspace_of_budgets_past_the_table(tris):
     need = _lib.load().tris_paged_cache_evict_workspace_bytes
     assert need(1, 1, 1213, 16, 1213 * 16) == need(1, 1, 1213, 16, 2 ** 31 - 1)
     assert need(1, 1, 1213, 16, 1213 * 16 - 1) == need(1, 1, 1213, 16, 1213 * 16) + 4 * (1213 * 16 - 1)
+
+
+@pytest.mark.parametrize("kw", [{}, dict(dtype=3, v=8192, k_scale=4096, v_scale=4096)], ids=["rows", "scales"])
+def test_keys_that_are_the_values_are_refused(tris, kw):
+    """Both would be moved in the same memory at the same time."""
+    import ctypes
+
+    from test_paged_cache import c_cache
+    from tris_moe_amd import _lib
+
+    lib, p = _lib.load(), ctypes.c_void_p(4096)
+    c = c_cache(**kw)
+    for n in ("k", "v"):
+        for field, stride in (("page", 32), ("head", 16), ("slot", 1)):
+            setattr(c, f"{n}_scale_{field}_stride", stride)
+    rc = lib.tris_paged_cache_evict(ctypes.byref(c), p, 96, 48, 8, 8, 1, 2, ctypes.c_void_p(8192), p, None, 0, None)
+    assert rc == -1 and b"share memory" in lib.tris_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache,shared", [(F16, "cache"), (E4M3, "scale")], ids=["rows", "scales"])
+def test_a_pool_given_twice_is_refused(tris, cuda, cache, shared):
+    a = evict_case(cuda, 2, 64, cache, 16, [100, 30])
+    a[f"v_{shared}"] = a[f"k_{shared}"]
+    with pytest.raises(RuntimeError, match="share memory"):
+        tris["ext"].paged_cache_evict(**a, budget=20)
