@@ -339,8 +339,11 @@ __global__ __launch_bounds__(kBlock) void evict_select_kernel(const EvictArgs a)
     const int ties = static_cast<int>(before >> 16) + __popcll(__ballot(tie) & below);
     if (sure || (tie && ties < equal)) {
       const int place = sures + min(ties, equal);
-      kept[place] = i;
-      sums[place] = weights[i];  // (the row's weights are all in LDS)
+      // (outside the budget, on either side, only if the lengths change meanwhile)
+      if (static_cast<uint32_t>(place) < static_cast<uint32_t>(a.budget)) {
+        kept[place] = i;
+        sums[place] = weights[i];  // (the row's weights are all in LDS)
+      }
     }
   }
   for (int i = a.budget + thread; i < n; i += kBlock) sums[i] = 0.0f;
@@ -583,7 +586,8 @@ __global__ __launch_bounds__(kThreads) void evict_place_kernel(const EvictArgs a
       const int t = tied + (past >> 16) + __popcll(tie[j] & below);
       const int place = sures + (past & 0xFFFF) + __popcll(sure[j] & below) + min(t, equal);
       const bool stays = (sure[j] >> lane & 1) || ((tie[j] >> lane & 1) && t < equal);
-      if (stays && place < a.budget) {  // (past it only if the sums change meanwhile)
+      // (outside the budget, on either side, only if the sums change meanwhile)
+      if (stays && static_cast<uint32_t>(place) < static_cast<uint32_t>(a.budget)) {
         kept[place] = i0 + j * kThreads + thread;
         moved[place] = now.w[j];
       }
