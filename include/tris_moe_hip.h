@@ -1005,7 +1005,8 @@ int64_t tris_paged_attention_weights_workspace_bytes(int32_t batch, int32_t q_he
  * 0 <= sink, 0 <= recent, sink + recent <= budget, 1 <= budget <= limit.  weight_sum as
  * tris_paged_attention_decode_weights takes it; new_lens [batch], apart from seq_lens; kept
  * [batch][kv_heads][budget], contiguous.  The cache's rows, scales and sums without shared memory, keys and values apart
- * (both move, at the same time).  workspace:
+ * (both move, at the same time; as parts of one buffer, one behind the other or interleaved under the same strides).
+ * workspace:
  * tris_paged_cache_evict_workspace_bytes of the same sizes (0: none needed), 16-byte aligned, no initial contents; calls
  * that may overlap need one each.
  */

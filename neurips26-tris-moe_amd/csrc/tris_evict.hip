@@ -784,7 +784,7 @@ extern "C" int tris_paged_cache_evict(const tris_paged_cache* cache, float* weig
                "%s: too many rows", who);
   TRIS_REQUIRE(s.bytes == 0 || (workspace && aligned16(workspace) && workspace_bytes >= s.bytes),
                "%s: workspace of %lld bytes needed", who, static_cast<long long>(s.bytes));
-  TRIS_REQUIRE(c.k != c.v && (!c.k_scale || c.k_scale != c.v_scale), "%s: keys and values must not share memory", who);
+  TRIS_REQUIRE(keys_and_values_apart(c), "%s: keys and values must not share memory", who);
   EvictArgs a{weight_sum, sum_seq_stride, sum_head_stride, budget, limit, sink, recent, new_lens, kept,
               PageDivision(c.page_size), c, s.segments, s.segment, nullptr, nullptr, nullptr, nullptr, nullptr};
   const hipStream_t st = static_cast<hipStream_t>(stream);

@@ -98,6 +98,47 @@ inline bool cache_scales_apart(const tris_paged_cache& c) {
                         cache_rows_apart(c, c.v_scale_page_stride, c.v_scale_head_stride, c.v_scale_slot_stride, 1));
 }
 
+// Whether two pools of rows of `row` bytes, `to` bytes from the first's beginning to the second's, share no memory, by their
+// strides (in bytes, largest first, each pool's own rows apart).  Parts of one buffer may interleave: under the same largest
+// stride P a unit of the second meets no units of the first but those `to` mod P and `to` mod P - P bytes from it, since no
+// unit is longer than P.  Pools whose strides differ before the ones' units end up beside the others' are taken as shared.
+template <size_t kDims>
+bool pools_apart(const std::array<RowDimension, kDims>& x, const std::array<RowDimension, kDims>& y, size_t from,
+                 __int128 to, int64_t row) {
+  __int128 x_end = row, y_end = to + row;
+  for (size_t i = from; i < kDims; ++i) {
+    x_end += static_cast<__int128>(x[i].size - 1) * x[i].stride;
+    y_end += static_cast<__int128>(y[i].size - 1) * y[i].stride;
+  }
+  if (to >= x_end || y_end <= 0) return true;
+  if (from == kDims || x[from].stride != y[from].stride) return false;
+  const __int128 step = x[from].stride;
+  if (step == 0) return false;  // (a dimension of one, and those behind it)
+  const __int128 rest = (to % step + step) % step;
+  return pools_apart(x, y, from + 1, rest, row) && pools_apart(x, y, from + 1, rest - step, row);
+}
+
+// The cache's keys and values, and their scales, for a call that moves both at the same time.
+inline bool keys_and_values_apart(const tris_paged_cache& c) {
+  const auto apart = [&c](const void* k, std::array<int64_t, 3> k_strides, const void* v, std::array<int64_t, 3> v_strides,
+                          int64_t values, int64_t bytes) {
+    const auto dims = [&](const std::array<int64_t, 3>& strides) {
+      const int32_t sizes[3] = {c.num_pages, c.kv_heads, c.page_size};
+      std::array<RowDimension, 3> d;
+      for (int i = 0; i < 3; ++i) d[i] = RowDimension{sizes[i], sizes[i] > 1 ? strides[i] * bytes : 0};
+      std::sort(d.begin(), d.end(), [](const RowDimension& x, const RowDimension& y) { return x.stride > y.stride; });
+      return d;
+    };
+    const __int128 to = static_cast<__int128>(reinterpret_cast<uintptr_t>(v)) - reinterpret_cast<uintptr_t>(k);
+    return pools_apart<3>(dims(k_strides), dims(v_strides), 0, to, values * bytes);
+  };
+  return apart(c.k, {c.k_page_stride, c.k_head_stride, c.k_slot_stride}, c.v,
+               {c.v_page_stride, c.v_head_stride, c.v_slot_stride}, c.head_dim, c.dtype == TRIS_DTYPE_E4M3 ? 1 : 2) &&
+         (!c.k_scale ||
+          apart(c.k_scale, {c.k_scale_page_stride, c.k_scale_head_stride, c.k_scale_slot_stride}, c.v_scale,
+                {c.v_scale_page_stride, c.v_scale_head_stride, c.v_scale_slot_stride}, 1, 4));
+}
+
 // Sums of attention weights, a row of all positions for each (sequence, kv head): strides that keep the rows apart.
 inline bool sum_rows_apart(const tris_paged_cache& c, int64_t seq_stride, int64_t head_stride) {
   return seq_stride >= 0 && head_stride >= 0 &&

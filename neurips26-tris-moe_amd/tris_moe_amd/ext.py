@@ -2393,8 +2393,9 @@ def paged_cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table:
     the old lengths before the new ones are copied there.
 
     The cache, block_table and seq_lens as rotary_append_paged takes them, weight_sum as paged_attention_decode does.  No
-    page of an evicted sequence may be another sequence's too, or its own twice; keys and values share no memory,
-    nor do their scales.  Rotary positions go on from the sequence's true length
+    page of an evicted sequence may be another sequence's too, or its own twice; keys and values share no memory, nor do
+    their scales (as views of one buffer, they lie one behind the other, or interleave with the same strides down to the
+    dimension that holds both).  Rotary positions go on from the sequence's true length
     (``positions`` of rotary_append_paged).  The launch depends on no value on the device, so a captured decode step may
     evict in every replay, with a limit above the budget every limit - budget + 1 steps.  No gradient."""
     who = "paged_cache_evict"
