@@ -1003,8 +1003,8 @@ int64_t tris_paged_attention_weights_workspace_bytes(int32_t batch, int32_t q_he
  * seq_lens[b], and kept[b] is -1 throughout.  The keys and values of positions budget .. n - 1 stay in the cache's memory.
  * No page below an evicted sequence's length may be another sequence's, or its own twice.
  * 0 <= sink, 0 <= recent, sink + recent <= budget, 1 <= budget <= limit.  weight_sum as
- * tris_paged_attention_decode_weights takes it; new_lens [batch], apart from seq_lens; kept
- * [batch][kv_heads][budget], contiguous.  The cache's rows, scales and sums without shared memory, keys and values apart
+ * tris_paged_attention_decode_weights takes it; new_lens [batch] and kept
+ * [batch][kv_heads][budget], contiguous, share no memory with seq_lens or each other.  The cache's rows, scales and sums without shared memory, keys and values apart
  * (both move, at the same time; as parts of one buffer, one behind the other or interleaved under the same strides).
  * workspace:
  * tris_paged_cache_evict_workspace_bytes of the same sizes (0: none needed), 16-byte aligned, no initial contents; calls

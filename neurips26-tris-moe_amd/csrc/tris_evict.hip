@@ -760,7 +760,6 @@ extern "C" int tris_paged_cache_evict(const tris_paged_cache* cache, float* weig
                "%s: sink and recent must be within the budget", who);
   if (c.batch == 0) return TRIS_OK;
   TRIS_REQUIRE((weight_sum || c.max_pages == 0) && new_lens && kept, "%s: null pointer", who);
-  TRIS_REQUIRE(new_lens != c.seq_lens, "%s: new_lens must not be seq_lens", who);
   TRIS_REQUIRE(cache_rows_apart(c), "%s: cache rows overlap", who);
   TRIS_REQUIRE(cache_scales_apart(c), "%s: cache scales overlap", who);
   TRIS_REQUIRE(sum_rows_apart(c, sum_seq_stride, sum_head_stride), "%s: rows of weight_sum overlap", who);
@@ -782,9 +781,17 @@ extern "C" int tris_paged_cache_evict(const tris_paged_cache* cache, float* weig
   TRIS_REQUIRE((rows + kXcds) * std::max(parts, s.segments) < (1LL << 32) / kThreads &&
                    rows * fetch_parts * splits < (1LL << 32) / kFetchThreads,
                "%s: too many rows", who);
+  // (the lengths are read after the first new ones, and the first of kept's places, are written)
+  const auto over = [](const int32_t* x, int64_t n, const int32_t* y, int64_t m) {
+    const auto x0 = reinterpret_cast<uintptr_t>(x), y0 = reinterpret_cast<uintptr_t>(y);
+    return x0 < y0 ? (y0 - x0) / 4 < static_cast<uint64_t>(n) : (x0 - y0) / 4 < static_cast<uint64_t>(m);
+  };
+  TRIS_REQUIRE(!over(new_lens, c.batch, c.seq_lens, c.batch), "%s: new_lens must not overlap seq_lens", who);
   TRIS_REQUIRE(s.bytes == 0 || (workspace && aligned16(workspace) && workspace_bytes >= s.bytes),
                "%s: workspace of %lld bytes needed", who, static_cast<long long>(s.bytes));
   TRIS_REQUIRE(keys_and_values_apart(c), "%s: keys and values must not share memory", who);
+  TRIS_REQUIRE(!over(kept, rows * budget, c.seq_lens, c.batch) && !over(kept, rows * budget, new_lens, c.batch),
+               "%s: kept must not overlap the lengths", who);
   EvictArgs a{weight_sum, sum_seq_stride, sum_head_stride, budget, limit, sink, recent, new_lens, kept,
               PageDivision(c.page_size), c, s.segments, s.segment, nullptr, nullptr, nullptr, nullptr, nullptr};
   const hipStream_t st = static_cast<hipStream_t>(stream);

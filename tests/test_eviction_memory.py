@@ -12,13 +12,14 @@ from test_paged_evict import evict_case, run_and_check
 F16, BF16 = torch.float16, torch.bfloat16
 
 
-def _evict(c, lens=1 << 40, new_lens=1 << 41):
+def _evict(c, lens=1 << 40, new_lens=1 << 41, kept=1 << 42):
     """The C entry on addresses that are never read: for calls that it refuses.  (rc, message)"""
     from tris_moe_amd import _lib
 
     lib, p = _lib.load(), ctypes.c_void_p(1 << 39)
     c.seq_lens = lens
-    rc = lib.tris_paged_cache_evict(ctypes.byref(c), p, 96, 48, 8, 8, 1, 2, ctypes.c_void_p(new_lens), p, None, 0, None)
+    rc = lib.tris_paged_cache_evict(ctypes.byref(c), p, 96, 48, 8, 8, 1, 2, ctypes.c_void_p(new_lens),
+                                    ctypes.c_void_p(kept), None, 0, None)
     return rc, lib.tris_last_error()
 
 
@@ -55,6 +56,22 @@ def test_scales_over_scales_are_refused(tris, to):
         for field, s in (("page", 32), ("head", 16), ("slot", 1)):
             setattr(c, f"{n}_scale_{field}_stride", s)
     assert _evict(c) == (-1, b"tris_paged_cache_evict: keys and values must not share memory")
+
+
+@pytest.mark.parametrize("batch,to", [(2, 0), (2, 4), (2, -4), (9, 32), (9, -32), (9, 2), (9, -35)])
+def test_new_lengths_over_lengths_are_refused(tris, batch, to):
+    c = c_cache(k=1 << 36, v=1 << 37, batch=batch)
+    rc, message = _evict(c, new_lens=(1 << 40) + to)
+    assert rc == -1 and b"new_lens must not overlap seq_lens" in message
+
+
+@pytest.mark.parametrize("of", ["lens", "new_lens"])
+@pytest.mark.parametrize("to", [0, 4, -4, -127, 7 - 4 * 2 * 2 * 8])
+def test_kept_over_lengths_is_refused(tris, of, to):
+    """Two sequences of two heads keep eight each: 128 bytes."""
+    at = dict(lens=1 << 40, new_lens=1 << 41)
+    rc, message = _evict(c_cache(k=1 << 36, v=1 << 37), **at, kept=at[of] + to)
+    assert rc == -1 and b"kept must not overlap the lengths" in message
 
 
 # one buffer of keys and values, by its dimensions (c: which of the two; o: a part that the pool leaves out)
