@@ -39,7 +39,8 @@ class PagedKVCache:
     its own type: under ``TrisPagedAttention``, whose projections are fp16, a cache is float16 or float8_e4m3fn.
     Which pages a sequence has is the block table's matter; a page's contents count only below the lengths given with
     it.  weight_sum: None, or after ``track_weights`` fp32 [batch, kv_heads, positions], the attention weights that each
-    place has had, row b for the block table's row b; a caller that gives row b to a new sequence sets it to zero."""
+    place has had, row b for the block table's row b; a caller that gives row b to a new sequence sets it to zero, and one
+    that moves a sequence to another row moves its sums too."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.float16,
                  device="cuda"):
@@ -54,9 +55,16 @@ class PagedKVCache:
             self.k_scale, self.v_scale = (torch.empty(shape[:3], dtype=torch.float32, device=device) for _ in range(2))
 
     def track_weights(self, batch: int, positions: int) -> None:
-        """From now on ``attend`` sums the attention weights of block tables of `batch` rows and up to `positions`
+        """From now on ``attend`` sums the attention weights of block tables of up to `batch` rows and `positions`
         positions (max_pages * page_size), from zero."""
         self.weight_sum = torch.zeros((batch, self.k.size(1), positions), dtype=torch.float32, device=self.k.device)
+
+    def _sums(self, block_table):
+        """The sums of a block table's rows: of fewer than `batch`, the first ones'."""
+        if self.weight_sum is None or not isinstance(block_table, torch.Tensor) or block_table.ndim != 2:
+            return self.weight_sum
+        rows = block_table.size(0)
+        return self.weight_sum if rows >= self.weight_sum.size(0) else self.weight_sum[:rows]
 
     def append(self, q, k, v, cos, sin, block_table, seq_lens, query_start=None, positions=None, sections=None,
                interleaved=False):
@@ -68,15 +76,16 @@ class PagedKVCache:
     def attend(self, q, block_table, seq_lens, scale=None, window=0):
         """ext.paged_attention_decode on this pool."""
         return ext.paged_attention_decode(q, self.k, self.v, block_table, seq_lens, scale, window,
-                                          k_scale=self.k_scale, v_scale=self.v_scale, weight_sum=self.weight_sum)
+                                          k_scale=self.k_scale, v_scale=self.v_scale,
+                                          weight_sum=self._sums(block_table))
 
     def evict(self, block_table, seq_lens, budget, limit=None, sink=0, recent=0):
         """ext.paged_cache_evict on this pool: (new lengths, kept positions).  With one pair of tables for all layers,
         every layer evicts by the old lengths; then seq_lens takes the new ones, which are the same for each."""
         if self.weight_sum is None:
             raise RuntimeError("evict: the cache has no sums of attention weights (track_weights)")
-        return ext.paged_cache_evict(self.k, self.v, block_table, seq_lens, self.weight_sum, budget, limit, sink, recent,
-                                     k_scale=self.k_scale, v_scale=self.v_scale)
+        return ext.paged_cache_evict(self.k, self.v, block_table, seq_lens, self._sums(block_table), budget, limit, sink,
+                                     recent, k_scale=self.k_scale, v_scale=self.v_scale)
 
 
 class TrisPagedAttention(nn.Module):
