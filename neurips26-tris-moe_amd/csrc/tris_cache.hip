@@ -6,9 +6,9 @@
 // and so are the cosines and sines, since a lane has the same part of each of its heads.  An 8-bit row's largest
 // magnitude is a maximum over the head's head_dim / 16 neighbouring lanes.
 //
-// Bound by memory where there are many tokens: 8189 of 32 query and 8 kv heads of 128, bf16 (205 MB), 39.9 us in a graph,
-// 5.15 TB/s, a large copy's rate; else by two memory latencies (boundaries and lengths, then page and angles): one token
-// for each of 16 sequences 3.7 us.  With positions of their own, on three axes, 42.5 (43.1 beside it without) and 4.2 us.
+// Bound by memory where there are many tokens: 8189 of 32 query and 8 kv heads of 128, bf16 (205 MB), 42.8 us in a graph over
+// three states, 4.8 TB/s (a large copy 5.15); else by two memory latencies (boundaries and lengths, then page and angles): one
+// token for each of 16 sequences 3.5 us.  With positions of their own, on three axes, 42.3 and 4.2 us, in turn with these.
 #include "tris_paged.h"
 
 // The rotation's two products and their sum are rounded one by one, as the same torch expression rounds them, so that
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(256) void rotary_append_kernel(const AppendArgs a) 
   constexpr int kPairUnits = kMostPairs / kWave;
   __shared__ float sh_cos[kAxes ? 4 : 1][kMostPairs], sh_sin[kAxes ? 4 : 1][kMostPairs];
   // each pair's angle once for the wavefront, asked for before the token's place is known, handed to the lanes that turn
-  // it through LDS (8189 tokens 42.5 us; asked for when the place is known 44.6, with every lane loading its own eight 53.2)
+  // it through LDS (8189 tokens 42.3 us; asked for when the place is known 44.6, with every lane loading its own eight 53.2)
   float pair_cos[kPairUnits] = {}, pair_sin[kPairUnits] = {};
   bool turnable = true;
   if constexpr (kAxes) {

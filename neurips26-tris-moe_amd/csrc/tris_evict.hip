@@ -704,11 +704,13 @@ constexpr int64_t kSmallMove = 64 << 10;
 constexpr int kManyRows = 160;
 // In a decode loop a sequence is due in one of limit - budget + 1 steps, and in the others a launch less is what counts: so
 // they move too where all sequences' moves come to so many bytes of a row a step (one sequence of 8 heads, 2048 positions of
-// 512 bytes, limit 2176: 3.9 / 5.5 us with nothing due, 40 / 20 when it is).
+// 512 bytes, limit 2176: 3.9 / 5.5 us with nothing due, 40 / 20 when it is).  A caller who makes the call only when it is due
+// gets the second by giving the budget as the limit.
 constexpr int64_t kRareMove = 16 << 10;
-// Budgets from which on the rows past them are moved by a launch of their own, where slices are few and the table has
-// twice as many positions (with it / without: 4 rows of 4096 of 32768 positions 43.5 / 46.1 us, 8192 of 65536 35.4 / 42.5;
-// 16 rows 53.5 / 51.1 and 56.8 / 67.7; 32 rows of 8192 of 32768 102.5 / 96.1).
+// Budgets past which the rows from past the budget are moved by a launch of their own, where slices are few and the table has
+// twice as many positions (with it / without: 4 rows of 8192 of 65536 positions 35.4 / 42.5 us, 16 rows 56.8 / 67.7; 32 rows of
+// 8192 of 32768, which are too many slices, 102.5 / 96.1).  4096 itself is left out, where it goes either way (of 32768, 4 rows
+// 43.5 / 46.1, 16 rows 53.5 / 51.1).
 constexpr int kFarBudget = 4096;
 
 struct EvictSpace {

@@ -2397,7 +2397,9 @@ def paged_cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table:
     their scales (as views of one buffer, they lie one behind the other, or interleave with the same strides down to the
     dimension that holds both).  Rotary positions go on from the sequence's true length
     (``positions`` of rotary_append_paged).  The launch depends on no value on the device, so a captured decode step may
-    evict in every replay, with a limit above the budget every limit - budget + 1 steps.  No gradient."""
+    evict in every replay, with a limit above the budget every limit - budget + 1 steps.  A limit far above the budget
+    makes the calls with nothing due cheap and those that evict dearer: where the host knows when one is due, leave it out
+    there (sequences between the budget and the limit are evicted from too).  No gradient."""
     who = "paged_cache_evict"
     if not (isinstance(k_cache, torch.Tensor) and k_cache.is_cuda):
         _check_on(who, "k_cache", k_cache, 4, _CACHE_DTYPES)
